@@ -15,6 +15,7 @@
 #include <string>
 #include <vector>
 
+#include "context.hpp"
 #include "gather.hpp"
 #include "gguf.hpp"
 #include "layout.hpp"
@@ -27,17 +28,6 @@
 // address: each device's copy is found with hipGetSymbolAddress (below) and
 // kept per device.
 static __device__ __align__(256) float scratch[CHARLOTTE_HIP_MATMUL_STATIC_SCRATCH_BYTES / sizeof(float)];
-
-struct charlotte_hip_matmul_context {
-    int device = 0;
-    uint32_t compute_units = 0;
-    float* scratch = nullptr;   // this device's copy of `scratch`
-    charlotte_hip_matmul_gemm_path gemm_path = CHARLOTTE_HIP_MATMUL_GEMM_AUTO;
-    charlotte_hip_matmul_gemv_path gemv_path = CHARLOTTE_HIP_MATMUL_GEMV_CANONICAL;
-    void* workspace = nullptr;  // the matrix-core path's, the caller's memory
-    uint64_t workspace_bytes = 0;
-    std::string error;
-};
 
 struct charlotte_hip_matmul_gguf {
     chm::GgufFile file;
@@ -55,20 +45,9 @@ namespace {
 
 using Status = charlotte_hip_matmul_status;
 
-Status fail(charlotte_hip_matmul_context* ctx, Status s, const std::string& message) {
-    if (ctx) ctx->error = message;
-    return s;
-}
-
-Status ok(charlotte_hip_matmul_context* ctx) {
-    if (ctx) ctx->error.clear();
-    return CHARLOTTE_HIP_MATMUL_OK;
-}
-
-Status hip_fail(charlotte_hip_matmul_context* ctx, hipError_t e, const char* what) {
-    return fail(ctx, e == hipErrorOutOfMemory ? CHARLOTTE_HIP_MATMUL_OUT_OF_MEMORY : CHARLOTTE_HIP_MATMUL_HIP_ERROR,
-                std::string(what) + ": " + hipGetErrorString(e));
-}
+using chm::fail;
+using chm::hip_fail;
+using chm::ok;
 
 // The formats a weight may hold: the reference's format table
 // (capability.cpp:57-65). The products and the gather read them all.

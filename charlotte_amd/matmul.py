@@ -199,6 +199,43 @@ class _GatherDesc(ctypes.Structure):
     ]
 
 
+class _Heads(ctypes.Structure):
+    _fields_ = [("input", ctypes.c_void_p), ("output", ctypes.c_void_p), ("input_stride", ctypes.c_uint64),
+                ("output_stride", ctypes.c_uint64), ("weight", ctypes.c_void_p), ("heads", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class _HeadNormRopeDesc(ctypes.Structure):
+    _fields_ = [("parts", _Heads * 2), ("part_count", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rope", ctypes.c_uint32), ("rope_dims", ctypes.c_uint32), ("cosines", ctypes.c_void_p),
+                ("sines", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("table_rows", ctypes.c_uint32),
+                ("epsilon", ctypes.c_float)]
+
+
+class _AttentionDesc(ctypes.Structure):
+    _fields_ = [("cache", ctypes.c_void_p), ("queries", ctypes.c_void_p), ("output", ctypes.c_void_p),
+                ("query_stride", ctypes.c_uint64), ("output_stride", ctypes.c_uint64), ("query_heads", ctypes.c_uint32),
+                ("window", ctypes.c_uint32), ("scale", ctypes.c_float), ("longest", ctypes.c_uint32),
+                ("past", ctypes.c_void_p), ("parents", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _ProbabilitiesDesc(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("output", ctypes.c_void_p), ("logit_stride", ctypes.c_uint64),
+                ("output_stride", ctypes.c_uint64), ("rows", ctypes.c_uint32), ("vocabulary", ctypes.c_uint32),
+                ("temperature", ctypes.c_float), ("reserved", ctypes.c_uint32), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _VerifyDesc(ctypes.Structure):
+    _fields_ = [("node_tokens", ctypes.c_void_p), ("target", ctypes.c_void_p), ("draft", ctypes.c_void_p),
+                ("uniforms", ctypes.c_void_p), ("accepts", ctypes.c_void_p), ("parents", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("path", ctypes.c_void_p), ("emitted", ctypes.c_void_p),
+                ("count", ctypes.c_void_p), ("target_stride", ctypes.c_uint64), ("draft_stride", ctypes.c_uint64),
+                ("vocabulary", ctypes.c_uint32), ("reserved", ctypes.c_uint32), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
 class _GgufTensor(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char_p),
@@ -254,6 +291,42 @@ SIGNATURES = {
         _c.c_int,
         [_c.c_void_p, _c.c_void_p, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_void_p, _c.c_void_p],
     ),
+    "charlotte_hip_matmul_head_norm_rope": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_HeadNormRopeDesc), _c.c_uint32, _c.c_void_p]),
+    "charlotte_hip_matmul_cache_bytes": (
+        _c.c_uint64, [_c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_cache_create": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.POINTER(_c.c_void_p)],
+    ),
+    "charlotte_hip_matmul_cache_wrap": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_void_p, _c.c_uint64,
+         _c.POINTER(_c.c_void_p)],
+    ),
+    "charlotte_hip_matmul_cache_free": (_c.c_int, [_c.c_void_p]),
+    "charlotte_hip_matmul_cache_append": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint64, _c.c_uint64, _c.c_void_p, _c.c_uint32,
+         _c.c_void_p],
+    ),
+    "charlotte_hip_matmul_cache_read": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint64, _c.c_uint64, _c.c_void_p, _c.c_uint32,
+         _c.c_void_p],
+    ),
+    "charlotte_hip_matmul_cache_keep": (
+        _c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint32, _c.c_void_p]),
+    "charlotte_hip_matmul_attention_workspace_bytes": (
+        _c.c_uint64, [_c.c_void_p, _c.c_void_p, _c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_attention": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_AttentionDesc), _c.c_uint32, _c.c_void_p]),
+    "charlotte_hip_matmul_probabilities_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_probabilities": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_ProbabilitiesDesc), _c.c_void_p]),
+    "charlotte_hip_matmul_verify_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_verify": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_VerifyDesc), _c.c_uint32, _c.c_uint32, _c.c_void_p]),
     "charlotte_hip_matmul_gguf_open": (_c.c_int, [_c.c_char_p, _c.POINTER(_c.c_void_p), _c.POINTER(_c.c_uint32)]),
     "charlotte_hip_matmul_gguf_read": (
         _c.c_int,

@@ -8,7 +8,9 @@
  * BF16 as stored) in device memory and is decoded in the kernels' load path;
  * x and y are f32. One token runs the decode form (a matrix-vector product
  * bound by HBM), more tokens the prefill form (a tiled matrix product). The
- * embedding gather decodes table rows through the same formats.
+ * embedding gather decodes table rows through the same formats. Between the
+ * products: norms and rotation of heads, a quantized cache, attention over it;
+ * after the head: probabilities, and drafted tokens verified.
  *
  * What each part replaces in the reference (paths relative to its root):
  *   charlotte_hip_matmul_desc       kernels::MatmulLaunch  src/core/kernels/matmul/matmul.h:602-632
@@ -427,6 +429,222 @@ charlotte_hip_matmul_status charlotte_hip_matmul_gather_positions(charlotte_hip_
                                                                   const charlotte_hip_matmul_weight* table,
                                                                   uint32_t positions, uint32_t grid_columns,
                                                                   uint32_t tokens, float* output, void* stream);
+
+/* ---- between a step's products: heads, cache, attention ------------------------- */
+
+/* What a decoder step runs between its QKV product and its output product, and
+ * after its head, for one token, a prompt's block or drafted tokens to verify:
+ * head_norm_rope on the Q and K the product wrote, cache_append of K and V,
+ * attention over the cache; then probabilities of the head's logits, verify,
+ * and cache_keep of the tokens accepted. Activations are f32, as the products'.
+ * A step holds `tokens` tokens of each of a cache's sequences, rows in
+ * sequence order: row s * tokens + t. Lengths and positions are device memory,
+ * so a captured step replays as they grow. Nothing here allocates but
+ * cache_create. Results are the same bits for the same call; they are not
+ * batch-invariant (the attention's splits follow the step's size). */
+
+/* How a head's values pair for the rotation: value i with i + rope_dims / 2, or
+ * 2i with 2i + 1. */
+typedef enum {
+    CHARLOTTE_HIP_MATMUL_ROPE_NONE = 0,
+    CHARLOTTE_HIP_MATMUL_ROPE_HALVES = 1,
+    CHARLOTTE_HIP_MATMUL_ROPE_NEIGHBOURS = 2
+} charlotte_hip_matmul_rope;
+
+/* The queries or the keys of a step: head h of token t is the head_dim floats at
+ * input + t * input_stride + h * head_dim, written likewise to output. */
+typedef struct {
+    const float* input;     /* device, 16-byte aligned */
+    float* output;          /* device, 16-byte aligned; input itself, or memory apart from it */
+    uint64_t input_stride;  /* floats from a token to the next, whole 4s; 0: heads * head_dim */
+    uint64_t output_stride;
+    const float* weight;    /* device, 16-byte aligned: the norm's head_dim weights, or NULL: not normalised */
+    uint32_t heads;
+    uint32_t reserved;      /* 0 */
+} charlotte_hip_matmul_heads;
+
+/* Each head x of each part becomes rotate(x / sqrt(mean(x^2) + epsilon) * weight):
+ * a pair (a, b) of its first rope_dims values becomes (a c - b s, b c + a s), c
+ * and s the pair's entries in row positions[t] of the tables. */
+typedef struct {
+    charlotte_hip_matmul_heads parts[2];
+    uint32_t part_count;        /* 1 or 2: queries, keys */
+    uint32_t head_dim;          /* 8 .. 256, whole 8s */
+    uint32_t rope;              /* charlotte_hip_matmul_rope */
+    uint32_t rope_dims;         /* whole 8s, at most head_dim; 0: head_dim. The rest is not rotated */
+    const float* cosines;       /* device, 16-byte aligned: table_rows rows of rope_dims / 2 */
+    const float* sines;
+    const uint32_t* positions;  /* device: each token's row; one past the tables makes the rotated values NaN */
+    uint32_t table_rows;
+    float epsilon;              /* finite, not negative */
+} charlotte_hip_matmul_head_norm_rope_desc;
+
+charlotte_hip_matmul_status charlotte_hip_matmul_head_norm_rope(charlotte_hip_matmul_context* ctx,
+                                                                const charlotte_hip_matmul_head_norm_rope_desc* desc,
+                                                                uint32_t tokens, void* stream);
+
+/* The keys and values of `sequences` sequences, `capacity` tokens each, in a
+ * format of blocks of 32 values of one head of one token:
+ *   Q8_0  d = f16(max|x| / 127), codes rint(x / d) within -127 .. 127
+ *   Q4_0  d = f16(m / -8), m the block's first value of the largest magnitude,
+ *         codes rint(x / d) within -8 .. 7
+ *   F16   binary16, rounded to nearest even
+ * (d = 0: codes 0). A block its format cannot hold - a NaN, an infinity, a
+ * scale or a value past binary16 - reads back as 32 NaNs, and reaches only the
+ * rows that see its token. The bytes are in an order of the library's own, the
+ * matrix cores' operands in 32-token tiles. head_dim: 32 .. 256, whole 32s. */
+typedef struct charlotte_hip_matmul_cache charlotte_hip_matmul_cache;
+
+/* Bytes a cache takes; 0 for a format or sizes it cannot have. */
+uint64_t charlotte_hip_matmul_cache_bytes(uint32_t gguf_type, uint32_t sequences, uint32_t kv_heads, uint32_t head_dim,
+                                          uint32_t capacity);
+/* A cache in memory of the library's (cleared, synchronously), or in the
+ * caller's: `device` 16-byte aligned, any contents, borrowed until freed. */
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_create(charlotte_hip_matmul_context* ctx, uint32_t gguf_type,
+                                                              uint32_t sequences, uint32_t kv_heads, uint32_t head_dim,
+                                                              uint32_t capacity, charlotte_hip_matmul_cache** out);
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_wrap(charlotte_hip_matmul_context* ctx, uint32_t gguf_type,
+                                                            uint32_t sequences, uint32_t kv_heads, uint32_t head_dim,
+                                                            uint32_t capacity, void* device, uint64_t bytes,
+                                                            charlotte_hip_matmul_cache** out);
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_free(charlotte_hip_matmul_cache* cache);
+
+/* Token t of sequence s, kv_heads * head_dim floats at keys + (s * tokens + t) *
+ * key_stride (and values), into slot past[s] + t. Strides in floats, whole 4s
+ * (0: kv_heads * head_dim), pointers 16-byte aligned. A slot past the capacity
+ * is not written. */
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_append(charlotte_hip_matmul_context* ctx,
+                                                              charlotte_hip_matmul_cache* cache, const float* keys,
+                                                              const float* values, uint64_t key_stride,
+                                                              uint64_t value_stride, const uint32_t* past,
+                                                              uint32_t tokens, void* stream);
+/* The reverse: slots first[s] .. first[s] + tokens - 1 as the values they stand
+ * for. A row whose slot lies past the capacity is left as it is. */
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_read(charlotte_hip_matmul_context* ctx,
+                                                            const charlotte_hip_matmul_cache* cache, float* keys,
+                                                            float* values, uint64_t key_stride, uint64_t value_stride,
+                                                            const uint32_t* first, uint32_t tokens, void* stream);
+/* The accepted path's slots moved together: slot past[s] + path[s * tokens + j]
+ * to past[s] + j, for j = 0 .. count[s] - 1 (at most `tokens`). A path rises:
+ * path[j] > path[j - 1] >= 0; it is taken to end before an entry that does not,
+ * or whose slot lies past the capacity. */
+charlotte_hip_matmul_status charlotte_hip_matmul_cache_keep(charlotte_hip_matmul_context* ctx,
+                                                            charlotte_hip_matmul_cache* cache, const uint32_t* past,
+                                                            const int32_t* path, const uint32_t* count, uint32_t tokens,
+                                                            void* stream);
+
+/* Attention of a step's tokens, already appended at slots past[s] .. past[s] +
+ * tokens - 1, over their sequence's cache:
+ *   o = sum_j p_j v_j,  p = softmax over the visible slots j of scale q . k_j.
+ * Query head h reads key head h / (query_heads / kv_heads). Visible to token t:
+ * the slots before past[s], and of the step's own tokens t itself and those
+ * above it: with parents NULL every one before it (a chain), else its parent,
+ * its parent's parent and so on (a tree of at most
+ * CHARLOTTE_HIP_MATMUL_TREE_TOKENS tokens a sequence). parents[s * tokens + t]
+ * is -1 (the cached tokens alone come before) or a token below t; any other
+ * value marks t unused: it, and all under it, see nothing and get zeros. With
+ * a window w > 0 a token sees only itself and the w - 1 places before it, a
+ * tree's token standing at the place of its depth. past[s] is taken as at most
+ * capacity - tokens. */
+#define CHARLOTTE_HIP_MATMUL_TREE_TOKENS 256u
+typedef struct {
+    const charlotte_hip_matmul_cache* cache;
+    const float* queries;     /* device, 16-byte aligned: row i's heads at queries + i * query_stride */
+    float* output;            /* device, 16-byte aligned, apart from queries: rows of query_heads * head_dim */
+    uint64_t query_stride;    /* floats, whole 4s; 0: query_heads * head_dim */
+    uint64_t output_stride;
+    uint32_t query_heads;     /* a multiple of the cache's kv_heads */
+    uint32_t window;          /* 0: none */
+    float scale;              /* finite */
+    /* The most past[s] + tokens the step may reach, for the choice of splits
+     * alone (0: the capacity): any value gives a right answer. */
+    uint32_t longest;
+    const uint32_t* past;     /* device: a word a sequence */
+    const int32_t* parents;   /* device, or NULL */
+    void* workspace;          /* device, 16-byte aligned: attention_workspace_bytes */
+    uint64_t workspace_bytes;
+} charlotte_hip_matmul_attention_desc;
+
+/* Bytes of workspace that serve every step of at most `tokens` tokens a
+ * sequence; 0 for sizes the launch refuses. The contents need no care; launches
+ * that share a workspace must be ordered on one stream. */
+uint64_t charlotte_hip_matmul_attention_workspace_bytes(const charlotte_hip_matmul_context* ctx,
+                                                        const charlotte_hip_matmul_cache* cache, uint32_t query_heads,
+                                                        uint32_t tokens);
+charlotte_hip_matmul_status charlotte_hip_matmul_attention(charlotte_hip_matmul_context* ctx,
+                                                           const charlotte_hip_matmul_attention_desc* desc,
+                                                           uint32_t tokens, void* stream);
+
+/* ---- after the head: probabilities, and drafted tokens verified ------------------- */
+
+/* Each row of `vocabulary` logits as softmax(logits / temperature); at
+ * temperature 0 a one for the largest logit (the first of equals) and zeros. A
+ * row of nothing but -inf becomes zeros; one with a NaN or +inf becomes NaNs,
+ * but at temperature 0, where a NaN counts as -inf. */
+typedef struct {
+    const float* logits;      /* device, 4-byte aligned: row i at logits + i * logit_stride */
+    float* output;            /* device, 4-byte aligned: the logits' memory with their stride, or memory apart */
+    uint64_t logit_stride;    /* floats; 0: vocabulary */
+    uint64_t output_stride;
+    uint32_t rows;
+    uint32_t vocabulary;
+    float temperature;        /* 0, or 1e-6 and above */
+    uint32_t reserved;        /* 0 */
+    void* workspace;          /* device, 16-byte aligned: probabilities_workspace_bytes */
+    uint64_t workspace_bytes;
+} charlotte_hip_matmul_probabilities_desc;
+
+uint64_t charlotte_hip_matmul_probabilities_workspace_bytes(uint32_t rows, uint32_t vocabulary);
+charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_matmul_context* ctx,
+                                                               const charlotte_hip_matmul_probabilities_desc* desc,
+                                                               void* stream);
+
+/* Drafted tokens against the target's probabilities, from given uniform numbers
+ * in [0, 1). A sequence's step holds `tokens` nodes: node 0 is the last token
+ * already taken, the others drafted ones. target's row i (of a sequence) is the
+ * target's distribution after node i.
+ *
+ * With `draft` (a chain; parents NULL) node i + 1's token x is accepted while
+ * accepts[i + 1] * draft_i(x) < target_i(x) (draft's row i is what the token of
+ * node i + 1 was drawn from). At the first refused, after node i, the next
+ * token is drawn from max(target_i - draft_i, 0); with none refused, from
+ * target's last row.
+ * Without `draft` the next token after every node is drawn from its target row,
+ * and from node 0 on the first child holding the drawn token is accepted.
+ * `parents` is attention's (NULL: a chain); only what hangs from node 0 is
+ * reached.
+ *
+ * A draw from row x with uniform number u (uniforms' of that node) is exact, in
+ * whole numbers: weights floor(min(max(x, 0), 1) 2^44) (a NaN: 0), W their sum,
+ * r = floor(u 2^31) within 0 .. 2^31 - 1, and the lowest index whose running sum
+ * passes floor(W r / 2^31); with W = 0, index 0.
+ *
+ * path gets the accepted nodes, node 0 first, emitted the tokens after each of
+ * them (the drafted ones accepted, then the one drawn): count of each, and -1
+ * in the rest of a sequence's `tokens` places. */
+typedef struct {
+    const int32_t* node_tokens; /* device: sequences rows of `tokens`; one outside the vocabulary is never accepted */
+    const float* target;        /* device, 4-byte aligned: sequences * tokens rows, target_stride apart */
+    const float* draft;         /* device, 4-byte aligned: sequences * (tokens - 1) rows, draft_stride apart; or NULL */
+    const float* uniforms;      /* device: sequences * tokens */
+    const float* accepts;       /* device: sequences * tokens (entry 0 of each unread); with draft */
+    const int32_t* parents;     /* device or NULL */
+    const uint32_t* lengths;    /* device or NULL: the nodes of each sequence, at most tokens; 0: count 0 */
+    int32_t* path;              /* device: sequences * tokens */
+    int32_t* emitted;           /* device: sequences * tokens */
+    uint32_t* count;            /* device: sequences */
+    uint64_t target_stride;     /* floats; 0: vocabulary */
+    uint64_t draft_stride;
+    uint32_t vocabulary;        /* at most 2^18 */
+    uint32_t reserved;          /* 0 */
+    void* workspace;            /* device, 16-byte aligned: verify_workspace_bytes */
+    uint64_t workspace_bytes;
+} charlotte_hip_matmul_verify_desc;
+
+uint64_t charlotte_hip_matmul_verify_workspace_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocabulary);
+charlotte_hip_matmul_status charlotte_hip_matmul_verify(charlotte_hip_matmul_context* ctx,
+                                                        const charlotte_hip_matmul_verify_desc* desc,
+                                                        uint32_t sequences, uint32_t tokens, void* stream);
 
 /* ---- GGUF files (gguf::read_index, src/core/gguf/reader.cpp) -------------------- */
 
