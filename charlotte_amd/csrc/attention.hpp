@@ -17,15 +17,18 @@
 // lo, about 22 bits; a cache's codes are exact in binary16. A block's key scale
 // multiplies its product in f32 (F16: none). Sums are f32 throughout.
 //
-// Range: p is at most 2^(10 - D), D the exponent of the largest value scale
-// met, so p d stays below 2^12 and its lo part's steps (2^-24) 34 bits below
-// the largest: D stands in the exponent's offset as the maximum does, and
-// grows as it does.
+// Range: values' scales, and so the outputs, are held over 2^D, D the exponent
+// of the largest scale met; the outputs follow where it grows, as they follow
+// the maximum. p is below 2^14 (the offset follows the maximum once a score
+// passes it by 2^8, which a tile seldom does) and p d below 2^15, so that the
+// parts' steps (2^-24) lie at least 30 bits below the largest.
 //
-// Split: a workgroup takes up to 16 or 32 rows of a key head and a run of its
-// tiles, each wave every fourth tile, and joins its four waves' outputs in
-// LDS; where a step has too few rows to fill the card its tiles are split
-// among several workgroups, joined by attention_combine.
+// Split: up to 32 rows of a key head (attend) - the rows one wave holds - its
+// four waves take every fourth tile each, operands straight from the record,
+// and are joined in LDS. More rows (attend_rows): each wave has rows of its
+// own, and a tile's codes become binary16 operands in LDS once for all of them.
+// Where a step has too few rows to fill the card its tiles are split among
+// several workgroups, joined by attention_combine.
 #pragma once
 
 #include "cache.hpp"
@@ -36,23 +39,18 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2E = 1.44269504088896340736f;
 constexpr uint32_t kAttentionWaves = 4;
+constexpr int kHeadroom = 6;      // a probability's exponent at the maximum last followed
+constexpr float kSlack = 8.0f;    // and how far past it a score may go (a half ends at 2^16)
 
 // A lane's codes of one unit (keys or values of a block by 32 tokens).
 template <uint32_t F>
-struct Codes;
-template <>
-struct Codes<kQ8_0> {
-    uint32_t w[4];
-};
-template <>
-struct Codes<kQ4_0> {
-    uint32_t w[2];
-};
-template <>
-struct Codes<kF16> {
-    uint32_t w[8];
+struct Codes {
+    uint32_t w[F == kQ8_0 ? 4 : F == kQ4_0 ? 2 : 8];
 };
 
 template <uint32_t F>
@@ -90,34 +88,35 @@ __device__ __forceinline__ half8_t join(half2_t a, half2_t b, half2_t c, half2_t
 // values u (cache.hpp).
 template <uint32_t F, bool VALUES>
 __device__ __forceinline__ half8_t operand(const Codes<F>& c, int part) {
-    half2_t a, b, d, e;
-    if constexpr (F == kQ8_0) {
-        halves_of<128>(c.w[2 * part], &a, &b);
-        halves_of<128>(c.w[2 * part + 1], &d, &e);
-    } else if constexpr (F == kQ4_0) {
-        if constexpr (VALUES) {
+    if constexpr (F == kF16) {
+        const uint4_t w = {c.w[4 * part], c.w[4 * part + 1], c.w[4 * part + 2], c.w[4 * part + 3]};
+        return __builtin_bit_cast(half8_t, w);
+    } else {
+        half2_t a, b, d, e;
+        if constexpr (F == kQ8_0) {
+            halves_of<128>(c.w[2 * part], &a, &b);
+            halves_of<128>(c.w[2 * part + 1], &d, &e);
+        } else if constexpr (VALUES) {
             halves_of<8>(c.w[0] >> (4 * part) & 0x0F0F0F0Fu, &a, &b);
             halves_of<8>(c.w[1] >> (4 * part) & 0x0F0F0F0Fu, &d, &e);
         } else {
             halves_of<8>(c.w[part] & 0x0F0F0F0Fu, &a, &b);
             halves_of<8>(c.w[part] >> 4 & 0x0F0F0F0Fu, &d, &e);
         }
-    } else {
-        uint4 w = {c.w[4 * part], c.w[4 * part + 1], c.w[4 * part + 2], c.w[4 * part + 3]};
-        return __builtin_bit_cast(half8_t, w);
+        return join(a, b, d, e);
     }
-    return join(a, b, d, e);
 }
 
 __device__ __forceinline__ float4_t multiply(half8_t a, half8_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// A dword's two halves, the dword passed by value: a bit cast straight from a
+// vector's element reads its first.
+__device__ __forceinline__ half2_t pair_of(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
+
 // Slot i's scale of a lane's eight, i a constant.
-__device__ __forceinline__ float scale_at(const uint4& s, int i) {
-    const uint32_t w = i < 2 ? s.x : i < 4 ? s.y : i < 6 ? s.z : s.w;
-    return static_cast<float>(__builtin_bit_cast(half2_t, w)[i & 1]);
-}
+__device__ __forceinline__ float scale_at(const uint4_t& s, int i) { return static_cast<float>(pair_of(s[i >> 1])[i & 1]); }
 
 // Two f32 as two binary16 parts of each: hi rounded towards zero, lo what it
 // leaves, rounded likewise (2^-21 of the value at the most).
@@ -125,6 +124,32 @@ __device__ __forceinline__ void split2(float a, float b, half2_t* hi, half2_t* l
     *hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     *lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi->x), -1.0f, a),
                                                                  __builtin_fmaf(static_cast<float>(hi->y), -1.0f, b)));
+}
+
+// Over the four lanes that share a row (lane % 16).
+__device__ __forceinline__ float most_of_row(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_of_row(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// What lies past the last token is no one's, and may be anything: `kept`
+// masks dword w of a lane's eight slots (two a dword) to those before `latest`.
+__device__ __forceinline__ uint32_t kept_of(uint32_t slot0, uint32_t g, uint32_t w, uint32_t latest) {
+    const uint32_t slot = slot0 + w / 2 * 16 + 4 * g + (w & 1) * 2;
+    return slot >= latest ? 0u : slot + 1 >= latest ? 0xFFFFu : 0xFFFFFFFFu;
+}
+// A scale there reads as never met: zero, or F16's one.
+template <uint32_t F>
+__device__ __forceinline__ uint32_t kept_scale(uint32_t scale, uint32_t kept) {
+    return (scale & kept) | ((F == kF16 ? 0x3C003C00u : 0u) & ~kept);
 }
 
 // The step's tree as a workgroup's rows see it: for each of its tokens, the
@@ -142,8 +167,8 @@ struct Tree {
 template <uint32_t TOKENS>
 __device__ void read_tree(Tree<TOKENS>& tree, const int32_t* parents, uint32_t tokens, uint32_t first, uint32_t count,
                           uint32_t reach) {
-    for (uint32_t i = threadIdx.x; i < tokens; i += 256) tree.parents[i] = parents[i];
-    for (uint32_t i = threadIdx.x; i < TOKENS * (kTreeTokens / 32); i += 256)
+    for (uint32_t i = threadIdx.x; i < tokens; i += blockDim.x) tree.parents[i] = parents[i];
+    for (uint32_t i = threadIdx.x; i < TOKENS * (kTreeTokens / 32); i += blockDim.x)
         (&tree.above[0][0])[i] = 0;
     __syncthreads();
     if (threadIdx.x < count) {
@@ -173,121 +198,120 @@ struct Sight {
     bool live;        // a row of the step, and used
 };
 
+// What a workgroup's rows, row0 .. row_end - 1 of a key head, have in common.
+struct Group {
+    uint32_t sequence, head, past, latest;
+    uint32_t row0, row_end, token0, token_end;
+    uint32_t tile_begin, tile_end;  // its split's tiles
+    uint32_t all_begin;             // every row sees the slots from here to past
+    uint64_t sequence_head;
+    uint32_t split;
+
+    // `rows` rows a workgroup, blockIdx.x = (head, row group, split).
+    __device__ __forceinline__ Group(const Attention& a, uint32_t rows) {
+        split = blockIdx.x % a.splits;
+        const uint32_t at = blockIdx.x / a.splits, row_groups = (a.rows + rows - 1) / rows;
+        row0 = at % row_groups * rows;
+        sequence_head = at / row_groups;
+        sequence = static_cast<uint32_t>(sequence_head) / a.cache.kv_heads;
+        head = static_cast<uint32_t>(sequence_head) % a.cache.kv_heads;
+        past = min(a.past[sequence], a.cache.capacity - a.tokens);
+        latest = past + a.tokens;
+        row_end = min(row0 + rows, a.rows);
+        token0 = row0 / a.group, token_end = (row_end - 1) / a.group + 1;
+        // From the window's first to the last token that its rows may see.
+        const uint32_t end = a.parents ? latest : past + token_end;
+        const uint32_t earliest = past + (a.parents ? 0u : token0) + 1;
+        const uint32_t begin = a.window && earliest > a.window ? earliest - a.window : 0u;
+        all_begin = a.window && latest > a.window ? latest - a.window : 0u;
+        const uint32_t first = begin / kTile, last = (end + kTile - 1) / kTile;
+        const uint32_t share = (last - first + a.splits - 1) / a.splits;
+        tile_begin = min(first + split * share, last);
+        tile_end = min(tile_begin + share, last);
+    }
+
+    __device__ __forceinline__ bool masked(uint32_t slot0) const { return slot0 + kTile > past || slot0 < all_begin; }
+};
+
+// A wave's RT x 16 rows as they go over the tiles: lane 16g + n holds, of rows
+// n, 16 + n, ..., the queries' operands and the outputs' values 4g .. 4g + 3 of
+// each 16.
 template <uint32_t F, uint32_t NB, uint32_t RT>
-__global__ __launch_bounds__(256) void attend(Attention a) {
-    constexpr uint32_t kRows = 16 * RT, kRecord = cache_record(F, NB), kUnit = cache_unit(F);
-    __shared__ Tree<kRows> tree;
-    __shared__ float4_t joined[2][RT * 2 * NB][64];
-    __shared__ float joined_offset[kAttentionWaves][kRows], joined_sum[kAttentionWaves][kRows];
-
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = lane & 15u, g = lane >> 4;
-    const uint32_t split = blockIdx.x % a.splits, at = blockIdx.x / a.splits;
-    const uint32_t row_groups = (a.rows + kRows - 1) / kRows;
-    const uint32_t row0 = at % row_groups * kRows, sequence_head = at / row_groups;
-    const uint32_t sequence = sequence_head / a.cache.kv_heads, head = sequence_head % a.cache.kv_heads;
-    const uint32_t past = min(a.past[sequence], a.cache.capacity - a.tokens);
-
-    // The workgroup's tokens, and its rows' sight.
-    const uint32_t row_end = min(row0 + kRows, a.rows);
-    const uint32_t token0 = row0 / a.group, token_end = (row_end - 1) / a.group + 1;
-    if (a.parents)
-        read_tree(tree, a.parents + static_cast<uint64_t>(sequence) * a.tokens, a.tokens, token0, token_end - token0,
-                  a.window);
-    Sight sight[RT];
-#pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        const uint32_t row = row0 + 16 * i + n;
-        const uint32_t token = min(row, row_end - 1) / a.group;
-        const uint32_t depth = a.parents ? tree.depth[token - token0] : token;
-        sight[i].live = row < row_end && depth != kUnused;
-        const uint32_t place = past + (sight[i].live ? depth : 0u) + 1;  // one past its own place
-        sight[i].first = a.window && place > a.window ? place - a.window : 0u;
-        sight[i].last = a.parents ? token - token0 : past + token;
-    }
-
-    // Its tiles: from the window's first to the last token its rows may see.
-    const uint32_t end = a.parents ? past + a.tokens : past + token_end;
-    const uint32_t earliest = past + (a.parents ? 0u : token0) + 1;
-    const uint32_t begin = a.window && earliest > a.window ? earliest - a.window : 0u;
-    const uint32_t tile_begin = begin / kTile, tile_end = (end + kTile - 1) / kTile;
-    const uint32_t share = (tile_end - tile_begin + a.splits - 1) / a.splits;
-    const uint32_t my_begin = min(tile_begin + split * share, tile_end), my_end = min(my_begin + share, tile_end);
-    // Slots that every row of the workgroup sees: from `all_begin` to `past`.
-    const uint32_t latest = past + a.tokens;
-    const uint32_t all_begin = a.window && latest > a.window ? latest - a.window : 0u;
-
-    // The rows' queries as operands, 2^(-shift) their power of two.
+struct Rows {
     half8_t high[RT][NB], low[RT][NB];
-    float unit[RT];
-#pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        const uint32_t row = min(row0 + 16 * i + n, row_end - 1);
-        const float* q = a.queries + (static_cast<uint64_t>(sequence) * a.tokens + row / a.group) * a.query_stride +
-                         static_cast<uint64_t>(head * a.group + row % a.group) * (32 * NB) + 8 * g;
-        float x[NB][8], largest = 0.0f;
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            const float4 u = *reinterpret_cast<const float4*>(q + 32 * b), v = *reinterpret_cast<const float4*>(q + 32 * b + 4);
-            x[b][0] = u.x, x[b][1] = u.y, x[b][2] = u.z, x[b][3] = u.w;
-            x[b][4] = v.x, x[b][5] = v.y, x[b][6] = v.z, x[b][7] = v.w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][e] *= a.scale * kLog2E, largest = fmaxf(largest, fabsf(x[b][e]));
-        }
-        largest = fmaxf(largest, __shfl_xor(largest, 16));
-        largest = fmaxf(largest, __shfl_xor(largest, 32));
-        int shift = 0;
-        if (largest > 0.0f && largest <= 3.4e38f) {
-            int e;
-            (void)frexpf(largest, &e);
-            shift = min(11 - e, 126);
-        }
-        unit[i] = ldexpf(1.0f, -shift);
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            half2_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(ldexpf(x[b][2 * e], shift), ldexpf(x[b][2 * e + 1], shift), &hi[e], &lo[e]);
-            high[i][b] = join(hi[0], hi[1], hi[2], hi[3]);
-            low[i][b] = join(lo[0], lo[1], lo[2], lo[3]);
-        }
-    }
-
+    float unit[RT];                          // what a raw score stands for, a power of two
     float4_t out[RT][2 * NB];
     float largest[RT], offset[RT], sum[RT];  // the raw maximum; exp2's offset; the lane's part of the sum
-    int exponent = -64;                      // D, the same in every lane
+    int exponent;                            // D, the same in every lane
+    Sight sight[RT];
+
+    // Rows from `row0` on; rows past the group's end repeat its last.
+    template <typename TREE>
+    __device__ __forceinline__ void begin(const Attention& a, const Group& group, const TREE& tree, uint32_t row0) {
+        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+        exponent = -64;
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        largest[i] = -INFINITY, offset[i] = INFINITY, sum[i] = 0.0f;
+        for (uint32_t i = 0; i < RT; ++i) {
+            const uint32_t row = row0 + 16 * i + n, inside = min(row, group.row_end - 1);
+            const uint32_t token = inside / a.group;
+            const uint32_t depth = a.parents ? tree.depth[token - group.token0] : token;
+            sight[i].live = row < group.row_end && depth != kUnused;
+            const uint32_t place = group.past + (depth != kUnused ? depth : 0u) + 1;  // one past its own place
+            sight[i].first = a.window && place > a.window ? place - a.window : 0u;
+            sight[i].last = a.parents ? token - group.token0 : group.past + token;
+
+            const float* q = a.queries +
+                             (static_cast<uint64_t>(group.sequence) * a.tokens + token) * a.query_stride +
+                             static_cast<uint64_t>(group.head * a.group + inside % a.group) * (32 * NB) + 8 * g;
+            float x[NB][8], most = 0.0f;
 #pragma unroll
-        for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t b = 0; b < NB; ++b) {
+                const float4 u = *reinterpret_cast<const float4*>(q + 32 * b);
+                const float4 v = *reinterpret_cast<const float4*>(q + 32 * b + 4);
+                x[b][0] = u.x, x[b][1] = u.y, x[b][2] = u.z, x[b][3] = u.w;
+                x[b][4] = v.x, x[b][5] = v.y, x[b][6] = v.z, x[b][7] = v.w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[b][e] *= a.scale * kLog2E, most = fmaxf(most, fabsf(x[b][e]));
+            }
+            most = most_of_row(most);
+            int shift = 0;
+            if (most > 0.0f && most <= 3.4e38f) {
+                int e;
+                (void)frexpf(most, &e);
+                shift = min(11 - e, 126);
+            }
+            unit[i] = ldexpf(1.0f, -shift);
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                half2_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    split2(ldexpf(x[b][2 * e], shift), ldexpf(x[b][2 * e + 1], shift), &hi[e], &lo[e]);
+                high[i][b] = join(hi[0], hi[1], hi[2], hi[3]);
+                low[i][b] = join(lo[0], lo[1], lo[2], lo[3]);
+            }
+            largest[i] = -INFINITY, offset[i] = INFINITY, sum[i] = 0.0f;
+#pragma unroll
+            for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
     }
 
-    const uint8_t* base = record_of(a.cache, F, sequence, head, 0);
-    for (uint32_t tile = my_begin + wave; tile < my_end; tile += kAttentionWaves) {
-        const uint8_t* record = base + static_cast<uint64_t>(tile) * kRecord;
-        Codes<F> keys[NB], values[NB];
-        uint4 key_scale[NB], value_scale[NB];
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            keys[b] = load_codes<F>(record + b * kUnit, lane);
-            if constexpr (key_scales(F))
-                key_scale[b] = *reinterpret_cast<const uint4*>(record + key_scales_at(F, NB) + 64 * b + 16 * g);
-        }
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            values[b] = load_codes<F>(record + values_at(F, NB) + b * kUnit, lane);
-            value_scale[b] = *reinterpret_cast<const uint4*>(record + value_scales_at(F, NB) + 64 * b + 16 * g);
-        }
-
+    // One tile. `source` gives the operands: key(b, h), key_scale(b), value(b, u), value_scale(b).
+    template <typename SOURCE, typename TREE>
+    __device__ __forceinline__ void tile(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
+                                         const SOURCE& source) {
+        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
         // Scores: s[i][h][r] of token 16h + 4g + r.
         float4_t s[RT][2];
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) s[i][0] = s[i][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
+            uint4_t scale;
+            if constexpr (key_scales(F)) scale = source.key_scale(b);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const half8_t k = operand<F, false>(keys[b], h);
+                const half8_t k = source.key(b, h);
 #pragma unroll
                 for (uint32_t i = 0; i < RT; ++i) {
                     if constexpr (key_scales(F)) {
@@ -295,7 +319,7 @@ __global__ __launch_bounds__(256) void attend(Attention a) {
                         p = multiply(k, low[i][b], p);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            s[i][h][r] = __builtin_fmaf(p[r], scale_at(key_scale[b], 4 * h + r), s[i][h][r]);
+                            s[i][h][r] = __builtin_fmaf(p[r], scale_at(scale, 4 * h + r), s[i][h][r]);
                     } else {
                         s[i][h] = multiply(k, high[i][b], s[i][h]);
                         s[i][h] = multiply(k, low[i][b], s[i][h]);
@@ -304,94 +328,100 @@ __global__ __launch_bounds__(256) void attend(Attention a) {
             }
         }
 
-        const uint32_t slot0 = tile * kTile;
-        const bool masked = slot0 + kTile > past || slot0 < all_begin;
-        bool seen[RT][8];
+        const bool masked = group.masked(slot0);
+        uint32_t seen[RT][4];  // a half's mask a slot
+#pragma unroll
+        for (uint32_t i = 0; i < RT; ++i) seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0xFFFFFFFFu;
         if (masked) {
 #pragma unroll
             for (uint32_t i = 0; i < RT; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t slot = slot0 + 16 * h + 4 * g + r;
-                        bool sees = slot >= sight[i].first;
-                        if (!a.parents) {
-                            sees = sees && slot <= sight[i].last;
-                        } else if (slot >= past) {
-                            const uint32_t node = slot - past;
-                            sees = node < a.tokens && (tree.above[sight[i].last][node >> 5] >> (node & 31u) & 1u);
-                        }
-                        seen[i][4 * h + r] = sees;
-                        if (!sees) s[i][h][r] = -INFINITY;
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t slot = slot0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                    bool sees = slot >= sight[i].first;
+                    if (!a.parents) {
+                        sees = sees && slot <= sight[i].last;
+                    } else if (slot >= group.past) {
+                        const uint32_t node = slot - group.past;
+                        sees = node < a.tokens && (tree.above[sight[i].last][node >> 5] >> (node & 31u) & 1u);
                     }
-            // What lies past the last token is no one's, and may be anything:
-            // scales as if never met, F16's values zero.
-            if (slot0 + kTile > latest) {
-#pragma unroll
-                for (uint32_t b = 0; b < NB; ++b) {
-                    constexpr uint32_t kPlain = F == kF16 ? 0x3C003C00u : 0u;
-                    uint32_t* const scale[4] = {&value_scale[b].x, &value_scale[b].y, &value_scale[b].z, &value_scale[b].w};
-#pragma unroll
-                    for (uint32_t w = 0; w < 4; ++w) {
-                        const uint32_t slot = slot0 + w / 2 * 16 + 4 * g + (w & 1) * 2;
-                        const uint32_t kept = slot >= latest ? 0u : slot + 1 >= latest ? 0xFFFFu : 0xFFFFFFFFu;
-                        *scale[w] = (*scale[w] & kept) | (kPlain & ~kept);
-                        if constexpr (F == kF16) values[b].w[w] &= kept, values[b].w[4 + w] &= kept;
+                    if (!sees) {
+                        s[i][e >> 2][e & 3] = -INFINITY;
+                        seen[i][e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
                     }
                 }
-            }
         }
 
-        // The largest value scale's exponent.
-        bool scaled = true;  // whether value scales are other than one
+        // The value scales: the largest's exponent, and all of them over 2^D.
+        uint4_t scale[NB];
+        bool scaled = true;  // whether any is other than one
         int grown = exponent;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) scale[b] = source.value_scale(b);
         if constexpr (F == kF16) {
             uint32_t other = 0;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
-                other |= (value_scale[b].x ^ 0x3C003C00u) | (value_scale[b].y ^ 0x3C003C00u) |
-                         (value_scale[b].z ^ 0x3C003C00u) | (value_scale[b].w ^ 0x3C003C00u);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) other |= scale[b][w] ^ 0x3C003C00u;
             scaled = __any(other != 0);
             grown = 0;
         } else {
-            uint32_t most = 0;
+            ushort2_t top = {0, 0};
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const uint32_t w[4] = {value_scale[b].x, value_scale[b].y, value_scale[b].z, value_scale[b].w};
+            for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t lo = w[e] & 0x7FFFu, hi = w[e] >> 16 & 0x7FFFu;
-                    // a NaN scale spoils its own rows alone
-                    most = max(most, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t size = F == kQ4_0 ? scale[b][w] & 0x7FFF7FFFu : scale[b][w];
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
                 }
+            uint32_t most = max(top.x, top.y);
+            if (__any(most > 0x7C00u)) {  // a NaN scale spoils the rows that see it, no other
+                most = 0;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t lo = scale[b][w] & 0x7FFFu, hi = scale[b][w] >> 16 & 0x7FFFu;
+                        most = max(most, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
+                    }
             }
-            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
-            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
-            // 2^grown <= the scale < 2^(grown + 1); subnormals count as the least normal
+            // the same in a group's 16 lanes; 2^grown <= the scale < 2^(grown + 1); subnormals count as the least normal
+            most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
+                       max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
             grown = max(exponent, static_cast<int>(max(most >> 10, 1u)) - 15);
+            const _Float16 down = static_cast<_Float16>(ldexpf(1.0f, -grown));
+            const half2_t by = {down, down};
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    scale[b][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][w]) * by);
         }
 
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) {
             float top = fmaxf(fmaxf(fmaxf(s[i][0][0], s[i][0][1]), fmaxf(s[i][0][2], s[i][0][3])),
                               fmaxf(fmaxf(s[i][1][0], s[i][1][1]), fmaxf(s[i][1][2], s[i][1][3])));
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float most = fmaxf(largest[i], top);
-            if (__any(most > largest[i]) || grown != exponent) {
+            top = most_of_row(top);
+            // the offset follows once a score passes it by kSlack (the first: -inf + inf is a NaN, no less than)
+            const bool follow = top > largest[i] && !((top - largest[i]) * unit[i] <= kSlack);
+            if (__any(follow) || grown != exponent) {
+                const float most = fmaxf(largest[i], top);
                 // the offset as used is what the factor is made of, so that its rounding cancels
-                const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit[i], static_cast<float>(10 - grown));
+                const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit[i], static_cast<float>(kHeadroom));
                 const float factor = largest[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - offset[i]);
+                const float down = factor * ldexpf(1.0f, exponent - grown);
                 largest[i] = most;
                 offset[i] = to;
                 sum[i] *= factor;
 #pragma unroll
-                for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= factor;
+                for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= down;
             }
         }
         exponent = grown;
 
+        half2_t hi[RT][4], lo[RT][4];
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) {
             // rows that have seen nothing: -inf + inf would be a NaN
@@ -402,47 +432,156 @@ __global__ __launch_bounds__(256) void attend(Attention a) {
                 p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], unit[i], to));
                 sum[i] += p[e];
             }
-            half8_t hi8, lo8;
-            auto split8 = [&](const float* x) {
-                half2_t hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split2(x[2 * e], x[2 * e + 1], &hi[e], &lo[e]);
-                hi8 = join(hi[0], hi[1], hi[2], hi[3]);
-                lo8 = join(lo[0], lo[1], lo[2], lo[3]);
-            };
-            if (F == kF16 && !scaled) split8(p);
+            for (int e = 0; e < 4; ++e) split2(p[2 * e], p[2 * e + 1], &hi[i][e], &lo[i][e]);
+        }
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                if (scaled) {
-                    float x[8];
+        for (uint32_t b = 0; b < NB; ++b) {
+            const half8_t v[2] = {source.value(b, 0), source.value(b, 1)};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = __builtin_fmaf(p[e], scale_at(value_scale[b], e), 0.0f);
+            for (uint32_t i = 0; i < RT; ++i) {
+                half8_t x, y;
+                if (F == kF16 && !scaled) {
+                    x = join(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
+                    y = join(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                } else {
+                    // (hi + lo) d in two parts: hi d rounded, what that leaves
+                    // (exact: 22 bits less their first 11) plus lo d
+                    half2_t u[4], w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
                         // a scale that the row does not see may be a NaN
-                        if (masked && !seen[i][e]) x[e] = 0.0f;
+                        const half2_t d = pair_of(scale[b][e] & seen[i][e]);
+                        u[e] = hi[i][e] * d;
+                        w[e] = __builtin_elementwise_fma(lo[i][e], d, __builtin_elementwise_fma(hi[i][e], d, -u[e]));
                     }
-                    split8(x);
+                    x = join(u[0], u[1], u[2], u[3]);
+                    y = join(w[0], w[1], w[2], w[3]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const half8_t v = operand<F, true>(values[b], u);
-                    out[i][2 * b + u] = multiply(v, hi8, out[i][2 * b + u]);
-                    out[i][2 * b + u] = multiply(v, lo8, out[i][2 * b + u]);
+                    out[i][2 * b + u] = multiply(v[u], x, out[i][2 * b + u]);
+                    out[i][2 * b + u] = multiply(v[u], y, out[i][2 * b + u]);
                 }
             }
         }
     }
 
+    // The last tile is done: the outputs, held over 2^D, as the sum is.
+    __device__ __forceinline__ void end() {
+        const float up = ldexpf(1.0f, exponent);
+#pragma unroll
+        for (uint32_t i = 0; i < RT; ++i)
+#pragma unroll
+            for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= up;
+    }
+
+    // A row's outputs, its sum whole (`total`) and its offset (`least`): to the
+    // step's output, or to the split's place.
+    __device__ __forceinline__ void finish(const Attention& a, const Group& group, uint32_t row0, const float (&total)[RT],
+                                           const float (&least)[RT]) const {
+        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+#pragma unroll
+        for (uint32_t i = 0; i < RT; ++i) {
+            const uint32_t row = row0 + 16 * i + n;
+            if (row >= group.row_end) continue;
+            // nothing seen: no maximum, and no NaN either
+            const bool empty = !sight[i].live || (least[i] == INFINITY && total[i] == 0.0f);
+            if (a.splits == 1) {
+                const float inverse = empty ? 0.0f : 1.0f / total[i];
+                float* to = a.output +
+                            (static_cast<uint64_t>(group.sequence) * a.tokens + row / a.group) * a.output_stride +
+                            static_cast<uint64_t>(group.head * a.group + row % a.group) * (32 * NB) + 4 * g;
+#pragma unroll
+                for (uint32_t t = 0; t < 2 * NB; ++t)
+                    *reinterpret_cast<float4_t*>(to + 16 * t) = empty ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : out[i][t] * inverse;
+            } else {
+                const uint64_t place = (group.sequence_head * a.rows + row) * a.splits + group.split;
+                float* to = a.partial + place * (32 * NB) + 4 * g;
+                if (!empty)
+#pragma unroll
+                    for (uint32_t t = 0; t < 2 * NB; ++t) *reinterpret_cast<float4_t*>(to + 16 * t) = out[i][t];
+                const bool spoilt = total[i] != total[i];
+                if (g == 0)
+                    a.stats[place] = make_float2(empty ? INFINITY : spoilt ? total[i] : least[i], empty ? 0.0f : total[i]);
+            }
+        }
+    }
+};
+
+// ---- few rows: the waves split the tiles ----------------------------------------
+
+// A tile's operands in registers, loaded as the record holds them.
+template <uint32_t F, uint32_t NB>
+struct Registers {
+    Codes<F> keys[NB], values[NB];
+    uint4_t key_scales_[NB], value_scales_[NB];
+
+    __device__ __forceinline__ void load(const uint8_t* record) {
+        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            keys[b] = load_codes<F>(record + b * cache_unit(F), lane);
+            if constexpr (key_scales(F))
+                key_scales_[b] = *reinterpret_cast<const uint4_t*>(record + key_scales_at(F, NB) + 64 * b + 16 * g);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            values[b] = load_codes<F>(record + values_at(F, NB) + b * cache_unit(F), lane);
+            value_scales_[b] = *reinterpret_cast<const uint4_t*>(record + value_scales_at(F, NB) + 64 * b + 16 * g);
+        }
+    }
+    __device__ __forceinline__ void cut(uint32_t slot0, uint32_t latest) {
+        const uint32_t g = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+            const uint32_t kept = kept_of(slot0, g, w, latest);
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                value_scales_[b][w] = kept_scale<F>(value_scales_[b][w], kept);
+                if constexpr (F == kF16) values[b].w[w] &= kept, values[b].w[4 + w] &= kept;
+            }
+        }
+    }
+    __device__ __forceinline__ half8_t key(uint32_t b, int h) const { return operand<F, false>(keys[b], h); }
+    __device__ __forceinline__ half8_t value(uint32_t b, int u) const { return operand<F, true>(values[b], u); }
+    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const { return key_scales_[b]; }
+    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const { return value_scales_[b]; }
+};
+
+template <uint32_t F, uint32_t NB, uint32_t RT>
+__global__ __launch_bounds__(256) void attend(Attention a) {
+    constexpr uint32_t kRows = 16 * RT, kRecord = cache_record(F, NB);
+    __shared__ Tree<kRows> tree;
+    __shared__ float4_t joined[2][RT * 2 * NB][64];
+    __shared__ float joined_offset[kAttentionWaves][kRows], joined_sum[kAttentionWaves][kRows];
+
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = lane & 15u, g = lane >> 4;
+    const Group group(a, kRows);
+    if (a.parents)
+        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                  group.token_end - group.token0, a.window);
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, group.row0);
+
+    const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
+    for (uint32_t tile = group.tile_begin + wave; tile < group.tile_end; tile += kAttentionWaves) {
+        Registers<F, NB> source;
+        source.load(base + static_cast<uint64_t>(tile) * kRecord);
+        if (tile * kTile + kTile > group.latest) source.cut(tile * kTile, group.latest);
+        rows.tile(a, group, tree, tile * kTile, source);
+    }
+    rows.end();
+
     // The four waves joined: each one's outputs on the least offset's (the
     // largest maximum's) scale, waves 2 and 3 into 0 and 1, then 1 into 0.
+    float total[RT], least[RT];
 #pragma unroll
     for (uint32_t i = 0; i < RT; ++i) {
-        sum[i] += __shfl_xor(sum[i], 16);
-        sum[i] += __shfl_xor(sum[i], 32);
-        if (g == 0) joined_offset[wave][16 * i + n] = offset[i], joined_sum[wave][16 * i + n] = sum[i];
+        const float mine = sum_of_row(rows.sum[i]);
+        if (g == 0) joined_offset[wave][16 * i + n] = rows.offset[i], joined_sum[wave][16 * i + n] = mine;
     }
     __syncthreads();
-    float total[RT], least[RT];
 #pragma unroll
     for (uint32_t i = 0; i < RT; ++i) {
         least[i] = INFINITY, total[i] = 0.0f;
@@ -456,21 +595,21 @@ __global__ __launch_bounds__(256) void attend(Attention a) {
             const float theirs = joined_offset[w][16 * i + n];
             total[i] += joined_sum[w][16 * i + n] * (theirs == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least[i] - theirs));
         }
-        const float factor = offset[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least[i] - offset[i]);
+        const float factor = rows.offset[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least[i] - rows.offset[i]);
 #pragma unroll
-        for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= factor;
+        for (uint32_t t = 0; t < 2 * NB; ++t) rows.out[i][t] *= factor;
     }
     auto give = [&](uint32_t place) {
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i)
 #pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) joined[place][i * 2 * NB + t][lane] = out[i][t];
+            for (uint32_t t = 0; t < 2 * NB; ++t) joined[place][i * 2 * NB + t][lane] = rows.out[i][t];
     };
     auto take = [&](uint32_t place) {
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i)
 #pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] += joined[place][i * 2 * NB + t][lane];
+            for (uint32_t t = 0; t < 2 * NB; ++t) rows.out[i][t] += joined[place][i * 2 * NB + t][lane];
     };
     if (wave >= 2) give(wave - 2);
     __syncthreads();
@@ -480,48 +619,138 @@ __global__ __launch_bounds__(256) void attend(Attention a) {
     __syncthreads();
     if (wave != 0) return;
     take(0);
+    rows.finish(a, group, group.row0, total, least);
+}
 
+// ---- many rows: the waves split the rows -------------------------------------------
+
+// A stage: kStage tiles' codes as binary16 operands, and their scales, in LDS,
+// laid out by the workgroup for all of its waves.
+template <uint32_t NB>
+constexpr uint32_t stage_tiles() {
+    return NB <= 4 ? 2 : 1;
+}
+
+template <uint32_t NB>
+struct Stage {
+    half8_t keys[2 * NB][64], values[2 * NB][64];  // [2 b + h], [2 b + u]
+    uint4_t key_scales_[NB][4], value_scales_[NB][4];
+
+    __device__ __forceinline__ half8_t key(uint32_t b, int h) const { return keys[2 * b + h][threadIdx.x & 63u]; }
+    __device__ __forceinline__ half8_t value(uint32_t b, int u) const { return values[2 * b + u][threadIdx.x & 63u]; }
+    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const { return key_scales_[b][(threadIdx.x & 63u) >> 4]; }
+    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const { return value_scales_[b][(threadIdx.x & 63u) >> 4]; }
+};
+
+template <uint32_t F, uint32_t NB, uint32_t RT, uint32_t W>
+__global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
+    constexpr uint32_t kRows = 16 * RT * W, kRecord = cache_record(F, NB), kTiles = stage_tiles<NB>();
+    constexpr uint32_t kUnits = 2 * NB * kTiles, kMine = (kUnits + W - 1) / W;  // units of a stage; a wave's, at most
+    constexpr uint32_t kScaleWords = (key_scales(F) ? 32 : 16) * NB;            // a tile's
+    static_assert(kScaleWords * kTiles <= 64 * W, "a thread a dword");
+    __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
+    __shared__ Stage<NB> stages[2][kTiles];
+
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const Group group(a, kRows);
+    if (a.parents)
+        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                  group.token_end - group.token0, a.window);
+    const uint32_t row0 = group.row0 + 16 * RT * wave;
+    const bool mine = row0 < group.row_end;  // a wave without rows still lays out its share
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, min(row0, group.row_end - 1));
+    // a chain's wave sees nothing past its last row's token
+    const uint32_t sees_to =
+        a.parents ? group.latest : group.past + (min(row0 + 16 * RT, group.row_end) - 1) / a.group + 1;
+
+    const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
+    Codes<F> codes[kMine];
+    uint32_t scale_word = 0;
+    // Unit u of a stage: tile u / 2NB, block u % NB, keys then values.
+    auto load = [&](uint32_t tile0) {
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        const uint32_t row = row0 + 16 * i + n;
-        if (row >= row_end) continue;
-        // nothing seen: no maximum, and no NaN either
-        const bool empty = !sight[i].live || (least[i] == INFINITY && total[i] == 0.0f);
-        if (a.splits == 1) {
-            const float inverse = empty ? 0.0f : 1.0f / total[i];
-            float* to = a.output + (static_cast<uint64_t>(sequence) * a.tokens + row / a.group) * a.output_stride +
-                        static_cast<uint64_t>(head * a.group + row % a.group) * (32 * NB) + 4 * g;
+        for (uint32_t j = 0; j < kMine; ++j) {
+            const uint32_t u = wave + W * j, t = tile0 + u / (2 * NB);
+            if (u < kUnits && t < group.tile_end)
+                codes[j] = load_codes<F>(base + static_cast<uint64_t>(t) * kRecord + u % (2 * NB) * cache_unit(F), lane);
+        }
+        const uint32_t t = tile0 + threadIdx.x / kScaleWords;
+        if (threadIdx.x < kScaleWords * kTiles && t < group.tile_end)
+            scale_word = reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord +
+                                                           key_scales_at(F, NB))[threadIdx.x % kScaleWords];
+    };
+    auto lay = [&](uint32_t tile0, Stage<NB>* stage) {
 #pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t)
-                *reinterpret_cast<float4*>(to + 16 * t) =
-                    empty ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                          : make_float4(out[i][t][0] * inverse, out[i][t][1] * inverse, out[i][t][2] * inverse,
-                                        out[i][t][3] * inverse);
-        } else {
-            const uint64_t place = (static_cast<uint64_t>(sequence_head) * a.rows + row) * a.splits + split;
-            float* to = a.partial + place * (32 * NB) + 4 * g;
-            if (!empty)
+        for (uint32_t j = 0; j < kMine; ++j) {
+            const uint32_t u = wave + W * j, t = u / (2 * NB), b = u % NB;
+            if (u >= kUnits || tile0 + t >= group.tile_end) continue;
+            if (u % (2 * NB) < NB) {
+                stage[t].keys[2 * b][lane] = operand<F, false>(codes[j], 0);
+                stage[t].keys[2 * b + 1][lane] = operand<F, false>(codes[j], 1);
+            } else {
+                if constexpr (F == kF16)
+                    if ((tile0 + t) * kTile + kTile > group.latest)
 #pragma unroll
-                for (uint32_t t = 0; t < 2 * NB; ++t)
-                    *reinterpret_cast<float4*>(to + 16 * t) = make_float4(out[i][t][0], out[i][t][1], out[i][t][2], out[i][t][3]);
-            if (g == 0) {
-                const bool spoilt = total[i] != total[i];
-                a.stats[place] = make_float2(empty ? INFINITY : spoilt ? total[i] : least[i], empty ? 0.0f : total[i]);
+                        for (uint32_t w = 0; w < 4; ++w) {
+                            const uint32_t kept = kept_of((tile0 + t) * kTile, lane >> 4, w, group.latest);
+                            codes[j].w[w] &= kept, codes[j].w[4 + w] &= kept;
+                        }
+                stage[t].values[2 * b][lane] = operand<F, true>(codes[j], 0);
+                stage[t].values[2 * b + 1][lane] = operand<F, true>(codes[j], 1);
             }
         }
+        const uint32_t t = threadIdx.x / kScaleWords, w = threadIdx.x % kScaleWords;
+        if (threadIdx.x < kScaleWords * kTiles && tile0 + t < group.tile_end) {
+            const bool values = !key_scales(F) || w >= 16 * NB;
+            if (values)
+                scale_word = kept_scale<F>(scale_word, kept_of((tile0 + t) * kTile, w / 4 & 3u, w & 3u, group.latest));
+            uint32_t* to = reinterpret_cast<uint32_t*>(values ? stage[t].value_scales_ : stage[t].key_scales_);
+            to[w % (16 * NB)] = scale_word;
+        }
+    };
+
+    if (group.tile_begin < group.tile_end) {
+        load(group.tile_begin);
+        lay(group.tile_begin, stages[0]);
     }
+    __syncthreads();
+    uint32_t turn = 0;
+    for (uint32_t tile0 = group.tile_begin; tile0 < group.tile_end; tile0 += kTiles, turn ^= 1) {
+        // the next stage's loads are in flight over this one's products
+        const bool more = tile0 + kTiles < group.tile_end;
+        if (more) load(tile0 + kTiles);
+#pragma unroll
+        for (uint32_t t = 0; t < kTiles; ++t) {
+            const uint32_t slot0 = (tile0 + t) * kTile;
+            if (mine && tile0 + t < group.tile_end && slot0 < sees_to) rows.tile(a, group, tree, slot0, stages[turn][t]);
+        }
+        // the other stage was read before the last barrier
+        if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
+        __syncthreads();
+    }
+    if (!mine) return;
+    rows.end();
+    float total[RT];
+#pragma unroll
+    for (uint32_t i = 0; i < RT; ++i) total[i] = sum_of_row(rows.sum[i]);
+    rows.finish(a, group, row0, total, rows.offset);
 }
 
 template <uint32_t F, uint32_t NB>
 static hipError_t launch_blocks(const Attention& a, const AttentionPlan& plan, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads * plan.row_groups * plan.splits);
-    if constexpr (NB <= 4) {
-        if (plan.row_tiles == 2) {
-            hipLaunchKernelGGL((attend<F, NB, 2>), grid, dim3(256), 0, stream, a);
-            return hipGetLastError();
-        }
-    }
-    hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(256), 0, stream, a);
+    constexpr uint32_t kWide = NB <= 4 ? 2 : 1;  // 16-row tiles a wave's registers hold
+    if (plan.waves == 8)
+        hipLaunchKernelGGL((attend_rows<F, NB, kWide, 8>), grid, dim3(512), 0, stream, a);
+    else if (plan.waves == 4 && plan.row_tiles == kWide)
+        hipLaunchKernelGGL((attend_rows<F, NB, kWide, 4>), grid, dim3(256), 0, stream, a);
+    else if (plan.waves == 4)
+        hipLaunchKernelGGL((attend_rows<F, NB, 1, 4>), grid, dim3(256), 0, stream, a);
+    else if (plan.row_tiles == kWide)
+        hipLaunchKernelGGL((attend<F, NB, kWide>), grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

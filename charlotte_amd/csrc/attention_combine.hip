@@ -77,18 +77,22 @@ hipError_t launch_attention_combine(const Attention& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Two workgroups a compute unit, but at least four tiles (one a wave) each.
+// The least rows a workgroup that hold the step's, at most 32 RT; then splits
+// until each compute unit has eight waves, a split of at least four tiles.
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units) {
     const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
+    const uint32_t wide = cache.head_dim <= 128 ? 2 : 1;  // 16-row tiles a wave's registers hold
     AttentionPlan plan{};
-    plan.row_tiles = rows > 16 && cache.head_dim <= 128 ? 2 : 1;
-    plan.row_groups = static_cast<uint32_t>((rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles));
+    plan.waves = rows <= 16 * wide ? 1 : rows <= 64 * wide ? 4 : 8;
+    plan.row_tiles = rows <= 16 || (plan.waves == 4 && rows <= 64) ? 1 : wide;
+    const uint64_t group = 16ull * plan.row_tiles * plan.waves;
+    plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
     const uint64_t workgroups = uint64_t{cache.sequences} * cache.kv_heads * plan.row_groups;
     uint64_t reach = std::min(longest ? longest : cache.capacity, cache.capacity);
     if (window) reach = std::min<uint64_t>(reach, uint64_t{window} + tokens + 31);
     const uint64_t tiles = (reach + 31) / 32;
-    const uint64_t wanted = 2ull * compute_units / workgroups;
+    const uint64_t wanted = (plan.waves == 8 ? 1ull : 2ull) * compute_units / workgroups;
     plan.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, (tiles + 3) / 4)));
     return plan;
 }
@@ -98,26 +102,18 @@ uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, 
     return uint64_t{cache.sequences} * query_heads * tokens * splits * (uint64_t{cache.head_dim} * 4 + 8);
 }
 
-// A step splits while its workgroups are at most the compute units (a split
-// more than one workgroup's share), so rows x splits is bounded by two
-// workgroups' rows a compute unit; and by what the step's own rows could take
-// were they split as far as its tiles allow.
+// Steps of every number of tokens up to `tokens`: of those in one number of
+// row groups the last needs most, and past the first that does not split none does.
 uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units) {
     uint64_t most = 0;
     const uint64_t group = query_heads / cache.kv_heads;
-    // rows x splits grows with the rows within a number of row groups, and
-    // falls from one to the next: the last step of each is its most
-    const auto need = [&](uint32_t t) {
-        const AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
-        return plan.splits;
-    };
     for (uint32_t t = 1; t <= tokens; ++t) {
-        // the last step whose row groups are t's
-        const uint64_t rows = t * group, tile = rows > 16 && cache.head_dim <= 128 ? 32 : 16;
-        const uint64_t full = (rows + tile - 1) / tile * tile / group;
-        t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, full)));
-        if (need(t) < 2) break;
+        AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
+        const uint64_t rows = 16ull * plan.row_tiles * plan.waves * plan.row_groups;
+        t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, rows / group)));
+        plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
+        most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
+        if (plan.waves == 8 && plan.splits < 2) break;
     }
     return most;
 }

@@ -248,6 +248,14 @@ def test_attention_at_every_head_width(ctx, dev, format_, dim):
     _check_attention(dev, format_, 1, 6, 2, dim, 13, [45], seed=dim + 1)  # 39 rows
 
 
+@pytest.mark.parametrize("format_", ["q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("tokens", [19, 41, 91])
+def test_attention_of_many_rows_at_every_head_width(ctx, dev, format_, dim, tokens):
+    """57, 123 and 273 rows of a key head: workgroups of four waves and of eight, the last with few rows."""
+    _check_attention(dev, format_, 1, 3, 1, dim, tokens, [150], seed=dim + tokens)
+
+
 @pytest.mark.parametrize("format_", ["q8_0", "f16"])
 @pytest.mark.parametrize("tokens,past,heads,kv_heads", [
     (1, 0, 4, 4), (1, 1, 8, 1), (1, 31, 2, 2), (1, 32, 2, 1), (1, 2000, 16, 8), (2, 0, 7, 1), (5, 27, 3, 3), (32, 0, 2, 1),
