@@ -23,8 +23,8 @@
 // passes it by 2^8, which a tile seldom does) and p d below 2^15, so that the
 // parts' steps (2^-24) lie at least 30 bits below the largest.
 //
-// Split: up to 32 rows of a key head (attend) - the rows one wave holds - its
-// four waves take every fourth tile each, operands straight from the record,
+// Split: up to 32 rows of a key head (attend) - the rows one wave holds - a
+// workgroup's waves take its tiles in turn, operands straight from the record,
 // and are joined in LDS. More rows (attend_rows): each wave has rows of its
 // own, and a tile's codes become binary16 operands in LDS once for all of them.
 // Where a step has too few rows to fill the card its tiles are split among
@@ -32,6 +32,7 @@
 #pragma once
 
 #include "cache.hpp"
+#include "stream.hpp"
 
 namespace chm {
 
@@ -43,7 +44,6 @@ typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2E = 1.44269504088896340736f;
-constexpr uint32_t kAttentionWaves = 4;
 constexpr int kHeadroom = 6;      // a probability's exponent at the maximum last followed
 constexpr float kSlack = 8.0f;    // and how far past it a score may go (a half ends at 2^16)
 
@@ -245,34 +245,50 @@ struct Rows {
     int exponent;                            // D, the same in every lane
     Sight sight[RT];
 
-    // Rows from `row0` on; rows past the group's end repeat its last.
-    template <typename TREE>
-    __device__ __forceinline__ void begin(const Attention& a, const Group& group, const TREE& tree, uint32_t row0) {
+    // The queries' loads alone, ahead of what the rows wait for: a lane's
+    // values 8g .. 8g + 7 of each block. Rows past the group's end repeat its last.
+    struct Queries {
+        float x[RT][NB][8];
+    };
+    __device__ __forceinline__ static void fetch(const Attention& a, const Group& group, uint32_t row0, Queries& q) {
         const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+#pragma unroll
+        for (uint32_t i = 0; i < RT; ++i) {
+            const uint32_t inside = min(row0 + 16 * i + n, group.row_end - 1);
+            const float* from = a.queries +
+                                (static_cast<uint64_t>(group.sequence) * a.tokens + inside / a.group) * a.query_stride +
+                                static_cast<uint64_t>(group.head * a.group + inside % a.group) * (32 * NB) + 8 * g;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const float4 u = *reinterpret_cast<const float4*>(from + 32 * b);
+                const float4 v = *reinterpret_cast<const float4*>(from + 32 * b + 4);
+                q.x[i][b][0] = u.x, q.x[i][b][1] = u.y, q.x[i][b][2] = u.z, q.x[i][b][3] = u.w;
+                q.x[i][b][4] = v.x, q.x[i][b][5] = v.y, q.x[i][b][6] = v.z, q.x[i][b][7] = v.w;
+            }
+        }
+    }
+
+    template <typename TREE>
+    __device__ __forceinline__ void begin(const Attention& a, const Group& group, const TREE& tree, uint32_t row0,
+                                          Queries& q) {
+        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u;
         exponent = -64;
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) {
-            const uint32_t row = row0 + 16 * i + n, inside = min(row, group.row_end - 1);
-            const uint32_t token = inside / a.group;
+            const uint32_t row = row0 + 16 * i + n;
+            const uint32_t token = min(row, group.row_end - 1) / a.group;
             const uint32_t depth = a.parents ? tree.depth[token - group.token0] : token;
             sight[i].live = row < group.row_end && depth != kUnused;
             const uint32_t place = group.past + (depth != kUnused ? depth : 0u) + 1;  // one past its own place
             sight[i].first = a.window && place > a.window ? place - a.window : 0u;
             sight[i].last = a.parents ? token - group.token0 : group.past + token;
 
-            const float* q = a.queries +
-                             (static_cast<uint64_t>(group.sequence) * a.tokens + token) * a.query_stride +
-                             static_cast<uint64_t>(group.head * a.group + inside % a.group) * (32 * NB) + 8 * g;
-            float x[NB][8], most = 0.0f;
+            float most = 0.0f;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const float4 u = *reinterpret_cast<const float4*>(q + 32 * b);
-                const float4 v = *reinterpret_cast<const float4*>(q + 32 * b + 4);
-                x[b][0] = u.x, x[b][1] = u.y, x[b][2] = u.z, x[b][3] = u.w;
-                x[b][4] = v.x, x[b][5] = v.y, x[b][6] = v.z, x[b][7] = v.w;
+            for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[b][e] *= a.scale * kLog2E, most = fmaxf(most, fabsf(x[b][e]));
-            }
+                for (int e = 0; e < 8; ++e)
+                    q.x[i][b][e] *= a.scale * kLog2E, most = fmaxf(most, fabsf(q.x[i][b][e]));
             most = most_of_row(most);
             int shift = 0;
             if (most > 0.0f && most <= 3.4e38f) {
@@ -286,7 +302,7 @@ struct Rows {
                 half2_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    split2(ldexpf(x[b][2 * e], shift), ldexpf(x[b][2 * e + 1], shift), &hi[e], &lo[e]);
+                    split2(ldexpf(q.x[i][b][2 * e], shift), ldexpf(q.x[i][b][2 * e + 1], shift), &hi[e], &lo[e]);
                 high[i][b] = join(hi[0], hi[1], hi[2], hi[3]);
                 low[i][b] = join(lo[0], lo[1], lo[2], lo[3]);
             }
@@ -475,151 +491,185 @@ struct Rows {
 #pragma unroll
             for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= up;
     }
-
-    // A row's outputs, its sum whole (`total`) and its offset (`least`): to the
-    // step's output, or to the split's place.
-    __device__ __forceinline__ void finish(const Attention& a, const Group& group, uint32_t row0, const float (&total)[RT],
-                                           const float (&least)[RT]) const {
-        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
-#pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            const uint32_t row = row0 + 16 * i + n;
-            if (row >= group.row_end) continue;
-            // nothing seen: no maximum, and no NaN either
-            const bool empty = !sight[i].live || (least[i] == INFINITY && total[i] == 0.0f);
-            if (a.splits == 1) {
-                const float inverse = empty ? 0.0f : 1.0f / total[i];
-                float* to = a.output +
-                            (static_cast<uint64_t>(group.sequence) * a.tokens + row / a.group) * a.output_stride +
-                            static_cast<uint64_t>(group.head * a.group + row % a.group) * (32 * NB) + 4 * g;
-#pragma unroll
-                for (uint32_t t = 0; t < 2 * NB; ++t)
-                    *reinterpret_cast<float4_t*>(to + 16 * t) = empty ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : out[i][t] * inverse;
-            } else {
-                const uint64_t place = (group.sequence_head * a.rows + row) * a.splits + group.split;
-                float* to = a.partial + place * (32 * NB) + 4 * g;
-                if (!empty)
-#pragma unroll
-                    for (uint32_t t = 0; t < 2 * NB; ++t) *reinterpret_cast<float4_t*>(to + 16 * t) = out[i][t];
-                const bool spoilt = total[i] != total[i];
-                if (g == 0)
-                    a.stats[place] = make_float2(empty ? INFINITY : spoilt ? total[i] : least[i], empty ? 0.0f : total[i]);
-            }
-        }
-    }
 };
+
+// Four values of a row's outputs, its sum `total` and its offset `least`: to
+// the step's output, or to the split's place. `stats`: whether this thread
+// writes the row's.
+template <uint32_t NB>
+__device__ __forceinline__ void finish(const Attention& a, const Group& group, uint32_t row, bool live, uint32_t at,
+                                       float4_t out, float total, float least, bool stats) {
+    // nothing seen: no maximum, and no NaN either
+    const bool empty = !live || (least == INFINITY && total == 0.0f);
+    if (a.splits == 1) {
+        float* to = a.output + (static_cast<uint64_t>(group.sequence) * a.tokens + row / a.group) * a.output_stride +
+                    static_cast<uint64_t>(group.head * a.group + row % a.group) * (32 * NB) + at;
+        *reinterpret_cast<float4_t*>(to) = empty ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : out * (1.0f / total);
+        return;
+    }
+    const uint64_t place = (group.sequence_head * a.rows + row) * a.splits + group.split;
+    if (!empty) *reinterpret_cast<float4_t*>(a.partial + place * (32 * NB) + at) = out;
+    if (stats) {
+        const bool spoilt = total != total;
+        a.stats[place] = make_float2(empty ? INFINITY : spoilt ? total : least, empty ? 0.0f : total);
+    }
+}
 
 // ---- few rows: the waves split the tiles ----------------------------------------
 
-// A tile's operands in registers, loaded as the record holds them.
-template <uint32_t F, uint32_t NB>
-struct Registers {
-    Codes<F> keys[NB], values[NB];
-    uint4_t key_scales_[NB], value_scales_[NB];
+// Records copied to LDS as they are, a wave's own ring of them: each copy is
+// 64 lanes of 16 bytes straight from memory to LDS, so that a wave's next
+// tiles are on their way while it works on one, with no registers for them.
+typedef __attribute__((address_space(3))) void* lds_pointer;
 
-    __device__ __forceinline__ void load(const uint8_t* record) {
-        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+template <uint32_t RECORD>
+__device__ __forceinline__ void copy_record(const uint8_t* from, uint8_t* to) {
+    const uint32_t lane = threadIdx.x & 63u;
 #pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            keys[b] = load_codes<F>(record + b * cache_unit(F), lane);
-            if constexpr (key_scales(F))
-                key_scales_[b] = *reinterpret_cast<const uint4_t*>(record + key_scales_at(F, NB) + 64 * b + 16 * g);
-        }
-#pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            values[b] = load_codes<F>(record + values_at(F, NB) + b * cache_unit(F), lane);
-            value_scales_[b] = *reinterpret_cast<const uint4_t*>(record + value_scales_at(F, NB) + 64 * b + 16 * g);
-        }
+    for (uint32_t at = 0; at < RECORD; at += 1024)
+        if (at + 1024 <= RECORD || at + 16 * lane < RECORD)
+            __builtin_amdgcn_global_load_lds(from + at + 16 * lane, (lds_pointer)(to + at), 16, 0, kStreamPolicy);
+}
+
+// Waits until at most `LEFT` of the wave's loads are on their way (they end in
+// order), what they write in LDS then being there. LEFT below 64: s_waitcnt's
+// vmcnt, its low four bits and its high two, the other counters at no wait.
+template <uint32_t LEFT>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(LEFT < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((LEFT & 15u) | (LEFT >> 4) << 14 | 0x7u << 4 | 0xFu << 8);
+    __asm__ __volatile__("" ::: "memory");
+}
+
+// A tile's operands out of its record in LDS.
+template <uint32_t F, uint32_t NB>
+struct Record {
+    const uint8_t* at;
+    uint32_t slot0, latest;  // what lies past the last token is cut: kept_of
+
+    __device__ __forceinline__ half8_t key(uint32_t b, int h) const {
+        return operand<F, false>(load_codes<F>(at + b * cache_unit(F), threadIdx.x & 63u), h);
     }
-    __device__ __forceinline__ void cut(uint32_t slot0, uint32_t latest) {
+    __device__ __forceinline__ half8_t value(uint32_t b, int u) const {
+        const uint32_t lane = threadIdx.x & 63u;
+        Codes<F> c = load_codes<F>(at + values_at(F, NB) + b * cache_unit(F), lane);
+        if constexpr (F == kF16)
+            if (slot0 + kTile > latest)
+#pragma unroll
+                for (uint32_t w = 0; w < 4; ++w) c.w[4 * u + w] &= kept_of(slot0, lane >> 4, w, latest);
+        return operand<F, true>(c, u);
+    }
+    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const {
+        return *reinterpret_cast<const uint4_t*>(at + key_scales_at(F, NB) + 64 * b + 16 * ((threadIdx.x & 63u) >> 4));
+    }
+    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const {
         const uint32_t g = (threadIdx.x & 63u) >> 4;
+        uint4_t s = *reinterpret_cast<const uint4_t*>(at + value_scales_at(F, NB) + 64 * b + 16 * g);
+        if (slot0 + kTile > latest)
 #pragma unroll
-        for (uint32_t w = 0; w < 4; ++w) {
-            const uint32_t kept = kept_of(slot0, g, w, latest);
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                value_scales_[b][w] = kept_scale<F>(value_scales_[b][w], kept);
-                if constexpr (F == kF16) values[b].w[w] &= kept, values[b].w[4 + w] &= kept;
-            }
-        }
+            for (uint32_t w = 0; w < 4; ++w) s[w] = kept_scale<F>(s[w], kept_of(slot0, g, w, latest));
+        return s;
     }
-    __device__ __forceinline__ half8_t key(uint32_t b, int h) const { return operand<F, false>(keys[b], h); }
-    __device__ __forceinline__ half8_t value(uint32_t b, int u) const { return operand<F, true>(values[b], u); }
-    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const { return key_scales_[b]; }
-    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const { return value_scales_[b]; }
+};
+
+// Waves a workgroup and records a wave's ring: eight waves where two fit a
+// SIMD's registers and two records of each fit the LDS, else four, else two.
+constexpr uint32_t kRingBytes = 144 * 1024;
+template <uint32_t F, uint32_t NB, uint32_t RT>
+struct AttendShape {
+    static constexpr uint32_t kRecord = cache_record(F, NB);
+    static constexpr uint32_t kWaves = NB * RT <= 4 && 16 * kRecord <= kRingBytes ? 8 : 8 * kRecord <= kRingBytes ? 4 : 2;
+    static constexpr uint32_t kRing = kRingBytes / (kWaves * kRecord) < 4 ? kRingBytes / (kWaves * kRecord) : 4;
+    static constexpr uint32_t kCopies = (kRecord + 1023) / 1024;
 };
 
 template <uint32_t F, uint32_t NB, uint32_t RT>
-__global__ __launch_bounds__(256) void attend(Attention a) {
-    constexpr uint32_t kRows = 16 * RT, kRecord = cache_record(F, NB);
+__global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(Attention a) {
+    using Shape = AttendShape<F, NB, RT>;
+    constexpr uint32_t kRows = 16 * RT, kRecord = Shape::kRecord, W = Shape::kWaves, D = Shape::kRing;
+    constexpr uint32_t kParts = RT * 2 * NB * 64;  // float4s of a wave's outputs
     __shared__ Tree<kRows> tree;
-    __shared__ float4_t joined[2][RT * 2 * NB][64];
-    __shared__ float joined_offset[kAttentionWaves][kRows], joined_sum[kAttentionWaves][kRows];
+    // The waves' rings; then, all tiles done, their outputs.
+    __shared__ __align__(16) uint8_t space[sizeof(uint8_t[W][D][kRecord]) > sizeof(float4_t[W][kParts])
+                                               ? sizeof(uint8_t[W][D][kRecord])
+                                               : sizeof(float4_t[W][kParts])];
+    __shared__ float joined_offset[W][kRows], joined_sum[W][kRows];
+    __shared__ uint32_t joined_live[kRows];
 
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15u, g = lane >> 4;
     const Group group(a, kRows);
+    typename Rows<F, NB, RT>::Queries queries;
+    Rows<F, NB, RT>::fetch(a, group, group.row0, queries);
     if (a.parents)
         read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
                   group.token_end - group.token0, a.window);
-    Rows<F, NB, RT> rows;
-    rows.begin(a, group, tree, group.row0);
 
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
-    for (uint32_t tile = group.tile_begin + wave; tile < group.tile_end; tile += kAttentionWaves) {
-        Registers<F, NB> source;
-        source.load(base + static_cast<uint64_t>(tile) * kRecord);
-        if (tile * kTile + kTile > group.latest) source.cut(tile * kTile, group.latest);
-        rows.tile(a, group, tree, tile * kTile, source);
+    uint8_t* ring = space + wave * (D * kRecord);
+    const uint32_t first = group.tile_begin + wave;
+    const uint32_t count = first < group.tile_end ? (group.tile_end - first + W - 1) / W : 0;  // the wave's tiles
+    auto copy = [&](uint32_t j) {
+        copy_record<kRecord>(base + static_cast<uint64_t>(first + j * W) * kRecord, ring + j % D * kRecord);
+    };
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, group.row0, queries);
+    // only the copies are on their way from here on
+    wait_loads<0>();
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < D; ++j)
+        if (j < count) copy(j);
+    for (uint32_t j = 0; j < count; ++j) {
+        // tile j + D - 1 into the place of tile j - 1, whose reads are done
+        if (j + D - 1 < count) {
+            copy(j + D - 1);
+            wait_loads<(D - 1) * Shape::kCopies>();
+        } else {
+            wait_loads<0>();
+        }
+        const uint32_t slot0 = (first + j * W) * kTile;
+        rows.tile(a, group, tree, slot0, Record<F, NB>{ring + j % D * kRecord, slot0, group.latest});
+        __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");  // the record's reads, before its place is copied to
     }
     rows.end();
+    __syncthreads();
+    float4_t(*joined)[kParts] = reinterpret_cast<float4_t(*)[kParts]>(space);
 
-    // The four waves joined: each one's outputs on the least offset's (the
-    // largest maximum's) scale, waves 2 and 3 into 0 and 1, then 1 into 0.
-    float total[RT], least[RT];
+    // The waves joined: each one's outputs on the least offset's (the largest
+    // maximum's) scale, added in wave order, a thread some of the values.
 #pragma unroll
     for (uint32_t i = 0; i < RT; ++i) {
         const float mine = sum_of_row(rows.sum[i]);
         if (g == 0) joined_offset[wave][16 * i + n] = rows.offset[i], joined_sum[wave][16 * i + n] = mine;
+        if (threadIdx.x < 16) joined_live[16 * i + n] = rows.sight[i].live;
     }
+#pragma unroll
+    for (uint32_t i = 0; i < RT; ++i)
+#pragma unroll
+        for (uint32_t t = 0; t < 2 * NB; ++t) joined[wave][(i * 2 * NB + t) * 64 + lane] = rows.out[i][t];
     __syncthreads();
+    for (uint32_t x = 0; x < (kParts + 64 * W - 1) / (64 * W); ++x) {
+        const uint32_t at = threadIdx.x + 64 * W * x;
+        if (at >= kParts) break;
+        const uint32_t i = at / (128 * NB), t = at / 64 % (2 * NB), in_row = 16 * i + n;
+        if (group.row0 + in_row >= group.row_end) continue;
+        float least = INFINITY, total = 0.0f;
+        float4_t out = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        least[i] = INFINITY, total[i] = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < kAttentionWaves; ++w) {
-            const float theirs = joined_offset[w][16 * i + n];
-            least[i] = theirs < least[i] || theirs != theirs ? theirs : least[i];
+        for (uint32_t w = 0; w < W; ++w) {
+            const float theirs = joined_offset[w][in_row];
+            least = theirs < least || theirs != theirs ? theirs : least;
         }
 #pragma unroll
-        for (uint32_t w = 0; w < kAttentionWaves; ++w) {
-            const float theirs = joined_offset[w][16 * i + n];
-            total[i] += joined_sum[w][16 * i + n] * (theirs == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least[i] - theirs));
+        for (uint32_t w = 0; w < W; ++w) {
+            // a wave that saw nothing has zeros, or the NaNs of scores that are
+            const float theirs = joined_offset[w][in_row];
+            const float factor = theirs == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least - theirs);
+            total = __builtin_fmaf(joined_sum[w][in_row], factor, total);
+            out += joined[w][at] * factor;
         }
-        const float factor = rows.offset[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least[i] - rows.offset[i]);
-#pragma unroll
-        for (uint32_t t = 0; t < 2 * NB; ++t) rows.out[i][t] *= factor;
+        finish<NB>(a, group, group.row0 + in_row, joined_live[in_row] != 0, 16 * t + 4 * g, out, total, least,
+                   t == 0 && g == 0);
     }
-    auto give = [&](uint32_t place) {
-#pragma unroll
-        for (uint32_t i = 0; i < RT; ++i)
-#pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) joined[place][i * 2 * NB + t][lane] = rows.out[i][t];
-    };
-    auto take = [&](uint32_t place) {
-#pragma unroll
-        for (uint32_t i = 0; i < RT; ++i)
-#pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) rows.out[i][t] += joined[place][i * 2 * NB + t][lane];
-    };
-    if (wave >= 2) give(wave - 2);
-    __syncthreads();
-    if (wave < 2) take(wave);
-    __syncthreads();
-    if (wave == 1) give(0);
-    __syncthreads();
-    if (wave != 0) return;
-    take(0);
-    rows.finish(a, group, group.row0, total, least);
 }
 
 // ---- many rows: the waves split the rows -------------------------------------------
@@ -653,13 +703,10 @@ __global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
 
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const Group group(a, kRows);
-    if (a.parents)
-        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
-                  group.token_end - group.token0, a.window);
     const uint32_t row0 = group.row0 + 16 * RT * wave;
     const bool mine = row0 < group.row_end;  // a wave without rows still lays out its share
-    Rows<F, NB, RT> rows;
-    rows.begin(a, group, tree, min(row0, group.row_end - 1));
+    typename Rows<F, NB, RT>::Queries queries;
+    Rows<F, NB, RT>::fetch(a, group, min(row0, group.row_end - 1), queries);
     // a chain's wave sees nothing past its last row's token
     const uint32_t sees_to =
         a.parents ? group.latest : group.past + (min(row0 + 16 * RT, group.row_end) - 1) / a.group + 1;
@@ -710,10 +757,13 @@ __global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
         }
     };
 
-    if (group.tile_begin < group.tile_end) {
-        load(group.tile_begin);
-        lay(group.tile_begin, stages[0]);
-    }
+    if (group.tile_begin < group.tile_end) load(group.tile_begin);
+    if (a.parents)
+        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                  group.token_end - group.token0, a.window);
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, min(row0, group.row_end - 1), queries);
+    if (group.tile_begin < group.tile_end) lay(group.tile_begin, stages[0]);
     __syncthreads();
     uint32_t turn = 0;
     for (uint32_t tile0 = group.tile_begin; tile0 < group.tile_end; tile0 += kTiles, turn ^= 1) {
@@ -729,12 +779,19 @@ __global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
         if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
         __syncthreads();
     }
-    if (!mine) return;
-    rows.end();
-    float total[RT];
+    if (mine) {
+        rows.end();
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) total[i] = sum_of_row(rows.sum[i]);
-    rows.finish(a, group, row0, total, rows.offset);
+        for (uint32_t i = 0; i < RT; ++i) {
+            const float total = sum_of_row(rows.sum[i]);
+            const uint32_t row = row0 + 16 * i + (lane & 15u);
+            if (row >= group.row_end) continue;
+#pragma unroll
+            for (uint32_t t = 0; t < 2 * NB; ++t)
+                finish<NB>(a, group, row, rows.sight[i].live, 16 * t + 4 * (lane >> 4), rows.out[i][t], total,
+                           rows.offset[i], t == 0 && lane < 16);
+        }
+    }
 }
 
 template <uint32_t F, uint32_t NB>
@@ -748,9 +805,9 @@ static hipError_t launch_blocks(const Attention& a, const AttentionPlan& plan, h
     else if (plan.waves == 4)
         hipLaunchKernelGGL((attend_rows<F, NB, 1, 4>), grid, dim3(256), 0, stream, a);
     else if (plan.row_tiles == kWide)
-        hipLaunchKernelGGL((attend<F, NB, kWide>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attend<F, NB, kWide>), grid, dim3(64 * AttendShape<F, NB, kWide>::kWaves), 0, stream, a);
     else
-        hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(64 * AttendShape<F, NB, 1>::kWaves), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -1,121 +1,96 @@
 // The splits of a step's attention joined (attention.hpp): a row's splits hold
-// outputs and a sum relative to their own offsets, o_s and l_s; the row is
+// outputs o_s and sums l_s relative to their own offsets c_s; the row is
 //   sum_s 2^(c - c_s) o_s / sum_s 2^(c - c_s) l_s,  c the least offset,
-// added in split order. And the step's plan.
+// added in an order that their number alone fixes.
 //
-// A wave a row: head_dim / 4 lanes hold the row's values, and as many such
-// groups as fit the wave take its splits in turn.
-#include <algorithm>
-
+// As many lanes as hold a row's values, four each, are a group; where the rows
+// are few a row's splits are shared among several groups of a workgroup and
+// added through LDS, so that all of its loads are on their way at once.
 #include "serving.hpp"
 
 namespace chm {
 
-template <uint32_t LANES>
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+// SHARES groups a row.
+template <uint32_t LANES, uint32_t SHARES>
 __global__ __launch_bounds__(256) void attention_combine(Attention a) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t id = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const uint64_t sequence_head = id / a.rows;
-    const uint32_t row = static_cast<uint32_t>(id % a.rows);
-    if (sequence_head >= static_cast<uint64_t>(a.cache.sequences) * a.cache.kv_heads) return;
-    const uint32_t sequence = static_cast<uint32_t>(sequence_head / a.cache.kv_heads);
-    const uint32_t head = static_cast<uint32_t>(sequence_head % a.cache.kv_heads);
-    const float2* stats = a.stats + id * a.splits;
+    constexpr uint32_t kGroups = 256 / LANES;
+    __shared__ float4_t sums[SHARES > 1 ? 256 : 1];
+    __shared__ float totals[kGroups];
+    const uint32_t part = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARES;
+    const uint64_t row_of_all = static_cast<uint64_t>(blockIdx.x) * (kGroups / SHARES) + group / SHARES;
+    const uint64_t sequence_head = row_of_all / a.rows;
+    const uint32_t row = static_cast<uint32_t>(row_of_all % a.rows);
+    const bool live = sequence_head < static_cast<uint64_t>(a.cache.sequences) * a.cache.kv_heads &&
+                      4 * part < a.cache.head_dim;
+    const uint64_t place = row_of_all * a.splits;
 
-    float least = INFINITY;
-    for (uint32_t s = lane; s < a.splits; s += 64) {
-        const float c = stats[s].x;
-        least = c < least || c != c ? c : least;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float c = __shfl_xor(least, o);
-        least = c < least || c != c ? c : least;
-    }
-
-    constexpr uint32_t kGroups = 64 / LANES;
-    const uint32_t part = lane % LANES, group = lane / LANES;
-    float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    float total = 0.0f;
-    if (4 * part < a.cache.head_dim) {
-        for (uint32_t s = group; s < a.splits; s += kGroups) {
-            const float2 st = stats[s];
+    // This share's splits relative to its own least offset, then all of them to the row's.
+    float least = INFINITY, total = 0.0f;
+    float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+#pragma unroll 4
+        for (uint32_t s = share; s < a.splits; s += SHARES) {
+            const float2 st = a.stats[place + s];
+            const float4_t v = *reinterpret_cast<const float4_t*>(a.partial + (place + s) * a.cache.head_dim + 4 * part);
             if (st.x == INFINITY) continue;  // nothing seen: its outputs were not written
-            const float w = __builtin_amdgcn_exp2f(least - st.x);
-            const float4 v = *reinterpret_cast<const float4*>(a.partial + (id * a.splits + s) * a.cache.head_dim + 4 * part);
-            total = __builtin_fmaf(w, st.y, total);
-            sum = {__builtin_fmaf(w, v.x, sum.x), __builtin_fmaf(w, v.y, sum.y), __builtin_fmaf(w, v.z, sum.z),
-                   __builtin_fmaf(w, v.w, sum.w)};
+            const float to = st.x < least || st.x != st.x ? st.x : least;
+            const float old = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - least);
+            const float w = __builtin_amdgcn_exp2f(to - st.x);
+            least = to;
+            total = __builtin_fmaf(w, st.y, total * old);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w, v[e], sum[e] * old);
         }
     }
-#pragma unroll
-    for (uint32_t o = LANES; o < 64; o <<= 1) {
-        sum.x += __shfl_xor(sum.x, o);
-        sum.y += __shfl_xor(sum.y, o);
-        sum.z += __shfl_xor(sum.z, o);
-        sum.w += __shfl_xor(sum.w, o);
-        total += __shfl_xor(total, o);
+    if constexpr (SHARES > 1) {
+        __shared__ float leasts[kGroups];
+        sums[threadIdx.x] = sum;
+        if (part == 0) totals[group] = total, leasts[group] = least;
+        __syncthreads();
+        if (share != 0) return;
+        for (uint32_t x = 1; x < SHARES; ++x) {
+            const float c = leasts[group + x];
+            least = c < least || c != c ? c : least;
+        }
+        sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        total = 0.0f;
+        for (uint32_t x = 0; x < SHARES; ++x) {
+            const float c = leasts[group + x];
+            if (c == INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(least - c);
+            total = __builtin_fmaf(w, totals[group + x], total);
+            sum += sums[threadIdx.x + x * LANES] * w;
+        }
     }
-    if (group != 0 || 4 * part >= a.cache.head_dim) return;
+    if (!live) return;
+    const uint32_t sequence = static_cast<uint32_t>(sequence_head / a.cache.kv_heads);
+    const uint32_t head = static_cast<uint32_t>(sequence_head % a.cache.kv_heads);
     const float inverse = least == INFINITY ? 0.0f : 1.0f / total;
     float* to = a.output + (static_cast<uint64_t>(sequence) * a.tokens + row / a.group) * a.output_stride +
                 static_cast<uint64_t>(head * a.group + row % a.group) * a.cache.head_dim + 4 * part;
-    *reinterpret_cast<float4*>(to) = make_float4(sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse);
+    *reinterpret_cast<float4_t*>(to) = sum * inverse;
 }
 
-hipError_t launch_attention_combine(const Attention& a, hipStream_t stream) {
+template <uint32_t LANES>
+static hipError_t launch_lanes(const Attention& a, hipStream_t stream) {
+    constexpr uint32_t kGroups = 256 / LANES;
     const uint64_t rows = uint64_t{a.cache.sequences} * a.cache.kv_heads * a.rows;
-    const dim3 grid(static_cast<uint32_t>((rows + 3) / 4));
-    if (a.cache.head_dim <= 32)
-        hipLaunchKernelGGL(attention_combine<8>, grid, dim3(256), 0, stream, a);
-    else if (a.cache.head_dim <= 64)
-        hipLaunchKernelGGL(attention_combine<16>, grid, dim3(256), 0, stream, a);
-    else if (a.cache.head_dim <= 128)
-        hipLaunchKernelGGL(attention_combine<32>, grid, dim3(256), 0, stream, a);
+    // a workgroup a row while that is at most four a compute unit
+    if (rows <= 1024)
+        hipLaunchKernelGGL((attention_combine<LANES, kGroups>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL(attention_combine<64>, grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attention_combine<LANES, 1>), dim3(static_cast<uint32_t>((rows + kGroups - 1) / kGroups)),
+                           dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
-// The least rows a workgroup that hold the step's, at most 32 RT; then splits
-// until each compute unit has eight waves, a split of at least four tiles.
-AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
-                             uint32_t window, uint32_t compute_units) {
-    const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
-    const uint32_t wide = cache.head_dim <= 128 ? 2 : 1;  // 16-row tiles a wave's registers hold
-    AttentionPlan plan{};
-    plan.waves = rows <= 16 * wide ? 1 : rows <= 64 * wide ? 4 : 8;
-    plan.row_tiles = rows <= 16 || (plan.waves == 4 && rows <= 64) ? 1 : wide;
-    const uint64_t group = 16ull * plan.row_tiles * plan.waves;
-    plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
-    const uint64_t workgroups = uint64_t{cache.sequences} * cache.kv_heads * plan.row_groups;
-    uint64_t reach = std::min(longest ? longest : cache.capacity, cache.capacity);
-    if (window) reach = std::min<uint64_t>(reach, uint64_t{window} + tokens + 31);
-    const uint64_t tiles = (reach + 31) / 32;
-    const uint64_t wanted = (plan.waves == 8 ? 1ull : 2ull) * compute_units / workgroups;
-    plan.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, (tiles + 3) / 4)));
-    return plan;
-}
-
-uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t splits) {
-    if (splits < 2) return 0;
-    return uint64_t{cache.sequences} * query_heads * tokens * splits * (uint64_t{cache.head_dim} * 4 + 8);
-}
-
-// Steps of every number of tokens up to `tokens`: of those in one number of
-// row groups the last needs most, and past the first that does not split none does.
-uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units) {
-    uint64_t most = 0;
-    const uint64_t group = query_heads / cache.kv_heads;
-    for (uint32_t t = 1; t <= tokens; ++t) {
-        AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        const uint64_t rows = 16ull * plan.row_tiles * plan.waves * plan.row_groups;
-        t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, rows / group)));
-        plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
-        if (plan.waves == 8 && plan.splits < 2) break;
-    }
-    return most;
+hipError_t launch_attention_combine(const Attention& a, hipStream_t stream) {
+    if (a.cache.head_dim <= 32) return launch_lanes<8>(a, stream);
+    if (a.cache.head_dim <= 64) return launch_lanes<16>(a, stream);
+    if (a.cache.head_dim <= 128) return launch_lanes<32>(a, stream);
+    return launch_lanes<64>(a, stream);
 }
 
 }  // namespace chm

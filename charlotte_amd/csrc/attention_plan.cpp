@@ -1,0 +1,53 @@
+// How a step of attention runs (attention.hpp), on the host alone.
+#include <algorithm>
+
+#include "serving.hpp"
+
+namespace chm {
+
+// The least rows a workgroup that hold the step's, at most 128 to one whose
+// waves split its tiles; then splits until each compute unit has a workgroup
+// (two of attend_rows' four waves), of kLeast tiles at the least: shorter, a
+// second launch to join them costs more than it gains.
+AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
+                             uint32_t window, uint32_t compute_units) {
+    const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
+    const uint32_t wide = cache.head_dim <= 128 ? 2 : 1;  // 16-row tiles a wave's registers hold
+    AttentionPlan plan{};
+    plan.waves = rows <= 128 ? 1 : rows <= 64 * wide ? 4 : 8;
+    plan.row_tiles = rows <= 16 ? 1 : wide;
+    const uint64_t group = 16ull * plan.row_tiles * plan.waves;
+    plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
+    const uint64_t workgroups = uint64_t{cache.sequences} * cache.kv_heads * plan.row_groups;
+    uint64_t reach = std::min(longest ? longest : cache.capacity, cache.capacity);
+    if (window) reach = std::min<uint64_t>(reach, uint64_t{window} + tokens + 31);
+    const uint64_t tiles = (reach + 31) / 32;
+    const uint64_t wanted = compute_units / workgroups;
+    constexpr uint64_t kLeast = 8;
+    plan.splits = static_cast<uint32_t>(
+        tiles <= 32 ? 1 : std::max<uint64_t>(1, std::min(wanted, (tiles + kLeast - 1) / kLeast)));
+    return plan;
+}
+
+uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t splits) {
+    if (splits < 2) return 0;
+    return uint64_t{cache.sequences} * query_heads * tokens * splits * (uint64_t{cache.head_dim} * 4 + 8);
+}
+
+// Steps of every number of tokens up to `tokens`: of those in one number of
+// row groups the last needs most, and past the first that does not split none does.
+uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units) {
+    uint64_t most = 0;
+    const uint64_t group = query_heads / cache.kv_heads;
+    for (uint32_t t = 1; t <= tokens; ++t) {
+        AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
+        const uint64_t rows = 16ull * plan.row_tiles * plan.waves * plan.row_groups;
+        t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, rows / group)));
+        plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
+        most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
+        if (plan.waves == 8 && plan.splits < 2) break;
+    }
+    return most;
+}
+
+}  // namespace chm

@@ -59,7 +59,7 @@ hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream);
 hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream);
 hipError_t launch_cache_keep(const CacheKeep& a, hipStream_t stream);
 
-// ---- attention (attention.hpp, attention_*.hip) ----
+// ---- attention (attention.hpp, attention_*.hip, attention_plan.cpp) ----
 
 constexpr uint32_t kTreeTokens = 256;
 
@@ -70,8 +70,8 @@ struct Attention {
     uint64_t query_stride, output_stride;
     const uint32_t* past;
     const int32_t* parents;  // or null: a chain
-    float* partial;          // splits > 1: each row's unnormalised outputs, [head][row][split][head_dim]
-    float2* stats;           // and their maximum and sum, [head][row][split]
+    float2* stats;           // splits > 1: each row's offset and sum, [head][row][split]
+    float* partial;          // and its outputs over neither, [head][row][split][head_dim]
     uint32_t tokens, group, rows;  // rows = tokens x group, of one key head
     uint32_t window, splits;
     float scale;
@@ -87,6 +87,7 @@ struct AttentionPlan {
 
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units);
+// The workspace of a step in `splits`: its outputs, then its stats.
 uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t splits);
 // What any step of at most `tokens` tokens a sequence may need of it.
 uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units);
