@@ -44,8 +44,11 @@ typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2E = 1.44269504088896340736f;
-constexpr int kHeadroom = 6;      // a probability's exponent at the maximum last followed
-constexpr float kSlack = 8.0f;    // and how far past it a score may go (a half ends at 2^16)
+// A probability is 2^kHeadroom at the maximum last followed, and a score may go
+// kSlack past it; the largest value scale met is 2^kScaleTop to twice it. Their
+// product stays below 2^15 (a half ends at 2^16).
+constexpr int kHeadroom = 7, kScaleTop = 3;
+constexpr float kSlack = 4.0f;
 
 // A lane's codes of one unit (keys or values of a block by 32 tokens).
 template <uint32_t F>
@@ -118,12 +121,26 @@ __device__ __forceinline__ half2_t pair_of(uint32_t w) { return __builtin_bit_ca
 // Slot i's scale of a lane's eight, i a constant.
 __device__ __forceinline__ float scale_at(const uint4_t& s, int i) { return static_cast<float>(pair_of(s[i >> 1])[i & 1]); }
 
-// Two f32 as two binary16 parts of each: hi rounded towards zero, lo what it
-// leaves, rounded likewise (2^-21 of the value at the most).
+// Two f32 as two binary16 parts of each: hi, and lo what it leaves, both
+// rounded to nearest (lo's bias, were it cut, would be every probability's):
+// within 2^-22 of the value, or 2^-25.
 __device__ __forceinline__ void split2(float a, float b, half2_t* hi, half2_t* lo) {
-    *hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-    *lo = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi->x), -1.0f, a),
-                                                                 __builtin_fmaf(static_cast<float>(hi->y), -1.0f, b)));
+    *hi = half2_t{static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    *lo = half2_t{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi->x), -1.0f, a)),
+                  static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi->y), -1.0f, b))};
+}
+
+// The larger of two scales' magnitudes as bits, a NaN's as none.
+__device__ __forceinline__ uint32_t larger_scale(uint32_t w) {
+    const uint32_t lo = w & 0x7FFFu, hi = w >> 16 & 0x7FFFu;
+    return max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi);
+}
+// D: 2^D <= the scale < 2^(D + 1); any below 2^-12 counts as that.
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return static_cast<int>(max(bits >> 10, 3u)) - 15; }
+// What a scale is multiplied by, a power of two: from 2^(3 - 15) to 2^(3 + 12), which binary16 holds.
+__device__ __forceinline__ half2_t over(int exponent) {
+    const _Float16 by = static_cast<_Float16>(ldexpf(1.0f, kScaleTop - exponent));
+    return half2_t{by, by};
 }
 
 // Over the four lanes that share a row (lane % 16).
@@ -197,6 +214,14 @@ struct Sight {
     uint32_t last;    // chain: the last; tree: its token's place in the workgroup's Tree
     bool live;        // a row of the step, and used
 };
+
+// Bits `from` .. `to` - 1 of a tile's 32 slots, the bounds counted from its
+// first and anywhere.
+__device__ __forceinline__ uint32_t bits_between(int64_t from, int64_t to) {
+    const uint32_t lo = static_cast<uint32_t>(from < 0 ? 0 : from > 32 ? 32 : from);
+    const uint32_t hi = static_cast<uint32_t>(to < 0 ? 0 : to > 32 ? 32 : to);
+    return static_cast<uint32_t>((1ull << hi) - 1) & ~static_cast<uint32_t>((1ull << lo) - 1);
+}
 
 // What a workgroup's rows, row0 .. row_end - 1 of a key head, have in common.
 struct Group {
@@ -272,7 +297,7 @@ struct Rows {
     __device__ __forceinline__ void begin(const Attention& a, const Group& group, const TREE& tree, uint32_t row0,
                                           Queries& q) {
         const uint32_t lane = threadIdx.x & 63u, n = lane & 15u;
-        exponent = -64;
+        exponent = F == kF16 ? kScaleTop : -64;
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) {
             const uint32_t row = row0 + 16 * i + n;
@@ -312,10 +337,38 @@ struct Rows {
         }
     }
 
-    // One tile. `source` gives the operands: key(b, h), key_scale(b), value(b, u), value_scale(b).
-    template <typename SOURCE, typename TREE>
+    // The slots of the tile at slot0 that row i of the lane sees, as bits.
+    template <typename TREE>
+    __device__ __forceinline__ uint32_t sees(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
+                                             uint32_t i) const {
+        const int64_t at = slot0;
+        if (!a.parents) return bits_between(sight[i].first - at, static_cast<int64_t>(sight[i].last) + 1 - at);
+        uint32_t seen = bits_between(sight[i].first - at, group.past - at);
+        if (slot0 + kTile > group.past) {
+            // the tree's tokens from `node` on: two words of the row's bits, shifted
+            const int32_t node = static_cast<int32_t>(slot0 - group.past);
+            const uint32_t* above = tree.above[sight[i].last];
+            uint64_t words = 0;
+            if (node < 0) {
+                words = static_cast<uint64_t>(above[0]) << -node;
+            } else if (node < static_cast<int32_t>(kTreeTokens)) {
+                const uint32_t w = static_cast<uint32_t>(node) >> 5;
+                words = above[w];
+                if (w + 1 < kTreeTokens / 32) words |= static_cast<uint64_t>(above[w + 1]) << 32;
+                words >>= node & 31;
+            }
+            seen |= static_cast<uint32_t>(words);
+        }
+        return seen;
+    }
+
+    // One tile. `source` gives the operands: key(b, h), key_scale(b), value(b, u),
+    // value_scale(b); and, PARTED, value_low(b, u), the values being scaled (over
+    // 2^D by 2^kScaleTop) and in two parts of their own: their scales are then
+    // looked at only where `spoilt`, some of them a NaN, stands.
+    template <bool PARTED, typename SOURCE, typename TREE>
     __device__ __forceinline__ void tile(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
-                                         const SOURCE& source) {
+                                         const SOURCE& source, bool spoilt = false) {
         const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
         // Scores: s[i][h][r] of token 16h + 4g + r.
         float4_t s[RT][2];
@@ -345,44 +398,32 @@ struct Rows {
         }
 
         const bool masked = group.masked(slot0);
-        uint32_t seen[RT][4];  // a half's mask a slot
+        if (masked)
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0xFFFFFFFFu;
-        if (masked) {
+            for (uint32_t i = 0; i < RT; ++i) {
+                const uint32_t bits = sees(a, group, tree, slot0, i) >> (4 * g);
 #pragma unroll
-            for (uint32_t i = 0; i < RT; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t slot = slot0 + 16 * (e >> 2) + 4 * g + (e & 3);
-                    bool sees = slot >= sight[i].first;
-                    if (!a.parents) {
-                        sees = sees && slot <= sight[i].last;
-                    } else if (slot >= group.past) {
-                        const uint32_t node = slot - group.past;
-                        sees = node < a.tokens && (tree.above[sight[i].last][node >> 5] >> (node & 31u) & 1u);
-                    }
-                    if (!sees) {
-                        s[i][e >> 2][e & 3] = -INFINITY;
-                        seen[i][e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
-                    }
-                }
-        }
+                for (int e = 0; e < 8; ++e)
+                    if (!(bits >> ((e >> 2) * 16 + (e & 3)) & 1u)) s[i][e >> 2][e & 3] = -INFINITY;
+            }
 
         // The value scales: the largest's exponent, and all of them over 2^D.
         uint4_t scale[NB];
-        bool scaled = true;  // whether any is other than one
         int grown = exponent;
+        constexpr bool kScaled = F != kF16 && !PARTED;
+        if (kScaled || F == kF16 || spoilt) {
 #pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) scale[b] = source.value_scale(b);
+            for (uint32_t b = 0; b < NB; ++b) scale[b] = source.value_scale(b);
+        }
         if constexpr (F == kF16) {
             uint32_t other = 0;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) other |= scale[b][w] ^ 0x3C003C00u;
-            scaled = __any(other != 0);
-            grown = 0;
-        } else {
+            spoilt = __any(other != 0);
+        }
+        if constexpr (kScaled) {
             ushort2_t top = {0, 0};
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
@@ -391,28 +432,28 @@ struct Rows {
                     const uint32_t size = F == kQ4_0 ? scale[b][w] & 0x7FFF7FFFu : scale[b][w];
                     top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
                 }
-            uint32_t most = max(top.x, top.y);
-            if (__any(most > 0x7C00u)) {  // a NaN scale spoils the rows that see it, no other
-                most = 0;
-#pragma unroll
-                for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t lo = scale[b][w] & 0x7FFFu, hi = scale[b][w] >> 16 & 0x7FFFu;
-                        most = max(most, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
-                    }
-            }
-            // the same in a group's 16 lanes; 2^grown <= the scale < 2^(grown + 1); subnormals count as the least normal
-            most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
-                       max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
-            grown = max(exponent, static_cast<int>(max(most >> 10, 1u)) - 15);
-            const _Float16 down = static_cast<_Float16>(ldexpf(1.0f, -grown));
-            const half2_t by = {down, down};
+            spoilt = __any(max(top.x, top.y) > 0x7C00);
+        }
+        if (spoilt) spoil(a, group, tree, slot0, masked, scale);
+        if constexpr (kScaled) {
+            ushort2_t top = {0, 0};
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    scale[b][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][w]) * by);
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t size = F == kQ4_0 ? scale[b][w] & 0x7FFF7FFFu : scale[b][w];
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
+                }
+            // the same in a group's 16 lanes
+            const uint32_t mine = max(top.x, top.y);
+            const uint32_t most = max(max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 16)),
+                                      max(__builtin_amdgcn_readlane(mine, 32), __builtin_amdgcn_readlane(mine, 48)));
+            grown = max(exponent, exponent_of(most));
+            const half2_t by = over(grown);
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) scale[b][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][w]) * by);
         }
 
 #pragma unroll
@@ -444,20 +485,23 @@ struct Rows {
             const float to = largest[i] == -INFINITY ? 0.0f : offset[i];
             float p[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], unit[i], to));
-                sum[i] += p[e];
-            }
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], unit[i], to));
+            sum[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
             for (int e = 0; e < 4; ++e) split2(p[2 * e], p[2 * e + 1], &hi[i][e], &lo[i][e]);
         }
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            const half8_t v[2] = {source.value(b, 0), source.value(b, 1)};
+            half8_t v[2], v_low[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                v[u] = source.value(b, u);
+                if constexpr (PARTED && F != kF16) v_low[u] = source.value_low(b, u);
+            }
 #pragma unroll
             for (uint32_t i = 0; i < RT; ++i) {
                 half8_t x, y;
-                if (F == kF16 && !scaled) {
+                if constexpr (!kScaled) {
                     x = join(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
                     y = join(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
                 } else {
@@ -466,8 +510,7 @@ struct Rows {
                     half2_t u[4], w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        // a scale that the row does not see may be a NaN
-                        const half2_t d = pair_of(scale[b][e] & seen[i][e]);
+                        const half2_t d = pair_of(scale[b][e]);
                         u[e] = hi[i][e] * d;
                         w[e] = __builtin_elementwise_fma(lo[i][e], d, __builtin_elementwise_fma(hi[i][e], d, -u[e]));
                     }
@@ -476,16 +519,43 @@ struct Rows {
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    out[i][2 * b + u] = multiply(v[u], x, out[i][2 * b + u]);
-                    out[i][2 * b + u] = multiply(v[u], y, out[i][2 * b + u]);
+                    float4_t& to = out[i][2 * b + u];
+                    to = multiply(v[u], x, to);
+                    to = multiply(v[u], y, to);
+                    if constexpr (PARTED && F != kF16) to = multiply(v_low[u], x, to);
                 }
             }
         }
     }
 
-    // The last tile is done: the outputs, held over 2^D, as the sum is.
+    // A tile with value scales that are NaNs: a row that sees such a token gets
+    // NaNs in its block, and the scale becomes 0, for the rows that do not.
+    template <typename TREE>
+    __device__ __forceinline__ void spoil(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
+                                                    bool masked, uint4_t (&scale)[NB]) {
+        const uint32_t g = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            uint32_t nans = 0;  // a bit a slot of the lane's eight
+#pragma unroll
+            for (int e = 0; e < 8; ++e) nans |= (scale[b][e >> 1] >> (16 * (e & 1)) & 0x7FFFu) > 0x7C00u ? 1u << e : 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < RT; ++i) {
+                const uint32_t bits = (masked ? sees(a, group, tree, slot0, i) : 0xFFFFFFFFu) >> (4 * g);
+                const float mine = nans & ((bits & 15u) | (bits >> 12 & 0xF0u)) ? 1.0f : 0.0f;
+                const float nan = most_of_row(mine) > 0.0f ? __builtin_nanf("") : 0.0f;
+                out[i][2 * b] += nan;
+                out[i][2 * b + 1] += nan;
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                scale[b][w] &= (nans >> (2 * w) & 1u ? 0u : 0xFFFFu) | (nans >> (2 * w + 1) & 1u ? 0u : 0xFFFF0000u);
+        }
+    }
+
+    // The last tile is done: the outputs, held over 2^(D - kScaleTop), as the sum is.
     __device__ __forceinline__ void end() {
-        const float up = ldexpf(1.0f, exponent);
+        const float up = ldexpf(1.0f, exponent - kScaleTop);
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i)
 #pragma unroll
@@ -598,12 +668,6 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15u, g = lane >> 4;
     const Group group(a, kRows);
-    typename Rows<F, NB, RT>::Queries queries;
-    Rows<F, NB, RT>::fetch(a, group, group.row0, queries);
-    if (a.parents)
-        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
-                  group.token_end - group.token0, a.window);
-
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
     uint8_t* ring = space + wave * (D * kRecord);
     const uint32_t first = group.tile_begin + wave;
@@ -611,13 +675,19 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
     auto copy = [&](uint32_t j) {
         copy_record<kRecord>(base + static_cast<uint64_t>(first + j * W) * kRecord, ring + j % D * kRecord);
     };
-    Rows<F, NB, RT> rows;
-    rows.begin(a, group, tree, group.row0, queries);
-    // only the copies are on their way from here on
-    wait_loads<0>();
+    // The first copies go out before anything that the rows wait for.
 #pragma unroll
     for (uint32_t j = 0; j + 1 < D; ++j)
         if (j < count) copy(j);
+    typename Rows<F, NB, RT>::Queries queries;
+    Rows<F, NB, RT>::fetch(a, group, group.row0, queries);
+    if (a.parents)
+        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                  group.token_end - group.token0, a.window);
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, group.row0, queries);
+    // Only copies are on their way from here on: the queries' own loads, the
+    // youngest, have been waited for.
     for (uint32_t j = 0; j < count; ++j) {
         // tile j + D - 1 into the place of tile j - 1, whose reads are done
         if (j + D - 1 < count) {
@@ -627,7 +697,8 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
             wait_loads<0>();
         }
         const uint32_t slot0 = (first + j * W) * kTile;
-        rows.tile(a, group, tree, slot0, Record<F, NB>{ring + j % D * kRecord, slot0, group.latest});
+        const Record<F, NB> record{ring + j % D * kRecord, slot0, group.latest};
+        rows.template tile<false>(a, group, tree, slot0, record);
         __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");  // the record's reads, before its place is copied to
     }
     rows.end();
@@ -674,34 +745,37 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
 
 // ---- many rows: the waves split the rows -------------------------------------------
 
-// A stage: kStage tiles' codes as binary16 operands, and their scales, in LDS,
-// laid out by the workgroup for all of its waves.
-template <uint32_t NB>
-constexpr uint32_t stage_tiles() {
-    return NB <= 4 ? 2 : 1;
-}
-
-template <uint32_t NB>
+// A tile laid out in LDS by the workgroup for all of its waves: the codes as
+// binary16 operands, the values' scaled, in two parts (the product of a code
+// and a scale is exact in them), so that a wave does no more than read them.
+// (A NaN among the scales, which is not every row's, goes in as 0: Rows::spoil.)
+template <uint32_t F, uint32_t NB>
 struct Stage {
-    half8_t keys[2 * NB][64], values[2 * NB][64];  // [2 b + h], [2 b + u]
+    half8_t keys[2 * NB][64], values[2 * NB][64];    // [2 b + h], [2 b + u]
+    half8_t values_low[F == kF16 ? 1 : 2 * NB][64];  // (F16's are exact in one)
     uint4_t key_scales_[NB][4], value_scales_[NB][4];
 
     __device__ __forceinline__ half8_t key(uint32_t b, int h) const { return keys[2 * b + h][threadIdx.x & 63u]; }
     __device__ __forceinline__ half8_t value(uint32_t b, int u) const { return values[2 * b + u][threadIdx.x & 63u]; }
+    __device__ __forceinline__ half8_t value_low(uint32_t b, int u) const { return values_low[2 * b + u][threadIdx.x & 63u]; }
     __device__ __forceinline__ uint4_t key_scale(uint32_t b) const { return key_scales_[b][(threadIdx.x & 63u) >> 4]; }
     __device__ __forceinline__ uint4_t value_scale(uint32_t b) const { return value_scales_[b][(threadIdx.x & 63u) >> 4]; }
 };
 
-template <uint32_t F, uint32_t NB, uint32_t RT, uint32_t W>
-__global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
-    constexpr uint32_t kRows = 16 * RT * W, kRecord = cache_record(F, NB), kTiles = stage_tiles<NB>();
+constexpr uint32_t kRowWaves = 8;
+
+template <uint32_t F, uint32_t NB, uint32_t RT>
+__global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
+    constexpr uint32_t W = kRowWaves, kRows = 16 * RT * W, kRecord = cache_record(F, NB);
+    constexpr uint32_t kTiles = NB <= 4 ? 2 : 1;                                // a stage's
     constexpr uint32_t kUnits = 2 * NB * kTiles, kMine = (kUnits + W - 1) / W;  // units of a stage; a wave's, at most
     constexpr uint32_t kScaleWords = (key_scales(F) ? 32 : 16) * NB;            // a tile's
     static_assert(kScaleWords * kTiles <= 64 * W, "a thread a dword");
     __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
-    __shared__ Stage<NB> stages[2][kTiles];
+    __shared__ Stage<F, NB> stages[2][kTiles];
+    __shared__ uint32_t wave_most[W], wave_spoilt[W];
 
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Group group(a, kRows);
     const uint32_t row0 = group.row0 + 16 * RT * wave;
     const bool mine = row0 < group.row_end;  // a wave without rows still lays out its share
@@ -710,41 +784,102 @@ __global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
     // a chain's wave sees nothing past its last row's token
     const uint32_t sees_to =
         a.parents ? group.latest : group.past + (min(row0 + 16 * RT, group.row_end) - 1) / a.group + 1;
-
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
-    Codes<F> codes[kMine];
-    uint32_t scale_word = 0;
+
+    // All the tiles' value scales, once: their largest exponent, and whether any is a NaN (F16: other than one).
+    uint32_t most = 0, spoilt = 0;
+#pragma unroll 4
+    for (uint32_t x = threadIdx.x; x < (group.tile_end - group.tile_begin) * 16 * NB; x += 64 * W) {
+        const uint32_t t = group.tile_begin + x / (16 * NB), w = x % (16 * NB);
+        const uint32_t word = kept_scale<F>(
+            reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord + value_scales_at(F, NB))[w],
+            kept_of(t * kTile, w / 4 & 3u, w & 3u, group.latest));
+        most = max(most, larger_scale(word));
+        spoilt |= F == kF16 ? word ^ 0x3C003C00u
+                            : static_cast<uint32_t>((word & 0x7FFFu) > 0x7C00u || (word & 0x7FFF0000u) > 0x7C000000u);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o)));
+    spoilt = __any(spoilt != 0);
+    if (lane == 0) wave_most[wave] = most, wave_spoilt[wave] = spoilt;
+    if (a.parents)
+        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                  group.token_end - group.token0, a.window);
+    __syncthreads();
+    most = spoilt = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) most = max(most, wave_most[w]), spoilt |= wave_spoilt[w];
+    spoilt = __builtin_amdgcn_readfirstlane(spoilt);
+    const int exponent = F == kF16 ? kScaleTop : exponent_of(__builtin_amdgcn_readfirstlane(most));
+    const half2_t by = over(exponent);
+
+    Rows<F, NB, RT> rows;
+    rows.begin(a, group, tree, min(row0, group.row_end - 1), queries);
+    rows.exponent = exponent;
+
     // Unit u of a stage: tile u / 2NB, block u % NB, keys then values.
+    Codes<F> codes[kMine];
+    uint4_t unit_scale[kMine];  // a value unit's
+    uint32_t scale_word = 0;    // of those that the waves read
     auto load = [&](uint32_t tile0) {
 #pragma unroll
         for (uint32_t j = 0; j < kMine; ++j) {
             const uint32_t u = wave + W * j, t = tile0 + u / (2 * NB);
-            if (u < kUnits && t < group.tile_end)
-                codes[j] = load_codes<F>(base + static_cast<uint64_t>(t) * kRecord + u % (2 * NB) * cache_unit(F), lane);
+            if (u >= kUnits || t >= group.tile_end) continue;
+            const uint8_t* record = base + static_cast<uint64_t>(t) * kRecord;
+            codes[j] = load_codes<F>(record + u % (2 * NB) * cache_unit(F), lane);
+            if (F != kF16 && u % (2 * NB) >= NB)
+                unit_scale[j] = *reinterpret_cast<const uint4_t*>(record + value_scales_at(F, NB) + 64 * (u % NB) + 16 * (lane >> 4));
         }
         const uint32_t t = tile0 + threadIdx.x / kScaleWords;
         if (threadIdx.x < kScaleWords * kTiles && t < group.tile_end)
             scale_word = reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord +
                                                            key_scales_at(F, NB))[threadIdx.x % kScaleWords];
     };
-    auto lay = [&](uint32_t tile0, Stage<NB>* stage) {
+    auto lay = [&](uint32_t tile0, Stage<F, NB>* stage) {
 #pragma unroll
         for (uint32_t j = 0; j < kMine; ++j) {
-            const uint32_t u = wave + W * j, t = u / (2 * NB), b = u % NB;
+            const uint32_t u = wave + W * j, t = u / (2 * NB), b = u % NB, slot0 = (tile0 + t) * kTile;
             if (u >= kUnits || tile0 + t >= group.tile_end) continue;
             if (u % (2 * NB) < NB) {
                 stage[t].keys[2 * b][lane] = operand<F, false>(codes[j], 0);
                 stage[t].keys[2 * b + 1][lane] = operand<F, false>(codes[j], 1);
-            } else {
-                if constexpr (F == kF16)
-                    if ((tile0 + t) * kTile + kTile > group.latest)
+                continue;
+            }
+            // what lies past the last token is no one's, and may be anything
+            if (slot0 + kTile > group.latest)
 #pragma unroll
-                        for (uint32_t w = 0; w < 4; ++w) {
-                            const uint32_t kept = kept_of((tile0 + t) * kTile, lane >> 4, w, group.latest);
-                            codes[j].w[w] &= kept, codes[j].w[4 + w] &= kept;
-                        }
-                stage[t].values[2 * b][lane] = operand<F, true>(codes[j], 0);
-                stage[t].values[2 * b + 1][lane] = operand<F, true>(codes[j], 1);
+                for (uint32_t w = 0; w < 4; ++w) {
+                    const uint32_t kept = kept_of(slot0, lane >> 4, w, group.latest);
+                    if constexpr (F == kF16)
+                        codes[j].w[w] &= kept, codes[j].w[4 + w] &= kept;
+                    else
+                        unit_scale[j][w] &= kept;
+                }
+            if (F != kF16 && spoilt)
+#pragma unroll
+                for (uint32_t w = 0; w < 4; ++w) {
+                    const uint32_t s = unit_scale[j][w];
+                    unit_scale[j][w] = ((s & 0x7FFFu) > 0x7C00u ? 0u : s & 0xFFFFu) |
+                                       ((s & 0x7FFF0000u) > 0x7C000000u ? 0u : s & 0xFFFF0000u);
+                }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                const half8_t code = operand<F, true>(codes[j], part);
+                half8_t high = code, low = {0, 0, 0, 0, 0, 0, 0, 0};
+                if constexpr (F != kF16) {
+                    half2_t hi[4], lo[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const half2_t c = {code[2 * w], code[2 * w + 1]}, d = pair_of(unit_scale[j][w]) * by;
+                        hi[w] = c * d;
+                        lo[w] = __builtin_elementwise_fma(c, d, -hi[w]);
+                    }
+                    high = join(hi[0], hi[1], hi[2], hi[3]);
+                    low = join(lo[0], lo[1], lo[2], lo[3]);
+                    stage[t].values_low[2 * b + part][lane] = low;
+                }
+                stage[t].values[2 * b + part][lane] = high;
             }
         }
         const uint32_t t = threadIdx.x / kScaleWords, w = threadIdx.x % kScaleWords;
@@ -756,24 +891,21 @@ __global__ __launch_bounds__(64 * W) void attend_rows(Attention a) {
             to[w % (16 * NB)] = scale_word;
         }
     };
-
-    if (group.tile_begin < group.tile_end) load(group.tile_begin);
-    if (a.parents)
-        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
-                  group.token_end - group.token0, a.window);
-    Rows<F, NB, RT> rows;
-    rows.begin(a, group, tree, min(row0, group.row_end - 1), queries);
-    if (group.tile_begin < group.tile_end) lay(group.tile_begin, stages[0]);
+    if (group.tile_begin < group.tile_end) {
+        load(group.tile_begin);
+        lay(group.tile_begin, stages[0]);
+    }
     __syncthreads();
     uint32_t turn = 0;
     for (uint32_t tile0 = group.tile_begin; tile0 < group.tile_end; tile0 += kTiles, turn ^= 1) {
         // the next stage's loads are in flight over this one's products
         const bool more = tile0 + kTiles < group.tile_end;
         if (more) load(tile0 + kTiles);
-#pragma unroll
+#pragma unroll 1
         for (uint32_t t = 0; t < kTiles; ++t) {
             const uint32_t slot0 = (tile0 + t) * kTile;
-            if (mine && tile0 + t < group.tile_end && slot0 < sees_to) rows.tile(a, group, tree, slot0, stages[turn][t]);
+            if (mine && tile0 + t < group.tile_end && slot0 < sees_to)
+                rows.template tile<true>(a, group, tree, slot0, stages[turn][t], spoilt != 0);
         }
         // the other stage was read before the last barrier
         if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
@@ -798,12 +930,8 @@ template <uint32_t F, uint32_t NB>
 static hipError_t launch_blocks(const Attention& a, const AttentionPlan& plan, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads * plan.row_groups * plan.splits);
     constexpr uint32_t kWide = NB <= 4 ? 2 : 1;  // 16-row tiles a wave's registers hold
-    if (plan.waves == 8)
-        hipLaunchKernelGGL((attend_rows<F, NB, kWide, 8>), grid, dim3(512), 0, stream, a);
-    else if (plan.waves == 4 && plan.row_tiles == kWide)
-        hipLaunchKernelGGL((attend_rows<F, NB, kWide, 4>), grid, dim3(256), 0, stream, a);
-    else if (plan.waves == 4)
-        hipLaunchKernelGGL((attend_rows<F, NB, 1, 4>), grid, dim3(256), 0, stream, a);
+    if (plan.waves > 1)
+        hipLaunchKernelGGL((attend_rows<F, NB, kWide>), grid, dim3(64 * kRowWaves), 0, stream, a);
     else if (plan.row_tiles == kWide)
         hipLaunchKernelGGL((attend<F, NB, kWide>), grid, dim3(64 * AttendShape<F, NB, kWide>::kWaves), 0, stream, a);
     else

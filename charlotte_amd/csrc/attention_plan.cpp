@@ -5,16 +5,16 @@
 
 namespace chm {
 
-// The least rows a workgroup that hold the step's, at most 128 to one whose
-// waves split its tiles; then splits until each compute unit has a workgroup
-// (two of attend_rows' four waves), of kLeast tiles at the least: shorter, a
-// second launch to join them costs more than it gains.
+// Up to 128 rows a key head take workgroups of 16 or 32 rows whose waves split
+// the tiles, more take eight waves of 32 (or 16) rows each; then splits until
+// each compute unit has a workgroup, of at least kLeast tiles, but one while
+// the tiles are few: the launch that joins them would cost more.
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units) {
     const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
     const uint32_t wide = cache.head_dim <= 128 ? 2 : 1;  // 16-row tiles a wave's registers hold
     AttentionPlan plan{};
-    plan.waves = rows <= 128 ? 1 : rows <= 64 * wide ? 4 : 8;
+    plan.waves = rows <= 128 ? 1 : 8;
     plan.row_tiles = rows <= 16 ? 1 : wide;
     const uint64_t group = 16ull * plan.row_tiles * plan.waves;
     plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
@@ -23,9 +23,9 @@ AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint
     if (window) reach = std::min<uint64_t>(reach, uint64_t{window} + tokens + 31);
     const uint64_t tiles = (reach + 31) / 32;
     const uint64_t wanted = compute_units / workgroups;
-    constexpr uint64_t kLeast = 8;
+    constexpr uint64_t kLeast = 4, kOne = 16;
     plan.splits = static_cast<uint32_t>(
-        tiles <= 32 ? 1 : std::max<uint64_t>(1, std::min(wanted, (tiles + kLeast - 1) / kLeast)));
+        tiles <= kOne ? 1 : std::max<uint64_t>(1, std::min(wanted, (tiles + kLeast - 1) / kLeast)));
     return plan;
 }
 
