@@ -39,6 +39,8 @@ namespace chm {
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
 typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
@@ -49,30 +51,6 @@ constexpr float kLog2E = 1.44269504088896340736f;
 // product stays below 2^15 (a half ends at 2^16).
 constexpr int kHeadroom = 7, kScaleTop = 3;
 constexpr float kSlack = 4.0f;
-
-// A lane's codes of one unit (keys or values of a block by 32 tokens).
-template <uint32_t F>
-struct Codes {
-    uint32_t w[F == kQ8_0 ? 4 : F == kQ4_0 ? 2 : 8];
-};
-
-template <uint32_t F>
-__device__ __forceinline__ Codes<F> load_codes(const uint8_t* unit, uint32_t lane) {
-    Codes<F> c;
-    if constexpr (F == kQ8_0) {
-        const uint4 v = *reinterpret_cast<const uint4*>(unit + 16 * lane);
-        c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
-    } else if constexpr (F == kQ4_0) {
-        const uint2 v = *reinterpret_cast<const uint2*>(unit + 8 * lane);
-        c.w[0] = v.x, c.w[1] = v.y;
-    } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(unit + 16 * lane);
-        const uint4 u = *reinterpret_cast<const uint4*>(unit + 1024 + 16 * lane);
-        c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
-        c.w[4] = u.x, c.w[5] = u.y, c.w[6] = u.z, c.w[7] = u.w;
-    }
-    return c;
-}
 
 // Four unsigned bytes, each raised by `raise`, as halves: under the high byte
 // 0x64 a byte c is 1,024 + c in binary16, and taking 1,024 + raise is exact.
@@ -86,32 +64,38 @@ __device__ __forceinline__ void halves_of(uint32_t bytes, half2_t* low, half2_t*
 __device__ __forceinline__ half8_t join(half2_t a, half2_t b, half2_t c, half2_t d) {
     return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
+template <int RAISE>
+__device__ __forceinline__ half8_t halves_of(uint32_t first, uint32_t second) {
+    half2_t a, b, c, d;
+    halves_of<RAISE>(first, &a, &b);
+    halves_of<RAISE>(second, &c, &d);
+    return join(a, b, c, d);
+}
 
-// The lane's operand of a key unit's token half h, or of a value unit's 16
-// values u (cache.hpp).
+// Eight codes as an operand: of lane `from` of a unit as cache.hpp lays it
+// out, for the keys those of token half `part`, for the values those of value
+// 16 part + from % 16.
 template <uint32_t F, bool VALUES>
-__device__ __forceinline__ half8_t operand(const Codes<F>& c, int part) {
+__device__ __forceinline__ half8_t operand(const uint8_t* unit, uint32_t from, uint32_t part) {
     if constexpr (F == kF16) {
-        const uint4_t w = {c.w[4 * part], c.w[4 * part + 1], c.w[4 * part + 2], c.w[4 * part + 3]};
-        return __builtin_bit_cast(half8_t, w);
+        return *reinterpret_cast<const half8_t*>(unit + 1024 * part + 16 * from);
+    } else if constexpr (F == kQ8_0) {
+        const uint2 w = *reinterpret_cast<const uint2*>(unit + 16 * from + 8 * part);
+        return halves_of<128>(w.x, w.y);
+    } else if constexpr (VALUES) {
+        const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * from);
+        return halves_of<8>(w.x >> (4 * part) & 0x0F0F0F0Fu, w.y >> (4 * part) & 0x0F0F0F0Fu);
     } else {
-        half2_t a, b, d, e;
-        if constexpr (F == kQ8_0) {
-            halves_of<128>(c.w[2 * part], &a, &b);
-            halves_of<128>(c.w[2 * part + 1], &d, &e);
-        } else if constexpr (VALUES) {
-            halves_of<8>(c.w[0] >> (4 * part) & 0x0F0F0F0Fu, &a, &b);
-            halves_of<8>(c.w[1] >> (4 * part) & 0x0F0F0F0Fu, &d, &e);
-        } else {
-            halves_of<8>(c.w[part] & 0x0F0F0F0Fu, &a, &b);
-            halves_of<8>(c.w[part] >> 4 & 0x0F0F0F0Fu, &d, &e);
-        }
-        return join(a, b, d, e);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(unit + 8 * from + 4 * part);
+        return halves_of<8>(w & 0x0F0F0F0Fu, w >> 4 & 0x0F0F0F0Fu);
     }
 }
 
 __device__ __forceinline__ float4_t multiply(half8_t a, half8_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16_t multiply(half8_t a, half8_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
 // A dword's two halves, the dword passed by value: a bit cast straight from a
@@ -125,9 +109,13 @@ __device__ __forceinline__ float scale_at(const uint4_t& s, int i) { return stat
 // rounded to nearest (lo's bias, were it cut, would be every probability's):
 // within 2^-22 of the value, or 2^-25.
 __device__ __forceinline__ void split2(float a, float b, half2_t* hi, half2_t* lo) {
-    *hi = half2_t{static_cast<_Float16>(a), static_cast<_Float16>(b)};
-    *lo = half2_t{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi->x), -1.0f, a)),
-                  static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi->y), -1.0f, b))};
+    *hi = __builtin_convertvector((float2_t{a, b}), half2_t);
+    // a factor the compiler does not know keeps each difference one mixed-precision instruction
+    float minus = -1.0f;
+    __asm__("" : "+s"(minus));
+    *lo = __builtin_convertvector((float2_t{__builtin_fmaf(static_cast<float>(hi->x), minus, a),
+                                            __builtin_fmaf(static_cast<float>(hi->y), minus, b)}),
+                                  half2_t);
 }
 
 // The larger of two scales' magnitudes as bits, a NaN's as none.
@@ -143,17 +131,23 @@ __device__ __forceinline__ half2_t over(int exponent) {
     return half2_t{by, by};
 }
 
-// Over the four lanes that share a row (lane % 16).
+// Over the lanes that share a row: lane % 16, four of them, or lane % 32, two.
+template <uint32_t X>
 __device__ __forceinline__ float most_of_row(float x) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    if constexpr (X == 1) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+template <uint32_t X>
 __device__ __forceinline__ float sum_of_row(float x) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    if constexpr (X == 1) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
@@ -258,96 +252,125 @@ struct Group {
     __device__ __forceinline__ bool masked(uint32_t slot0) const { return slot0 + kTile > past || slot0 < all_begin; }
 };
 
-// A wave's RT x 16 rows as they go over the tiles: lane 16g + n holds, of rows
-// n, 16 + n, ..., the queries' operands and the outputs' values 4g .. 4g + 3 of
-// each 16.
-template <uint32_t F, uint32_t NB, uint32_t RT>
-struct Rows {
-    half8_t high[RT][NB], low[RT][NB];
-    float unit[RT];                          // what a raw score stands for, a power of two
-    float4_t out[RT][2 * NB];
-    float largest[RT], offset[RT], sum[RT];  // the raw maximum; exp2's offset; the lane's part of the sum
-    int exponent;                            // D, the same in every lane
-    Sight sight[RT];
+// A wave's 16 X rows as they go over the tiles. X = 1: the 16 x 16 x 32
+// instruction, lane 16g + n row n, its eight tokens those of group g. X = 2: the
+// 32 x 32 x 16 one, which does twice the work in little more time; lane 32f + n
+// row n, its 16 tokens those of groups f and 2 + f, octets 0 and 1. That takes
+// the keys' rows in the order of their slots: row 16 (g / 2) + 8h + 4 (g % 2) + r
+// is token 16h + 4g + r, so that a result's octet is a group's eight slots in
+// the record's order, and they are the operands along the next sum, 16 tokens
+// an instruction.
+template <uint32_t X>
+__device__ __forceinline__ uint32_t group_of(uint32_t octet) {
+    const uint32_t lane = threadIdx.x & 63u;
+    return X == 1 ? lane >> 4 : 2 * octet + (lane >> 5);
+}
 
-    // The queries' loads alone, ahead of what the rows wait for: a lane's
-    // values 8g .. 8g + 7 of each block. Rows past the group's end repeat its last.
+template <uint32_t X>
+struct Result {
+    typedef float4_t type;
+};
+template <>
+struct Result<2> {
+    typedef float16_t type;
+};
+
+template <uint32_t F, uint32_t NB, uint32_t X>
+struct Rows {
+    typedef typename Result<X>::type result_t;
+    static constexpr uint32_t kOuts = X == 1 ? 2 * NB : NB;    // results: 16 values of 16 rows, or 32 of 32
+    static constexpr uint32_t kQuads = X == 1 ? 2 * NB : 4 * NB;  // a lane's runs of four values
+
+    half8_t high[NB * X], low[NB * X];  // the queries
+    float unit;                         // what a raw score stands for, a power of two
+    result_t out[kOuts];
+    float largest, offset, sum;         // the raw maximum; exp2's offset; the lane's part of the sum
+    int exponent;                       // D, the same in every lane
+    Sight sight;
+
+    // Where a lane's run of four output values stands in its row.
+    __device__ __forceinline__ static uint32_t quad_at(uint32_t quad) {
+        const uint32_t lane = threadIdx.x & 63u;
+        return X == 1 ? 16 * quad + 4 * (lane >> 4) : 8 * quad + 4 * (lane >> 5);
+    }
+    __device__ __forceinline__ float4_t quad(uint32_t q) const {
+        if constexpr (X == 1) {
+            return out[q];
+        } else {
+            const uint32_t r = 4 * (q & 3u);
+            return float4_t{out[q >> 2][r], out[q >> 2][r + 1], out[q >> 2][r + 2], out[q >> 2][r + 3]};
+        }
+    }
+
+    // The queries' loads alone, ahead of what the rows wait for: eight values an
+    // operand. Rows past the group's end repeat its last.
     struct Queries {
-        float x[RT][NB][8];
+        float x[NB * X][8];
     };
     __device__ __forceinline__ static void fetch(const Attention& a, const Group& group, uint32_t row0, Queries& q) {
-        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+        const uint32_t lane = threadIdx.x & 63u, n = lane % (16 * X);
+        const uint32_t inside = min(row0 + n, group.row_end - 1);
+        const float* from = a.queries +
+                            (static_cast<uint64_t>(group.sequence) * a.tokens + inside / a.group) * a.query_stride +
+                            static_cast<uint64_t>(group.head * a.group + inside % a.group) * (32 * NB) + 8 * (lane / (16 * X));
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            const uint32_t inside = min(row0 + 16 * i + n, group.row_end - 1);
-            const float* from = a.queries +
-                                (static_cast<uint64_t>(group.sequence) * a.tokens + inside / a.group) * a.query_stride +
-                                static_cast<uint64_t>(group.head * a.group + inside % a.group) * (32 * NB) + 8 * g;
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const float4 u = *reinterpret_cast<const float4*>(from + 32 * b);
-                const float4 v = *reinterpret_cast<const float4*>(from + 32 * b + 4);
-                q.x[i][b][0] = u.x, q.x[i][b][1] = u.y, q.x[i][b][2] = u.z, q.x[i][b][3] = u.w;
-                q.x[i][b][4] = v.x, q.x[i][b][5] = v.y, q.x[i][b][6] = v.z, q.x[i][b][7] = v.w;
-            }
+        for (uint32_t b = 0; b < NB * X; ++b) {
+            const float4 u = *reinterpret_cast<const float4*>(from + 32 / X * b);
+            const float4 v = *reinterpret_cast<const float4*>(from + 32 / X * b + 4);
+            q.x[b][0] = u.x, q.x[b][1] = u.y, q.x[b][2] = u.z, q.x[b][3] = u.w;
+            q.x[b][4] = v.x, q.x[b][5] = v.y, q.x[b][6] = v.z, q.x[b][7] = v.w;
         }
     }
 
     template <typename TREE>
     __device__ __forceinline__ void begin(const Attention& a, const Group& group, const TREE& tree, uint32_t row0,
                                           Queries& q) {
-        const uint32_t lane = threadIdx.x & 63u, n = lane & 15u;
-        exponent = F == kF16 ? kScaleTop : -64;
-#pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            const uint32_t row = row0 + 16 * i + n;
-            const uint32_t token = min(row, group.row_end - 1) / a.group;
-            const uint32_t depth = a.parents ? tree.depth[token - group.token0] : token;
-            sight[i].live = row < group.row_end && depth != kUnused;
-            const uint32_t place = group.past + (depth != kUnused ? depth : 0u) + 1;  // one past its own place
-            sight[i].first = a.window && place > a.window ? place - a.window : 0u;
-            sight[i].last = a.parents ? token - group.token0 : group.past + token;
+        const uint32_t row = row0 + (threadIdx.x & 63u) % (16 * X);
+        const uint32_t token = min(row, group.row_end - 1) / a.group;
+        const uint32_t depth = a.parents ? tree.depth[token - group.token0] : token;
+        sight.live = row < group.row_end && depth != kUnused;
+        const uint32_t place = group.past + (depth != kUnused ? depth : 0u) + 1;  // one past its own place
+        sight.first = a.window && place > a.window ? place - a.window : 0u;
+        sight.last = a.parents ? token - group.token0 : group.past + token;
 
-            float most = 0.0f;
+        float most = 0.0f;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
+        for (uint32_t b = 0; b < NB * X; ++b)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    q.x[i][b][e] *= a.scale * kLog2E, most = fmaxf(most, fabsf(q.x[i][b][e]));
-            most = most_of_row(most);
-            int shift = 0;
-            if (most > 0.0f && most <= 3.4e38f) {
-                int e;
-                (void)frexpf(most, &e);
-                shift = min(11 - e, 126);
-            }
-            unit[i] = ldexpf(1.0f, -shift);
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                half2_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    split2(ldexpf(q.x[i][b][2 * e], shift), ldexpf(q.x[i][b][2 * e + 1], shift), &hi[e], &lo[e]);
-                high[i][b] = join(hi[0], hi[1], hi[2], hi[3]);
-                low[i][b] = join(lo[0], lo[1], lo[2], lo[3]);
-            }
-            largest[i] = -INFINITY, offset[i] = INFINITY, sum[i] = 0.0f;
-#pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = 0; e < 8; ++e) q.x[b][e] *= a.scale * kLog2E, most = fmaxf(most, fabsf(q.x[b][e]));
+        most = most_of_row<X>(most);
+        int shift = 0;
+        if (most > 0.0f && most <= 3.4e38f) {
+            int e;
+            (void)frexpf(most, &e);
+            shift = min(11 - e, 126);
         }
+        unit = ldexpf(1.0f, -shift);
+#pragma unroll
+        for (uint32_t b = 0; b < NB * X; ++b) {
+            half2_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                split2(ldexpf(q.x[b][2 * e], shift), ldexpf(q.x[b][2 * e + 1], shift), &hi[e], &lo[e]);
+            high[b] = join(hi[0], hi[1], hi[2], hi[3]);
+            low[b] = join(lo[0], lo[1], lo[2], lo[3]);
+        }
+        exponent = F == kF16 ? kScaleTop : -64;
+        largest = -INFINITY, offset = INFINITY, sum = 0.0f;
+#pragma unroll
+        for (uint32_t t = 0; t < kOuts; ++t) out[t] = result_t(0.0f);
     }
 
-    // The slots of the tile at slot0 that row i of the lane sees, as bits.
+    // The slots of the tile at slot0 that the lane's row sees, as bits.
     template <typename TREE>
-    __device__ __forceinline__ uint32_t sees(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
-                                             uint32_t i) const {
+    __device__ __forceinline__ uint32_t sees(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0) const {
         const int64_t at = slot0;
-        if (!a.parents) return bits_between(sight[i].first - at, static_cast<int64_t>(sight[i].last) + 1 - at);
-        uint32_t seen = bits_between(sight[i].first - at, group.past - at);
+        if (!a.parents) return bits_between(sight.first - at, static_cast<int64_t>(sight.last) + 1 - at);
+        uint32_t seen = bits_between(sight.first - at, group.past - at);
         if (slot0 + kTile > group.past) {
             // the tree's tokens from `node` on: two words of the row's bits, shifted
             const int32_t node = static_cast<int32_t>(slot0 - group.past);
-            const uint32_t* above = tree.above[sight[i].last];
+            const uint32_t* above = tree.above[sight.last];
             uint64_t words = 0;
             if (node < 0) {
                 words = static_cast<uint64_t>(above[0]) << -node;
@@ -361,195 +384,219 @@ struct Rows {
         }
         return seen;
     }
+    // Those of an octet, a bit a slot of its eight.
+    __device__ __forceinline__ static uint32_t octet_bits(uint32_t seen, uint32_t octet) {
+        const uint32_t bits = seen >> (4 * group_of<X>(octet));
+        return (bits & 15u) | (bits >> 12 & 0xF0u);
+    }
 
-    // One tile. `source` gives the operands: key(b, h), key_scale(b), value(b, u),
-    // value_scale(b); and, PARTED, value_low(b, u), the values being scaled (over
-    // 2^D by 2^kScaleTop) and in two parts of their own: their scales are then
-    // looked at only where `spoilt`, some of them a NaN, stands.
+    // One tile. `source` gives the operands: keys(b, i) and values(b, i), i = 0, 1
+    // (X = 1: token half, 16 values; X = 2: 16 dims, 16 tokens), and an octet's
+    // scales, key_scale(b, x) and value_scale(b, x); and, PARTED, values_low(b, i),
+    // the values being scaled (over 2^D by 2^kScaleTop) and in two parts of their
+    // own: their scales are then looked at only where `spoilt`, some a NaN, stands.
     template <bool PARTED, typename SOURCE, typename TREE>
     __device__ __forceinline__ void tile(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
                                          const SOURCE& source, bool spoilt = false) {
-        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
-        // Scores: s[i][h][r] of token 16h + 4g + r.
-        float4_t s[RT][2];
+        float s[X][8];
+        if constexpr (X == 1) {
+            float4_t sums[2] = {float4_t(0.0f), float4_t(0.0f)};
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) s[i][0] = s[i][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t b = 0; b < NB; ++b) {
+                uint4_t scale;
+                if constexpr (key_scales(F)) scale = source.key_scale(b, 0);
 #pragma unroll
-        for (uint32_t b = 0; b < NB; ++b) {
-            uint4_t scale;
-            if constexpr (key_scales(F)) scale = source.key_scale(b);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const half8_t k = source.key(b, h);
-#pragma unroll
-                for (uint32_t i = 0; i < RT; ++i) {
+                for (int h = 0; h < 2; ++h) {
+                    const half8_t k = source.keys(b, h);
                     if constexpr (key_scales(F)) {
-                        float4_t p = multiply(k, high[i][b], float4_t{0.0f, 0.0f, 0.0f, 0.0f});
-                        p = multiply(k, low[i][b], p);
+                        const float4_t p = multiply(k, low[b], multiply(k, high[b], float4_t(0.0f)));
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            s[i][h][r] = __builtin_fmaf(p[r], scale_at(scale, 4 * h + r), s[i][h][r]);
+                        for (int r = 0; r < 4; ++r) sums[h][r] = __builtin_fmaf(p[r], scale_at(scale, 4 * h + r), sums[h][r]);
                     } else {
-                        s[i][h] = multiply(k, high[i][b], s[i][h]);
-                        s[i][h] = multiply(k, low[i][b], s[i][h]);
+                        sums[h] = multiply(k, low[b], multiply(k, high[b], sums[h]));
                     }
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[0][e] = sums[e >> 2][e & 3];
+        } else {
+            float16_t sums = float16_t(0.0f);
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                float16_t p = key_scales(F) ? float16_t(0.0f) : sums;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const half8_t k = source.keys(b, y);
+                    p = multiply(k, low[2 * b + y], multiply(k, high[2 * b + y], p));
+                }
+                if constexpr (key_scales(F)) {
+#pragma unroll
+                    for (uint32_t x = 0; x < 2; ++x) {
+                        const uint4_t scale = source.key_scale(b, x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            sums[8 * x + e] = __builtin_fmaf(p[8 * x + e], scale_at(scale, e), sums[8 * x + e]);
+                    }
+                } else {
+                    sums = p;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e >> 3][e & 7] = sums[e];
         }
 
         const bool masked = group.masked(slot0);
-        if (masked)
+        if (masked) {
+            const uint32_t seen = sees(a, group, tree, slot0);
 #pragma unroll
-            for (uint32_t i = 0; i < RT; ++i) {
-                const uint32_t bits = sees(a, group, tree, slot0, i) >> (4 * g);
+            for (uint32_t x = 0; x < X; ++x) {
+                const uint32_t bits = octet_bits(seen, x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (!(bits >> ((e >> 2) * 16 + (e & 3)) & 1u)) s[i][e >> 2][e & 3] = -INFINITY;
+                    if (!(bits >> e & 1u)) s[x][e] = -INFINITY;
             }
+        }
 
         // The value scales: the largest's exponent, and all of them over 2^D.
-        uint4_t scale[NB];
+        uint4_t scale[NB][X];
         int grown = exponent;
         constexpr bool kScaled = F != kF16 && !PARTED;
         if (kScaled || F == kF16 || spoilt) {
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) scale[b] = source.value_scale(b);
+            for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                for (uint32_t x = 0; x < X; ++x) scale[b][x] = source.value_scale(b, x);
         }
         if constexpr (F == kF16) {
             uint32_t other = 0;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) other |= scale[b][w] ^ 0x3C003C00u;
+                for (uint32_t x = 0; x < X; ++x)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) other |= scale[b][x][w] ^ 0x3C003C00u;
             spoilt = __any(other != 0);
         }
-        if constexpr (kScaled) {
-            ushort2_t top = {0, 0};
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t size = F == kQ4_0 ? scale[b][w] & 0x7FFF7FFFu : scale[b][w];
-                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
-                }
-            spoilt = __any(max(top.x, top.y) > 0x7C00);
-        }
+        if constexpr (kScaled) spoilt = __any(largest_scale(scale) > 0x7C00u);
         if (spoilt) spoil(a, group, tree, slot0, masked, scale);
         if constexpr (kScaled) {
-            ushort2_t top = {0, 0};
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t size = F == kQ4_0 ? scale[b][w] & 0x7FFF7FFFu : scale[b][w];
-                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
-                }
-            // the same in a group's 16 lanes
-            const uint32_t mine = max(top.x, top.y);
-            const uint32_t most = max(max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 16)),
-                                      max(__builtin_amdgcn_readlane(mine, 32), __builtin_amdgcn_readlane(mine, 48)));
+            // the same in the lanes of a group
+            const uint32_t mine = largest_scale(scale);
+            const uint32_t most = X == 1 ? max(max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 16)),
+                                               max(__builtin_amdgcn_readlane(mine, 32), __builtin_amdgcn_readlane(mine, 48)))
+                                         : max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 32));
             grown = max(exponent, exponent_of(most));
             const half2_t by = over(grown);
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) scale[b][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][w]) * by);
+                for (uint32_t x = 0; x < X; ++x)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) scale[b][x][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][x][w]) * by);
         }
 
+        float top = s[0][0];
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            float top = fmaxf(fmaxf(fmaxf(s[i][0][0], s[i][0][1]), fmaxf(s[i][0][2], s[i][0][3])),
-                              fmaxf(fmaxf(s[i][1][0], s[i][1][1]), fmaxf(s[i][1][2], s[i][1][3])));
-            top = most_of_row(top);
-            // the offset follows once a score passes it by kSlack (the first: -inf + inf is a NaN, no less than)
-            const bool follow = top > largest[i] && !((top - largest[i]) * unit[i] <= kSlack);
-            if (__any(follow) || grown != exponent) {
-                const float most = fmaxf(largest[i], top);
-                // the offset as used is what the factor is made of, so that its rounding cancels
-                const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit[i], static_cast<float>(kHeadroom));
-                const float factor = largest[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - offset[i]);
-                const float down = factor * ldexpf(1.0f, exponent - grown);
-                largest[i] = most;
-                offset[i] = to;
-                sum[i] *= factor;
+        for (int e = 1; e < 8 * static_cast<int>(X); ++e) top = fmaxf(top, s[e >> 3][e & 7]);
+        top = most_of_row<X>(top);
+        // the offset follows once a score passes it by kSlack (the first: -inf + inf is a NaN, no less than)
+        const bool follow = top > largest && !((top - largest) * unit <= kSlack);
+        if (__any(follow) || grown != exponent) {
+            const float most = fmaxf(largest, top);
+            // the offset as used is what the factor is made of, so that its rounding cancels
+            const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit, static_cast<float>(kHeadroom));
+            const float factor = largest == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - offset);
+            const float down = factor * ldexpf(1.0f, exponent - grown);
+            largest = most;
+            offset = to;
+            sum *= factor;
 #pragma unroll
-                for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= down;
-            }
+            for (uint32_t t = 0; t < kOuts; ++t) out[t] *= down;
         }
         exponent = grown;
 
-        half2_t hi[RT][4], lo[RT][4];
+        // rows that have seen nothing: -inf + inf would be a NaN
+        const float to = largest == -INFINITY ? 0.0f : offset;
+        half2_t hi[X][4], lo[X][4];
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            // rows that have seen nothing: -inf + inf would be a NaN
-            const float to = largest[i] == -INFINITY ? 0.0f : offset[i];
+        for (uint32_t x = 0; x < X; ++x) {
             float p[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], unit[i], to));
-            sum[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], unit, to));
+            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split2(p[2 * e], p[2 * e + 1], &hi[i][e], &lo[i][e]);
+            for (int e = 0; e < 4; ++e) split2(p[2 * e], p[2 * e + 1], &hi[x][e], &lo[x][e]);
         }
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            half8_t v[2], v_low[2];
+            half8_t first[X], second[X];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                v[u] = source.value(b, u);
-                if constexpr (PARTED && F != kF16) v_low[u] = source.value_low(b, u);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < RT; ++i) {
-                half8_t x, y;
+            for (uint32_t x = 0; x < X; ++x) {
                 if constexpr (!kScaled) {
-                    x = join(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
-                    y = join(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                    first[x] = join(hi[x][0], hi[x][1], hi[x][2], hi[x][3]);
+                    second[x] = join(lo[x][0], lo[x][1], lo[x][2], lo[x][3]);
                 } else {
                     // (hi + lo) d in two parts: hi d rounded, what that leaves
                     // (exact: 22 bits less their first 11) plus lo d
                     half2_t u[4], w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const half2_t d = pair_of(scale[b][e]);
-                        u[e] = hi[i][e] * d;
-                        w[e] = __builtin_elementwise_fma(lo[i][e], d, __builtin_elementwise_fma(hi[i][e], d, -u[e]));
+                        const half2_t d = pair_of(scale[b][x][e]);
+                        u[e] = hi[x][e] * d;
+                        w[e] = __builtin_elementwise_fma(lo[x][e], d, __builtin_elementwise_fma(hi[x][e], d, -u[e]));
                     }
-                    x = join(u[0], u[1], u[2], u[3]);
-                    y = join(w[0], w[1], w[2], w[3]);
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float4_t& to = out[i][2 * b + u];
-                    to = multiply(v[u], x, to);
-                    to = multiply(v[u], y, to);
-                    if constexpr (PARTED && F != kF16) to = multiply(v_low[u], x, to);
+                    first[x] = join(u[0], u[1], u[2], u[3]);
+                    second[x] = join(w[0], w[1], w[2], w[3]);
                 }
             }
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                const half8_t v = source.values(b, i);
+                result_t& to = out[X == 1 ? 2 * b + i : b];
+                to = multiply(v, second[X == 1 ? 0 : i], multiply(v, first[X == 1 ? 0 : i], to));
+                if constexpr (PARTED && F != kF16) to = multiply(source.values_low(b, i), first[X == 1 ? 0 : i], to);
+            }
         }
+    }
+
+    // The largest of the lane's value scales' magnitudes, as bits (a NaN's above every other's).
+    __device__ __forceinline__ static uint32_t largest_scale(const uint4_t (&scale)[NB][X]) {
+        ushort2_t top = {0, 0};
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t x = 0; x < X; ++x)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t size = F == kQ4_0 ? scale[b][x][w] & 0x7FFF7FFFu : scale[b][x][w];
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
+                }
+        return max(top.x, top.y);
     }
 
     // A tile with value scales that are NaNs: a row that sees such a token gets
     // NaNs in its block, and the scale becomes 0, for the rows that do not.
     template <typename TREE>
     __device__ __forceinline__ void spoil(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
-                                                    bool masked, uint4_t (&scale)[NB]) {
-        const uint32_t g = (threadIdx.x & 63u) >> 4;
+                                          bool masked, uint4_t (&scale)[NB][X]) {
+        const uint32_t seen = masked ? sees(a, group, tree, slot0) : 0xFFFFFFFFu;
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            uint32_t nans = 0;  // a bit a slot of the lane's eight
+            float mine = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) nans |= (scale[b][e >> 1] >> (16 * (e & 1)) & 0x7FFFu) > 0x7C00u ? 1u << e : 0u;
+            for (uint32_t x = 0; x < X; ++x) {
+                uint32_t nans = 0;  // a bit a slot of the octet
 #pragma unroll
-            for (uint32_t i = 0; i < RT; ++i) {
-                const uint32_t bits = (masked ? sees(a, group, tree, slot0, i) : 0xFFFFFFFFu) >> (4 * g);
-                const float mine = nans & ((bits & 15u) | (bits >> 12 & 0xF0u)) ? 1.0f : 0.0f;
-                const float nan = most_of_row(mine) > 0.0f ? __builtin_nanf("") : 0.0f;
-                out[i][2 * b] += nan;
-                out[i][2 * b + 1] += nan;
+                for (int e = 0; e < 8; ++e)
+                    nans |= (scale[b][x][e >> 1] >> (16 * (e & 1)) & 0x7FFFu) > 0x7C00u ? 1u << e : 0u;
+                if (nans & octet_bits(seen, x)) mine = 1.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    scale[b][x][w] &= (nans >> (2 * w) & 1u ? 0u : 0xFFFFu) | (nans >> (2 * w + 1) & 1u ? 0u : 0xFFFF0000u);
             }
+            const float nan = most_of_row<X>(mine) > 0.0f ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-                scale[b][w] &= (nans >> (2 * w) & 1u ? 0u : 0xFFFFu) | (nans >> (2 * w + 1) & 1u ? 0u : 0xFFFF0000u);
+            for (uint32_t t = 0; t < kOuts / NB; ++t) out[kOuts / NB * b + t] += nan;
         }
     }
 
@@ -557,9 +604,7 @@ struct Rows {
     __device__ __forceinline__ void end() {
         const float up = ldexpf(1.0f, exponent - kScaleTop);
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i)
-#pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t) out[i][t] *= up;
+        for (uint32_t t = 0; t < kOuts; ++t) out[t] *= up;
     }
 };
 
@@ -611,29 +656,39 @@ __device__ __forceinline__ void wait_loads() {
     __asm__ __volatile__("" ::: "memory");
 }
 
-// A tile's operands out of its record in LDS.
-template <uint32_t F, uint32_t NB>
+// A tile's operands out of its record in LDS. X = 2 reads them by lanes of its
+// own order (Rows).
+template <uint32_t F, uint32_t NB, uint32_t X>
 struct Record {
     const uint8_t* at;
     uint32_t slot0, latest;  // what lies past the last token is cut: kept_of
 
-    __device__ __forceinline__ half8_t key(uint32_t b, int h) const {
-        return operand<F, false>(load_codes<F>(at + b * cache_unit(F), threadIdx.x & 63u), h);
-    }
-    __device__ __forceinline__ half8_t value(uint32_t b, int u) const {
+    __device__ __forceinline__ half8_t keys(uint32_t b, uint32_t i) const {
         const uint32_t lane = threadIdx.x & 63u;
-        Codes<F> c = load_codes<F>(at + values_at(F, NB) + b * cache_unit(F), lane);
+        const uint8_t* unit = at + b * cache_unit(F);
+        if constexpr (X == 1) return operand<F, false>(unit, lane, i);
+        // row n = 16 (g / 2) + 8h + 4 (g % 2) + r, values 16i + 8f on
+        const uint32_t column = (lane >> 4 & 1u) * 8 + (lane >> 2 & 1u) * 4 + (lane & 3u);
+        return operand<F, false>(unit, 16 * (2 * i + (lane >> 5)) + column, lane >> 3 & 1u);
+    }
+    __device__ __forceinline__ half8_t values(uint32_t b, uint32_t i) const {
+        const uint32_t lane = threadIdx.x & 63u, g = group_of<X>(i);
+        const uint8_t* unit = at + values_at(F, NB) + b * cache_unit(F);
+        half8_t v = X == 1 ? operand<F, true>(unit, lane, i) : operand<F, true>(unit, 16 * g + (lane & 15u), lane >> 4 & 1u);
         if constexpr (F == kF16)
-            if (slot0 + kTile > latest)
+            if (slot0 + kTile > latest) {
+                uint4_t w = __builtin_bit_cast(uint4_t, v);
 #pragma unroll
-                for (uint32_t w = 0; w < 4; ++w) c.w[4 * u + w] &= kept_of(slot0, lane >> 4, w, latest);
-        return operand<F, true>(c, u);
+                for (uint32_t x = 0; x < 4; ++x) w[x] &= kept_of(slot0, g, x, latest);
+                v = __builtin_bit_cast(half8_t, w);
+            }
+        return v;
     }
-    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const {
-        return *reinterpret_cast<const uint4_t*>(at + key_scales_at(F, NB) + 64 * b + 16 * ((threadIdx.x & 63u) >> 4));
+    __device__ __forceinline__ uint4_t key_scale(uint32_t b, uint32_t x) const {
+        return *reinterpret_cast<const uint4_t*>(at + key_scales_at(F, NB) + 64 * b + 16 * group_of<X>(x));
     }
-    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const {
-        const uint32_t g = (threadIdx.x & 63u) >> 4;
+    __device__ __forceinline__ uint4_t value_scale(uint32_t b, uint32_t x) const {
+        const uint32_t g = group_of<X>(x);
         uint4_t s = *reinterpret_cast<const uint4_t*>(at + value_scales_at(F, NB) + 64 * b + 16 * g);
         if (slot0 + kTile > latest)
 #pragma unroll
@@ -645,19 +700,19 @@ struct Record {
 // Waves a workgroup and records a wave's ring: eight waves where two fit a
 // SIMD's registers and two records of each fit the LDS, else four, else two.
 constexpr uint32_t kRingBytes = 144 * 1024;
-template <uint32_t F, uint32_t NB, uint32_t RT>
+template <uint32_t F, uint32_t NB, uint32_t X>
 struct AttendShape {
     static constexpr uint32_t kRecord = cache_record(F, NB);
-    static constexpr uint32_t kWaves = NB * RT <= 4 && 16 * kRecord <= kRingBytes ? 8 : 8 * kRecord <= kRingBytes ? 4 : 2;
+    static constexpr uint32_t kWaves = NB * X <= 4 && 16 * kRecord <= kRingBytes ? 8 : 8 * kRecord <= kRingBytes ? 4 : 2;
     static constexpr uint32_t kRing = kRingBytes / (kWaves * kRecord) < 4 ? kRingBytes / (kWaves * kRecord) : 4;
     static constexpr uint32_t kCopies = (kRecord + 1023) / 1024;
 };
 
-template <uint32_t F, uint32_t NB, uint32_t RT>
-__global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(Attention a) {
-    using Shape = AttendShape<F, NB, RT>;
-    constexpr uint32_t kRows = 16 * RT, kRecord = Shape::kRecord, W = Shape::kWaves, D = Shape::kRing;
-    constexpr uint32_t kParts = RT * 2 * NB * 64;  // float4s of a wave's outputs
+template <uint32_t F, uint32_t NB, uint32_t X>
+__global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend(Attention a) {
+    using Shape = AttendShape<F, NB, X>;
+    constexpr uint32_t kRows = 16 * X, kRecord = Shape::kRecord, W = Shape::kWaves, D = Shape::kRing;
+    constexpr uint32_t kQuads = Rows<F, NB, X>::kQuads, kParts = kQuads * 64;  // float4s of a wave's outputs
     __shared__ Tree<kRows> tree;
     // The waves' rings; then, all tiles done, their outputs.
     __shared__ __align__(16) uint8_t space[sizeof(uint8_t[W][D][kRecord]) > sizeof(float4_t[W][kParts])
@@ -666,7 +721,7 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
     __shared__ float joined_offset[W][kRows], joined_sum[W][kRows];
     __shared__ uint32_t joined_live[kRows];
 
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane % kRows;
     const Group group(a, kRows);
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
     uint8_t* ring = space + wave * (D * kRecord);
@@ -679,12 +734,12 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
 #pragma unroll
     for (uint32_t j = 0; j + 1 < D; ++j)
         if (j < count) copy(j);
-    typename Rows<F, NB, RT>::Queries queries;
-    Rows<F, NB, RT>::fetch(a, group, group.row0, queries);
+    typename Rows<F, NB, X>::Queries queries;
+    Rows<F, NB, X>::fetch(a, group, group.row0, queries);
     if (a.parents)
         read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
                   group.token_end - group.token0, a.window);
-    Rows<F, NB, RT> rows;
+    Rows<F, NB, X> rows;
     rows.begin(a, group, tree, group.row0, queries);
     // Only copies are on their way from here on: the queries' own loads, the
     // youngest, have been waited for.
@@ -697,7 +752,7 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
             wait_loads<0>();
         }
         const uint32_t slot0 = (first + j * W) * kTile;
-        const Record<F, NB> record{ring + j % D * kRecord, slot0, group.latest};
+        const Record<F, NB, X> record{ring + j % D * kRecord, slot0, group.latest};
         rows.template tile<false>(a, group, tree, slot0, record);
         __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");  // the record's reads, before its place is copied to
     }
@@ -707,69 +762,66 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, RT>::kWaves)) void attend(
 
     // The waves joined: each one's outputs on the least offset's (the largest
     // maximum's) scale, added in wave order, a thread some of the values.
+    const float mine = sum_of_row<X>(rows.sum);
+    if (lane < kRows) joined_offset[wave][n] = rows.offset, joined_sum[wave][n] = mine;
+    if (threadIdx.x < kRows) joined_live[n] = rows.sight.live;
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-        const float mine = sum_of_row(rows.sum[i]);
-        if (g == 0) joined_offset[wave][16 * i + n] = rows.offset[i], joined_sum[wave][16 * i + n] = mine;
-        if (threadIdx.x < 16) joined_live[16 * i + n] = rows.sight[i].live;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < RT; ++i)
-#pragma unroll
-        for (uint32_t t = 0; t < 2 * NB; ++t) joined[wave][(i * 2 * NB + t) * 64 + lane] = rows.out[i][t];
+    for (uint32_t t = 0; t < kQuads; ++t) joined[wave][t * 64 + lane] = rows.quad(t);
     __syncthreads();
-    for (uint32_t x = 0; x < (kParts + 64 * W - 1) / (64 * W); ++x) {
-        const uint32_t at = threadIdx.x + 64 * W * x;
-        if (at >= kParts) break;
-        const uint32_t i = at / (128 * NB), t = at / 64 % (2 * NB), in_row = 16 * i + n;
-        if (group.row0 + in_row >= group.row_end) continue;
+    for (uint32_t at = threadIdx.x; at < kParts; at += 64 * W) {
+        if (group.row0 + n >= group.row_end) continue;
         float least = INFINITY, total = 0.0f;
-        float4_t out = {0.0f, 0.0f, 0.0f, 0.0f};
+        float4_t out = float4_t(0.0f);
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
-            const float theirs = joined_offset[w][in_row];
+            const float theirs = joined_offset[w][n];
             least = theirs < least || theirs != theirs ? theirs : least;
         }
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
             // a wave that saw nothing has zeros, or the NaNs of scores that are
-            const float theirs = joined_offset[w][in_row];
+            const float theirs = joined_offset[w][n];
             const float factor = theirs == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least - theirs);
-            total = __builtin_fmaf(joined_sum[w][in_row], factor, total);
+            total = __builtin_fmaf(joined_sum[w][n], factor, total);
             out += joined[w][at] * factor;
         }
-        finish<NB>(a, group, group.row0 + in_row, joined_live[in_row] != 0, 16 * t + 4 * g, out, total, least,
-                   t == 0 && g == 0);
+        finish<NB>(a, group, group.row0 + n, joined_live[n] != 0, Rows<F, NB, X>::quad_at(at / 64), out, total, least,
+                   at < kRows);
     }
 }
 
 // ---- many rows: the waves split the rows -------------------------------------------
 
 // A tile laid out in LDS by the workgroup for all of its waves: the codes as
-// binary16 operands, the values' scaled, in two parts (the product of a code
-// and a scale is exact in them), so that a wave does no more than read them.
-// (A NaN among the scales, which is not every row's, goes in as 0: Rows::spoil.)
+// binary16 operands in the order of Rows (X = 2), the values' scaled, in two
+// parts (the product of a code and a scale is exact in them), so that a wave
+// does no more than read them. (A NaN among the scales, which is not every
+// row's, goes in as 0: Rows::spoil.)
 template <uint32_t F, uint32_t NB>
 struct Stage {
-    half8_t keys[2 * NB][64], values[2 * NB][64];    // [2 b + h], [2 b + u]
-    half8_t values_low[F == kF16 ? 1 : 2 * NB][64];  // (F16's are exact in one)
+    half8_t keys_[2 * NB][64], values_[2 * NB][64];   // [2 b + i]
+    half8_t values_low_[F == kF16 ? 1 : 2 * NB][64];  // (F16's are exact in one)
     uint4_t key_scales_[NB][4], value_scales_[NB][4];
 
-    __device__ __forceinline__ half8_t key(uint32_t b, int h) const { return keys[2 * b + h][threadIdx.x & 63u]; }
-    __device__ __forceinline__ half8_t value(uint32_t b, int u) const { return values[2 * b + u][threadIdx.x & 63u]; }
-    __device__ __forceinline__ half8_t value_low(uint32_t b, int u) const { return values_low[2 * b + u][threadIdx.x & 63u]; }
-    __device__ __forceinline__ uint4_t key_scale(uint32_t b) const { return key_scales_[b][(threadIdx.x & 63u) >> 4]; }
-    __device__ __forceinline__ uint4_t value_scale(uint32_t b) const { return value_scales_[b][(threadIdx.x & 63u) >> 4]; }
+    __device__ __forceinline__ half8_t keys(uint32_t b, uint32_t i) const { return keys_[2 * b + i][threadIdx.x & 63u]; }
+    __device__ __forceinline__ half8_t values(uint32_t b, uint32_t i) const { return values_[2 * b + i][threadIdx.x & 63u]; }
+    __device__ __forceinline__ half8_t values_low(uint32_t b, uint32_t i) const {
+        return values_low_[2 * b + i][threadIdx.x & 63u];
+    }
+    __device__ __forceinline__ uint4_t key_scale(uint32_t b, uint32_t x) const { return key_scales_[b][group_of<2>(x)]; }
+    __device__ __forceinline__ uint4_t value_scale(uint32_t b, uint32_t x) const { return value_scales_[b][group_of<2>(x)]; }
 };
 
-constexpr uint32_t kRowWaves = 8;
+// Waves of 32 rows a workgroup: two a SIMD where their registers allow.
+constexpr uint32_t row_waves(uint32_t blocks) { return blocks <= 4 ? 8 : 4; }
 
-template <uint32_t F, uint32_t NB, uint32_t RT>
-__global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
-    constexpr uint32_t W = kRowWaves, kRows = 16 * RT * W, kRecord = cache_record(F, NB);
+template <uint32_t F, uint32_t NB>
+__global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
+    constexpr uint32_t W = row_waves(NB), kRows = 32 * W, kRecord = cache_record(F, NB), kUnit = cache_unit(F);
     constexpr uint32_t kTiles = NB <= 4 ? 2 : 1;                                // a stage's
     constexpr uint32_t kUnits = 2 * NB * kTiles, kMine = (kUnits + W - 1) / W;  // units of a stage; a wave's, at most
     constexpr uint32_t kScaleWords = (key_scales(F) ? 32 : 16) * NB;            // a tile's
+    constexpr uint32_t kLoads = kUnit / 1024 + (kUnit < 1024 ? 1 : 0);          // 16-byte (Q4_0: 8-byte) loads a lane a unit
     static_assert(kScaleWords * kTiles <= 64 * W, "a thread a dword");
     __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
     __shared__ Stage<F, NB> stages[2][kTiles];
@@ -777,13 +829,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Group group(a, kRows);
-    const uint32_t row0 = group.row0 + 16 * RT * wave;
+    const uint32_t row0 = group.row0 + 32 * wave;
     const bool mine = row0 < group.row_end;  // a wave without rows still lays out its share
-    typename Rows<F, NB, RT>::Queries queries;
-    Rows<F, NB, RT>::fetch(a, group, min(row0, group.row_end - 1), queries);
+    typename Rows<F, NB, 2>::Queries queries;
+    Rows<F, NB, 2>::fetch(a, group, min(row0, group.row_end - 1), queries);
     // a chain's wave sees nothing past its last row's token
     const uint32_t sees_to =
-        a.parents ? group.latest : group.past + (min(row0 + 16 * RT, group.row_end) - 1) / a.group + 1;
+        a.parents ? group.latest : group.past + (min(row0 + 32, group.row_end) - 1) / a.group + 1;
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
 
     // All the tiles' value scales, once: their largest exponent, and whether any is a NaN (F16: other than one).
@@ -813,12 +865,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
     const int exponent = F == kF16 ? kScaleTop : exponent_of(__builtin_amdgcn_readfirstlane(most));
     const half2_t by = over(exponent);
 
-    Rows<F, NB, RT> rows;
+    Rows<F, NB, 2> rows;
     rows.begin(a, group, tree, min(row0, group.row_end - 1), queries);
     rows.exponent = exponent;
 
-    // Unit u of a stage: tile u / 2NB, block u % NB, keys then values.
-    Codes<F> codes[kMine];
+    // Unit u of a stage: tile u / 2NB, block u % NB, keys then values. A lane
+    // holds what it will lay out: as the unit has it, lane for lane.
+    struct Held {
+        uint4_t w[kLoads];
+    } held[kMine];
     uint4_t unit_scale[kMine];  // a value unit's
     uint32_t scale_word = 0;    // of those that the waves read
     auto load = [&](uint32_t tile0) {
@@ -827,7 +882,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
             const uint32_t u = wave + W * j, t = tile0 + u / (2 * NB);
             if (u >= kUnits || t >= group.tile_end) continue;
             const uint8_t* record = base + static_cast<uint64_t>(t) * kRecord;
-            codes[j] = load_codes<F>(record + u % (2 * NB) * cache_unit(F), lane);
+            const uint8_t* unit = record + u % (2 * NB) * kUnit;
+            if constexpr (F == kQ4_0) {
+                const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * lane);
+                held[j].w[0][0] = w.x, held[j].w[0][1] = w.y;
+            } else {
+#pragma unroll
+                for (uint32_t x = 0; x < kLoads; ++x) held[j].w[x] = *reinterpret_cast<const uint4_t*>(unit + 1024 * x + 16 * lane);
+            }
             if (F != kF16 && u % (2 * NB) >= NB)
                 unit_scale[j] = *reinterpret_cast<const uint4_t*>(record + value_scales_at(F, NB) + 64 * (u % NB) + 16 * (lane >> 4));
         }
@@ -837,60 +899,78 @@ __global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
                                                            key_scales_at(F, NB))[threadIdx.x % kScaleWords];
     };
     auto lay = [&](uint32_t tile0, Stage<F, NB>* stage) {
+        const uint32_t quarter = lane >> 4, column = lane & 15u;
 #pragma unroll
         for (uint32_t j = 0; j < kMine; ++j) {
             const uint32_t u = wave + W * j, t = u / (2 * NB), b = u % NB, slot0 = (tile0 + t) * kTile;
             if (u >= kUnits || tile0 + t >= group.tile_end) continue;
+            uint32_t w[8];
+#pragma unroll
+            for (uint32_t x = 0; x < 4 * kLoads; ++x) w[x] = held[j].w[x >> 2][x & 3];
             if (u % (2 * NB) < NB) {
-                stage[t].keys[2 * b][lane] = operand<F, false>(codes[j], 0);
-                stage[t].keys[2 * b + 1][lane] = operand<F, false>(codes[j], 1);
+                // token 16h + column, its row; values 8 quarter on
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    half8_t k;
+                    if constexpr (F == kF16)
+                        k = __builtin_bit_cast(half8_t, held[j].w[h]);
+                    else if constexpr (F == kQ8_0)
+                        k = halves_of<128>(w[2 * h], w[2 * h + 1]);
+                    else
+                        k = halves_of<8>(w[h] & 0x0F0F0F0Fu, w[h] >> 4 & 0x0F0F0F0Fu);
+                    const uint32_t row = column / 8 * 16 + 8 * h + column % 8;
+                    stage[t].keys_[2 * b + quarter / 2][32 * (quarter & 1u) + row] = k;
+                }
                 continue;
             }
             // what lies past the last token is no one's, and may be anything
+            uint32_t kept[4] = {~0u, ~0u, ~0u, ~0u};
             if (slot0 + kTile > group.latest)
 #pragma unroll
-                for (uint32_t w = 0; w < 4; ++w) {
-                    const uint32_t kept = kept_of(slot0, lane >> 4, w, group.latest);
-                    if constexpr (F == kF16)
-                        codes[j].w[w] &= kept, codes[j].w[4 + w] &= kept;
-                    else
-                        unit_scale[j][w] &= kept;
-                }
-            if (F != kF16 && spoilt)
+                for (uint32_t x = 0; x < 4; ++x) kept[x] = kept_of(slot0, quarter, x, group.latest);
+            half2_t d[4];
+            if constexpr (F != kF16)
 #pragma unroll
-                for (uint32_t w = 0; w < 4; ++w) {
-                    const uint32_t s = unit_scale[j][w];
-                    unit_scale[j][w] = ((s & 0x7FFFu) > 0x7C00u ? 0u : s & 0xFFFFu) |
-                                       ((s & 0x7FFF0000u) > 0x7C000000u ? 0u : s & 0xFFFF0000u);
+                for (uint32_t x = 0; x < 4; ++x) {
+                    uint32_t s = unit_scale[j][x] & kept[x];
+                    if (spoilt)
+                        s = ((s & 0x7FFFu) > 0x7C00u ? 0u : s & 0xFFFFu) | ((s & 0x7FFF0000u) > 0x7C000000u ? 0u : s & 0xFFFF0000u);
+                    d[x] = pair_of(s) * by;
                 }
+            // tokens of group `quarter`, value 16 part + column
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                const half8_t code = operand<F, true>(codes[j], part);
-                half8_t high = code, low = {0, 0, 0, 0, 0, 0, 0, 0};
-                if constexpr (F != kF16) {
+            for (uint32_t part = 0; part < 2; ++part) {
+                const uint32_t to = 32 * (quarter & 1u) + 16 * part + column, i = 2 * b + quarter / 2;
+                if constexpr (F == kF16) {
+                    uint4_t v = held[j].w[part];
+#pragma unroll
+                    for (uint32_t x = 0; x < 4; ++x) v[x] &= kept[x];
+                    stage[t].values_[i][to] = __builtin_bit_cast(half8_t, v);
+                } else {
+                    const half8_t code = F == kQ8_0 ? halves_of<128>(w[2 * part], w[2 * part + 1])
+                                                    : halves_of<8>(w[0] >> (4 * part) & 0x0F0F0F0Fu, w[1] >> (4 * part) & 0x0F0F0F0Fu);
                     half2_t hi[4], lo[4];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const half2_t c = {code[2 * w], code[2 * w + 1]}, d = pair_of(unit_scale[j][w]) * by;
-                        hi[w] = c * d;
-                        lo[w] = __builtin_elementwise_fma(c, d, -hi[w]);
+                    for (int x = 0; x < 4; ++x) {
+                        const half2_t c = {code[2 * x], code[2 * x + 1]};
+                        hi[x] = c * d[x];
+                        lo[x] = __builtin_elementwise_fma(c, d[x], -hi[x]);
                     }
-                    high = join(hi[0], hi[1], hi[2], hi[3]);
-                    low = join(lo[0], lo[1], lo[2], lo[3]);
-                    stage[t].values_low[2 * b + part][lane] = low;
+                    stage[t].values_[i][to] = join(hi[0], hi[1], hi[2], hi[3]);
+                    stage[t].values_low_[i][to] = join(lo[0], lo[1], lo[2], lo[3]);
                 }
-                stage[t].values[2 * b + part][lane] = high;
             }
         }
-        const uint32_t t = threadIdx.x / kScaleWords, w = threadIdx.x % kScaleWords;
+        const uint32_t t = threadIdx.x / kScaleWords, x = threadIdx.x % kScaleWords;
         if (threadIdx.x < kScaleWords * kTiles && tile0 + t < group.tile_end) {
-            const bool values = !key_scales(F) || w >= 16 * NB;
+            const bool values = !key_scales(F) || x >= 16 * NB;
             if (values)
-                scale_word = kept_scale<F>(scale_word, kept_of((tile0 + t) * kTile, w / 4 & 3u, w & 3u, group.latest));
+                scale_word = kept_scale<F>(scale_word, kept_of((tile0 + t) * kTile, x / 4 & 3u, x & 3u, group.latest));
             uint32_t* to = reinterpret_cast<uint32_t*>(values ? stage[t].value_scales_ : stage[t].key_scales_);
-            to[w % (16 * NB)] = scale_word;
+            to[x % (16 * NB)] = scale_word;
         }
     };
+
     if (group.tile_begin < group.tile_end) {
         load(group.tile_begin);
         lay(group.tile_begin, stages[0]);
@@ -911,29 +991,24 @@ __global__ __launch_bounds__(64 * kRowWaves) void attend_rows(Attention a) {
         if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
         __syncthreads();
     }
-    if (mine) {
-        rows.end();
+    if (!mine) return;
+    rows.end();
+    const float total = sum_of_row<2>(rows.sum);
+    const uint32_t row = row0 + (lane & 31u);
+    if (row >= group.row_end) return;
 #pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) {
-            const float total = sum_of_row(rows.sum[i]);
-            const uint32_t row = row0 + 16 * i + (lane & 15u);
-            if (row >= group.row_end) continue;
-#pragma unroll
-            for (uint32_t t = 0; t < 2 * NB; ++t)
-                finish<NB>(a, group, row, rows.sight[i].live, 16 * t + 4 * (lane >> 4), rows.out[i][t], total,
-                           rows.offset[i], t == 0 && lane < 16);
-        }
-    }
+    for (uint32_t t = 0; t < Rows<F, NB, 2>::kQuads; ++t)
+        finish<NB>(a, group, row, rows.sight.live, Rows<F, NB, 2>::quad_at(t), rows.quad(t), total, rows.offset,
+                   t == 0 && lane < 32);
 }
 
 template <uint32_t F, uint32_t NB>
 static hipError_t launch_blocks(const Attention& a, const AttentionPlan& plan, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads * plan.row_groups * plan.splits);
-    constexpr uint32_t kWide = NB <= 4 ? 2 : 1;  // 16-row tiles a wave's registers hold
     if (plan.waves > 1)
-        hipLaunchKernelGGL((attend_rows<F, NB, kWide>), grid, dim3(64 * kRowWaves), 0, stream, a);
-    else if (plan.row_tiles == kWide)
-        hipLaunchKernelGGL((attend<F, NB, kWide>), grid, dim3(64 * AttendShape<F, NB, kWide>::kWaves), 0, stream, a);
+        hipLaunchKernelGGL((attend_rows<F, NB>), grid, dim3(64 * row_waves(NB)), 0, stream, a);
+    else if (plan.octets == 2)
+        hipLaunchKernelGGL((attend<F, NB, 2>), grid, dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
     else
         hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(64 * AttendShape<F, NB, 1>::kWaves), 0, stream, a);
     return hipGetLastError();

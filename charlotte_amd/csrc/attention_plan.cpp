@@ -6,17 +6,16 @@
 namespace chm {
 
 // Up to 128 rows a key head take workgroups of 16 or 32 rows whose waves split
-// the tiles, more take eight waves of 32 (or 16) rows each; then splits until
+// the tiles, more take eight (or four) waves of 32 rows each; then splits until
 // each compute unit has a workgroup, of at least kLeast tiles, but one while
 // the tiles are few: the launch that joins them would cost more.
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units) {
     const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
-    const uint32_t wide = cache.head_dim <= 128 ? 2 : 1;  // 16-row tiles a wave's registers hold
     AttentionPlan plan{};
-    plan.waves = rows <= 128 ? 1 : 8;
-    plan.row_tiles = rows <= 16 ? 1 : wide;
-    const uint64_t group = 16ull * plan.row_tiles * plan.waves;
+    plan.octets = rows <= 16 ? 1 : 2;
+    plan.waves = rows <= 128 ? 1 : cache.head_dim <= 128 ? 8 : 4;
+    const uint64_t group = 16ull * plan.octets * plan.waves;
     plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
     const uint64_t workgroups = uint64_t{cache.sequences} * cache.kv_heads * plan.row_groups;
     uint64_t reach = std::min(longest ? longest : cache.capacity, cache.capacity);
@@ -41,11 +40,11 @@ uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads
     const uint64_t group = query_heads / cache.kv_heads;
     for (uint32_t t = 1; t <= tokens; ++t) {
         AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        const uint64_t rows = 16ull * plan.row_tiles * plan.waves * plan.row_groups;
+        const uint64_t rows = 16ull * plan.octets * plan.waves * plan.row_groups;
         t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, rows / group)));
         plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
         most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
-        if (plan.waves == 8 && plan.splits < 2) break;
+        if (plan.waves > 1 && plan.splits < 2) break;
     }
     return most;
 }

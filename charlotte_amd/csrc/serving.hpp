@@ -79,8 +79,8 @@ struct Attention {
 
 // How a step runs: rows a workgroup, workgroups along its rows and its keys.
 struct AttentionPlan {
-    uint32_t row_tiles;   // 16-row tiles a wave holds
-    uint32_t waves;       // waves with rows of their own: 8 (attend_rows); 1: the waves split the tiles (attend)
+    uint32_t octets;      // a wave's rows, in 16s
+    uint32_t waves;       // waves with rows of their own: 8 or 4 (attend_rows); 1: the waves split the tiles (attend)
     uint32_t row_groups;  // workgroups along the rows of a key head
     uint32_t splits;      // workgroups along the keys
 };
