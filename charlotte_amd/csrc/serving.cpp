@@ -386,7 +386,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_mat
 
 uint64_t charlotte_hip_matmul_verify_workspace_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocabulary) {
     if (sequences == 0 || tokens == 0 || vocabulary == 0 || vocabulary > (1u << 18) ||
-        uint64_t{sequences} * tokens > 0xFFFFFFull)
+        tokens > chm::kVerifyTokens || uint64_t{sequences} * tokens > 0xFFFFFull)
         return 0;
     return chm::verify_bytes(sequences, tokens, vocabulary);
 }
@@ -419,11 +419,8 @@ charlotte_hip_matmul_status charlotte_hip_matmul_verify(charlotte_hip_matmul_con
         a.target_stride = stride_of(d.target_stride, d.vocabulary, 1, "target stride");
         a.draft_stride = stride_of(d.draft_stride, d.vocabulary, 1, "draft stride");
         a.vocabulary = d.vocabulary, a.sequences = sequences, a.tokens = tokens;
-        const uint32_t rows = d.draft ? sequences : sequences * tokens;
-        a.chunks = chm::verify_chunks(rows, d.vocabulary);
-        need_grid(uint64_t{rows} * a.chunks);
         a.sums = static_cast<uint64_t*>(d.workspace);
-        a.drawn = reinterpret_cast<int32_t*>(a.sums + uint64_t{rows} * a.chunks);
+        a.drawn = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(d.workspace) + bytes - uint64_t{sequences} * 4);
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
         return chm::launch_verify(a, static_cast<hipStream_t>(stream));
     });

@@ -129,13 +129,15 @@ struct Verify {
     int32_t* emitted;
     uint32_t* count;
     uint64_t target_stride, draft_stride;
-    uint32_t vocabulary, sequences, tokens, chunks;
-    uint64_t* sums;   // [drawn rows][chunks]: a chunk's weights summed
-    int32_t* drawn;   // [sequences * tokens]: without a draft, each node's draw
+    uint32_t vocabulary, sequences, tokens;
+    uint32_t share, chunks;  // segments a workgroup, workgroups a row (launch_verify's)
+    uint64_t* sums;          // [drawn rows][segments]: a segment's weights summed
+    int32_t* drawn;          // [sequences]: with a draft, the last node accepted
 };
 
-uint32_t verify_chunks(uint32_t rows, uint32_t vocabulary);
+constexpr uint32_t kVerifyTokens = 1024;  // nodes a sequence
+
 uint64_t verify_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocabulary);
-hipError_t launch_verify(const Verify& a, hipStream_t stream);
+hipError_t launch_verify(Verify a, hipStream_t stream);
 
 }  // namespace chm

@@ -4,14 +4,14 @@
 // the token drawn is the lowest index whose running sum passes W r / 2^31, r =
 // floor(u 2^31); so however a row is cut, the token is the same.
 //
-// Two launches. draw_sums: each row to draw from, in chunks, a workgroup a
-// chunk, each chunk's units summed: the one pass over the probabilities. A
-// chain with a draft draws once a sequence, from the row where its walk ends;
-// every workgroup walks it anew (a lane a token, three reads each), which
-// costs less than a launch. walk: a workgroup a sequence finds the chunk that
-// holds the draw from the sums, reads it again (from cache) for the index, and
-// writes what was accepted; without a draft, each of its waves draws nodes and
-// the first lane then walks the tree.
+// Two launches. draw_sums: each row to draw from, in segments of 256 entries, a
+// wave a segment at a time, each segment's units summed: the one pass over the
+// probabilities. A chain with a draft draws once a sequence, from the row where
+// its walk ends; every workgroup walks it anew (a lane a token, three reads
+// each), which costs less than a launch. walk_*: a wave a draw sums the
+// segments, a lane a run of them, finds the segment, and reads it again (from
+// cache) for the index: two dependent reads. Without a draft a workgroup a
+// sequence draws for every node and its first wave then walks the tree.
 //
 // Bound by bytes: 4 a probability of the rows drawn from, once.
 #include <algorithm>
@@ -77,9 +77,10 @@ __device__ __forceinline__ uint64_t units_of(float x) {
     return (static_cast<uint64_t>(high) << 22) + low;
 }
 
-__device__ __forceinline__ uint32_t share_of(const Verify& a) {
-    return ((a.vocabulary + 3 + a.chunks - 1) / a.chunks + 3) / 4 * 4;
-}
+constexpr uint32_t kSegment = 256;  // entries: four a lane
+
+// Segments of a row, counted from its boundary (rows.hpp).
+__host__ __device__ constexpr uint32_t segments_of(uint32_t vocabulary) { return (vocabulary + 3 + kSegment - 1) / kSegment; }
 
 // Entries at .. at + 3 of a draw's row, counted from its target's boundary
 // (rows.hpp): a refused draft's taken off. Where the draft's rows lie otherwise
@@ -102,8 +103,20 @@ __device__ __forceinline__ float4 weights4(const DrawRow& r, uint32_t lead, uint
     return v;
 }
 
+// The sum over the wave's lanes, in every lane.
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+    // within rows of 16 lanes, rotated by 1, 2, 4 and 8
+    x += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x121, 0xF, 0xF, true));
+    x += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x122, 0xF, 0xF, true));
+    x += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x124, 0xF, 0xF, true));
+    x += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x128, 0xF, 0xF, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = a[0] + a[1];
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return b[0] + b[1];
+}
+
 __global__ __launch_bounds__(256) void draw_sums(Verify a) {
-    __shared__ uint64_t parts[4];
     const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const uint32_t sequence = a.draft ? row : row / a.tokens;
     const uint32_t length = length_of(a, sequence);
@@ -113,29 +126,22 @@ __global__ __launch_bounds__(256) void draw_sums(Verify a) {
     if (a.draft) {
         node = accepted_of(a, sequence, length);
         refused = node + 1 < length;
+        if (chunk == 0 && threadIdx.x == 0) a.drawn[sequence] = static_cast<int32_t>(node);
     }
     const DrawRow r = row_of(a, sequence, node, refused);
-    const uint32_t lead = lead_of(r.target), share = share_of(a);
-    const uint32_t end = min((chunk + 1) * share, lead + a.vocabulary);
-    // a thread adds at most 256 entries' 2^22 before it widens: below 2^32
-    uint32_t high = 0, low = 0;
-    for (uint32_t at = chunk * share + 4 * threadIdx.x; at < end; at += 1024) {
-        const float4 v = weights4(r, lead, a.vocabulary, at);
-        const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            uint32_t h, l;
-            units_of(x[e], &h, &l);
-            high += h;
-            low += l;
-        }
+    const uint32_t lead = lead_of(r.target), all = segments_of(a.vocabulary);
+    const uint32_t end = min((chunk + 1) * a.share, all);
+    for (uint32_t segment = chunk * a.share + (threadIdx.x >> 6); segment < end; segment += 4) {
+        const float4 v = weights4(r, lead, a.vocabulary, segment * kSegment + 4 * (threadIdx.x & 63u));
+        uint32_t high[4], low[4];
+        units_of(v.x, &high[0], &low[0]);
+        units_of(v.y, &high[1], &low[1]);
+        units_of(v.z, &high[2], &low[2]);
+        units_of(v.w, &high[3], &low[3]);
+        // 256 entries of at most 2^22 each
+        const uint32_t h = wave_sum(high[0] + high[1] + high[2] + high[3]), l = wave_sum(low[0] + low[1] + low[2] + low[3]);
+        if ((threadIdx.x & 63u) == 0) a.sums[static_cast<uint64_t>(row) * all + segment] = (static_cast<uint64_t>(h) << 22) + l;
     }
-    uint64_t sum = (static_cast<uint64_t>(high) << 22) + low;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(static_cast<unsigned long long>(sum), o);
-    if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = parts[0] + parts[1] + parts[2] + parts[3];
 }
 
 // The wave's running sum: each lane's, itself included.
@@ -149,71 +155,62 @@ __device__ __forceinline__ uint64_t running(uint64_t x) {
     return x;
 }
 
-// The token drawn from `r` by uniform number u, its chunks' sums at `sums`: by
-// one wave, every lane the same.
+// The token drawn from `r` by uniform number u, its segments' sums at `sums`:
+// by one wave, every lane the same.
 __device__ uint32_t drawn_from(const Verify& a, const DrawRow& r, const uint64_t* sums, float u) {
-    const uint32_t lane = threadIdx.x & 63u;
-    uint64_t total = 0;
-    for (uint32_t c = lane; c < a.chunks; c += 64) total += sums[c];
+    const uint32_t lane = threadIdx.x & 63u, all = segments_of(a.vocabulary);
+    // a lane's run of the segments, at most kRun (of 2^18 entries: 1,025 segments)
+    constexpr uint32_t kRun = 17;
+    const uint32_t run = (all + 63) / 64;
+    uint64_t held[kRun], mine = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(static_cast<unsigned long long>(total), o);
+    for (uint32_t i = 0; i < kRun; ++i) {
+        held[i] = i < run && lane * run + i < all ? sums[lane * run + i] : 0;
+        mine += held[i];
+    }
+    uint64_t to = running(mine);
+    const uint64_t total = __shfl(static_cast<unsigned long long>(to), 63);
     if (total == 0) return 0;
     // floor(u 2^31) within 0 .. 2^31 - 1 (a NaN: 0), and floor(W r / 2^31)
     const float scaled = fminf(fmaxf(u, 0.0f), 0.99999994f) * 2147483648.0f;
     const uint64_t by = static_cast<uint32_t>(scaled);
     const uint64_t passed = __umul64hi(total, by) << 33 | (total * by) >> 31;
 
-    // the chunk: the first whose running sum passes it
-    uint64_t before = 0;
-    uint32_t chunk = a.chunks - 1;
-    for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
-        const uint64_t mine = c0 + lane < a.chunks ? sums[c0 + lane] : 0;
-        const uint64_t run = before + running(mine);
-        const uint64_t past = __ballot(run > passed);
-        if (past) {
-            const int first = __builtin_ctzll(past);
-            chunk = c0 + first;
-            before = __shfl(static_cast<unsigned long long>(run - mine), first);
-            break;
-        }
-        before = __shfl(static_cast<unsigned long long>(run), 63);
-    }
-    // within it: 256 entries a step
-    const uint32_t lead = lead_of(r.target), share = share_of(a);
-    const uint32_t end = min((chunk + 1) * share, lead + a.vocabulary);
-    for (uint32_t at0 = chunk * share; at0 < end; at0 += 256) {
-        const uint32_t at = at0 + 4 * lane;
-        uint64_t w[4] = {0, 0, 0, 0};
-        if (at < end) {
-            const float4 v = weights4(r, lead, a.vocabulary, at);
-            w[0] = units_of(v.x), w[1] = units_of(v.y), w[2] = units_of(v.z), w[3] = units_of(v.w);
-        }
-        const uint64_t mine = w[0] + w[1] + w[2] + w[3];
-        const uint64_t run = before + running(mine);
-        const uint64_t past = __ballot(run > passed);
-        if (past) {
-            const int first = __builtin_ctzll(past);
-            uint64_t so_far = run - mine;
-            uint32_t e = 0;
-            while (e < 3 && so_far + w[e] <= passed) so_far += w[e++];
-            return __shfl(at + e - lead, first);
-        }
-        before = __shfl(static_cast<unsigned long long>(run), 63);
-    }
-    return a.vocabulary - 1;  // not reached: the chunk's sum passes
+    // the lane whose run passes it, its first segment that does, and the sum before that
+    const int owner = __builtin_ctzll(__ballot(to > passed));
+    uint64_t before = to - mine;
+    uint32_t segment = lane * run;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i)
+        if (segment == lane * run + i && before + held[i] <= passed) before += held[i], ++segment;
+    before = __shfl(static_cast<unsigned long long>(before), owner);
+    segment = __shfl(segment, owner);
+
+    const uint32_t lead = lead_of(r.target), at = segment * kSegment + 4 * lane;
+    const float4 v = weights4(r, lead, a.vocabulary, at);
+    const uint64_t w[4] = {units_of(v.x), units_of(v.y), units_of(v.z), units_of(v.w)};
+    mine = w[0] + w[1] + w[2] + w[3];
+    to = before + running(mine);
+    const int first = __builtin_ctzll(__ballot(to > passed));
+    before = to - mine;
+    uint32_t e = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i)
+        if (e == i && before + w[i] <= passed) before += w[i], ++e;
+    return __shfl(at + e - lead, first);
 }
 
-// A chain with a draft: a wave a sequence.
+// A chain with a draft: a wave a sequence; draw_sums left where its walk ended.
 __global__ __launch_bounds__(64) void walk_chain(Verify a) {
     const uint32_t sequence = blockIdx.x, lane = threadIdx.x;
     const uint32_t length = length_of(a, sequence);
     const uint64_t first = static_cast<uint64_t>(sequence) * a.tokens;
     uint32_t count = 0, token = 0;
     if (length > 0) {
-        const uint32_t node = accepted_of(a, sequence, length);
+        const uint32_t node = static_cast<uint32_t>(a.drawn[sequence]);
         count = node + 1;
-        token = drawn_from(a, row_of(a, sequence, node, count < length), a.sums + static_cast<uint64_t>(sequence) * a.chunks,
-                           a.uniforms[first + node]);
+        token = drawn_from(a, row_of(a, sequence, node, count < length),
+                           a.sums + static_cast<uint64_t>(sequence) * segments_of(a.vocabulary), a.uniforms[first + node]);
     }
     for (uint32_t i = lane; i < a.tokens; i += 64) {
         a.path[first + i] = i < count ? static_cast<int32_t>(i) : -1;
@@ -222,22 +219,27 @@ __global__ __launch_bounds__(64) void walk_chain(Verify a) {
     if (lane == 0) a.count[sequence] = count;
 }
 
-// Without a draft: every node's draw, then the walk from node 0, each step by
-// the first wave: the first child with the token drawn.
+// Without a draft: every node's draw, a wave a node; then the first wave walks
+// from node 0, each step to the first child with the token drawn.
 __global__ __launch_bounds__(64 * kWalkWaves) void walk_tree(Verify a) {
+    __shared__ int32_t drawn[kVerifyTokens], tokens[kVerifyTokens], parents[kVerifyTokens];
     const uint32_t sequence = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t length = length_of(a, sequence);
     const uint64_t first = static_cast<uint64_t>(sequence) * a.tokens;
+    for (uint32_t i = threadIdx.x; i < length; i += 64 * kWalkWaves) {
+        tokens[i] = a.node_tokens[first + i];
+        parents[i] = a.parents ? a.parents[first + i] : static_cast<int32_t>(i) - 1;
+    }
     for (uint32_t node = wave; node < length; node += kWalkWaves) {
-        const uint32_t token = drawn_from(a, row_of(a, sequence, node, false), a.sums + (first + node) * a.chunks,
+        const uint32_t token = drawn_from(a, row_of(a, sequence, node, false), a.sums + (first + node) * segments_of(a.vocabulary),
                                           a.uniforms[first + node]);
-        if (lane == 0) a.drawn[first + node] = static_cast<int32_t>(token);
+        if (lane == 0) drawn[node] = static_cast<int32_t>(token);
     }
     __syncthreads();
     if (wave != 0) return;
     uint32_t count = 0, node = 0;
     while (count < length) {
-        const int32_t token = a.drawn[first + node];
+        const int32_t token = drawn[node];
         if (lane == 0) {
             a.path[first + count] = static_cast<int32_t>(node);
             a.emitted[first + count] = token;
@@ -246,9 +248,7 @@ __global__ __launch_bounds__(64 * kWalkWaves) void walk_tree(Verify a) {
         uint32_t next = 0;
         for (uint32_t i0 = node + 1; i0 < length; i0 += 64) {
             const uint32_t i = i0 + lane;
-            const bool child = i < length && a.node_tokens[first + i] == token &&
-                               (a.parents ? a.parents[first + i] == static_cast<int32_t>(node) : i == node + 1);
-            const uint64_t some = __ballot(child);
+            const uint64_t some = __ballot(i < length && tokens[i] == token && parents[i] == static_cast<int32_t>(node));
             if (some) {
                 next = i0 + static_cast<uint32_t>(__builtin_ctzll(some));
                 break;
@@ -261,20 +261,21 @@ __global__ __launch_bounds__(64 * kWalkWaves) void walk_tree(Verify a) {
     if (lane == 0) a.count[sequence] = count;
 }
 
-// Chunks of 2,048 to 8,192 entries, about a thousand of them where the rows are few.
-uint32_t verify_chunks(uint32_t rows, uint32_t vocabulary) {
-    const uint64_t share = std::clamp<uint64_t>(uint64_t{rows} * vocabulary / 1024, 2048, 8192);
-    return static_cast<uint32_t>((vocabulary + share - 1) / share);
+// Workgroups of at least two segments a wave, about two thousand of them.
+uint32_t verify_share(uint32_t rows, uint32_t vocabulary) {
+    const uint64_t all = segments_of(vocabulary);
+    return static_cast<uint32_t>(std::max<uint64_t>(8, (rows * all / 2048 + 3) / 4 * 4));
 }
 
 uint64_t verify_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocabulary) {
-    // the most chunks any number of rows gives; then the draws
     const uint64_t rows = uint64_t{sequences} * tokens;
-    return rows * ((vocabulary + 2047) / 2048) * 8 + rows * 4;
+    return rows * segments_of(vocabulary) * 8 + uint64_t{sequences} * 4;
 }
 
-hipError_t launch_verify(const Verify& a, hipStream_t stream) {
+hipError_t launch_verify(Verify a, hipStream_t stream) {
     const uint32_t rows = a.draft ? a.sequences : a.sequences * a.tokens;
+    a.share = verify_share(rows, a.vocabulary);
+    a.chunks = (segments_of(a.vocabulary) + a.share - 1) / a.share;
     hipLaunchKernelGGL(draw_sums, dim3(rows * a.chunks), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.draft)

@@ -600,8 +600,8 @@ charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_mat
                                                                void* stream);
 
 /* Drafted tokens against the target's probabilities, from given uniform numbers
- * in [0, 1). A sequence's step holds `tokens` nodes: node 0 is the last token
- * already taken, the others drafted ones. target's row i (of a sequence) is the
+ * in [0, 1). A sequence's step holds `tokens` nodes (at most
+ * CHARLOTTE_HIP_MATMUL_VERIFY_TOKENS): node 0 is the last token already taken, the others drafted ones. target's row i (of a sequence) is the
  * target's distribution after node i.
  *
  * With `draft` (a chain; parents NULL) node i + 1's token x is accepted while
@@ -622,6 +622,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_mat
  * path gets the accepted nodes, node 0 first, emitted the tokens after each of
  * them (the drafted ones accepted, then the one drawn): count of each, and -1
  * in the rest of a sequence's `tokens` places. */
+#define CHARLOTTE_HIP_MATMUL_VERIFY_TOKENS 1024u
 typedef struct {
     const int32_t* node_tokens; /* device: sequences rows of `tokens`; one outside the vocabulary is never accepted */
     const float* target;        /* device, 4-byte aligned: sequences * tokens rows, target_stride apart */

@@ -23,7 +23,8 @@ def test_cache_bytes():
 def test_workspaces():
     assert sv.probabilities_workspace_bytes(0, 5) == 0
     assert sv.verify_workspace_bytes(1, 1, (1 << 18) + 1) == 0
-    assert sv.verify_workspace_bytes(2, 3, 2048) == 6 * 8 + 6 * 4
+    assert sv.verify_workspace_bytes(2, 3, 2048) == 6 * 9 * 8 + 2 * 4  # segments of 256, at any alignment
+    assert sv.verify_workspace_bytes(1, 1025, 2048) == 0
 
 
 def test_rope_table():
