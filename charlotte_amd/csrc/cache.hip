@@ -1,10 +1,18 @@
 // The quantized cache (its layout: cache.hpp): tokens written as they are
 // quantized, slots read back, an accepted path's slots moved together.
 //
-// append and read: eight lanes a block of 32 values, four values a lane, so
-// the f32 side is read or written in whole 128-byte runs; the block's largest
-// magnitude is three shuffles. A key's four codes of a lane are neighbours in
-// the record, a value's are in four lanes' operands.
+// A few tokens (cache_append, cache_read): eight lanes a block of 32 values,
+// four values a lane, so the f32 side is read or written in whole 128-byte
+// runs and the block's largest magnitude is three shuffles. A key's four codes
+// of a lane are neighbours in the record, a value's are in four lanes' operands,
+// each stored alone.
+//
+// From a tile's worth of tokens on (append_units, read_units): a wave a unit -
+// a block's 32 values of a tile's 32 tokens - each lane with the codes that
+// the unit has at its place, so that the record is read and written in whole
+// runs too; the largest magnitudes are over 4 lanes (keys) or 16 (values). A
+// unit that the step covers in part keeps its other tokens' codes.
+// Bound by bytes: 4 a value on the f32 side and the codes.
 #include "cache.hpp"
 
 namespace chm {
@@ -47,53 +55,76 @@ __device__ __forceinline__ uint32_t half_bits(float x) {
 
 constexpr uint32_t kNanHalf = 0x7E00u;
 
-// A lane's four codes, raised to be unsigned, and its block's scale as f16
-// bits; every lane of the block calls it. F16's codes are the halves.
+// A block's scale as f16 bits, from its largest magnitude's bits (a NaN's rank
+// above every number's) and whether the first value of it is negative. F16:
+// one, or a NaN.
+template <uint32_t F>
+__device__ __forceinline__ uint32_t scale_of(uint32_t largest, bool negative) {
+    const float most = __uint_as_float(largest);
+    if constexpr (F == kF16) return (half_bits(most) & 0x7C00u) == 0x7C00u ? kNanHalf : 0x3C00u;
+    const uint32_t d = half_bits(F == kQ8_0 ? most / 127.0f : (negative ? most : -most) / 8.0f);
+    return (d & 0x7C00u) == 0x7C00u ? kNanHalf : d;
+}
+
+// A scale as the codes are found by it: d and 1 / d, both 0 where every code is.
+// 1 / d, rounded to nearest, is one Newton step on the reciprocal instruction
+// (for every one of binary16's scales; the tests go through them all).
+struct Step {
+    float d, inverse;
+};
+__device__ __forceinline__ Step step_of(uint32_t scale) {
+    const float d = half_to_float(scale);
+    if (d == 0.0f || scale == kNanHalf) return {0.0f, 0.0f};
+    const float y = __builtin_amdgcn_rcpf(d);
+    return {d, __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y)};
+}
+
+// The code nearest to x / d, ties to even, raised to be unsigned; F16's is the
+// half. The quotient is rounded once: with 1 / d rounded to nearest, q = x (1 /
+// d) corrected by its exact remainder is x / d rounded to nearest (Markstein).
+template <uint32_t F>
+__device__ __forceinline__ uint32_t code_of(float x, const Step& step, uint32_t scale, bool values) {
+    if constexpr (F == kF16) return scale != kNanHalf ? half_bits(x) : values ? 0u : kNanHalf;
+    constexpr float kLow = F == kQ8_0 ? -127.0f : -8.0f, kHigh = F == kQ8_0 ? 127.0f : 7.0f;
+    const float y = step.d == 0.0f ? 0.0f : x;  // what a block that is not held has may be a NaN
+    const float guess = y * step.inverse;
+    const float q = __builtin_fmaf(__builtin_fmaf(-guess, step.d, y), step.inverse, guess);
+    return static_cast<uint32_t>(static_cast<int>(__builtin_amdgcn_fmed3f(rintf(q), kLow, kHigh)) + (F == kQ8_0 ? 128 : 8));
+}
+
+template <uint32_t F>
+__device__ __forceinline__ float value_of(uint32_t code, float d) {
+    return F == kF16 ? half_to_float(code) * d : static_cast<float>(static_cast<int>(code) - (F == kQ8_0 ? 128 : 8)) * d;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// What the block's lanes find the sign of its largest magnitude by: the least of
+// twice the place of a value of it plus whether it is negative.
+__device__ __forceinline__ uint32_t place_of(float x, uint32_t largest, uint32_t place) {
+    return magnitude(x) == largest ? 2 * place + (__float_as_uint(x) >> 31) : 0xFFu;
+}
+
+// A lane's four codes and its block's scale; every lane of the block calls it.
 template <uint32_t F>
 __device__ __forceinline__ uint32_t quantize(const float4& v, uint32_t lane, bool values, uint32_t code[4]) {
     const float x[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (F == kF16) {
-        uint32_t bad = 0;
+    uint32_t largest = max(max(magnitude(x[0]), magnitude(x[1])), max(magnitude(x[2]), magnitude(x[3])));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            code[e] = half_bits(x[e]);
-            bad |= (code[e] & 0x7C00u) == 0x7C00u ? 1u : 0u;
-        }
+    for (int o = 4; o > 0; o >>= 1) largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), o, 8)));
+    uint32_t place = 0;
+    if constexpr (F == kQ4_0) {
+        place = 0xFFu;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) bad |= __shfl_xor(bad, o, 8);
-        if (bad)
+        for (uint32_t e = 0; e < 4; ++e) place = min(place, place_of(x[e], largest, 4 * lane + e));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) code[e] = values ? 0u : kNanHalf;
-        return bad ? kNanHalf : 0x3C00u;
-    } else {
-        // the largest magnitude, the first of equals; a NaN's bits rank above every magnitude's
-        uint32_t largest = 0, at = 0;
-        float extreme = 0.0f;
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-            const uint32_t bits = __float_as_uint(x[e]) & 0x7FFFFFFFu;
-            if (e == 0 || bits > largest) largest = bits, at = 4 * lane + e, extreme = x[e];
-        }
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            const uint32_t theirs = __shfl_xor(largest, o, 8), their_at = __shfl_xor(at, o, 8);
-            const float their_extreme = __shfl_xor(extreme, o, 8);
-            if (theirs > largest || (theirs == largest && their_at < at))
-                largest = theirs, at = their_at, extreme = their_extreme;
-        }
-        const uint32_t d = half_bits(F == kQ8_0 ? fabsf(extreme) / 127.0f : extreme / -8.0f);
-        const bool bad = (d & 0x7C00u) == 0x7C00u;
-        const float step = half_to_float(d);
-        constexpr float kLow = F == kQ8_0 ? -127.0f : -8.0f, kHigh = F == kQ8_0 ? 127.0f : 7.0f;
-        constexpr int kRaise = F == kQ8_0 ? 128 : 8;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            // the code nearest to x / d, ties to even; the division is rounded once
-            const float q = step == 0.0f || bad ? 0.0f : fminf(fmaxf(rintf(x[e] / step), kLow), kHigh);
-            code[e] = static_cast<uint32_t>(static_cast<int>(q) + kRaise);
-        }
-        return bad ? kNanHalf : d;
+        for (int o = 4; o > 0; o >>= 1) place = min(place, static_cast<uint32_t>(__shfl_xor(static_cast<int>(place), o, 8)));
     }
+    const uint32_t d = scale_of<F>(largest, place & 1u);
+    const Step step = step_of(d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) code[e] = code_of<F>(x[e], step, d, values);
+    return d;
 }
 
 template <uint32_t F>
@@ -190,15 +221,271 @@ __global__ __launch_bounds__(256) void cache_read(CacheRows a) {
     }
     float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if constexpr (F == kF16)
-            x[e] = half_to_float(code[e]) * d;
-        else
-            x[e] = static_cast<float>(static_cast<int>(code[e]) - (F == kQ8_0 ? 128 : 8)) * d;
-    }
+    for (int e = 0; e < 4; ++e) x[e] = value_of<F>(code[e], d);
     float* to = const_cast<float*>(p.values ? a.values + p.row * a.value_stride : a.keys + p.row * a.key_stride) +
                 static_cast<uint64_t>(p.head) * a.cache.head_dim + 32 * p.block + 4 * p.lane;
     *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// ---- whole units ---------------------------------------------------------------
+
+// Over the 16 lanes of a row (values) or the four lanes 16 apart (keys).
+template <bool VALUES>
+__device__ __forceinline__ uint32_t most_of_block(uint32_t x) {
+    if constexpr (VALUES) {
+        x = max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x121, 0xF, 0xF, true)));
+        x = max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x122, 0xF, 0xF, true)));
+        x = max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x124, 0xF, 0xF, true)));
+        return max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x128, 0xF, 0xF, true)));
+    } else {
+        const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = max(a[0], a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return max(b[0], b[1]);
+    }
+}
+
+// A wave's unit, its lane's 16 values in it and which of them the step holds.
+// Value e of token part p: keys - value 8 (lane / 16) + e of token 16p + lane %
+// 16; values - value 16p + lane % 16 of the token of slot e of group lane / 16.
+template <bool VALUES>
+struct Unit {
+    uint32_t sequence, head, block, lane;
+    uint64_t tile;
+    int32_t ahead;    // the tile's first slot, counted from the step's first
+    uint32_t limit;   // the step's tokens that have slots
+    bool live, whole;
+    float* first;     // the lane's first value at the tile's first token
+    uint64_t stride;
+
+    __device__ __forceinline__ explicit Unit(const CacheRows& a, uint32_t tiles) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint64_t id = static_cast<uint64_t>(blockIdx.x) * 4 + wave;
+        const uint32_t blocks = a.cache.head_dim / 32, units = blocks * a.cache.kv_heads;
+        lane = threadIdx.x & 63u;
+        const uint64_t at = id / units;  // sequence, tile
+        head = static_cast<uint32_t>(id % units) / blocks;
+        block = static_cast<uint32_t>(id % units) % blocks;
+        live = at / tiles < a.cache.sequences;
+        sequence = live ? static_cast<uint32_t>(at / tiles) : 0u;
+        const uint32_t past = a.first[sequence];
+        tile = past / kTile + at % tiles;
+        limit = past < a.cache.capacity ? min(a.tokens, a.cache.capacity - past) : 0u;
+        const int64_t from = static_cast<int64_t>(tile * kTile) - past;
+        live = live && from < limit;
+        ahead = static_cast<int32_t>(from);
+        whole = ahead >= 0 && ahead + static_cast<int32_t>(kTile) <= static_cast<int32_t>(limit);
+        stride = VALUES ? a.value_stride : a.key_stride;
+        const int64_t row = static_cast<int64_t>(static_cast<uint64_t>(sequence) * a.tokens) + ahead +
+                            (VALUES ? 4 * (lane >> 4) : lane & 15u);
+        first = const_cast<float*>(VALUES ? a.values : a.keys) + row * static_cast<int64_t>(stride) +
+                static_cast<uint64_t>(head) * a.cache.head_dim + 32 * block + (VALUES ? lane & 15u : 8 * (lane >> 4));
+    }
+    // a token of the tile: past the lane's first one
+    __device__ __forceinline__ static uint32_t token(uint32_t part, uint32_t e) { return VALUES ? 16 * (e >> 2) + (e & 3) : 16 * part; }
+    __device__ __forceinline__ bool inside(uint32_t part, uint32_t e) const {
+        const uint32_t mine = VALUES ? 4 * (lane >> 4) : lane & 15u;
+        return static_cast<uint32_t>(ahead + static_cast<int32_t>(mine + token(part, e))) < limit;
+    }
+    // where it is one of the step's
+    __device__ __forceinline__ float* row(uint32_t part, uint32_t e) const {
+        return first + token(part, e) * stride + (VALUES ? 16 * part : 0u);
+    }
+};
+
+// A lane's codes as its unit holds them: Q8_0 16 bytes, 8 a part; Q4_0 8 bytes;
+// F16 16 bytes a part, 1,024 apart. And a mask of those that a code covers.
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void pack(const uint32_t (&code)[2][8], uint32_t (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (F == kQ8_0)
+                w[2 * p + (e >> 2)] |= code[p][e] << (8 * (e & 3));
+            else if constexpr (F == kF16)
+                w[4 * p + (e >> 1)] |= code[p][e] << (16 * (e & 1));
+            else if constexpr (VALUES)
+                w[e >> 2] |= code[p][e] << (8 * (e & 3) + 4 * p);
+            else
+                w[p] |= code[p][e] << (8 * (e & 3) + 4 * (e >> 2));
+        }
+}
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void unpack(const uint32_t (&w)[8], uint32_t (&code)[2][8]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (F == kQ8_0)
+                code[p][e] = w[2 * p + (e >> 2)] >> (8 * (e & 3)) & 0xFFu;
+            else if constexpr (F == kF16)
+                code[p][e] = w[4 * p + (e >> 1)] >> (16 * (e & 1)) & 0xFFFFu;
+            else if constexpr (VALUES)
+                code[p][e] = w[e >> 2] >> (8 * (e & 3) + 4 * p) & 0xFu;
+            else
+                code[p][e] = w[p] >> (8 * (e & 3) + 4 * (e >> 2)) & 0xFu;
+        }
+}
+template <uint32_t F>
+__device__ __forceinline__ void load_unit(const uint8_t* unit, uint32_t lane, uint32_t (&w)[8]) {
+    if constexpr (F == kQ4_0) {
+        const uint2 v = *reinterpret_cast<const uint2*>(unit + 8 * lane);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int p = 0; p < (F == kF16 ? 2 : 1); ++p) {
+            const uint4 v = *reinterpret_cast<const uint4*>(unit + 1024 * p + 16 * lane);
+            w[4 * p] = v.x, w[4 * p + 1] = v.y, w[4 * p + 2] = v.z, w[4 * p + 3] = v.w;
+        }
+    }
+}
+template <uint32_t F>
+__device__ __forceinline__ void store_unit(uint8_t* unit, uint32_t lane, const uint32_t (&w)[8]) {
+    if constexpr (F == kQ4_0) {
+        *reinterpret_cast<uint2*>(unit + 8 * lane) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int p = 0; p < (F == kF16 ? 2 : 1); ++p)
+            *reinterpret_cast<uint4*>(unit + 1024 * p + 16 * lane) = make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+    }
+}
+
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void append_unit(const CacheRows& a, uint32_t tiles) {
+    const Unit<VALUES> u(a, tiles);
+    if (!u.live) return;
+    float x[2][8];
+#pragma unroll
+    for (uint32_t p = 0; p < 2; ++p) {
+        if constexpr (VALUES) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) x[p][e] = u.whole || u.inside(p, e) ? *u.row(p, e) : 0.0f;
+        } else {
+            float4 v = {0.0f, 0.0f, 0.0f, 0.0f}, w = v;
+            if (u.whole || u.inside(p, 0)) {
+                const float4* from = reinterpret_cast<const float4*>(u.row(p, 0));
+                v = from[0], w = from[1];
+            }
+            x[p][0] = v.x, x[p][1] = v.y, x[p][2] = v.z, x[p][3] = v.w;
+            x[p][4] = w.x, x[p][5] = w.y, x[p][6] = w.z, x[p][7] = w.w;
+        }
+    }
+    // A block is a token's: for the keys a part, over its eight values here and
+    // three more lanes'; for the values a slot, over both parts and 15 more lanes'.
+    constexpr uint32_t kBlocks = VALUES ? 8 : 2;
+    uint32_t code[2][8], d[kBlocks];
+#pragma unroll
+    for (uint32_t t = 0; t < kBlocks; ++t) {
+        uint32_t largest = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i) largest = max(largest, magnitude(VALUES ? x[i][t] : x[t][i]));
+        largest = most_of_block<VALUES>(largest);
+        uint32_t place = 0;
+        if constexpr (F == kQ4_0) {
+#pragma unroll
+            for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i)
+                place = max(place, 0xFFu - place_of(VALUES ? x[i][t] : x[t][i], largest,
+                                                    VALUES ? 16 * i + (u.lane & 15u) : 8 * (u.lane >> 4) + i));
+            place = 0xFFu - most_of_block<VALUES>(place);
+        }
+        d[t] = scale_of<F>(largest, place & 1u);
+        const Step step = step_of(d[t]);
+#pragma unroll
+        for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i) {
+            uint32_t& c = VALUES ? code[i][t] : code[t][i];
+            c = code_of<F>(VALUES ? x[i][t] : x[t][i], step, d[t], VALUES);
+        }
+    }
+
+    const uint32_t blocks = a.cache.head_dim / 32;
+    uint8_t* record = record_of(a.cache, F, u.sequence, u.head, u.tile);
+    uint8_t* unit = record + (VALUES ? values_at(F, blocks) : 0u) + u.block * cache_unit(F);
+    uint32_t w[8];
+    pack<F, VALUES>(code, w);
+    if (!u.whole) {  // other tokens' codes stay
+        uint32_t old[8], old_code[2][8];
+        load_unit<F>(unit, u.lane, old);
+        unpack<F, VALUES>(old, old_code);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) code[p][e] = u.inside(p, e) ? code[p][e] : old_code[p][e];
+        pack<F, VALUES>(code, w);
+    }
+    store_unit<F>(unit, u.lane, w);
+
+    if constexpr (VALUES) {
+        if ((u.lane & 15u) == 0) {  // a group's eight tokens
+            uint16_t* scales = reinterpret_cast<uint16_t*>(record + value_scales_at(F, blocks) + 64 * u.block) + 8 * (u.lane >> 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (u.whole || u.inside(0, e)) scales[e] = static_cast<uint16_t>(d[e]);
+        }
+    } else if constexpr (key_scales(F)) {
+        if (u.lane < 16) {
+            uint16_t* scales = reinterpret_cast<uint16_t*>(record + key_scales_at(F, blocks) + 64 * u.block);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                if (u.whole || u.inside(p, 0)) scales[8 * (u.lane >> 2) + 4 * p + (u.lane & 3u)] = static_cast<uint16_t>(d[p]);
+        }
+    }
+}
+
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void read_unit(const CacheRows& a, uint32_t tiles) {
+    const Unit<VALUES> u(a, tiles);
+    if (!u.live) return;
+    const uint32_t blocks = a.cache.head_dim / 32;
+    const uint8_t* record = record_of(a.cache, F, u.sequence, u.head, u.tile);
+    uint32_t w[8], code[2][8];
+    load_unit<F>(record + (VALUES ? values_at(F, blocks) : 0u) + u.block * cache_unit(F), u.lane, w);
+    uint16_t d[8];
+    if constexpr (VALUES || key_scales(F)) {
+        const uint16_t* scales = reinterpret_cast<const uint16_t*>(
+            record + (VALUES ? value_scales_at(F, blocks) : key_scales_at(F, blocks)) + 64 * u.block);
+        if constexpr (VALUES) {
+            const uint4 v = *reinterpret_cast<const uint4*>(scales + 8 * (u.lane >> 4));
+            d[0] = v.x, d[1] = v.x >> 16, d[2] = v.y, d[3] = v.y >> 16, d[4] = v.z, d[5] = v.z >> 16, d[6] = v.w, d[7] = v.w >> 16;
+        } else {
+            const uint32_t token = u.lane & 15u;
+            d[0] = scales[8 * (token >> 2) + (token & 3u)], d[1] = scales[8 * (token >> 2) + 4 + (token & 3u)];
+        }
+    }
+    unpack<F, VALUES>(w, code);
+#pragma unroll
+    for (uint32_t p = 0; p < 2; ++p) {
+        if constexpr (VALUES) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                if (u.whole || u.inside(p, e)) *u.row(p, e) = value_of<F>(code[p][e], half_to_float(d[e]));
+        } else {
+            if (!u.whole && !u.inside(p, 0)) continue;
+            const float by = key_scales(F) ? half_to_float(d[p]) : 1.0f;
+            float4* to = reinterpret_cast<float4*>(u.row(p, 0));
+            to[0] = make_float4(value_of<F>(code[p][0], by), value_of<F>(code[p][1], by), value_of<F>(code[p][2], by),
+                                value_of<F>(code[p][3], by));
+            to[1] = make_float4(value_of<F>(code[p][4], by), value_of<F>(code[p][5], by), value_of<F>(code[p][6], by),
+                                value_of<F>(code[p][7], by));
+        }
+    }
+}
+
+template <uint32_t F>
+__global__ __launch_bounds__(256) void append_units(CacheRows a, uint32_t tiles) {
+    if (blockIdx.y == 0)
+        append_unit<F, false>(a, tiles);
+    else
+        append_unit<F, true>(a, tiles);
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void read_units(CacheRows a, uint32_t tiles) {
+    if (blockIdx.y == 0)
+        read_unit<F, false>(a, tiles);
+    else
+        read_unit<F, true>(a, tiles);
 }
 
 // keep: a workgroup a head of a sequence, a thread a byte run of a token
@@ -306,31 +593,41 @@ __global__ __launch_bounds__(256) void cache_keep(CacheKeep a) {
     }
 }
 
-template <typename A>
-static dim3 rows_grid(const A& a) {
-    const uint64_t blocks = uint64_t{a.cache.sequences} * a.tokens * a.cache.kv_heads * (a.cache.head_dim / 32);
-    return dim3(static_cast<uint32_t>((blocks * 8 + 255) / 256), 2);
+// From 32 tokens on a step has whole units, wherever it begins.
+constexpr uint32_t kUnitTokens = 32;
+
+template <uint32_t F>
+static void launch_rows(const CacheRows& a, bool read, hipStream_t stream) {
+    const uint64_t units = uint64_t{a.cache.kv_heads} * (a.cache.head_dim / 32);
+    if (a.tokens < kUnitTokens) {
+        const uint64_t blocks = uint64_t{a.cache.sequences} * a.tokens * units;
+        const dim3 grid(static_cast<uint32_t>((blocks * 8 + 255) / 256), 2);
+        if (read)
+            hipLaunchKernelGGL(cache_read<F>, grid, dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL(cache_append<F>, grid, dim3(256), 0, stream, a);
+        return;
+    }
+    const uint32_t tiles = a.tokens / kTile + (a.tokens % kTile > 1 ? 2 : 1);  // touched at the most
+    const dim3 grid(static_cast<uint32_t>((a.cache.sequences * uint64_t{tiles} * units + 3) / 4), 2);
+    if (read)
+        hipLaunchKernelGGL(read_units<F>, grid, dim3(256), 0, stream, a, tiles);
+    else
+        hipLaunchKernelGGL(append_units<F>, grid, dim3(256), 0, stream, a, tiles);
 }
 
-hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream) {
+static hipError_t launch_rows(const CacheRows& a, bool read, hipStream_t stream) {
     switch (a.cache.format) {
-        case kF16: hipLaunchKernelGGL(cache_append<kF16>, rows_grid(a), dim3(256), 0, stream, a); break;
-        case kQ4_0: hipLaunchKernelGGL(cache_append<kQ4_0>, rows_grid(a), dim3(256), 0, stream, a); break;
-        case kQ8_0: hipLaunchKernelGGL(cache_append<kQ8_0>, rows_grid(a), dim3(256), 0, stream, a); break;
+        case kF16: launch_rows<kF16>(a, read, stream); break;
+        case kQ4_0: launch_rows<kQ4_0>(a, read, stream); break;
+        case kQ8_0: launch_rows<kQ8_0>(a, read, stream); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
 }
 
-hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream) {
-    switch (a.cache.format) {
-        case kF16: hipLaunchKernelGGL(cache_read<kF16>, rows_grid(a), dim3(256), 0, stream, a); break;
-        case kQ4_0: hipLaunchKernelGGL(cache_read<kQ4_0>, rows_grid(a), dim3(256), 0, stream, a); break;
-        case kQ8_0: hipLaunchKernelGGL(cache_read<kQ8_0>, rows_grid(a), dim3(256), 0, stream, a); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
-}
+hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream) { return launch_rows(a, false, stream); }
+hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream) { return launch_rows(a, true, stream); }
 
 hipError_t launch_cache_keep(const CacheKeep& a, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads);

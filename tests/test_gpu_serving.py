@@ -161,6 +161,37 @@ def test_a_cache_reads_back_what_its_format_holds(ctx, dev, format_, sequences, 
     c.free()
 
 
+@pytest.mark.parametrize("format_,most", [("q8_0", 127), ("q4_0", 8)])
+@pytest.mark.parametrize("tokens", [16, 64])
+def test_codes_at_every_scale(ctx, dev, format_, most, tokens):
+    """Every finite scale of binary16 above zero, and around each tie between two codes
+    the values next to it: the code is that of the quotient, rounded once."""
+    from charlotte_amd import harness as hx
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(51)
+    d = np.arange(1, 0x7C00, dtype=np.uint16).view(np.float16).astype(np.float32)
+    blocks = -(-len(d) // (tokens * 8)) * tokens * 8
+    d = np.concatenate([d, np.ones(blocks - len(d), np.float32)])
+    half = rng.integers(-most, most, (blocks, 32)) + np.float32(0.5)
+    x = (half * d[:, None]).astype(np.float32)
+    beside = [x, np.nextafter(x, np.float32(np.inf)), np.nextafter(x, np.float32(-np.inf))]
+    x = np.choose(rng.integers(0, 3, x.shape), beside)
+    x[:, 5] = -most * d  # the scale is d
+    assert (np.abs(x) <= most * d[:, None]).all()
+    sequences = blocks // (tokens * 8)
+    x = x.reshape(sequences * tokens, 8 * 32)
+    c = dev.cache(format_, np.zeros((sequences, 0, 2, 128)), None, tokens)
+    zero = dev.put(np.zeros(sequences, np.uint32))
+    c.append(dev.put(x), dev.put(x), zero, tokens)
+    (ko, kr), (vo, vr) = dev.room(x.size), dev.room(x.size)
+    c.read(ko, vo, zero, tokens)
+    hx.sync()
+    want = ref.stored(x, format_)
+    assert np.array_equal(kr().reshape(x.shape), want) and np.array_equal(vr().reshape(x.shape), want)
+    c.free()
+
+
 @pytest.mark.parametrize("format_", ["q8_0", "q4_0", "f16"])
 def test_appending_leaves_the_other_slots(ctx, dev, format_):
     from charlotte_amd import harness as hx
