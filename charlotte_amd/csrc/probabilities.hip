@@ -1,11 +1,19 @@
-// Softmax of the head's logits at a temperature: p = exp((x - m) / T) / sum.
-// Two passes over chunks of the rows: each chunk's maximum and sum in one read
-// (the sum kept relative to the running maximum), then, from all of a row's
-// chunks, its probabilities. The second read of the logits comes from cache
-// where a step's rows fit it. Few rows are cut into as many chunks as fill
-// the card. At temperature 0 the chunks keep the largest's first index.
+// Softmax of the head's logits at a temperature: p = exp((x - m) / T) / sum. At
+// temperature 0 the largest's first index stands in the sum's place.
 //
-// Bound by bytes: 4 read and 4 written a logit, and 4 more read from cache.
+// Few rows: two passes over chunks of the rows, as many as fill the card: each
+// chunk's maximum and sum in one read (the sum kept relative to the running
+// maximum), then, from all of a row's chunks, its probabilities; the second
+// read comes from cache.
+//
+// Rows past what the caches hold (kWholeBytes), read once: a workgroup keeps
+// its chunk in registers, publishes its maximum and sum, waits for those of the
+// row's other chunks, and writes its probabilities. The wait is bounded: a
+// workgroup that has not seen them all by then reads the row itself, so that
+// none depends on when another runs. (That needs the logits as they were, so a
+// step in place takes the two passes.)
+//
+// Bound by bytes: 4 read and 4 written a logit.
 #include <algorithm>
 
 #include "rows.hpp"
@@ -95,12 +103,145 @@ __global__ __launch_bounds__(256) void row_probabilities(Probabilities a) {
     }
 }
 
-// About a thousand workgroups, a chunk of at least 2,048 logits.
-uint32_t probabilities_chunks(uint32_t rows, uint32_t vocabulary) {
-    return std::max(1u, std::min((1024 + rows - 1) / rows, (vocabulary + 2047) / 2048));
+// ---- whole rows in one read ---------------------------------------------------------
+
+constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWholeThreads * kWholeFours;
+constexpr uint64_t kWholeBytes = 64ull << 20;  // logits, past which the second read would be memory's again
+constexpr uint32_t kPolls = 1u << 16;          // looks at the other chunks, some 0.1 s of them
+
+// What a chunk publishes, in one word that is never 0: the sum is at least 1
+// where the maximum is a number, and 0 only beside -inf; the index is raised by 1.
+__device__ __forceinline__ uint64_t published(const RowStats& s, bool at) {
+    return static_cast<uint64_t>(__float_as_uint(s.largest)) << 32 | (at ? s.at + 1 : __float_as_uint(s.sum));
 }
 
-hipError_t launch_probabilities(const Probabilities& a, hipStream_t stream) {
+// The workgroup's statistics from its threads', in every thread.
+__device__ __forceinline__ RowStats joined(RowStats s, float rate, RowStats* parts) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
+    if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = parts[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWholeThreads / 64; ++w) s = join_stats(s, parts[w], rate);
+    return s;
+}
+
+// A chunk's fours from `at0` on, in registers, and the thread's part of its statistics.
+__device__ __forceinline__ RowStats chunk_stats(const float* x, uint32_t lead, uint32_t vocabulary, uint32_t at0, float rate,
+                                                float4 (&q)[kWholeFours]) {
+#pragma unroll
+    for (uint32_t i = 0; i < kWholeFours; ++i) q[i] = read4(x, lead, vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
+    RowStats s = {-INFINITY, 0.0f, kNowhere};
+#pragma unroll
+    for (uint32_t i = 0; i < kWholeFours; ++i) s.largest = fmaxf(s.largest, fmaxf(fmaxf(q[i].x, q[i].y), fmaxf(q[i].z, q[i].w)));
+#pragma unroll
+    for (uint32_t i = 0; i < kWholeFours; ++i) {
+        const float v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            s.sum += v[e] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v[e] - s.largest) * rate);
+            if (v[e] == s.largest && v[e] != -INFINITY) s.at = min(s.at, at0 + 4 * kWholeThreads * i + e - lead);
+        }
+    }
+    return s;
+}
+
+__global__ __launch_bounds__(256) void clear_words(uint64_t* words, uint32_t count) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i < count) words[i] = 0;
+}
+
+__global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
+    __shared__ RowStats parts[kWholeThreads / 64];
+    __shared__ RowStats whole;
+    __shared__ uint32_t late;
+    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const float* x = a.logits + row * a.logit_stride;
+    float* y = a.output + row * a.output_stride;
+    const uint32_t lead = lead_of(x), at0 = chunk * kWholeChunk + 4 * threadIdx.x;
+    const bool at = a.temperature == 0.0f;
+    const float rate = at ? 0.0f : kPerOctave / a.temperature;
+    uint64_t* words = reinterpret_cast<uint64_t*>(a.stats) + static_cast<uint64_t>(row) * a.chunks;
+
+    float4 q[kWholeFours];
+    RowStats s = joined(chunk_stats(x, lead, a.vocabulary, at0, rate, q), rate, parts);
+    if (threadIdx.x == 0)
+        __hip_atomic_store(words + chunk, published(s, at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x < 64) {
+        // the first wave looks at every chunk's word, a lane a chunk, until none is 0
+        uint64_t word = 1;
+        bool all = false;
+        for (uint32_t poll = 0; poll < kPolls && !all; ++poll) {
+            if (threadIdx.x < a.chunks) word = __hip_atomic_load(words + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            all = __all(word != 0);
+            if (!all) __builtin_amdgcn_s_sleep(8);
+        }
+        s = {-INFINITY, 0.0f, kNowhere};
+        if (threadIdx.x < a.chunks) {
+            s.largest = __uint_as_float(static_cast<uint32_t>(word >> 32));
+            if (at)
+                s.at = static_cast<uint32_t>(word) - 1;
+            else
+                s.sum = __uint_as_float(static_cast<uint32_t>(word));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
+        if (threadIdx.x == 0) whole = s, late = !all;
+    }
+    __syncthreads();
+    if (late) {  // the row's statistics by this workgroup alone
+        s = {-INFINITY, 0.0f, kNowhere};
+        for (uint32_t c = 0; c < a.chunks; ++c) {
+            float4 other[kWholeFours];
+            s = join_stats(s, joined(chunk_stats(x, lead, a.vocabulary, c * kWholeChunk + 4 * threadIdx.x, rate, other), rate, parts), rate);
+            __syncthreads();
+        }
+    } else {
+        s = whole;
+    }
+    const float inverse = s.sum == 0.0f ? 0.0f : 1.0f / s.sum;
+    const float largest = s.largest == -INFINITY ? 0.0f : s.largest;
+#pragma unroll
+    for (uint32_t i = 0; i < kWholeFours; ++i) {
+        const uint32_t to = at0 + 4 * kWholeThreads * i;
+        if (to >= lead + a.vocabulary) break;
+        float4 p;
+        if (at) {
+            const uint32_t hit = s.at == kNowhere ? kNowhere : s.at + lead - to;
+            p = {hit == 0 ? 1.0f : 0.0f, hit == 1 ? 1.0f : 0.0f, hit == 2 ? 1.0f : 0.0f, hit == 3 ? 1.0f : 0.0f};
+        } else {
+            p = {__builtin_amdgcn_exp2f((q[i].x - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].y - largest) * rate) * inverse,
+                 __builtin_amdgcn_exp2f((q[i].z - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].w - largest) * rate) * inverse};
+        }
+        write4(y, lead, a.vocabulary, to, p);
+    }
+}
+
+// Chunks of the two passes: about a thousand workgroups, a chunk of at least 2,048 logits.
+static uint32_t pass_chunks(uint32_t rows, uint32_t vocabulary) {
+    return std::max(1u, std::min((1024 + rows - 1) / rows, (vocabulary + 2047) / 2048));
+}
+// Of a row read once (a lane a chunk); 0 where it is not.
+static uint32_t whole_chunks(uint32_t rows, uint32_t vocabulary) {
+    const uint32_t chunks = (vocabulary + 3 + kWholeChunk - 1) / kWholeChunk;
+    return uint64_t{rows} * vocabulary * 4 > kWholeBytes && chunks <= 64 ? chunks : 0;
+}
+
+uint64_t probabilities_bytes(uint32_t rows, uint32_t vocabulary) {
+    return rows * std::max<uint64_t>(pass_chunks(rows, vocabulary) * sizeof(RowStats), whole_chunks(rows, vocabulary) * 8ull);
+}
+
+hipError_t launch_probabilities(Probabilities a, hipStream_t stream) {
+    a.chunks = whole_chunks(a.rows, a.vocabulary);
+    if (a.chunks && a.logits != a.output) {
+        const uint32_t words = a.rows * a.chunks;
+        hipLaunchKernelGGL(clear_words, dim3((words + 255) / 256), dim3(256), 0, stream, reinterpret_cast<uint64_t*>(a.stats), words);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        hipLaunchKernelGGL(row_whole, dim3(words), dim3(kWholeThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    a.chunks = pass_chunks(a.rows, a.vocabulary);
     const dim3 grid(a.rows * a.chunks);
     hipLaunchKernelGGL(row_stats, grid, dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;

@@ -351,7 +351,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_attention(charlotte_hip_matmul_
 
 uint64_t charlotte_hip_matmul_probabilities_workspace_bytes(uint32_t rows, uint32_t vocabulary) {
     if (rows == 0 || vocabulary == 0) return 0;
-    return uint64_t{rows} * chm::probabilities_chunks(rows, vocabulary) * sizeof(chm::RowStats);
+    return chm::probabilities_bytes(rows, vocabulary);
 }
 
 charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_matmul_context* ctx,
@@ -373,8 +373,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_mat
         if (d.logits == d.output && a.logit_stride != a.output_stride) refuse("in place with two strides");
         a.rows = d.rows, a.vocabulary = d.vocabulary;
         a.temperature = d.temperature;
-        a.chunks = chm::probabilities_chunks(d.rows, d.vocabulary);
-        need_grid(uint64_t{d.rows} * a.chunks);
+        need_grid(uint64_t{d.rows} * ((uint64_t{d.vocabulary} + 2047) / 2048));
         need(d.workspace, "workspace", 16);
         if (d.workspace_bytes < charlotte_hip_matmul_probabilities_workspace_bytes(d.rows, d.vocabulary))
             refuse("workspace shorter than probabilities_workspace_bytes");

@@ -107,13 +107,13 @@ struct Probabilities {
     const float* logits;
     float* output;
     uint64_t logit_stride, output_stride;
-    uint32_t rows, vocabulary, chunks;
+    uint32_t rows, vocabulary, chunks;  // chunks a row: launch_probabilities'
     float temperature;
-    RowStats* stats;  // [rows][chunks]
+    RowStats* stats;  // [rows][chunks], or words of 8 bytes
 };
 
-uint32_t probabilities_chunks(uint32_t rows, uint32_t vocabulary);
-hipError_t launch_probabilities(const Probabilities& a, hipStream_t stream);
+uint64_t probabilities_bytes(uint32_t rows, uint32_t vocabulary);
+hipError_t launch_probabilities(Probabilities a, hipStream_t stream);
 
 // ---- verify (verify.hip) ----
 

@@ -582,7 +582,10 @@ def _probabilities(ctx, dev, rows, temperature, stride=0, offset=0, output_offse
 @pytest.mark.parametrize("rows,vocabulary,temperature,layout", [
     (1, 1, 1.0, {}), (2, 3, 0.5, {}), (3, 2047, 1.0, {"offset": 4}), (1, 151936, 0.7, {}), (5, 32001, 1.3, {"offset": 8}),
     (7, 4099, 1.0, {"in_place": True}), (4, 5000, 0.8, {"stride": 5003, "in_place": True}),
-    (3, 30001, 1.0, {"output_offset": 4}), (300, 6001, 1.0, {"stride": 6007}), (2, 262144, 1e-3, {})])
+    (3, 30001, 1.0, {"output_offset": 4}), (300, 6001, 1.0, {"stride": 6007}), (2, 262144, 1e-3, {}),
+    # past what the caches hold: rows read once
+    (130, 131072, 0.9, {}), (513, 32769, 1.0, {"stride": 32773, "offset": 4, "output_offset": 8}), (300, 60001, 1.0, {"offset": 12}),
+    (140, 120003, 1.1, {"in_place": True}), (3000, 5700, 1.0, {"output_offset": 12})])
 def test_probabilities(ctx, dev, rows, vocabulary, temperature, layout):
     rng = np.random.default_rng(vocabulary)
     x = (rng.standard_normal((rows, vocabulary)) * 3).astype(np.float32)
@@ -601,9 +604,10 @@ def test_probabilities(ctx, dev, rows, vocabulary, temperature, layout):
     assert (np.abs(got - want) <= bound).all()
 
 
-def test_probabilities_at_temperature_zero_take_the_first_largest(ctx, dev):
+@pytest.mark.parametrize("rows,vocabulary", [(6, 9001), (200, 90001)])  # two passes, and rows read once
+def test_probabilities_at_temperature_zero_take_the_first_largest(ctx, dev, rows, vocabulary):
     rng = np.random.default_rng(31)
-    x = rng.integers(-5, 6, (6, 9001)).astype(np.float32)
+    x = rng.integers(-5, 6, (rows, vocabulary)).astype(np.float32)
     x[1] = -np.inf
     x[2, :] = np.nan
     x[2, 77] = -4.0
@@ -611,14 +615,15 @@ def test_probabilities_at_temperature_zero_take_the_first_largest(ctx, dev):
     x[4] = 2.0
     got = _probabilities(ctx, dev, x, 0.0)
     want = np.zeros_like(x)
-    for i in (0, 3, 4, 5):
+    for i in (0, 3, 4, *range(5, rows)):
         want[i, x[i].argmax()] = 1
     want[2, 77] = 1
     assert (got == want).all()
 
 
-def test_probabilities_of_rows_with_nothing_or_not_finite(ctx, dev):
-    x = np.zeros((5, 5001), np.float32)
+@pytest.mark.parametrize("rows,vocabulary", [(5, 5001), (250, 70001)])
+def test_probabilities_of_rows_with_nothing_or_not_finite(ctx, dev, rows, vocabulary):
+    x = np.zeros((rows, vocabulary), np.float32)
     x[0] = -np.inf
     x[1] = -np.inf
     x[1, 4000] = -3e38
@@ -628,7 +633,7 @@ def test_probabilities_of_rows_with_nothing_or_not_finite(ctx, dev):
     assert (got[0] == 0).all()
     assert got[1, 4000] == 1 and got[1].sum() == 1
     assert np.isnan(got[2]).all() and np.isnan(got[3]).all()
-    assert np.abs(got[4] * 5001 - 1).max() < 100 * U
+    assert np.abs(got[4:] * np.float64(vocabulary) - 1).max() < 100 * U
 
 
 # ---- verify ----------------------------------------------------------------------
