@@ -23,12 +23,13 @@
 // passes it by 2^8, which a tile seldom does) and p d below 2^15, so that the
 // parts' steps (2^-24) lie at least 30 bits below the largest.
 //
-// Split: up to 32 rows of a key head (attend) - the rows one wave holds - a
-// workgroup's waves take its tiles in turn, operands straight from the record,
-// and are joined in LDS. More rows (attend_rows): each wave has rows of its
-// own, and a tile's codes become binary16 operands in LDS once for all of them.
-// Where a step has too few rows to fill the card its tiles are split among
-// several workgroups, joined by attention_combine.
+// Split: where there are few products for each compute unit (attend), a
+// workgroup has 16 or 32 rows, those one wave holds; its waves take the tiles in
+// turn, operands straight from the record, and are joined in LDS. Where there
+// are many (attend_rows), each wave has rows of its own, and a tile's codes
+// become binary16 operands in LDS once for all of them. Where rows do not fill
+// the card, tiles are split among several workgroups, joined by
+// attention_combine. attention_plan.cpp chooses, with what each side measured.
 #pragma once
 
 #include "cache.hpp"
@@ -1005,9 +1006,10 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
 template <uint32_t F, uint32_t NB>
 static hipError_t launch_blocks(const Attention& a, const AttentionPlan& plan, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads * plan.row_groups * plan.splits);
-    if (plan.waves > 1)
-        hipLaunchKernelGGL((attend_rows<F, NB>), grid, dim3(64 * row_waves(NB)), 0, stream, a);
-    else if (plan.octets == 2)
+    if (plan.waves > 1) {
+        if constexpr (NB <= 4 || F == kF16)  // wider quantized heads take attend alone: plan_attention
+            hipLaunchKernelGGL((attend_rows<F, NB>), grid, dim3(64 * row_waves(NB)), 0, stream, a);
+    } else if (plan.octets == 2)
         hipLaunchKernelGGL((attend<F, NB, 2>), grid, dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
     else
         hipLaunchKernelGGL((attend<F, NB, 1>), grid, dim3(64 * AttendShape<F, NB, 1>::kWaves), 0, stream, a);

@@ -1,30 +1,75 @@
 // How a step of attention runs (attention.hpp), on the host alone.
 #include <algorithm>
 
+#include "formats.hpp"
 #include "serving.hpp"
 
 namespace chm {
 
-// Up to 128 rows a key head take workgroups of 16 or 32 rows whose waves split
-// the tiles, more take eight (or four) waves of 32 rows each; then splits until
-// each compute unit has a workgroup, of at least kLeast tiles, but one while
-// the tiles are few: the launch that joins them would cost more.
+namespace {
+
+// Tiles a split takes at least: of wide binary16 heads two, but four once that
+// makes more than 32 splits (126 tiles of one head: 17.8 us in 63, 16.5 in 32).
+uint64_t least_tiles(const CacheShape& cache, uint64_t tiles) {
+    return cache.format == kF16 && cache.head_dim > 128 && tiles <= 64 ? 2 : 4;
+}
+
+// Waves of 32 rows a workgroup of attend_rows holds.
+uint32_t row_waves(uint32_t head_dim) { return head_dim <= 128 ? 8 : 4; }
+
+uint64_t groups_of(uint64_t rows, uint64_t group) { return (rows + group - 1) / group; }
+
+// A workgroup for each compute unit, while each split has least_tiles.
+uint64_t splits_of(const CacheShape& cache, uint64_t row_groups, uint64_t tiles, uint32_t compute_units) {
+    const uint64_t wanted = compute_units / (uint64_t{cache.sequences} * cache.kv_heads * row_groups);
+    return std::max<uint64_t>(1, std::min(wanted, groups_of(tiles, least_tiles(cache, tiles))));
+}
+
+}  // namespace
+
+// `load`: the step's blocks of 16 or 32 rows by a tile, for each compute unit.
+//
+// Workgroups of 16 rows (attend, one octet pair a wave) have the shorter chain
+// of products, and read the cache once for every 16 rows; they are taken while
+// load16 <= 24 and none has to wait for another's compute unit. 8 key heads of
+// 128, 20 rows over 8,000: 16.0 us, by 32 rows 18.6; 48 rows over 1,000 in
+// binary16 10.2 and 15.2, over 8,000 (load16 = 24) 26.8 and 23.7. Quantized
+// heads past 64, whose codes cost more to widen than to read, up to 64: 84 rows
+// over 8,000 (48) 31.5 and 34.5, over 60,000 (352) 153 and 136.
+//
+// A tile's codes laid out once for 128 or 256 rows (attend_rows) pay where each
+// compute unit has many products to feed: 1,024 rows of 8 key heads of 128 over
+// 16,000 in Q8_0 (load32 = 531) 182 us, by 32 rows 325; over 1,000 (47) 38.3 and
+// 39.9; over 400 (28) 32.5 and 29.1. Heads of 64, over 8,000 (266) 62 and 72,
+// 512 rows over 8,000 (129) 43.2 and 41.3. Heads of 256 hold 4 waves' rows, too
+// few to pay for laying codes out (Q8_0, 1,024 over 8,000: 396 and 321), but in
+// binary16 there is little to lay out: 328 and 609, 192 over 2,000 (13) 49 and 56.
+//
+// Few tiles are not split: the launch that joins them costs 2.5 us. One token, 2
+// rows of 8 heads, in one and in splits of four tiles: heads of 64, 19 tiles 8.1
+// and 8.9 us, 26 tiles 9.5 and 9.1; of 128, 11 tiles 7.9 and 9.0, 15 tiles 9.2
+// and 9.0; of 256, 8 tiles 14.0 and 13.0 (binary16 16.4 and 13.6, in splits of
+// two tiles 11.7). 512 tokens with none before, attend_rows: 46.5 and 28.3.
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units) {
     const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
-    AttentionPlan plan{};
-    plan.octets = rows <= 16 ? 1 : 2;
-    plan.waves = rows <= 128 ? 1 : cache.head_dim <= 128 ? 8 : 4;
-    const uint64_t group = 16ull * plan.octets * plan.waves;
-    plan.row_groups = static_cast<uint32_t>((rows + group - 1) / group);
-    const uint64_t workgroups = uint64_t{cache.sequences} * cache.kv_heads * plan.row_groups;
     uint64_t reach = std::min(longest ? longest : cache.capacity, cache.capacity);
     if (window) reach = std::min<uint64_t>(reach, uint64_t{window} + tokens + 31);
-    const uint64_t tiles = (reach + 31) / 32;
-    const uint64_t wanted = compute_units / workgroups;
-    constexpr uint64_t kLeast = 4, kOne = 16;
-    plan.splits = static_cast<uint32_t>(
-        tiles <= kOne ? 1 : std::max<uint64_t>(1, std::min(wanted, (tiles + kLeast - 1) / kLeast)));
+    const uint64_t tiles = groups_of(reach, 32), heads = uint64_t{cache.sequences} * cache.kv_heads;
+
+    const bool quantized = cache.format != kF16;
+    const uint64_t most16 = quantized && cache.head_dim > 64 ? 64 : 24;
+    const uint64_t load16 = groups_of(rows, 16) * heads * tiles, load32 = groups_of(rows, 32) * heads * tiles;
+    const uint32_t waves = row_waves(cache.head_dim);
+    const uint64_t least32 = cache.head_dim <= 64 ? 112 : cache.head_dim <= 128 ? 44 : quantized ? UINT64_MAX : 8;
+    AttentionPlan plan{1, 1, 0, 0};
+    if (rows > 16 * waves && load32 / compute_units >= least32)
+        plan.octets = 2, plan.waves = waves;
+    else if (rows > 16 && (load16 > most16 * compute_units || groups_of(rows, 16) * heads > compute_units))
+        plan.octets = 2;
+    plan.row_groups = static_cast<uint32_t>(groups_of(rows, 16ull * plan.octets * plan.waves));
+    const uint64_t one = plan.waves > 1 || cache.head_dim > 128 ? least_tiles(cache, tiles) : cache.head_dim > 64 ? 12 : 24;
+    plan.splits = tiles <= one ? 1 : static_cast<uint32_t>(splits_of(cache, plan.row_groups, tiles, compute_units));
     return plan;
 }
 
@@ -33,18 +78,21 @@ uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, 
     return uint64_t{cache.sequences} * query_heads * tokens * splits * (uint64_t{cache.head_dim} * 4 + 8);
 }
 
-// Steps of every number of tokens up to `tokens`: of those in one number of
-// row groups the last needs most, and past the first that does not split none does.
+// Over every number of tokens up to `tokens` and every `longest`: most splits
+// come of the fewest workgroups and of all the tiles, or the 64 that are still
+// split by two; of the tokens that make as many groups the last needs most.
 uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units) {
+    const uint64_t tiles = groups_of(cache.capacity, 32), shared = query_heads / cache.kv_heads;
+    const uint32_t waves = row_waves(cache.head_dim);
     uint64_t most = 0;
-    const uint64_t group = query_heads / cache.kv_heads;
-    for (uint32_t t = 1; t <= tokens; ++t) {
-        AttentionPlan plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        const uint64_t rows = 16ull * plan.octets * plan.waves * plan.row_groups;
-        t = static_cast<uint32_t>(std::min<uint64_t>(tokens, std::max<uint64_t>(t, rows / group)));
-        plan = plan_attention(cache, query_heads, t, 0, 0, compute_units);
-        most = std::max(most, attention_partial_bytes(cache, query_heads, t, plan.splits));
-        if (plan.waves > 1 && plan.splits < 2) break;
+    for (uint64_t t = 1; t <= tokens; ++t) {
+        const uint64_t rows = t * shared, group = rows <= 16 ? 16 : rows <= 16 * waves ? 32 : 32 * waves;
+        const uint64_t row_groups = groups_of(rows, group);
+        const uint64_t splits = std::max(splits_of(cache, row_groups, tiles, compute_units),
+                                         splits_of(cache, row_groups, std::min<uint64_t>(tiles, 64), compute_units));
+        most = std::max(most, attention_partial_bytes(cache, query_heads, static_cast<uint32_t>(t),
+                                                      static_cast<uint32_t>(splits)));
+        if (group == 32 * waves && splits < 2) break;
     }
     return most;
 }
