@@ -88,6 +88,8 @@ uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads
     for (uint64_t t = 1; t <= tokens; ++t) {
         const uint64_t rows = t * shared, group = rows <= 16 ? 16 : rows <= 16 * waves ? 32 : 32 * waves;
         const uint64_t row_groups = groups_of(rows, group);
+        const uint64_t last = std::min<uint64_t>(row_groups * group, rows <= 16 * waves ? 16 * waves : UINT64_MAX);
+        t = std::max(t, std::min<uint64_t>(tokens, last / shared));
         const uint64_t splits = std::max(splits_of(cache, row_groups, tiles, compute_units),
                                          splits_of(cache, row_groups, std::min<uint64_t>(tiles, 64), compute_units));
         most = std::max(most, attention_partial_bytes(cache, query_heads, static_cast<uint32_t>(t),

@@ -495,7 +495,7 @@ __global__ __launch_bounds__(256) void read_units(CacheRows a, uint32_t tiles) {
 // writes reach no later batch's source.
 constexpr uint32_t kKeepBatch = 16;
 
-// The path's entries a sequence moves: rising, inside the step and the capacity.
+// The path's entries a sequence moves: rising, their slots inside the capacity.
 __device__ __forceinline__ uint32_t path_length(const CacheKeep& a, uint32_t sequence) {
     uint32_t most = a.count[sequence];
     if (most > a.tokens) most = a.tokens;

@@ -22,7 +22,7 @@ using chm::hip_fail;
 using chm::ok;
 using Status = charlotte_hip_matmul_status;
 
-constexpr uint64_t kGrid = 0x7FFFFFFFull;  // workgroups a launch may have
+constexpr uint64_t kGrid = 0x7FFFFFull;  // workgroups a launch may have: of up to 512 threads, below 2^32 of them
 
 // A failed check, thrown to `guarded` within this file alone.
 struct Refused {
@@ -78,8 +78,9 @@ bool cache_type(uint32_t type) {
 
 // Sizes a cache may have: at most 2^40 records, whose bytes stay below 2^56.
 bool cache_sizes(uint32_t sequences, uint32_t kv_heads, uint32_t head_dim, uint32_t capacity) {
-    return (uint64_t{capacity} + 31) / 32 * sequences * kv_heads <= (1ull << 40) && sequences > 0 && sequences <= 65535 && kv_heads > 0 && kv_heads <= 65535 && head_dim >= 32 &&
-           head_dim <= 256 && head_dim % 32 == 0 && capacity > 0 && capacity <= 0x7FFFFFFFu;
+    return sequences > 0 && sequences <= 65535 && kv_heads > 0 && kv_heads <= 65535 && head_dim >= 32 && head_dim <= 256 &&
+           head_dim % 32 == 0 && capacity > 0 && capacity <= 0x7FFFFFFFu &&
+           (uint64_t{capacity} + 31) / 32 * sequences * kv_heads <= (1ull << 40);
 }
 
 chm::CacheShape shape_of(uint32_t type, uint32_t sequences, uint32_t kv_heads, uint32_t head_dim, uint32_t capacity,
@@ -134,7 +135,7 @@ chm::CacheRows rows_of(const charlotte_hip_matmul_context* ctx, const charlotte_
 uint64_t rows_a_head(const chm::CacheShape& c, uint32_t query_heads, uint32_t tokens) {
     if (query_heads == 0 || query_heads % c.kv_heads != 0 || tokens == 0 || tokens > c.capacity) return 0;
     const uint64_t rows = uint64_t{tokens} * (query_heads / c.kv_heads);
-    return rows * c.sequences * c.kv_heads <= kGrid / 1024 ? rows : 0;
+    return rows * c.sequences * c.kv_heads <= 16 * kGrid ? rows : 0;
 }
 
 }  // namespace

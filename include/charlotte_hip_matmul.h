@@ -492,7 +492,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_head_norm_rope(charlotte_hip_ma
  * (d = 0: codes 0). A block its format cannot hold - a NaN, an infinity, a
  * scale or a value past binary16 - reads back as 32 NaNs, and reaches only the
  * rows that see its token. The bytes are in an order of the library's own, the
- * matrix cores' operands in 32-token tiles. head_dim: 32 .. 256, whole 32s. */
+ * matrix cores' operands in 32-token tiles. Calls on one cache are ordered by
+ * the caller (one stream, or events): an append may write a tile's other
+ * slots again, as they were. head_dim: 32 .. 256, whole 32s. */
 typedef struct charlotte_hip_matmul_cache charlotte_hip_matmul_cache;
 
 /* Bytes a cache takes; 0 for a format or sizes it cannot have. */

@@ -156,3 +156,16 @@ def test_one_workspace_serves_every_bound_on_the_lengths(ctx, dev, format_, dim)
             print("bound", format_, dim, tokens, longest, flush=True)
             _close(dev.attend(c, q, [past], dim ** -0.5, longest=longest)[0], q[0], k[0], v[0], format_, past, dim ** -0.5)
         c.free()
+
+
+def test_a_long_prompt_in_one_step(ctx, dev):
+    """33,000 tokens of 64 query heads: past 2^21 rows, their memory past 2^28 bytes."""
+    rng = np.random.default_rng(33)
+    tokens, heads, dim = 33_000, 64, 32
+    k, v = _random(rng, 1, tokens, 1, dim), _random(rng, 1, tokens, 1, dim)
+    q = rng.random((1, tokens, heads, dim), np.float32) - np.float32(0.5)
+    c = dev.cache("q8_0", k, v, tokens)
+    got = dev.attend(c, q, [0], 0.5)[0]
+    for t in (0, 1, 31, 32, 8191, 16_384, 29_999, 32_999):
+        _close(got[t:t + 1], q[0, t:t + 1], k[0, :t + 1], v[0, :t + 1], "q8_0", t, 0.5)
+    c.free()
