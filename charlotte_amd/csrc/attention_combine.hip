@@ -5,7 +5,9 @@
 //
 // As many lanes as hold a row's values, four each, are a group; where the rows
 // are few a row's splits are shared among several groups of a workgroup and
-// added through LDS, so that all of its loads are on their way at once.
+// added through LDS, so that all of its loads are on their way at once. Bound by
+// the latency of a launch and of two dependent reads: 3 - 5 us, 8 for 16,384 rows
+// of 128 in 4 splits (34 MB).
 #include "serving.hpp"
 
 namespace chm {
@@ -77,7 +79,9 @@ template <uint32_t LANES>
 static hipError_t launch_lanes(const Attention& a, hipStream_t stream) {
     constexpr uint32_t kGroups = 256 / LANES;
     const uint64_t rows = uint64_t{a.cache.sequences} * a.cache.kv_heads * a.rows;
-    // a workgroup a row while that is at most four a compute unit
+    // a workgroup a row while that is at most four a compute unit; a step's time so
+    // and with a group a row: of 32 rows in 32 splits 10.3 and 21.3 us, of 672 17.1
+    // and 19.9, of 1,024 17.1 and 19.1, of 2,048 25.0 and 25.2
     if (rows <= 1024)
         hipLaunchKernelGGL((attention_combine<LANES, kGroups>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, stream, a);
     else

@@ -11,7 +11,9 @@
 // whole eights), exchanged by shuffle; neighbours are in one lane.
 //
 // Bound by bytes, each value read and written once; a token's table rows are
-// read by every head of it, from cache. A decode is one launch's latency.
+// read by every head of it, from cache. 2,048 tokens of 32 + 8 heads of 128 (85
+// MB): 19 us, 4.4 TB/s, where a large copy moves 5.1. A decode is one launch's
+// latency, 3 us.
 #include "serving.hpp"
 
 #include "charlotte_hip_matmul.h"

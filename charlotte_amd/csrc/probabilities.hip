@@ -13,7 +13,9 @@
 // none depends on when another runs. (That needs the logits as they were, so a
 // step in place takes the two passes.)
 //
-// Bound by bytes: 4 read and 4 written a logit.
+// Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 80 us (4.4 TB/s;
+// two passes 94), 1,024 x 131,072: 205 us (5.2 TB/s; 324); 6 x 151,936: passes of
+// 4.0 and 4.8 us, a launch's latency each.
 #include <algorithm>
 
 #include "rows.hpp"
@@ -106,7 +108,10 @@ __global__ __launch_bounds__(256) void row_probabilities(Probabilities a) {
 // ---- whole rows in one read ---------------------------------------------------------
 
 constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWholeThreads * kWholeFours;
-constexpr uint64_t kWholeBytes = 64ull << 20;  // logits, past which the second read would be memory's again
+// Logits past which the second read would be memory's again, and rows are read
+// once: of 151,936, 32 rows (19 MB) 14.7 us read once and 13.8 in two passes, 64
+// (39 MB) 23.7 and 23.6, 100 (61 MB) 29.0 and 33.7, 128 (78 MB) 36.2 and 40.7.
+constexpr uint64_t kWholeBytes = 40ull << 20;
 constexpr uint32_t kPolls = 1u << 16;          // looks at the other chunks, some 0.1 s of them
 
 // What a chunk publishes, in one word that is never 0: the sum is at least 1
