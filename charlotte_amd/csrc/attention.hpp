@@ -37,12 +37,13 @@
 //   us, 4.7 TB/s, and 4.6 to join its 32 splits;
 //   16 heads over 911, by the latency of a launch and its reads: 6.4 and 3.5 us;
 //   a tree of 21 tokens of 32 heads of 64 over 8,191 in Q4_0, by the VALU - some
-//   400 instructions a tile of 32 rows: codes widened, the probabilities scaled
+//   500 instructions a tile of 32 rows: codes widened, the probabilities scaled
 //   and parted for each block of values: 15.9 and 4.0 us;
 //   512 tokens of 32 heads of 128 over 15,873 in Q8_0 (attend_rows), by the matrix
 //   instructions: 339 GFLOP with queries, probabilities and values in parts (135
-//   by the formula), 330 - 340 us, 1.0 PFLOP/s; matrix cores busy 51% and the VALU
-//   44% of the time, waves' priorities and staggered stages changing nothing.
+//   by the formula), 320 - 340 us, 1.06 PFLOP/s; matrix cores busy 51% and the VALU
+//   44% of the time; priorities, operands read further ahead and the waves of a
+//   SIMD half a tile apart changed nothing or cost time.
 #pragma once
 
 #include "cache.hpp"
