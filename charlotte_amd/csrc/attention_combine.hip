@@ -21,12 +21,11 @@ __global__ __launch_bounds__(256) void attention_combine(Attention a) {
     __shared__ float4_t sums[SHARES > 1 ? 256 : 1];
     __shared__ float totals[kGroups];
     const uint32_t part = threadIdx.x % LANES, group = threadIdx.x / LANES, share = group % SHARES;
-    const uint64_t row_of_all = static_cast<uint64_t>(blockIdx.x) * (kGroups / SHARES) + group / SHARES;
-    const uint64_t sequence_head = row_of_all / a.rows;
-    const uint32_t row = static_cast<uint32_t>(row_of_all % a.rows);
+    const uint32_t row_of_all = blockIdx.x * (kGroups / SHARES) + group / SHARES;
+    const uint32_t sequence_head = row_of_all / a.rows, row = row_of_all % a.rows;
     const bool live = sequence_head < static_cast<uint64_t>(a.cache.sequences) * a.cache.kv_heads &&
                       4 * part < a.cache.head_dim;
-    const uint64_t place = row_of_all * a.splits;
+    const uint64_t place = static_cast<uint64_t>(row_of_all) * a.splits;
 
     // This share's splits relative to its own least offset, then all of them to the row's.
     float least = INFINITY, total = 0.0f;
@@ -67,8 +66,7 @@ __global__ __launch_bounds__(256) void attention_combine(Attention a) {
         }
     }
     if (!live) return;
-    const uint32_t sequence = static_cast<uint32_t>(sequence_head / a.cache.kv_heads);
-    const uint32_t head = static_cast<uint32_t>(sequence_head % a.cache.kv_heads);
+    const uint32_t sequence = sequence_head / a.cache.kv_heads, head = sequence_head % a.cache.kv_heads;
     const float inverse = least == INFINITY ? 0.0f : 1.0f / total;
     float* to = a.output + (static_cast<uint64_t>(sequence) * a.tokens + row / a.group) * a.output_stride +
                 static_cast<uint64_t>(head * a.group + row % a.group) * a.cache.head_dim + 4 * part;

@@ -7,17 +7,18 @@
 // of a lane are neighbours in the record, a value's are in four lanes' operands,
 // each stored alone.
 //
-// From a tile's worth of tokens on (append_units, read_units): a wave a unit -
-// a block's 32 values of a tile's 32 tokens - each lane with the codes that
-// the unit has at its place, so that the record is read and written in whole
-// runs too; the largest magnitudes are over 4 lanes (keys) or 16 (values). A
-// unit that the step covers in part keeps its other tokens' codes.
+// From half a tile's worth of tokens on (append_units; read_units from a whole
+// one): a wave a unit - a block's 32 values of a tile's 32 tokens - each lane
+// with the codes that the unit has at its place, so that the record is read and
+// written in whole runs too; the largest magnitudes are over 4 lanes (keys) or 16
+// (values). A unit that the step covers in part keeps its other tokens' codes.
+//
 // Bound by bytes: 4 a value on the f32 side and the codes. 2 sequences of 2,048
-// tokens, 8 heads of 128, keys and values: into Q8_0 (42 MB) 10.4 us by units,
-// 20.6 by tokens; Q4_0 11.1 and 16.1; F16 9.4 and 31.4; read back 9.3 - 10.9 and
-// 14.6 - 23.5. Up to 256 tokens of one sequence either is a launch's latency (3
-// us), and below 32 a unit would hold more lanes than tokens (32 sequences of 16
-// into Q4_0: 5.8 by units, 5.2 by tokens; read back 5.2 and 4.3).
+// tokens, 8 heads of 128, keys and values: into Q8_0 (42 MB) 9.6 us by units, 20.3
+// by tokens; Q4_0 9.4 and 15.9; F16 9.4 and 31.1; read back 9.2 - 10.6 and 14.4 -
+// 23.3 (a copy of as many bytes 6.5 - 7.3). 32 sequences of 16 tokens: 4.9 and 5.7,
+// 5.1 and 5.2, 4.7 and 7.0; read back 4.4 - 5.2 by units, 4.4 - 4.5 by tokens. Up to
+// 256 tokens of one sequence either is a launch's latency (3 us).
 #include "cache.hpp"
 
 namespace chm {
@@ -37,18 +38,18 @@ struct Piece {
 
 __device__ __forceinline__ Piece piece_of(const CacheRows& a) {
     Piece p;
-    const uint64_t id = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) / 8;
+    const uint32_t id = (blockIdx.x * 256 + threadIdx.x) / 8;  // a launch has below 2^32 threads
     const uint32_t blocks = a.cache.head_dim / 32, row_blocks = blocks * a.cache.kv_heads;
     p.lane = threadIdx.x & 7u;
     p.values = blockIdx.y != 0;
-    p.row = id / row_blocks;
-    const uint32_t in_row = static_cast<uint32_t>(id % row_blocks);
+    const uint32_t in_row = id % row_blocks;
     p.head = in_row / blocks;
     p.block = in_row % blocks;
-    const uint64_t sequence = p.row / a.tokens;
+    const uint32_t row = id / row_blocks, sequence = row / a.tokens;
+    p.row = row;
     p.live = sequence < a.cache.sequences;
-    p.sequence = p.live ? static_cast<uint32_t>(sequence) : 0u;
-    p.slot = static_cast<uint64_t>(a.first[p.sequence]) + p.row % a.tokens;
+    p.sequence = p.live ? sequence : 0u;
+    p.slot = static_cast<uint64_t>(a.first[p.sequence]) + row % a.tokens;
     p.live = p.live && p.slot < a.cache.capacity;
     return p;
 }
@@ -87,6 +88,8 @@ __device__ __forceinline__ Step step_of(uint32_t scale) {
 // The code nearest to x / d, ties to even, raised to be unsigned; F16's is the
 // half. The quotient is rounded once: with 1 / d rounded to nearest, q = x (1 /
 // d) corrected by its exact remainder is x / d rounded to nearest (Markstein).
+// It is rounded to a whole number, and raised, as the last bits of a float of
+// 1.5 * 2^23 (the bounds are whole, so the clamp may come first).
 template <uint32_t F>
 __device__ __forceinline__ uint32_t code_of(float x, const Step& step, uint32_t scale, bool values) {
     if constexpr (F == kF16) return scale != kNanHalf ? half_bits(x) : values ? 0u : kNanHalf;
@@ -94,7 +97,8 @@ __device__ __forceinline__ uint32_t code_of(float x, const Step& step, uint32_t 
     const float y = step.d == 0.0f ? 0.0f : x;  // what a block that is not held has may be a NaN
     const float guess = y * step.inverse;
     const float q = __builtin_fmaf(__builtin_fmaf(-guess, step.d, y), step.inverse, guess);
-    return static_cast<uint32_t>(static_cast<int>(__builtin_amdgcn_fmed3f(rintf(q), kLow, kHigh)) + (F == kQ8_0 ? 128 : 8));
+    constexpr float kRaise = 12582912.0f + (F == kQ8_0 ? 128.0f : 8.0f);
+    return __float_as_uint(__builtin_amdgcn_fmed3f(q, kLow, kHigh) + kRaise) & (F == kQ8_0 ? 0xFFu : 0xFu);
 }
 
 template <uint32_t F>
@@ -250,9 +254,25 @@ __device__ __forceinline__ uint32_t most_of_block(uint32_t x) {
     }
 }
 
+// Lane t of each row of 16, in all of its lanes.
+__device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t t) {
+    const int v = static_cast<int>(x);
+    switch (t) {  // (an operand of the instruction)
+        case 0: return __builtin_amdgcn_mov_dpp(v, 0x150, 0xF, 0xF, true);
+        case 1: return __builtin_amdgcn_mov_dpp(v, 0x151, 0xF, 0xF, true);
+        case 2: return __builtin_amdgcn_mov_dpp(v, 0x152, 0xF, 0xF, true);
+        case 3: return __builtin_amdgcn_mov_dpp(v, 0x153, 0xF, 0xF, true);
+        case 4: return __builtin_amdgcn_mov_dpp(v, 0x154, 0xF, 0xF, true);
+        case 5: return __builtin_amdgcn_mov_dpp(v, 0x155, 0xF, 0xF, true);
+        case 6: return __builtin_amdgcn_mov_dpp(v, 0x156, 0xF, 0xF, true);
+        default: return __builtin_amdgcn_mov_dpp(v, 0x157, 0xF, 0xF, true);
+    }
+}
+
 // A wave's unit, its lane's 16 values in it and which of them the step holds.
 // Value e of token part p: keys - value 8 (lane / 16) + e of token 16p + lane %
-// 16; values - value 16p + lane % 16 of the token of slot e of group lane / 16.
+// 16 (in memory, `exchange`: 4 (lane / 16) + e, 16 further on for e >=
+// 4, so that a wave's load or store has 64 bytes of each token); values - value 16p + lane % 16 of the token of slot e of group lane / 16.
 template <bool VALUES>
 struct Unit {
     uint32_t sequence, head, block, lane;
@@ -265,16 +285,16 @@ struct Unit {
 
     __device__ __forceinline__ explicit Unit(const CacheRows& a, uint32_t tiles) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint64_t id = static_cast<uint64_t>(blockIdx.x) * 4 + wave;
+        const uint32_t id = blockIdx.x * 4 + wave;
         const uint32_t blocks = a.cache.head_dim / 32, units = blocks * a.cache.kv_heads;
         lane = threadIdx.x & 63u;
-        const uint64_t at = id / units;  // sequence, tile
-        head = static_cast<uint32_t>(id % units) / blocks;
-        block = static_cast<uint32_t>(id % units) % blocks;
+        const uint32_t at = id / units;  // sequence, tile
+        head = id % units / blocks;
+        block = id % units % blocks;
         live = at / tiles < a.cache.sequences;
-        sequence = live ? static_cast<uint32_t>(at / tiles) : 0u;
+        sequence = live ? at / tiles : 0u;
         const uint32_t past = a.first[sequence];
-        tile = past / kTile + at % tiles;
+        tile = uint64_t{past / kTile} + at % tiles;
         limit = past < a.cache.capacity ? min(a.tokens, a.cache.capacity - past) : 0u;
         const int64_t from = static_cast<int64_t>(tile * kTile) - past;
         live = live && from < limit;
@@ -284,7 +304,7 @@ struct Unit {
         const int64_t row = static_cast<int64_t>(static_cast<uint64_t>(sequence) * a.tokens) + ahead +
                             (VALUES ? 4 * (lane >> 4) : lane & 15u);
         first = const_cast<float*>(VALUES ? a.values : a.keys) + row * static_cast<int64_t>(stride) +
-                static_cast<uint64_t>(head) * a.cache.head_dim + 32 * block + (VALUES ? lane & 15u : 8 * (lane >> 4));
+                static_cast<uint64_t>(head) * a.cache.head_dim + 32 * block + (VALUES ? lane & 15u : 4 * (lane >> 4));
     }
     // a token of the tile: past the lane's first one
     __device__ __forceinline__ static uint32_t token(uint32_t part, uint32_t e) { return VALUES ? 16 * (e >> 2) + (e & 3) : 16 * part; }
@@ -297,6 +317,30 @@ struct Unit {
         return first + token(part, e) * stride + (VALUES ? 16 * part : 0u);
     }
 };
+
+// Of four lanes 16 apart, g their number: values 8g .. 8g + 7 (a, then b) to and
+// from values 4g .. 4g + 3 (a) and 16 + 4g .. 16 + 4g + 3 (b).
+__device__ __forceinline__ void exchange(float4& a, float4& b, bool to_memory) {
+    float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t u = __float_as_uint(x[e]), v = __float_as_uint(y[e]);
+        auto swap16 = [&] {
+            const auto s = __builtin_amdgcn_permlane16_swap(u, v, false, false);
+            u = s[0], v = s[1];
+        };
+        auto swap32 = [&] {
+            const auto s = __builtin_amdgcn_permlane32_swap(u, v, false, false);
+            u = s[0], v = s[1];
+        };
+        if (to_memory)
+            swap16(), swap32();
+        else
+            swap32(), swap16();
+        x[e] = __uint_as_float(u), y[e] = __uint_as_float(v);
+    }
+    a = {x[0], x[1], x[2], x[3]}, b = {y[0], y[1], y[2], y[3]};
+}
 
 // A lane's codes as its unit holds them: Q8_0 16 bytes, 8 a part; Q4_0 8 bytes;
 // F16 16 bytes a part, 1,024 apart. And a mask of those that a code covers.
@@ -372,37 +416,76 @@ __device__ __forceinline__ void append_unit(const CacheRows& a, uint32_t tiles) 
             float4 v = {0.0f, 0.0f, 0.0f, 0.0f}, w = v;
             if (u.whole || u.inside(p, 0)) {
                 const float4* from = reinterpret_cast<const float4*>(u.row(p, 0));
-                v = from[0], w = from[1];
+                v = from[0], w = from[4];
             }
+            exchange(v, w, false);
             x[p][0] = v.x, x[p][1] = v.y, x[p][2] = v.z, x[p][3] = v.w;
             x[p][4] = w.x, x[p][5] = w.y, x[p][6] = w.z, x[p][7] = w.w;
         }
     }
     // A block is a token's: for the keys a part, over its eight values here and
     // three more lanes'; for the values a slot, over both parts and 15 more lanes'.
-    constexpr uint32_t kBlocks = VALUES ? 8 : 2;
-    uint32_t code[2][8], d[kBlocks];
+    constexpr uint32_t kBlocks = VALUES ? 8 : 2, kHere = VALUES ? 2 : 8;
+    auto value = [&](uint32_t t, uint32_t i) { return VALUES ? x[i][t] : x[t][i]; };
+    // Twice the largest magnitude, plus, Q4_0, whether the first value of it is
+    // negative: where only one sign has it, the largest of the values' bits with
+    // the sign put last. (Both signs' is as rare as +m and -m in a block; ~0 is a
+    // NaN, in a block that is not held.)
+    uint32_t most[kBlocks];
+    bool both = false;
 #pragma unroll
     for (uint32_t t = 0; t < kBlocks; ++t) {
         uint32_t largest = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i) largest = max(largest, magnitude(VALUES ? x[i][t] : x[t][i]));
+        for (uint32_t i = 0; i < kHere; ++i) {
+            const uint32_t bits = __float_as_uint(value(t, i));
+            largest = max(largest, F == kQ4_0 ? __builtin_amdgcn_alignbit(bits, bits, 31) : bits & 0x7FFFFFFFu);
+        }
         largest = most_of_block<VALUES>(largest);
-        uint32_t place = 0;
+        most[t] = F == kQ4_0 ? largest : largest << 1;
         if constexpr (F == kQ4_0) {
+            const uint32_t other = largest & 1u ? largest >> 1 : ~0u;
 #pragma unroll
-            for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i)
-                place = max(place, 0xFFu - place_of(VALUES ? x[i][t] : x[t][i], largest,
-                                                    VALUES ? 16 * i + (u.lane & 15u) : 8 * (u.lane >> 4) + i));
-            place = 0xFFu - most_of_block<VALUES>(place);
+            for (uint32_t i = 0; i < kHere; ++i) both |= __float_as_uint(value(t, i)) == other;
         }
-        d[t] = scale_of<F>(largest, place & 1u);
-        const Step step = step_of(d[t]);
+    }
+    if (F == kQ4_0 && __any(both)) {
 #pragma unroll
-        for (uint32_t i = 0; i < (VALUES ? 2 : 8); ++i) {
-            uint32_t& c = VALUES ? code[i][t] : code[t][i];
-            c = code_of<F>(VALUES ? x[i][t] : x[t][i], step, d[t], VALUES);
+        for (uint32_t t = 0; t < kBlocks; ++t) {
+            uint32_t place = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kHere; ++i)
+                place = max(place, 0xFFu - place_of(value(t, i), most[t] >> 1, VALUES ? 16 * i + (u.lane & 15u) : 8 * (u.lane >> 4) + i));
+            most[t] = (most[t] & ~1u) | ((0xFFu - most_of_block<VALUES>(place)) & 1u);
         }
+    }
+    // Their scales: of the values lane t of a row of 16 finds token t's, for all of it.
+    constexpr uint32_t kOwn = VALUES ? 1 : 2;
+    uint32_t own_scale[kOwn];
+    Step own[kOwn];
+#pragma unroll
+    for (uint32_t t = 0; t < kOwn; ++t) {
+        uint32_t mine = most[t];
+        if constexpr (VALUES)
+#pragma unroll
+            for (uint32_t e = 1; e < 8; ++e) mine = (u.lane & 7u) == e ? most[e] : mine;
+        own_scale[t] = scale_of<F>(mine >> 1, mine & 1u);
+        own[t] = step_of(own_scale[t]);
+    }
+    uint32_t code[2][8];
+#pragma unroll
+    for (uint32_t t = 0; t < kBlocks; ++t) {
+        Step step;
+        uint32_t scale;
+        if constexpr (VALUES) {
+            step.d = __uint_as_float(of_lane(__float_as_uint(own[0].d), t));
+            step.inverse = __uint_as_float(of_lane(__float_as_uint(own[0].inverse), t));
+            scale = of_lane(own_scale[0], t);
+        } else {
+            step = own[t], scale = own_scale[t];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kHere; ++i) (VALUES ? code[i][t] : code[t][i]) = code_of<F>(value(t, i), step, scale, VALUES);
     }
 
     const uint32_t blocks = a.cache.head_dim / 32;
@@ -423,18 +506,16 @@ __device__ __forceinline__ void append_unit(const CacheRows& a, uint32_t tiles) 
     store_unit<F>(unit, u.lane, w);
 
     if constexpr (VALUES) {
-        if ((u.lane & 15u) == 0) {  // a group's eight tokens
-            uint16_t* scales = reinterpret_cast<uint16_t*>(record + value_scales_at(F, blocks) + 64 * u.block) + 8 * (u.lane >> 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (u.whole || u.inside(0, e)) scales[e] = static_cast<uint16_t>(d[e]);
-        }
+        const uint32_t e = u.lane & 15u;
+        if (e < 8 && (u.whole || u.inside(0, e)))  // a group's eight tokens
+            reinterpret_cast<uint16_t*>(record + value_scales_at(F, blocks) + 64 * u.block)[8 * (u.lane >> 4) + e] =
+                static_cast<uint16_t>(own_scale[0]);
     } else if constexpr (key_scales(F)) {
         if (u.lane < 16) {
             uint16_t* scales = reinterpret_cast<uint16_t*>(record + key_scales_at(F, blocks) + 64 * u.block);
 #pragma unroll
             for (int p = 0; p < 2; ++p)
-                if (u.whole || u.inside(p, 0)) scales[8 * (u.lane >> 2) + 4 * p + (u.lane & 3u)] = static_cast<uint16_t>(d[p]);
+                if (u.whole || u.inside(p, 0)) scales[8 * (u.lane >> 2) + 4 * p + (u.lane & 3u)] = static_cast<uint16_t>(own_scale[p]);
         }
     }
 }
@@ -467,13 +548,15 @@ __device__ __forceinline__ void read_unit(const CacheRows& a, uint32_t tiles) {
             for (uint32_t e = 0; e < 8; ++e)
                 if (u.whole || u.inside(p, e)) *u.row(p, e) = value_of<F>(code[p][e], half_to_float(d[e]));
         } else {
-            if (!u.whole && !u.inside(p, 0)) continue;
             const float by = key_scales(F) ? half_to_float(d[p]) : 1.0f;
+            float4 v = make_float4(value_of<F>(code[p][0], by), value_of<F>(code[p][1], by), value_of<F>(code[p][2], by),
+                                   value_of<F>(code[p][3], by));
+            float4 w = make_float4(value_of<F>(code[p][4], by), value_of<F>(code[p][5], by), value_of<F>(code[p][6], by),
+                                   value_of<F>(code[p][7], by));
+            exchange(v, w, true);
+            if (!u.whole && !u.inside(p, 0)) continue;
             float4* to = reinterpret_cast<float4*>(u.row(p, 0));
-            to[0] = make_float4(value_of<F>(code[p][0], by), value_of<F>(code[p][1], by), value_of<F>(code[p][2], by),
-                                value_of<F>(code[p][3], by));
-            to[1] = make_float4(value_of<F>(code[p][4], by), value_of<F>(code[p][5], by), value_of<F>(code[p][6], by),
-                                value_of<F>(code[p][7], by));
+            to[0] = v, to[4] = w;
         }
     }
 }
@@ -598,13 +681,13 @@ __global__ __launch_bounds__(256) void cache_keep(CacheKeep a) {
     }
 }
 
-// From 32 tokens on (both sides' times: above).
-constexpr uint32_t kUnitTokens = 32;
+// From how many tokens on (both sides' times: above).
+constexpr uint32_t kAppendUnits = 16, kReadUnits = 32;
 
 template <uint32_t F>
 static void launch_rows(const CacheRows& a, bool read, hipStream_t stream) {
     const uint64_t units = uint64_t{a.cache.kv_heads} * (a.cache.head_dim / 32);
-    if (a.tokens < kUnitTokens) {
+    if (a.tokens < (read ? kReadUnits : kAppendUnits)) {
         const uint64_t blocks = uint64_t{a.cache.sequences} * a.tokens * units;
         const dim3 grid(static_cast<uint32_t>((blocks * 8 + 255) / 256), 2);
         if (read)

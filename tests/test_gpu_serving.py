@@ -889,3 +889,29 @@ def test_probabilities_and_verify_refuse(ctx, dev):
               check(sequences=1 << 14, tokens=1 << 12)):
         _refused(b, bad)
     _refused(check(parents=x), mm.Status.UNSUPPORTED)
+
+
+@pytest.mark.parametrize("format_", ["q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("tokens", [5, 32, 71])
+def test_blocks_whose_largest_magnitude_has_both_signs(ctx, dev, format_, tokens):
+    """Q4_0's scale takes the sign of the first value of the largest magnitude, by a few tokens and by whole units;
+    zeros of both signs, and blocks that are not held beside them."""
+    from charlotte_amd import harness as hx
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(tokens)
+    k, v = (rng.integers(-3, 4, (2, tokens, 2, 96)).astype(np.float32) for _ in range(2))
+    for x in (k, v):
+        x *= np.float32(0.37)
+        x[0, 0, 0, :32] = np.where(np.arange(32) % 2, np.float32(0.0), np.float32(-0.0))
+        x[0, 1, 1, 32:64] = 5.0
+        x[0, 1, 1, 40] = x[1, 2, 0, 95] = -5.0
+        x[1, 2, 0, 64:95] = 5.0
+        x[1, 3, 0, 0], x[1, 3, 0, 1], x[1, 3, 0, 33], x[1, 3, 1, 70] = np.nan, -np.nan, -np.inf, 1e30
+    c = dev.cache(format_, k, v, tokens + 9, past=7)
+    (ko, kr), (vo, vr) = dev.room(k.size), dev.room(v.size)
+    c.read(ko, vo, dev.put(np.full(2, 7, np.uint32)), tokens)
+    hx.sync()
+    assert np.array_equal(kr().reshape(k.shape), ref.stored(k, format_), equal_nan=True)
+    assert np.array_equal(vr().reshape(v.shape), ref.stored(v, format_), equal_nan=True)
+    c.free()
