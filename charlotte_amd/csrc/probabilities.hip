@@ -1,7 +1,9 @@
 // Softmax of the head's logits at a temperature: p = exp((x - m) / T) / sum. At
 // temperature 0 the largest's first index stands in the sum's place.
 //
-// Few rows: two passes over chunks of the rows, as many as fill the card: each
+// Rows that a workgroup's registers hold: one launch, a workgroup a row.
+//
+// Few longer rows: two passes over chunks of the rows, as many as fill the card: each
 // chunk's maximum and sum in one read (the sum kept relative to the running
 // maximum), then, from all of a row's chunks, its probabilities; the second
 // read comes from cache.
@@ -112,6 +114,12 @@ constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWhol
 // once: of 151,936, 32 rows (19 MB) 14.7 us read once and 13.8 in two passes, 64
 // (39 MB) 23.7 and 23.6, 100 (61 MB) 29.0 and 33.7, 128 (78 MB) 36.2 and 40.7.
 constexpr uint64_t kWholeBytes = 40ull << 20;
+// Rows from which a row of one to two chunks is one workgroup's, in one launch:
+// of 32,000, 6 rows 8.0 us so and 7.1 in two passes (one compute unit reads 128
+// KB in 4), 48 rows 8.7 and 8.8, 168 rows 11.0 and 14.6, 1,000 rows 39.8 and 46.7.
+// Rows of at most a chunk always are: 1 x 4,096 4.8 and 6.6, 6 x 16,000 5.4 and
+// 7.0, 168 x 16,000 6.6 and 11.2, 4,000 x 16,000 97.5 and 100.7.
+constexpr uint32_t kAloneRows = 48;
 constexpr uint32_t kPolls = 1u << 16;          // looks at the other chunks, some 0.1 s of them
 
 // What a chunk publishes, in one word that is never 0: the sum is at least 1
@@ -126,22 +134,23 @@ __device__ __forceinline__ RowStats joined(RowStats s, float rate, RowStats* par
     for (int o = 32; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
     if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = s;
     __syncthreads();
-    s = parts[0];
+    s = parts[threadIdx.x % (kWholeThreads / 64)];
 #pragma unroll
-    for (uint32_t w = 1; w < kWholeThreads / 64; ++w) s = join_stats(s, parts[w], rate);
+    for (int o = kWholeThreads / 128; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
     return s;
 }
 
 // A chunk's fours from `at0` on, in registers, and the thread's part of its statistics.
+template <uint32_t FOURS>
 __device__ __forceinline__ RowStats chunk_stats(const float* x, uint32_t lead, uint32_t vocabulary, uint32_t at0, float rate,
-                                                float4 (&q)[kWholeFours]) {
+                                                float4 (&q)[FOURS]) {
 #pragma unroll
-    for (uint32_t i = 0; i < kWholeFours; ++i) q[i] = read4(x, lead, vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
+    for (uint32_t i = 0; i < FOURS; ++i) q[i] = read4(x, lead, vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
     RowStats s = {-INFINITY, 0.0f, kNowhere};
 #pragma unroll
-    for (uint32_t i = 0; i < kWholeFours; ++i) s.largest = fmaxf(s.largest, fmaxf(fmaxf(q[i].x, q[i].y), fmaxf(q[i].z, q[i].w)));
+    for (uint32_t i = 0; i < FOURS; ++i) s.largest = fmaxf(s.largest, fmaxf(fmaxf(q[i].x, q[i].y), fmaxf(q[i].z, q[i].w)));
 #pragma unroll
-    for (uint32_t i = 0; i < kWholeFours; ++i) {
+    for (uint32_t i = 0; i < FOURS; ++i) {
         const float v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
@@ -150,6 +159,40 @@ __device__ __forceinline__ RowStats chunk_stats(const float* x, uint32_t lead, u
         }
     }
     return s;
+}
+
+// The chunk's probabilities, by its row's statistics.
+template <uint32_t FOURS>
+__device__ __forceinline__ void write_chunk(const Probabilities& a, float* y, uint32_t lead, uint32_t at0, const RowStats& s,
+                                            float rate, const float4 (&q)[FOURS]) {
+    const float inverse = s.sum == 0.0f ? 0.0f : 1.0f / s.sum;
+    const float largest = s.largest == -INFINITY ? 0.0f : s.largest;
+#pragma unroll
+    for (uint32_t i = 0; i < FOURS; ++i) {
+        const uint32_t to = at0 + 4 * kWholeThreads * i;
+        if (to >= lead + a.vocabulary) break;
+        float4 p;
+        if (a.temperature == 0.0f) {
+            const uint32_t hit = s.at == kNowhere ? kNowhere : s.at + lead - to;
+            p = {hit == 0 ? 1.0f : 0.0f, hit == 1 ? 1.0f : 0.0f, hit == 2 ? 1.0f : 0.0f, hit == 3 ? 1.0f : 0.0f};
+        } else {
+            p = {__builtin_amdgcn_exp2f((q[i].x - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].y - largest) * rate) * inverse,
+                 __builtin_amdgcn_exp2f((q[i].z - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].w - largest) * rate) * inverse};
+        }
+        write4(y, lead, a.vocabulary, to, p);
+    }}
+
+// A row by one workgroup, in one launch: FOURS fours of logits a thread.
+template <uint32_t FOURS>
+__global__ __launch_bounds__(kWholeThreads) void row_alone(Probabilities a) {
+    __shared__ RowStats parts[kWholeThreads / 64];
+    const float* x = a.logits + blockIdx.x * a.logit_stride;
+    const uint32_t lead = lead_of(x), at0 = 4 * threadIdx.x;
+    const float rate = a.temperature > 0.0f ? kPerOctave / a.temperature : 0.0f;
+    float4 q[FOURS];
+    // every thread's reads are before the barrier in `joined`: the output may be the logits
+    const RowStats s = joined(chunk_stats(x, lead, a.vocabulary, at0, rate, q), rate, parts);
+    write_chunk(a, a.output + blockIdx.x * a.output_stride, lead, at0, s, rate, q);
 }
 
 __global__ __launch_bounds__(256) void clear_words(uint64_t* words, uint32_t count) {
@@ -199,28 +242,14 @@ __global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
         s = {-INFINITY, 0.0f, kNowhere};
         for (uint32_t c = 0; c < a.chunks; ++c) {
             float4 other[kWholeFours];
-            s = join_stats(s, joined(chunk_stats(x, lead, a.vocabulary, c * kWholeChunk + 4 * threadIdx.x, rate, other), rate, parts), rate);
+            const RowStats part = chunk_stats(x, lead, a.vocabulary, c * kWholeChunk + 4 * threadIdx.x, rate, other);
+            s = join_stats(s, joined(part, rate, parts), rate);
             __syncthreads();
         }
     } else {
         s = whole;
     }
-    const float inverse = s.sum == 0.0f ? 0.0f : 1.0f / s.sum;
-    const float largest = s.largest == -INFINITY ? 0.0f : s.largest;
-#pragma unroll
-    for (uint32_t i = 0; i < kWholeFours; ++i) {
-        const uint32_t to = at0 + 4 * kWholeThreads * i;
-        if (to >= lead + a.vocabulary) break;
-        float4 p;
-        if (at) {
-            const uint32_t hit = s.at == kNowhere ? kNowhere : s.at + lead - to;
-            p = {hit == 0 ? 1.0f : 0.0f, hit == 1 ? 1.0f : 0.0f, hit == 2 ? 1.0f : 0.0f, hit == 3 ? 1.0f : 0.0f};
-        } else {
-            p = {__builtin_amdgcn_exp2f((q[i].x - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].y - largest) * rate) * inverse,
-                 __builtin_amdgcn_exp2f((q[i].z - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].w - largest) * rate) * inverse};
-        }
-        write4(y, lead, a.vocabulary, to, p);
-    }
+    write_chunk(a, y, lead, at0, s, rate, q);
 }
 
 // Chunks of the two passes: about a thousand workgroups, a chunk of at least 2,048 logits.
@@ -238,6 +267,14 @@ uint64_t probabilities_bytes(uint32_t rows, uint32_t vocabulary) {
 }
 
 hipError_t launch_probabilities(Probabilities a, hipStream_t stream) {
+    if (a.vocabulary + 3 <= kWholeChunk) {
+        hipLaunchKernelGGL(row_alone<kWholeFours>, dim3(a.rows), dim3(kWholeThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    if (a.vocabulary + 3 <= 2 * kWholeChunk && a.rows >= kAloneRows) {
+        hipLaunchKernelGGL(row_alone<2 * kWholeFours>, dim3(a.rows), dim3(kWholeThreads), 0, stream, a);
+        return hipGetLastError();
+    }
     a.chunks = whole_chunks(a.rows, a.vocabulary);
     if (a.chunks && a.logits != a.output) {
         const uint32_t words = a.rows * a.chunks;

@@ -915,3 +915,22 @@ def test_blocks_whose_largest_magnitude_has_both_signs(ctx, dev, format_, tokens
     assert np.array_equal(kr().reshape(k.shape), ref.stored(k, format_), equal_nan=True)
     assert np.array_equal(vr().reshape(v.shape), ref.stored(v, format_), equal_nan=True)
     c.free()
+
+
+@pytest.mark.parametrize("rows,vocabulary,temperature,layout", [
+    # a workgroup a row up to a chunk of 16,384 (at any alignment), from 48 rows up to two; else two passes
+    (3, 16381, 1.0, {"offset": 4}), (2, 16382, 1.0, {}), (5, 16384, 0.5, {"in_place": True}), (47, 20001, 1.0, {"offset": 8}),
+    (48, 16382, 1.0, {"offset": 12}), (50, 32765, 0.9, {"in_place": True}), (64, 32765, 1.0, {"stride": 32771, "offset": 4}),
+    (70, 20001, 1.0, {"output_offset": 4}), (60, 32766, 1.0, {}), (6, 70001, 0.7, {"stride": 70003, "in_place": True})])
+def test_probabilities_by_one_workgroup_and_by_several(ctx, dev, rows, vocabulary, temperature, layout):
+    test_probabilities(ctx, dev, rows, vocabulary, temperature, layout)
+
+
+@pytest.mark.parametrize("rows,vocabulary", [(6, 40001), (60, 20001), (6, 12001)])
+def test_probabilities_at_temperature_zero_by_each_form(ctx, dev, rows, vocabulary):
+    test_probabilities_at_temperature_zero_take_the_first_largest(ctx, dev, rows, vocabulary)
+
+
+@pytest.mark.parametrize("rows,vocabulary", [(6, 40001), (60, 20001), (6, 12001)])
+def test_probabilities_of_rows_not_finite_by_each_form(ctx, dev, rows, vocabulary):
+    test_probabilities_of_rows_with_nothing_or_not_finite(ctx, dev, rows, vocabulary)
