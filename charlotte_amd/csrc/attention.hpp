@@ -33,12 +33,12 @@
 //
 // Bound and measured (8 key heads; a large copy moves 5.1 TB/s, a large binary16
 // product of the library's runs at 1.1 - 1.16 PFLOP/s):
-//   one token of 32 heads of 128 over 65,536 in Q8_0, by the cache's 142 MB: 30.4
-//   us, 4.7 TB/s, and 4.6 to join its 32 splits;
-//   16 heads over 911, by the latency of a launch and its reads: 6.4 and 3.5 us;
+//   one token of 32 heads of 128 over 65,536 in Q8_0, by the cache's 142 MB: 30.2
+//   us, 4.7 TB/s, and 4.5 to join its 32 splits;
+//   16 heads over 911, by the latency of a launch and its reads: 6.4 and 3.2 us;
 //   a tree of 21 tokens of 32 heads of 64 over 8,191 in Q4_0, by the VALU - some
 //   500 instructions a tile of 32 rows: codes widened, the probabilities scaled
-//   and parted for each block of values: 15.9 and 4.0 us;
+//   and parted for each block of values: 15.6 and 4.0 us;
 //   512 tokens of 32 heads of 128 over 15,873 in Q8_0 (attend_rows), by the matrix
 //   instructions: 339 GFLOP with queries, probabilities and values in parts (135
 //   by the formula), 320 - 340 us, 1.06 PFLOP/s; matrix cores busy 51% and the VALU

@@ -9,9 +9,10 @@ namespace chm {
 namespace {
 
 // Tiles a split takes at least: of wide binary16 heads two, but four once that
-// makes more than 32 splits (126 tiles of one head: 17.8 us in 63, 16.5 in 32).
+// makes more than 64 splits (126 tiles of one head: 13.9 us in 63, 15.6 in 32; 501
+// tiles: 24.4 in 250, 20.8 in 126).
 uint64_t least_tiles(const CacheShape& cache, uint64_t tiles) {
-    return cache.format == kF16 && cache.head_dim > 128 && tiles <= 64 ? 2 : 4;
+    return cache.format == kF16 && cache.head_dim > 128 && tiles <= 128 ? 2 : 4;
 }
 
 // Waves of 32 rows a workgroup of attend_rows holds.
@@ -79,7 +80,7 @@ uint64_t attention_partial_bytes(const CacheShape& cache, uint32_t query_heads, 
 }
 
 // Over every number of tokens up to `tokens` and every `longest`: most splits
-// come of the fewest workgroups and of all the tiles, or the 64 that are still
+// come of the fewest workgroups and of all the tiles, or the 128 that are still
 // split by two; of the tokens that make as many groups the last needs most.
 uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t compute_units) {
     const uint64_t tiles = groups_of(cache.capacity, 32), shared = query_heads / cache.kv_heads;
@@ -91,7 +92,7 @@ uint64_t attention_workspace_bytes(const CacheShape& cache, uint32_t query_heads
         const uint64_t last = std::min<uint64_t>(row_groups * group, rows <= 16 * waves ? 16 * waves : UINT64_MAX);
         t = std::max(t, std::min<uint64_t>(tokens, last / shared));
         const uint64_t splits = std::max(splits_of(cache, row_groups, tiles, compute_units),
-                                         splits_of(cache, row_groups, std::min<uint64_t>(tiles, 64), compute_units));
+                                         splits_of(cache, row_groups, std::min<uint64_t>(tiles, 128), compute_units));
         most = std::max(most, attention_partial_bytes(cache, query_heads, static_cast<uint32_t>(t),
                                                       static_cast<uint32_t>(splits)));
         if (group == 32 * waves && splits < 2) break;
