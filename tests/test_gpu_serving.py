@@ -934,3 +934,63 @@ def test_probabilities_at_temperature_zero_by_each_form(ctx, dev, rows, vocabula
 @pytest.mark.parametrize("rows,vocabulary", [(6, 40001), (60, 20001), (6, 12001)])
 def test_probabilities_of_rows_not_finite_by_each_form(ctx, dev, rows, vocabulary):
     test_probabilities_of_rows_with_nothing_or_not_finite(ctx, dev, rows, vocabulary)
+
+
+@pytest.mark.parametrize("sequences,tokens,vocabulary", [(2, 7, 5003), (2, 7, 40001), (3, 26, 140001)])
+def test_a_captured_verification_replays_on_new_logits(ctx, dev, sequences, tokens, vocabulary):
+    """Probabilities (a workgroup a row, two passes, rows read once), a tree's verification and the slots kept, in one
+    graph, each replay against the same calls made eagerly."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+
+    rng = np.random.default_rng(vocabulary)
+    rows, past, dim = sequences * tokens, 40, 64
+    parents = np.stack([_random_tree(rng, tokens) for _ in range(sequences)])
+    k = rng.standard_normal((sequences, past + tokens, 1, dim)).astype(np.float32)
+    logits, uniforms, nodes = hx.Buffer(4 * rows * vocabulary), hx.Buffer(4 * rows), hx.Buffer(4 * rows)
+    need = max(sv.probabilities_workspace_bytes(rows, vocabulary), sv.verify_workspace_bytes(sequences, tokens, vocabulary))
+    work, _ = dev.room(need, np.uint8)
+    at, tree = dev.put(np.full(sequences, past, np.uint32)), dev.put(parents)
+
+    class Side:
+        def __init__(self):
+            self.out, self.read = dev.room(rows * vocabulary)
+            self.cache = dev.cache("q8_0", k, k, past + tokens)
+            self.results = [dev.room(rows, np.int32), dev.room(rows, np.int32), dev.room(sequences, np.uint32)]
+            self.soft = sv.Probabilities(logits.ptr, self.out, rows, vocabulary, 0.9, workspace=work, workspace_bytes=need)
+            self.check = sv.Verify(nodes.ptr, self.out, uniforms.ptr, vocabulary, *(r[0] for r in self.results), parents=tree,
+                                   workspace=work, workspace_bytes=need)
+            self.slots = dev.room(k.size), dev.room(k.size)
+
+        def run(self, stream):
+            sv.probabilities(ctx, self.soft, stream=stream)
+            sv.verify(ctx, self.check, sequences, tokens, stream=stream)
+            self.cache.keep(at, self.results[0][0], self.results[2][0], tokens, stream=stream)
+
+        def all(self):
+            (ko, kr), (vo, vr) = self.slots
+            self.cache.read(ko, vo, dev.put(np.zeros(sequences, np.uint32)), past + tokens)
+            hx.sync()
+            return [self.read(), *(r[1]() for r in self.results), kr(), vr()]
+
+    eager, captured = Side(), Side()
+    stream = hx.Stream()
+    graph = hx.Graph(stream, lambda: captured.run(stream.handle), global_mode=True)
+    for replay in range(4):
+        x = rng.standard_normal((rows, vocabulary)).astype(np.float32)
+        x[:, :3] += 8 + replay
+        logits.write(x)
+        uniforms.write(rng.random(rows, np.float32))
+        nodes.write(rng.integers(0, 3, rows).astype(np.int32))
+        graph.launch()
+        stream.sync()
+        eager.run(None)
+        hx.sync()
+        for a, b in zip(captured.all(), eager.all()):
+            assert np.array_equal(a, b)
+    graph.destroy()
+    stream.destroy()
+    for b in (logits, uniforms, nodes):
+        b.free()
+    for side in (eager, captured):
+        side.cache.free()
