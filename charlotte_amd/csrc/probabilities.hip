@@ -48,16 +48,12 @@ __device__ __forceinline__ uint32_t share_of(const Probabilities& a) {
     return ((a.vocabulary + 3 + a.chunks - 1) / a.chunks + 3) / 4 * 4;
 }
 
-__global__ __launch_bounds__(256) void row_stats(Probabilities a) {
-    __shared__ RowStats parts[4];
-    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const float* x = a.logits + row * a.logit_stride;
-    const uint32_t lead = lead_of(x), share = share_of(a);
-    const float rate = a.temperature > 0.0f ? kPerOctave / a.temperature : 0.0f;
+// A thread's part of a row's statistics: fours from `at` to `end`, `step` apart.
+__device__ __forceinline__ RowStats running_stats(const float* x, uint32_t lead, uint32_t vocabulary, uint32_t at, uint32_t end,
+                                                  uint32_t step, float rate) {
     RowStats s = {-INFINITY, 0.0f, kNowhere};
-    const uint32_t end = min((chunk + 1) * share, lead + a.vocabulary);
-    for (uint32_t at = chunk * share + 4 * threadIdx.x; at < end; at += 1024) {
-        const float4 q = read4(x, lead, a.vocabulary, at, -INFINITY);
+    for (; at < end; at += step) {
+        const float4 q = read4(x, lead, vocabulary, at, -INFINITY);
         const float v[4] = {q.x, q.y, q.z, q.w};
         const float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
         if (top > s.largest) {
@@ -69,6 +65,17 @@ __global__ __launch_bounds__(256) void row_stats(Probabilities a) {
         for (int e = 0; e < 4; ++e)
             s.sum += v[e] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v[e] - s.largest) * rate);
     }
+    return s;
+}
+
+__global__ __launch_bounds__(256) void row_stats(Probabilities a) {
+    __shared__ RowStats parts[4];
+    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const float* x = a.logits + row * a.logit_stride;
+    const uint32_t lead = lead_of(x), share = share_of(a);
+    const float rate = a.temperature > 0.0f ? kPerOctave / a.temperature : 0.0f;
+    RowStats s = running_stats(x, lead, a.vocabulary, chunk * share + 4 * threadIdx.x,
+                               min((chunk + 1) * share, lead + a.vocabulary), 1024, rate);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
     if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = s;
@@ -239,13 +246,7 @@ __global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
     }
     __syncthreads();
     if (late) {  // the row's statistics by this workgroup alone
-        s = {-INFINITY, 0.0f, kNowhere};
-        for (uint32_t c = 0; c < a.chunks; ++c) {
-            float4 other[kWholeFours];
-            const RowStats part = chunk_stats(x, lead, a.vocabulary, c * kWholeChunk + 4 * threadIdx.x, rate, other);
-            s = join_stats(s, joined(part, rate, parts), rate);
-            __syncthreads();
-        }
+        s = joined(running_stats(x, lead, a.vocabulary, 4 * threadIdx.x, lead + a.vocabulary, 4 * kWholeThreads, rate), rate, parts);
     } else {
         s = whole;
     }
