@@ -15,8 +15,8 @@
 // none depends on when another runs. (That needs the logits as they were, so a
 // step in place takes the two passes.)
 //
-// Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 80 us (4.4 TB/s;
-// two passes 94), 1,024 x 131,072: 205 us (5.2 TB/s; 324); 6 x 151,936: passes of
+// Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 66 us (5.3 TB/s;
+// two passes 94), 1,024 x 131,072: 186 us (5.8 TB/s; 324); 6 x 151,936: passes of
 // 4.0 and 4.8 us, a launch's latency each.
 #include <algorithm>
 
@@ -121,6 +121,12 @@ constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWhol
 // once: of 151,936, 32 rows (19 MB) 14.7 us read once and 13.8 in two passes, 64
 // (39 MB) 23.7 and 23.6, 100 (61 MB) 29.0 and 33.7, 128 (78 MB) 36.2 and 40.7.
 constexpr uint64_t kWholeBytes = 40ull << 20;
+// Logits past which, with as many probabilities, they leave the caches anyway and
+// are read without being kept there: 102 MB 42.4 us either way, 176 MB 66.0 and,
+// kept, 72.3 (the logits written before and their verification after: 171 and
+// 183); of 51 MB, which an earlier launch may have left there, 27.8 and 24.0.
+// (Probabilities written past the caches would cost their reader more.)
+constexpr uint64_t kOnceBytes = 128ull << 20;
 // Rows from which a row of one to two chunks is one workgroup's, in one launch:
 // of 32,000, 6 rows 8.0 us so and 7.1 in two passes (one compute unit reads 128
 // KB in 4), 48 rows 8.7 and 8.8, 168 rows 11.0 and 14.6, 1,000 rows 39.8 and 46.7.
@@ -148,11 +154,11 @@ __device__ __forceinline__ RowStats joined(RowStats s, float rate, RowStats* par
 }
 
 // A chunk's fours from `at0` on, in registers, and the thread's part of its statistics.
-template <uint32_t FOURS>
+template <bool ONCE, uint32_t FOURS>
 __device__ __forceinline__ RowStats chunk_stats(const float* x, uint32_t lead, uint32_t vocabulary, uint32_t at0, float rate,
                                                 float4 (&q)[FOURS]) {
 #pragma unroll
-    for (uint32_t i = 0; i < FOURS; ++i) q[i] = read4(x, lead, vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
+    for (uint32_t i = 0; i < FOURS; ++i) q[i] = read4<ONCE>(x, lead, vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
     RowStats s = {-INFINITY, 0.0f, kNowhere};
 #pragma unroll
     for (uint32_t i = 0; i < FOURS; ++i) s.largest = fmaxf(s.largest, fmaxf(fmaxf(q[i].x, q[i].y), fmaxf(q[i].z, q[i].w)));
@@ -198,7 +204,7 @@ __global__ __launch_bounds__(kWholeThreads) void row_alone(Probabilities a) {
     const float rate = a.temperature > 0.0f ? kPerOctave / a.temperature : 0.0f;
     float4 q[FOURS];
     // every thread's reads are before the barrier in `joined`: the output may be the logits
-    const RowStats s = joined(chunk_stats(x, lead, a.vocabulary, at0, rate, q), rate, parts);
+    const RowStats s = joined(chunk_stats<false>(x, lead, a.vocabulary, at0, rate, q), rate, parts);
     write_chunk(a, a.output + blockIdx.x * a.output_stride, lead, at0, s, rate, q);
 }
 
@@ -207,6 +213,7 @@ __global__ __launch_bounds__(256) void clear_words(uint64_t* words, uint32_t cou
     if (i < count) words[i] = 0;
 }
 
+template <bool ONCE>
 __global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
     __shared__ RowStats parts[kWholeThreads / 64];
     __shared__ RowStats whole;
@@ -220,7 +227,7 @@ __global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
     uint64_t* words = reinterpret_cast<uint64_t*>(a.stats) + static_cast<uint64_t>(row) * a.chunks;
 
     float4 q[kWholeFours];
-    RowStats s = joined(chunk_stats(x, lead, a.vocabulary, at0, rate, q), rate, parts);
+    RowStats s = joined(chunk_stats<ONCE>(x, lead, a.vocabulary, at0, rate, q), rate, parts);
     if (threadIdx.x == 0)
         __hip_atomic_store(words + chunk, published(s, at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (threadIdx.x < 64) {
@@ -281,7 +288,10 @@ hipError_t launch_probabilities(Probabilities a, hipStream_t stream) {
         const uint32_t words = a.rows * a.chunks;
         hipLaunchKernelGGL(clear_words, dim3((words + 255) / 256), dim3(256), 0, stream, reinterpret_cast<uint64_t*>(a.stats), words);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        hipLaunchKernelGGL(row_whole, dim3(words), dim3(kWholeThreads), 0, stream, a);
+        if (uint64_t{a.rows} * a.vocabulary * 4 > kOnceBytes)
+            hipLaunchKernelGGL(row_whole<true>, dim3(words), dim3(kWholeThreads), 0, stream, a);
+        else
+            hipLaunchKernelGGL(row_whole<false>, dim3(words), dim3(kWholeThreads), 0, stream, a);
         return hipGetLastError();
     }
     a.chunks = pass_chunks(a.rows, a.vocabulary);

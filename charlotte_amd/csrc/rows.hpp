@@ -14,9 +14,15 @@ __device__ __forceinline__ uint32_t lead_of(const float* row) {
 }
 
 // Entries at .. at + 3 counted from the boundary, `at` a multiple of 4;
-// `outside` for those not of the row's `length`.
+// `outside` for those not of the row's `length`. ONCE: not kept in the caches.
+template <bool ONCE = false>
 __device__ __forceinline__ float4 read4(const float* row, uint32_t lead, uint32_t length, uint32_t at, float outside) {
-    if (at >= lead && at + 4 <= lead + length) return *reinterpret_cast<const float4*>(row - lead + at);
+    if (at >= lead && at + 4 <= lead + length) {
+        typedef float vector_t __attribute__((ext_vector_type(4)));
+        const auto* from = reinterpret_cast<const vector_t*>(row - lead + at);
+        const vector_t v = ONCE ? __builtin_nontemporal_load(from) : *from;
+        return {v.x, v.y, v.z, v.w};
+    }
     float v[4];
 #pragma unroll
     for (uint32_t e = 0; e < 4; ++e) v[e] = at + e >= lead && at + e < lead + length ? row[at + e - lead] : outside;
