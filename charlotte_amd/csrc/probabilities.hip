@@ -117,10 +117,11 @@ __global__ __launch_bounds__(256) void row_probabilities(Probabilities a) {
 // ---- whole rows in one read ---------------------------------------------------------
 
 constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWholeThreads * kWholeFours;
-// Logits past which the second read would be memory's again, and rows are read
-// once: of 151,936, 32 rows (19 MB) 14.7 us read once and 13.8 in two passes, 64
-// (39 MB) 23.7 and 23.6, 100 (61 MB) 29.0 and 33.7, 128 (78 MB) 36.2 and 40.7.
-constexpr uint64_t kWholeBytes = 40ull << 20;
+// Logits past which rows are read once, their second read no longer all from
+// cache: of 151,936, 12 rows (7 MB) 10.6 us read once and 10.1 in two passes, 32
+// (19 MB) 14.9 and 14.0, 42 (26 MB) 15.7 and 16.9, 64 (39 MB) 18.9 and 23.5, 100 (61
+// MB) 25.7 and 33.5; of 262,144, 21 rows (22 MB) 15.4 and 15.6.
+constexpr uint64_t kWholeBytes = 22ull << 20;
 // Logits past which, with as many probabilities, they leave the caches anyway and
 // are read without being kept there: 102 MB 42.4 us either way, 176 MB 66.0 and,
 // kept, 72.3 (the logits written before and their verification after: 171 and
