@@ -9,13 +9,14 @@
 // probabilities. A chain with a draft draws once a sequence, from the row where
 // its walk ends; every workgroup walks it anew (a lane a token, three reads
 // each), which costs less than a launch. walk_*: a wave a draw sums the
-// segments, a lane a run of them, finds the segment, and reads it again (from
-// cache) for the index: two dependent reads. Without a draft a workgroup a
+// segments, a lane a run of them, finds the segment, and reads its entries again
+// (from cache) for the index: two dependent reads. Without a draft a workgroup a
 // sequence draws for every node and its first wave then walks the tree.
 //
 // Bound by bytes: 4 a probability of the rows drawn from, once. A tree of 21 nodes
-// over 151,936 (12.8 MB): 5.1 us, and its walk 7.8: one compute unit reads the 21
-// rows' sums, 100 KB. Chains of 6 in 8 sequences over 128,256: 4.2 and 4.8.
+// over 151,936 (12.8 MB): 5.1 us, and its walk 6.4: one compute unit reads the 21
+// rows' sums, 100 KB (7.8 with each lane's run read where it lies, through no
+// LDS). Chains of 6 in 8 sequences over 128,256: 4.1 and 4.4.
 #include <algorithm>
 
 #include "rows.hpp"
@@ -146,30 +147,44 @@ __global__ __launch_bounds__(256) void draw_sums(Verify a) {
     }
 }
 
-// The wave's running sum: each lane's, itself included.
+// The wave's running sum: each lane's, itself included. Within rows of 16 lanes,
+// then over the rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t x) {
+    const int low = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xF, false);
+    const int high = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), CTRL, ROWS, 0xF, false);
+    return static_cast<uint64_t>(static_cast<uint32_t>(high)) << 32 | static_cast<uint32_t>(low);
+}
 __device__ __forceinline__ uint64_t running(uint64_t x) {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up(static_cast<unsigned long long>(x), o);
-        if (lane >= o) x += y;
-    }
+    x += moved<0x111, 0xF>(x);  // from 1, 2, 4 and 8 lanes before, in the row
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    x += moved<0x142, 0xA>(x);  // the last of rows 0 and 2 to rows 1 and 3
+    x += moved<0x143, 0xC>(x);  // the last of the first two to the others
     return x;
 }
 
+// The segments a row may have, 2^18 entries at any boundary, and of them a lane's.
+constexpr uint32_t kSegments = segments_of(1u << 18), kRun = (kSegments + 63) / 64;
+
 // The token drawn from `r` by uniform number u, its segments' sums at `sums`:
-// by one wave, every lane the same.
-__device__ uint32_t drawn_from(const Verify& a, const DrawRow& r, const uint64_t* sums, float u) {
-    const uint32_t lane = threadIdx.x & 63u, all = segments_of(a.vocabulary);
-    // a lane's run of the segments, at most kRun (of 2^18 entries: 1,025 segments)
-    constexpr uint32_t kRun = 17;
-    const uint32_t run = (all + 63) / 64;
-    uint64_t held[kRun], mine = 0;
+// by one wave, every lane the same. `held` (LDS) is the wave's: a lane's run of
+// the sums, read there side by side, is one of neighbours. Runs are odd, so that
+// the lanes' places fall on all banks.
+__device__ __forceinline__ uint32_t drawn_from(const Verify& a, const DrawRow& r, const uint64_t* sums, float u, uint64_t* held) {
+    const uint32_t lane = threadIdx.x & 63u, all = segments_of(a.vocabulary), run = (all + 63) / 64 | 1u;
+    uint64_t got[kRun];
 #pragma unroll
-    for (uint32_t i = 0; i < kRun; ++i) {
-        held[i] = i < run && lane * run + i < all ? sums[lane * run + i] : 0;
-        mine += held[i];
-    }
+    for (uint32_t i = 0; i < kRun; ++i) got[i] = 64 * i + lane < all ? sums[64 * i + lane] : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i)
+        if (64 * i + lane < all) held[64 * i + lane] = got[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint64_t mine = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < run; ++i)
+        if (lane * run + i < all) mine += held[lane * run + i];
     uint64_t to = running(mine);
     const uint64_t total = __shfl(static_cast<unsigned long long>(to), 63);
     if (total == 0) return 0;
@@ -178,15 +193,15 @@ __device__ uint32_t drawn_from(const Verify& a, const DrawRow& r, const uint64_t
     const uint64_t by = static_cast<uint32_t>(scaled);
     const uint64_t passed = __umul64hi(total, by) << 33 | (total * by) >> 31;
 
-    // the lane whose run passes it, its first segment that does, and the sum before that
-    const int owner = __builtin_ctzll(__ballot(to > passed));
-    uint64_t before = to - mine;
-    uint32_t segment = lane * run;
-#pragma unroll
-    for (uint32_t i = 0; i < kRun; ++i)
-        if (segment == lane * run + i && before + held[i] <= passed) before += held[i], ++segment;
-    before = __shfl(static_cast<unsigned long long>(before), owner);
-    segment = __shfl(segment, owner);
+    // the first run that passes it, a lane a segment of that run (at most 17), and
+    // its first segment that does
+    const uint32_t owner = static_cast<uint32_t>(__builtin_ctzll(__ballot(to > passed)));
+    uint64_t before = __shfl(static_cast<unsigned long long>(to - mine), owner);
+    mine = lane < run && owner * run + lane < all ? held[owner * run + lane] : 0;
+    to = before + running(mine);
+    const uint32_t place = static_cast<uint32_t>(__builtin_ctzll(__ballot(to > passed)));
+    before = __shfl(static_cast<unsigned long long>(to - mine), place);
+    const uint32_t segment = owner * run + place;
 
     const uint32_t lead = lead_of(r.target), at = segment * kSegment + 4 * lane;
     const float4 v = weights4(r, lead, a.vocabulary, at);
@@ -204,6 +219,7 @@ __device__ uint32_t drawn_from(const Verify& a, const DrawRow& r, const uint64_t
 
 // A chain with a draft: a wave a sequence; draw_sums left where its walk ended.
 __global__ __launch_bounds__(64) void walk_chain(Verify a) {
+    __shared__ uint64_t held[kSegments];
     const uint32_t sequence = blockIdx.x, lane = threadIdx.x;
     const uint32_t length = length_of(a, sequence);
     const uint64_t first = static_cast<uint64_t>(sequence) * a.tokens;
@@ -212,7 +228,7 @@ __global__ __launch_bounds__(64) void walk_chain(Verify a) {
         const uint32_t node = static_cast<uint32_t>(a.drawn[sequence]);
         count = node + 1;
         token = drawn_from(a, row_of(a, sequence, node, count < length),
-                           a.sums + static_cast<uint64_t>(sequence) * segments_of(a.vocabulary), a.uniforms[first + node]);
+                           a.sums + static_cast<uint64_t>(sequence) * segments_of(a.vocabulary), a.uniforms[first + node], held);
     }
     for (uint32_t i = lane; i < a.tokens; i += 64) {
         a.path[first + i] = i < count ? static_cast<int32_t>(i) : -1;
@@ -225,6 +241,7 @@ __global__ __launch_bounds__(64) void walk_chain(Verify a) {
 // from node 0, each step to the first child with the token drawn.
 __global__ __launch_bounds__(64 * kWalkWaves) void walk_tree(Verify a) {
     __shared__ int32_t drawn[kVerifyTokens], tokens[kVerifyTokens], parents[kVerifyTokens];
+    __shared__ uint64_t held[kWalkWaves][kSegments];
     const uint32_t sequence = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t length = length_of(a, sequence);
     const uint64_t first = static_cast<uint64_t>(sequence) * a.tokens;
@@ -234,7 +251,7 @@ __global__ __launch_bounds__(64 * kWalkWaves) void walk_tree(Verify a) {
     }
     for (uint32_t node = wave; node < length; node += kWalkWaves) {
         const uint32_t token = drawn_from(a, row_of(a, sequence, node, false), a.sums + (first + node) * segments_of(a.vocabulary),
-                                          a.uniforms[first + node]);
+                                          a.uniforms[first + node], held[wave]);
         if (lane == 0) drawn[node] = static_cast<int32_t>(token);
     }
     __syncthreads();
