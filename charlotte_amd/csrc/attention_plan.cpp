@@ -30,11 +30,12 @@ uint64_t splits_of(const CacheShape& cache, uint64_t row_groups, uint64_t tiles,
 
 // `load`: the step's blocks of 16 or 32 rows by a tile, for each compute unit.
 //
-// Workgroups of 16 rows (attend, one octet pair a wave) have the shorter chain
-// of products, and read the cache once for every 16 rows; they are taken while
-// load16 <= 24 and none has to wait for another's compute unit. 8 key heads of
-// 128, 20 rows over 8,000: 16.0 us, by 32 rows 18.6; 48 rows over 1,000 in
-// binary16 10.2 and 15.2, over 8,000 (load16 = 24) 26.8 and 23.7. Quantized
+// Workgroups of 16 rows (attend) have the shorter chain of products, and read
+// the cache once for every 16 rows; they are taken while load16 <= 24 and none
+// has to wait for another's compute unit. 8 key heads of 128, 20 rows over 8,000
+// in Q8_0: 16.0 us, by 32 rows 18.6; in binary16 over 500 10.2 and 15.3, 48 rows
+// over 8,000 (load16 = 24) 26.8 and 23.7; 128 rows of 8 sequences with none before
+// (twice as many workgroups as compute units) 13.6 and 10.5. Quantized
 // heads past 64, whose codes cost more to widen than to read, up to 64: 84 rows
 // over 8,000 (48) 31.5 and 34.5, over 60,000 (352) 153 and 136.
 //

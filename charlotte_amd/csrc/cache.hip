@@ -270,9 +270,10 @@ __device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t t) {
 }
 
 // A wave's unit, its lane's 16 values in it and which of them the step holds.
-// Value e of token part p: keys - value 8 (lane / 16) + e of token 16p + lane %
-// 16 (in memory, `exchange`: 4 (lane / 16) + e, 16 further on for e >=
-// 4, so that a wave's load or store has 64 bytes of each token); values - value 16p + lane % 16 of the token of slot e of group lane / 16.
+// Value e of token part p: keys - value 8 (lane / 16) + e of token 16p + lane % 16
+// (in memory, `exchange`, 4 (lane / 16) + e, and 16 further on for e >= 4, so that
+// a wave's load or store has 64 bytes of each token); values - value 16p + lane %
+// 16 of the token of slot e of group lane / 16.
 template <bool VALUES>
 struct Unit {
     uint32_t sequence, head, block, lane;
