@@ -298,7 +298,7 @@ struct Unit {
         tile = uint64_t{past / kTile} + at % tiles;
         limit = past < a.cache.capacity ? min(a.tokens, a.cache.capacity - past) : 0u;
         const int64_t from = static_cast<int64_t>(tile * kTile) - past;
-        live = live && from < limit;
+        live = live && limit > 0 && from < limit;  // a step past the capacity has no unit at all
         ahead = static_cast<int32_t>(from);
         whole = ahead >= 0 && ahead + static_cast<int32_t>(kTile) <= static_cast<int32_t>(limit);
         stride = VALUES ? a.value_stride : a.key_stride;

@@ -994,3 +994,34 @@ def test_a_captured_verification_replays_on_new_logits(ctx, dev, sequences, toke
         b.free()
     for side in (eager, captured):
         side.cache.free()
+
+
+@pytest.mark.parametrize("format_", ["q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("tokens", [16, 40])
+def test_blocks_behind_the_capacity_reach_nothing(ctx, dev, format_, tokens):
+    """Steps written and read by whole units whose first slot lies past the capacity, at any place
+    of a tile: no slot of the cache, of any sequence or head, and no row read back changes."""
+    from charlotte_amd import harness as hx
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(7)
+    k, v = (rng.standard_normal((2, 70, 2, 64)).astype(np.float32) for _ in range(2))
+    c = dev.cache(format_, k, v, 70)
+    step = dev.put(rng.standard_normal((2 * tokens, 2 * 64)).astype(np.float32))
+    rows = np.full((2 * tokens, 2 * 64), 5.0, np.float32)
+    for past in ([70, 71], [95, 96], [101, 1000], [0x7FFFFFF1, 0xFFFFFFFF]):
+        slots = dev.put(np.array(past, np.uint32))
+        c.append(step, step, slots, tokens)
+        (ko, kr), (vo, vr) = dev.room(rows.size), dev.room(rows.size)
+        c.read(ko, vo, dev.put(np.zeros(2, np.uint32)), tokens)
+        hx.sync()
+        before = kr().copy(), vr().copy()
+        c.read(ko, vo, slots, tokens)
+        hx.sync()
+        assert np.array_equal(kr(), before[0]) and np.array_equal(vr(), before[1])
+    (ko, kr), (vo, vr) = dev.room(k.size), dev.room(v.size)
+    c.read(ko, vo, dev.put(np.zeros(2, np.uint32)), 70)
+    hx.sync()
+    assert np.array_equal(kr().reshape(k.shape), ref.stored(k, format_))
+    assert np.array_equal(vr().reshape(v.shape), ref.stored(v, format_))
+    c.free()
