@@ -194,7 +194,8 @@ __device__ __forceinline__ void write_chunk(const Probabilities& a, float* y, ui
                  __builtin_amdgcn_exp2f((q[i].z - largest) * rate) * inverse, __builtin_amdgcn_exp2f((q[i].w - largest) * rate) * inverse};
         }
         write4(y, lead, a.vocabulary, to, p);
-    }}
+    }
+}
 
 // A row by one workgroup, in one launch: FOURS fours of logits a thread.
 template <uint32_t FOURS>
