@@ -12,16 +12,28 @@
 // lane, and the maximum and the sum of a row are four lanes' (two shuffles).
 //
 // Precision: activations are f32 and keep their bits. A query, times scale /
-// ln 2 and a power of two that puts its largest value in [2^10, 2^11), and a
-// probability times a value's scale are each taken as two binary16 parts, hi +
-// lo, about 22 bits; a cache's codes are exact in binary16. A block's key scale
-// multiplies its product in f32 (F16: none). Sums are f32 throughout.
+// ln 2 and a power of two that puts its largest value in [2^14, 2^15), and a
+// probability (attend_rows, F16) or its product with a value's scale are each
+// taken as two binary16 parts, hi + lo: 22 bits, but no less than the half of
+// binary16's least step, 2^-25. A cache's codes are exact in binary16. A block's
+// key scale multiplies its product in f32 (F16: none). Sums are f32 throughout.
 //
-// Range: values' scales, and so the outputs, are held over 2^D, D the exponent
-// of the largest scale met; the outputs follow where it grows, as they follow
-// the maximum. p is below 2^14 (the offset follows the maximum once a score
-// passes it by 2^8, which a tile seldom does) and p d below 2^15, so that the
-// parts' steps (2^-24) lie at least 30 bits below the largest.
+// Range: a query's parts leave 2^-22 of it, or 2^-39 of the row's largest. p is
+// 2^up at the maximum last followed, which follows once a score passes it by
+// 2^kSlack, so below 2^(up + kSlack):
+//   F16 and attend_rows  up = 11, p below 2^15: its parts leave 2^-22 of it, or
+//     2^-36 of the row's largest;
+//   attend, quantized    up = 7, and p d over 2^held below 2^15. held is that of
+//     the tile's largest scale, and stays while the tiles' scales lie within 2^-8
+//     to 2 of it; the outputs are held over it and follow. The parts leave 2^-21 of
+//     p d, or 2^-25 of the row's largest p times d. A tile whose own scales lie
+//     further apart - whether its rows see the tokens or not - takes p d in f32,
+//     and parts them over each row's largest, lo over a step of its own (wide).
+// attend_rows lays values out as code times scale over 2^held, in two parts that
+// are exact while the scale is 2^-14 or more: while the split's scales lie within
+// 2^22. It does so while they lie within 2^16, so that 2^-36 of a row's largest p
+// times any value is 2^-20 of the least block's; else its waves take the tiles as
+// attend's do.
 //
 // Split: where there are few products for each compute unit (attend), a
 // workgroup has 16 or 32 rows, those one wave holds; its waves take the tiles in
@@ -61,11 +73,16 @@ typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2E = 1.44269504088896340736f;
-// A probability is 2^kHeadroom at the maximum last followed, and a score may go
-// kSlack past it; the largest value scale met is 2^kScaleTop to twice it. Their
-// product stays below 2^15 (a half ends at 2^16).
-constexpr int kHeadroom = 7, kScaleTop = 3;
-constexpr float kSlack = 4.0f;
+// A probability is 2^up at the maximum last followed, and a score may go kSlack
+// past it; the largest value scale is held as 2^top to twice that. What is
+// parted stays below 2^15 or, a code of at most 7 bits times its scale, 2^16.
+constexpr int kSlack = 4;
+constexpr int kProductUp = 7, kScaleTop = 3;  // p d, of quantized values in attend
+constexpr int kAloneUp = 11, kCodeTop = 8;    // p, and code times scale
+static_assert(kProductUp + kSlack + kScaleTop + 1 <= 15 && kAloneUp + kSlack <= 15 && 7 + kCodeTop + 1 <= 16,
+              "past binary16");
+// How far below the largest, in octaves, scales may lie: of a tile in attend, of a split in attend_rows.
+constexpr int kTileSpread = 8, kSplitSpread = 16;
 
 // Four unsigned bytes, each raised by `raise`, as halves: under the high byte
 // 0x64 a byte c is 1,024 + c in binary16, and taking 1,024 + raise is exact.
@@ -133,18 +150,60 @@ __device__ __forceinline__ void split2(float a, float b, half2_t* hi, half2_t* l
                                   half2_t);
 }
 
-// The larger of two scales' magnitudes as bits, a NaN's as none.
-__device__ __forceinline__ uint32_t larger_scale(uint32_t w) {
-    const uint32_t lo = w & 0x7FFFu, hi = w >> 16 & 0x7FFFu;
-    return max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi);
+// A wave's scales, two a dword: the largest and least magnitudes as bits, of
+// those that are neither zero, which weighs nothing, nor a NaN.
+struct Scales {
+    uint32_t most = 0, least = 0x7FFFu;
+    bool nan = false;
+    __device__ __forceinline__ void add(uint32_t word) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t size = word >> (16 * h) & 0x7FFFu;
+            nan |= size > 0x7C00u;
+            most = max(most, size > 0x7C00u ? 0u : size);
+            least = min(least, size - 1 < 0x7C00u ? size : 0x7FFFu);
+        }
+    }
+    // The wave's, in every lane.
+    __device__ __forceinline__ void join() {
+        uint32_t both = most | (0x7FFFu - least) << 16;
+        auto more = [&](uint32_t other) {
+            both = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, both),
+                                                                          __builtin_bit_cast(ushort2_t, other)));
+        };
+        // within rows of 16 lanes, rotated by 1, 2, 4 and 8, then over the rows
+        more(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(both), 0x121, 0xF, 0xF, true)));
+        more(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(both), 0x122, 0xF, 0xF, true)));
+        more(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(both), 0x124, 0xF, 0xF, true)));
+        more(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(both), 0x128, 0xF, 0xF, true)));
+        const auto a = __builtin_amdgcn_permlane16_swap(both, both, false, false);
+        both = a[0], more(a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(both, both, false, false);
+        both = b[0], more(b[1]);
+        both = __builtin_amdgcn_readfirstlane(both);
+        most = both & 0xFFFFu, least = 0x7FFFu - (both >> 16);
+        nan = __any(nan);
+    }
+};
+// Where scales up to `most` are held over 2^held: the largest as 2^TOP to twice
+// that, but none times more than 2^15, which binary16 holds.
+template <int TOP>
+__device__ __forceinline__ int held_of(uint32_t most) {
+    return static_cast<int>(max(most >> 10, static_cast<uint32_t>(TOP))) - 15 - TOP;
 }
-// D: 2^D <= the scale < 2^(D + 1); any below 2^-12 counts as that.
-__device__ __forceinline__ int exponent_of(uint32_t bits) { return static_cast<int>(max(bits >> 10, 3u)) - 15; }
-// What a scale is multiplied by, a power of two: from 2^(3 - 15) to 2^(3 + 12), which binary16 holds.
-__device__ __forceinline__ half2_t over(int exponent) {
-    const _Float16 by = static_cast<_Float16>(ldexpf(1.0f, kScaleTop - exponent));
+// 2^-held, what a scale is multiplied by.
+__device__ __forceinline__ half2_t over(int held) {
+    const _Float16 by = static_cast<_Float16>(ldexpf(1.0f, -held));
     return half2_t{by, by};
 }
+// 2^x as binary16's bits; what lies below its least, as that.
+__device__ __forceinline__ uint32_t power_bits(int x) {
+    return x >= -14 ? static_cast<uint32_t>(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 1u;
+}
+
+// How a tile's values come: as codes and scales (attend), or laid out, scaled, in
+// two parts (attend_rows).
+enum Values : uint32_t { kCodes, kLaidOut };
 
 // Over the lanes that share a row: lane % 16, four of them, or lane % 32, two.
 template <uint32_t X>
@@ -300,7 +359,8 @@ struct Rows {
     float unit;                         // what a raw score stands for, a power of two
     result_t out[kOuts];
     float largest, offset, sum;         // the raw maximum; exp2's offset; the lane's part of the sum
-    int exponent;                       // D, the same in every lane
+    int held;                           // outputs are over 2^held, the same in every lane
+    uint32_t scale_low, scale_high;     // the scales that it stays for, each twice in its dword: the least's bits less one; the largest's
     Sight sight;
 
     // Where a lane's run of four output values stands in its row.
@@ -358,7 +418,7 @@ struct Rows {
         if (most > 0.0f && most <= 3.4e38f) {
             int e;
             (void)frexpf(most, &e);
-            shift = min(11 - e, 126);
+            shift = min(15 - e, 126);
         }
         unit = ldexpf(1.0f, -shift);
 #pragma unroll
@@ -370,7 +430,8 @@ struct Rows {
             high[b] = join(hi[0], hi[1], hi[2], hi[3]);
             low[b] = join(lo[0], lo[1], lo[2], lo[3]);
         }
-        exponent = F == kF16 ? kScaleTop : -64;
+        held = 0;
+        scale_low = 0xFFFEFFFEu, scale_high = 0x7FFF7FFFu;  // zeros alone
         largest = -INFINITY, offset = INFINITY, sum = 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < kOuts; ++t) out[t] = result_t(0.0f);
@@ -407,12 +468,29 @@ struct Rows {
 
     // One tile. `source` gives the operands: keys(b, i) and values(b, i), i = 0, 1
     // (X = 1: token half, 16 values; X = 2: 16 dims, 16 tokens), and an octet's
-    // scales, key_scale(b, x) and value_scale(b, x); and, PARTED, values_low(b, i),
-    // the values being scaled (over 2^D by 2^kScaleTop) and in two parts of their
-    // own: their scales are then looked at only where `spoilt`, some a NaN, stands.
-    template <bool PARTED, typename SOURCE, typename TREE>
+    // scales, key_scale(b, x) and value_scale(b, x), a dword a lane scale_word(i);
+    // and, kLaidOut, values_low(b, i): then held is the split's, and `spoilt` says
+    // whether some value scale of it is a NaN.
+    template <Values HOW, typename SOURCE, typename TREE>
     __device__ __forceinline__ void tile(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
                                          const SOURCE& source, bool spoilt = false) {
+        constexpr bool kFollowed = F != kF16 && HOW == kCodes;
+        // The value scales, each looked at by one lane, ahead of what waits for the products.
+        constexpr uint32_t kWords = (16 * NB + 63) / 64;
+        [[maybe_unused]] uint32_t word[kWords], outside = 0;
+        if constexpr (HOW == kCodes)
+#pragma unroll
+            for (uint32_t i = 0; i < kWords; ++i) {
+                word[i] = source.scale_word(i);
+                if constexpr (F == kF16) {
+                    outside |= word[i] ^ 0x3C003C00u;
+                } else {
+                    const auto size = __builtin_bit_cast(ushort2_t, F == kQ4_0 ? word[i] & 0x7FFF7FFFu : word[i]);
+                    const auto low = __builtin_bit_cast(ushort2_t, scale_low), high = __builtin_bit_cast(ushort2_t, scale_high);
+                    outside |= __builtin_bit_cast(uint32_t, __builtin_elementwise_min(ushort2_t(size - ushort2_t(1)), low)) ^ scale_low;
+                    outside |= __builtin_bit_cast(uint32_t, __builtin_elementwise_max(size, high)) ^ scale_high;
+                }
+            }
         float s[X][8];
         if constexpr (X == 1) {
             float4_t sums[2] = {float4_t(0.0f), float4_t(0.0f)};
@@ -435,25 +513,37 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[0][e] = sums[e >> 2][e & 3];
         } else {
-            float16_t sums = float16_t(0.0f);
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                float16_t p = key_scales(F) ? float16_t(0.0f) : sums;
+            float16_t sums = float16_t(0.0f), p[2];
+            auto product = [&](uint32_t b, float16_t from) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     const half8_t k = source.keys(b, y);
-                    p = multiply(k, low[2 * b + y], multiply(k, high[2 * b + y], p));
+                    from = multiply(k, low[2 * b + y], multiply(k, high[2 * b + y], from));
                 }
-                if constexpr (key_scales(F)) {
+                return from;
+            };
+            // attend_rows: a block's products are out before those of the one before it
+            // are scaled (512 tokens over 15,873: 327 us, else 330)
+            constexpr bool kAhead = HOW == kLaidOut && key_scales(F);
+            if constexpr (kAhead) p[0] = product(0, float16_t(0.0f));
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                if constexpr (!key_scales(F)) {
+                    sums = product(b, sums);
+                } else {
+                    if constexpr (kAhead) {
+                        if (b + 1 < NB) p[(b + 1) & 1] = product(b + 1, float16_t(0.0f));
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else {
+                        p[b & 1] = product(b, float16_t(0.0f));
+                    }
 #pragma unroll
                     for (uint32_t x = 0; x < 2; ++x) {
                         const uint4_t scale = source.key_scale(b, x);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            sums[8 * x + e] = __builtin_fmaf(p[8 * x + e], scale_at(scale, e), sums[8 * x + e]);
+                            sums[8 * x + e] = __builtin_fmaf(p[b & 1][8 * x + e], scale_at(scale, e), sums[8 * x + e]);
                     }
-                } else {
-                    sums = p;
                 }
             }
 #pragma unroll
@@ -472,91 +562,101 @@ struct Rows {
             }
         }
 
-        // The value scales: the largest's exponent, and all of them over 2^D.
-        uint4_t scale[NB][X];
-        int grown = exponent;
-        constexpr bool kScaled = F != kF16 && !PARTED;
-        if (kScaled || F == kF16 || spoilt) {
+        // Where some scale lies outside what the outputs are held for, all of them say over what.
+        int grown = held;
+        bool wide = false;
+        constexpr int kUp = kFollowed ? kProductUp : kAloneUp;
+        if constexpr (HOW == kCodes) {
+            spoilt = __any(outside != 0);
+            if constexpr (kFollowed)
+                if (spoilt) {
+                    Scales reach;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (uint32_t x = 0; x < X; ++x) scale[b][x] = source.value_scale(b, x);
+                    for (uint32_t i = 0; i < kWords; ++i) reach.add(word[i]);
+                    reach.join();
+                    spoilt = reach.nan;
+                    if (reach.most != 0) {
+                        grown = held_of<kScaleTop>(reach.most);
+                        const uint32_t from = power_bits(grown + kScaleTop - kTileSpread);
+                        scale_low = (from - 1) * 0x10001u;
+                        scale_high = (power_bits(grown + kScaleTop + 1) - 1) * 0x10001u;
+                        wide = reach.least < from;
+                    }
+                }
         }
-        if constexpr (F == kF16) {
-            uint32_t other = 0;
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (uint32_t x = 0; x < X; ++x)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) other |= scale[b][x][w] ^ 0x3C003C00u;
-            spoilt = __any(other != 0);
-        }
-        if constexpr (kScaled) spoilt = __any(largest_scale(scale) > 0x7C00u);
-        if (spoilt) spoil(a, group, tree, slot0, masked, scale);
-        if constexpr (kScaled) {
-            // the same in the lanes of a group
-            const uint32_t mine = largest_scale(scale);
-            const uint32_t most = X == 1 ? max(max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 16)),
-                                               max(__builtin_amdgcn_readlane(mine, 32), __builtin_amdgcn_readlane(mine, 48)))
-                                         : max(__builtin_amdgcn_readlane(mine, 0), __builtin_amdgcn_readlane(mine, 32));
-            grown = max(exponent, exponent_of(most));
-            const half2_t by = over(grown);
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
-#pragma unroll
-                for (uint32_t x = 0; x < X; ++x)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) scale[b][x][w] = __builtin_bit_cast(uint32_t, pair_of(scale[b][x][w]) * by);
-        }
+        if (__builtin_expect(spoilt, false)) spoil(a, group, tree, slot0, masked, source);
 
         float top = s[0][0];
 #pragma unroll
         for (int e = 1; e < 8 * static_cast<int>(X); ++e) top = fmaxf(top, s[e >> 3][e & 7]);
         top = most_of_row<X>(top);
         // the offset follows once a score passes it by kSlack (the first: -inf + inf is a NaN, no less than)
-        const bool follow = top > largest && !((top - largest) * unit <= kSlack);
-        if (__any(follow) || grown != exponent) {
+        const bool follow = top > largest && !((top - largest) * unit <= static_cast<float>(kSlack));
+        if (__any(follow) || grown != held) {
             const float most = fmaxf(largest, top);
             // the offset as used is what the factor is made of, so that its rounding cancels
-            const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit, static_cast<float>(kHeadroom));
+            const float to = most == -INFINITY ? INFINITY : __builtin_fmaf(-most, unit, static_cast<float>(kUp));
             const float factor = largest == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - offset);
-            const float down = factor * ldexpf(1.0f, exponent - grown);
+            const float down = factor * ldexpf(1.0f, held - grown);
             largest = most;
             offset = to;
             sum *= factor;
 #pragma unroll
             for (uint32_t t = 0; t < kOuts; ++t) out[t] *= down;
         }
-        exponent = grown;
+        held = grown;
 
         // rows that have seen nothing: -inf + inf would be a NaN
         const float to = largest == -INFINITY ? 0.0f : offset;
+        float p[X][8];
+        auto weigh = [&](uint32_t x) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], unit, to));
+            sum += ((p[x][0] + p[x][1]) + (p[x][2] + p[x][3])) + ((p[x][4] + p[x][5]) + (p[x][6] + p[x][7]));
+        };
+        if constexpr (kFollowed) {
+#pragma unroll
+            for (uint32_t x = 0; x < X; ++x) weigh(x);
+            if (__builtin_expect(wide, false)) {
+                widely(source, p, spoilt);
+                return;
+            }
+        }
+        [[maybe_unused]] const half2_t by = over(held);
         half2_t hi[X][4], lo[X][4];
 #pragma unroll
         for (uint32_t x = 0; x < X; ++x) {
-            float p[8];
+            if constexpr (!kFollowed) weigh(x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], unit, to));
-            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(p[2 * e], p[2 * e + 1], &hi[x][e], &lo[x][e]);
+            for (int e = 0; e < 4; ++e) split2(p[x][2 * e], p[x][2 * e + 1], &hi[x][e], &lo[x][e]);
         }
+        [[maybe_unused]] uint4_t ahead[X];
+        if constexpr (kFollowed)
+#pragma unroll
+            for (uint32_t x = 0; x < X; ++x) ahead[x] = finite_scale(source, 0, x, spoilt);
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
             half8_t first[X], second[X];
+            [[maybe_unused]] uint4_t scales[X];
+            if constexpr (kFollowed)
+#pragma unroll
+                for (uint32_t x = 0; x < X; ++x) {
+                    scales[x] = ahead[x];
+                    if (b + 1 < NB) ahead[x] = finite_scale(source, b + 1, x, spoilt);
+                }
 #pragma unroll
             for (uint32_t x = 0; x < X; ++x) {
-                if constexpr (!kScaled) {
+                if constexpr (!kFollowed) {
                     first[x] = join(hi[x][0], hi[x][1], hi[x][2], hi[x][3]);
                     second[x] = join(lo[x][0], lo[x][1], lo[x][2], lo[x][3]);
                 } else {
                     // (hi + lo) d in two parts: hi d rounded, what that leaves
                     // (exact: 22 bits less their first 11) plus lo d
+                    const uint4_t scale = scales[x];
                     half2_t u[4], w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const half2_t d = pair_of(scale[b][x][e]);
+                        const half2_t d = pair_of(scale[e]) * by;
                         u[e] = hi[x][e] * d;
                         w[e] = __builtin_elementwise_fma(lo[x][e], d, __builtin_elementwise_fma(hi[x][e], d, -u[e]));
                     }
@@ -569,55 +669,105 @@ struct Rows {
                 const half8_t v = source.values(b, i);
                 result_t& to = out[X == 1 ? 2 * b + i : b];
                 to = multiply(v, second[X == 1 ? 0 : i], multiply(v, first[X == 1 ? 0 : i], to));
-                if constexpr (PARTED && F != kF16) to = multiply(source.values_low(b, i), first[X == 1 ? 0 : i], to);
+                if constexpr (HOW == kLaidOut && F != kF16) to = multiply(source.values_low(b, i), first[X == 1 ? 0 : i], to);
+            }
+            if constexpr (HOW == kLaidOut && F != kF16) {
+                // a block's LDS reads among the products of the block before it
+                if (b == 0) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                if (b + 1 < NB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+                if (b + 1 < NB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
             }
         }
     }
 
-    // The largest of the lane's value scales' magnitudes, as bits (a NaN's above every other's).
-    __device__ __forceinline__ static uint32_t largest_scale(const uint4_t (&scale)[NB][X]) {
-        ushort2_t top = {0, 0};
+    // The outputs of a tile whose scales lie far apart: p d in f32, times the power
+    // of two that puts the row's largest in [2^14, 2^15); hi, and lo times 2^11, so
+    // that what is 2^-28 of the largest still has 22 bits. The outputs so far go
+    // through the same powers, which stay far from f32's ends.
+    template <typename SOURCE>
+    __device__ __forceinline__ void widely(const SOURCE& source, const float (&p)[X][8], bool nan) {
 #pragma unroll
-        for (uint32_t b = 0; b < NB; ++b)
+        for (uint32_t b = 0; b < NB; ++b) {
+            __builtin_amdgcn_sched_barrier(0);  // a block's registers after another's
+            float w[X][8], most = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < X; ++x) {
+                const uint4_t scale = finite_scale(source, b, x, nan);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[x][e] = p[x][e] * scale_at(scale, e), most = fmaxf(most, fabsf(w[x][e]));
+            }
+            const int shift = min(15 - __builtin_amdgcn_frexp_expf(most_of_row<X>(most)), 40);
+            half8_t hi[X], lo[X];
 #pragma unroll
             for (uint32_t x = 0; x < X; ++x)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t size = F == kQ4_0 ? scale[b][x][w] & 0x7FFF7FFFu : scale[b][x][w];
-                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, size));
+                for (int e = 0; e < 8; ++e) {
+                    const float y = ldexpf(w[x][e], shift);
+                    hi[x][e] = static_cast<_Float16>(y);
+                    lo[x][e] = static_cast<_Float16>((y - static_cast<float>(hi[x][e])) * 2048.0f);
                 }
-        return max(top.x, top.y);
+            const float there = ldexpf(2048.0f, held + shift), back = ldexpf(1.0f, -held - shift);
+#pragma unroll
+            for (uint32_t t = 0; t < kOuts / NB; ++t) out[kOuts / NB * b + t] *= there;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                result_t& to = out[X == 1 ? 2 * b + i : b];
+                to = multiply(source.values(b, i), lo[X == 1 ? 0 : i], to);
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < kOuts / NB; ++t) out[kOuts / NB * b + t] *= 1.0f / 2048.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                result_t& to = out[X == 1 ? 2 * b + i : b];
+                to = multiply(source.values(b, i), hi[X == 1 ? 0 : i], to);
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < kOuts / NB; ++t) out[kOuts / NB * b + t] *= back;
+        }
     }
 
-    // A tile with value scales that are NaNs: a row that sees such a token gets
-    // NaNs in its block, and the scale becomes 0, for the rows that do not.
-    template <typename TREE>
+    // Bit e: slot e of an octet has a scale that is a NaN.
+    __device__ __forceinline__ static uint32_t nans_of(const uint4_t& scale) {
+        uint32_t nans = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) nans |= (scale[e >> 1] >> (16 * (e & 1)) & 0x7FFFu) > 0x7C00u ? 1u << e : 0u;
+        return nans;
+    }
+    // An octet's scales, zeros for NaNs where the tile has some: those are in the outputs already.
+    template <typename SOURCE>
+    __device__ __forceinline__ static uint4_t finite_scale(const SOURCE& source, uint32_t b, uint32_t x, bool nan) {
+        uint4_t scale = source.value_scale(b, x);
+        if (__builtin_expect(nan, false)) {
+            const uint32_t nans = nans_of(scale);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                scale[w] &= (nans >> (2 * w) & 1u ? 0u : 0xFFFFu) | (nans >> (2 * w + 1) & 1u ? 0u : 0xFFFF0000u);
+        }
+        return scale;
+    }
+
+    // A tile with value scales that are NaNs: a row that sees such a token gets NaNs in its block.
+    template <typename SOURCE, typename TREE>
     __device__ __forceinline__ void spoil(const Attention& a, const Group& group, const TREE& tree, uint32_t slot0,
-                                          bool masked, uint4_t (&scale)[NB][X]) {
+                                          bool masked, const SOURCE& source) {
         const uint32_t seen = masked ? sees(a, group, tree, slot0) : 0xFFFFFFFFu;
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
             float mine = 0.0f;
 #pragma unroll
-            for (uint32_t x = 0; x < X; ++x) {
-                uint32_t nans = 0;  // a bit a slot of the octet
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    nans |= (scale[b][x][e >> 1] >> (16 * (e & 1)) & 0x7FFFu) > 0x7C00u ? 1u << e : 0u;
-                if (nans & octet_bits(seen, x)) mine = 1.0f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    scale[b][x][w] &= (nans >> (2 * w) & 1u ? 0u : 0xFFFFu) | (nans >> (2 * w + 1) & 1u ? 0u : 0xFFFF0000u);
-            }
+            for (uint32_t x = 0; x < X; ++x)
+                if (nans_of(source.value_scale(b, x)) & octet_bits(seen, x)) mine = 1.0f;
             const float nan = most_of_row<X>(mine) > 0.0f ? __builtin_nanf("") : 0.0f;
 #pragma unroll
             for (uint32_t t = 0; t < kOuts / NB; ++t) out[kOuts / NB * b + t] += nan;
         }
     }
 
-    // The last tile is done: the outputs, held over 2^(D - kScaleTop), as the sum is.
+    // The last tile is done: the outputs, over 2^held, as the sum is.
     __device__ __forceinline__ void end() {
-        const float up = ldexpf(1.0f, exponent - kScaleTop);
+        const float up = ldexpf(1.0f, held);
 #pragma unroll
         for (uint32_t t = 0; t < kOuts; ++t) out[t] *= up;
     }
@@ -710,6 +860,13 @@ struct Record {
             for (uint32_t w = 0; w < 4; ++w) s[w] = kept_scale<F>(s[w], kept_of(slot0, g, w, latest));
         return s;
     }
+    // The lane's of the tile's value scales, two; past the last, that.
+    __device__ __forceinline__ uint32_t scale_word(uint32_t i) const {
+        const uint32_t w = min(64 * i + (threadIdx.x & 63u), 16 * NB - 1);
+        uint32_t s = reinterpret_cast<const uint32_t*>(at + value_scales_at(F, NB))[w];
+        if (slot0 + kTile > latest) s = kept_scale<F>(s, kept_of(slot0, w / 4 & 3u, w & 3u, latest));
+        return s;
+    }
 };
 
 // Waves a workgroup and records a wave's ring: eight waves where two fit a
@@ -768,7 +925,7 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend(A
         }
         const uint32_t slot0 = (first + j * W) * kTile;
         const Record<F, NB, X> record{ring + j % D * kRecord, slot0, group.latest};
-        rows.template tile<false>(a, group, tree, slot0, record);
+        rows.template tile<kCodes>(a, group, tree, slot0, record);
         __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");  // the record's reads, before its place is copied to
     }
     rows.end();
@@ -830,6 +987,38 @@ struct Stage {
 // Waves of 32 rows a workgroup: two a SIMD where their registers allow.
 constexpr uint32_t row_waves(uint32_t blocks) { return blocks <= 4 ? 8 : 4; }
 
+// A wave's rows, their last tile done.
+template <uint32_t F, uint32_t NB, uint32_t X>
+__device__ __forceinline__ void write_rows(const Attention& a, const Group& group, Rows<F, NB, X>& rows, uint32_t row0) {
+    rows.end();
+    const uint32_t lane = threadIdx.x & 63u, row = row0 + lane % (16 * X);
+    const float total = sum_of_row<X>(rows.sum);
+    if (row >= group.row_end) return;
+#pragma unroll
+    for (uint32_t t = 0; t < Rows<F, NB, X>::kQuads; ++t)
+        finish<NB>(a, group, row, rows.sight.live, Rows<F, NB, X>::quad_at(t), rows.quad(t), total, rows.offset,
+                   t == 0 && lane < 16 * X);
+}
+
+// A wave's 32 rows by themselves, straight from the records, 16 at a time.
+template <uint32_t F, uint32_t NB, typename TREE>
+__device__ __forceinline__ void attend_alone(const Attention& a, const Group& group, const TREE& tree, const uint8_t* base,
+                                             uint32_t row0) {
+#pragma unroll 1
+    for (uint32_t first = row0; first < min(row0 + 32, group.row_end); first += 16) {
+        typename Rows<F, NB, 1>::Queries queries;
+        Rows<F, NB, 1>::fetch(a, group, first, queries);
+        Rows<F, NB, 1> rows;
+        rows.begin(a, group, tree, first, queries);
+#pragma unroll 1
+        for (uint32_t t = group.tile_begin; t < group.tile_end; ++t) {
+            const Record<F, NB, 1> record{base + static_cast<uint64_t>(t) * cache_record(F, NB), t * kTile, group.latest};
+            rows.template tile<kCodes>(a, group, tree, t * kTile, record);
+        }
+        write_rows(a, group, rows, first);
+    }
+}
+
 template <uint32_t F, uint32_t NB>
 __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     constexpr uint32_t W = row_waves(NB), kRows = 32 * W, kRecord = cache_record(F, NB), kUnit = cache_unit(F);
@@ -840,7 +1029,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     static_assert(kScaleWords * kTiles <= 64 * W, "a thread a dword");
     __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
     __shared__ Stage<F, NB> stages[2][kTiles];
-    __shared__ uint32_t wave_most[W], wave_spoilt[W];
+    __shared__ uint32_t wave_most[W], wave_least[W], wave_spoilt[W];
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Group group(a, kRows);
@@ -853,36 +1042,43 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
         a.parents ? group.latest : group.past + (min(row0 + 32, group.row_end) - 1) / a.group + 1;
     const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
 
-    // All the tiles' value scales, once: their largest exponent, and whether any is a NaN (F16: other than one).
-    uint32_t most = 0, spoilt = 0;
+    // All the tiles' value scales, once: how far they reach, and whether any is a NaN (F16: other than one).
+    Scales reach;
+    uint32_t spoilt = 0;
 #pragma unroll 4
     for (uint32_t x = threadIdx.x; x < (group.tile_end - group.tile_begin) * 16 * NB; x += 64 * W) {
         const uint32_t t = group.tile_begin + x / (16 * NB), w = x % (16 * NB);
         const uint32_t word = kept_scale<F>(
             reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord + value_scales_at(F, NB))[w],
             kept_of(t * kTile, w / 4 & 3u, w & 3u, group.latest));
-        most = max(most, larger_scale(word));
-        spoilt |= F == kF16 ? word ^ 0x3C003C00u
-                            : static_cast<uint32_t>((word & 0x7FFFu) > 0x7C00u || (word & 0x7FFF0000u) > 0x7C000000u);
+        if constexpr (F == kF16)
+            spoilt |= word ^ 0x3C003C00u;
+        else
+            reach.add(word);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o)));
-    spoilt = __any(spoilt != 0);
-    if (lane == 0) wave_most[wave] = most, wave_spoilt[wave] = spoilt;
+    reach.join();
+    spoilt = F == kF16 ? __any(spoilt != 0) : reach.nan;
+    if (lane == 0) wave_most[wave] = reach.most, wave_least[wave] = reach.least, wave_spoilt[wave] = spoilt;
     if (a.parents)
         read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
                   group.token_end - group.token0, a.window);
     __syncthreads();
-    most = spoilt = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < W; ++w) most = max(most, wave_most[w]), spoilt |= wave_spoilt[w];
+    for (uint32_t w = 0; w < W; ++w)
+        reach.most = max(reach.most, wave_most[w]), reach.least = min(reach.least, wave_least[w]), spoilt |= wave_spoilt[w];
     spoilt = __builtin_amdgcn_readfirstlane(spoilt);
-    const int exponent = F == kF16 ? kScaleTop : exponent_of(__builtin_amdgcn_readfirstlane(most));
+    const int exponent = F == kF16 ? 0 : held_of<kCodeTop>(__builtin_amdgcn_readfirstlane(reach.most));
     const half2_t by = over(exponent);
 
+    if constexpr (F != kF16)
+        if (__builtin_amdgcn_readfirstlane(reach.least) < power_bits(exponent + kCodeTop - kSplitSpread)) {
+            // scales further apart than a layout is made for
+            attend_alone<F, NB>(a, group, tree, base, row0);
+            return;
+        }
     Rows<F, NB, 2> rows;
     rows.begin(a, group, tree, min(row0, group.row_end - 1), queries);
-    rows.exponent = exponent;
+    rows.held = exponent;
 
     // Unit u of a stage: tile u / 2NB, block u % NB, keys then values. A lane
     // holds what it will lay out: as the unit has it, lane for lane.
@@ -1000,21 +1196,13 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
         for (uint32_t t = 0; t < kTiles; ++t) {
             const uint32_t slot0 = (tile0 + t) * kTile;
             if (mine && tile0 + t < group.tile_end && slot0 < sees_to)
-                rows.template tile<true>(a, group, tree, slot0, stages[turn][t], spoilt != 0);
+                rows.template tile<kLaidOut>(a, group, tree, slot0, stages[turn][t], spoilt != 0);
         }
         // the other stage was read before the last barrier
         if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
         __syncthreads();
     }
-    if (!mine) return;
-    rows.end();
-    const float total = sum_of_row<2>(rows.sum);
-    const uint32_t row = row0 + (lane & 31u);
-    if (row >= group.row_end) return;
-#pragma unroll
-    for (uint32_t t = 0; t < Rows<F, NB, 2>::kQuads; ++t)
-        finish<NB>(a, group, row, rows.sight.live, Rows<F, NB, 2>::quad_at(t), rows.quad(t), total, rows.offset,
-                   t == 0 && lane < 32);
+    if (mine) write_rows(a, group, rows, row0);
 }
 
 template <uint32_t F, uint32_t NB>

@@ -547,7 +547,11 @@ charlotte_hip_matmul_status charlotte_hip_matmul_cache_keep(charlotte_hip_matmul
  * value marks t unused: it, and all under it, see nothing and get zeros. With
  * a window w > 0 a token sees only itself and the w - 1 places before it, a
  * tree's token standing at the place of its depth. past[s] is taken as at most
- * capacity - tokens. */
+ * capacity - tokens.
+ * Sums are f32. A query's values count to 2^-22 of each or 2^-39 of its row's
+ * largest, a probability to 2^-21 of itself or 2^-25 of its row's largest (2^-36
+ * over F16), times the value beside it, whatever the sizes of other values and
+ * of tokens that the row does not see. */
 #define CHARLOTTE_HIP_MATMUL_TREE_TOKENS 256u
 typedef struct {
     const charlotte_hip_matmul_cache* cache;
