@@ -17,6 +17,7 @@ struct charlotte_hip_matmul_context {
     charlotte_hip_matmul_gemv_path gemv_path = CHARLOTTE_HIP_MATMUL_GEMV_CANONICAL;
     void* workspace = nullptr;  // the matrix-core path's, the caller's memory
     uint64_t workspace_bytes = 0;
+    uint32_t patience = CHARLOTTE_HIP_MATMUL_PATIENCE;
     std::string error;
 };
 

@@ -11,8 +11,8 @@
 // Rows past what the caches hold (kWholeBytes), read once: a workgroup keeps
 // its chunk in registers, publishes its maximum and sum, waits for those of the
 // row's other chunks, and writes its probabilities. The wait is bounded: a
-// workgroup that has not seen them all by then reads the row itself, so that
-// none depends on when another runs. (That needs the logits as they were, so a
+// workgroup that has not seen them all by then reads the row itself and adds it
+// in the same order, so that none depends on when another runs. (That needs the logits as they were, so a
 // step in place takes the two passes.)
 //
 // Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 66 us (5.3 TB/s;
@@ -134,7 +134,6 @@ constexpr uint64_t kOnceBytes = 128ull << 20;
 // Rows of at most a chunk always are: 1 x 4,096 4.8 and 6.6, 6 x 16,000 5.4 and
 // 7.0, 168 x 16,000 6.6 and 11.2, 4,000 x 16,000 97.5 and 100.7.
 constexpr uint32_t kAloneRows = 48;
-constexpr uint32_t kPolls = 1u << 16;          // looks at the other chunks, some 0.1 s of them
 
 // What a chunk publishes, in one word that is never 0: the sum is at least 1
 // where the maximum is a number, and 0 only beside -inf; the index is raised by 1.
@@ -232,33 +231,49 @@ __global__ __launch_bounds__(kWholeThreads) void row_whole(Probabilities a) {
     RowStats s = joined(chunk_stats<ONCE>(x, lead, a.vocabulary, at0, rate, q), rate, parts);
     if (threadIdx.x == 0)
         __hip_atomic_store(words + chunk, published(s, at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // the first wave: the row's statistics from its chunks' words, a lane a chunk
+    uint64_t word = 1;
+    auto join_words = [&] {
+        RowStats r = {-INFINITY, 0.0f, kNowhere};
+        if (threadIdx.x < a.chunks) {
+            r.largest = __uint_as_float(static_cast<uint32_t>(word >> 32));
+            if (at)
+                r.at = static_cast<uint32_t>(word) - 1;
+            else
+                r.sum = __uint_as_float(static_cast<uint32_t>(word));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) r = join_stats(r, shuffled(r, o), rate);
+        if (threadIdx.x == 0) whole = r;
+    };
     if (threadIdx.x < 64) {
-        // the first wave looks at every chunk's word, a lane a chunk, until none is 0
-        uint64_t word = 1;
+        // it looks until none is 0
         bool all = false;
-        for (uint32_t poll = 0; poll < kPolls && !all; ++poll) {
+        for (uint32_t look = 0; look < a.looks && !all; ++look) {
             if (threadIdx.x < a.chunks) word = __hip_atomic_load(words + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             all = __all(word != 0);
             if (!all) __builtin_amdgcn_s_sleep(8);
         }
-        s = {-INFINITY, 0.0f, kNowhere};
-        if (threadIdx.x < a.chunks) {
-            s.largest = __uint_as_float(static_cast<uint32_t>(word >> 32));
-            if (at)
-                s.at = static_cast<uint32_t>(word) - 1;
-            else
-                s.sum = __uint_as_float(static_cast<uint32_t>(word));
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s = join_stats(s, shuffled(s, o), rate);
-        if (threadIdx.x == 0) whole = s, late = !all;
+        join_words();
+        if (threadIdx.x == 0) late = !all;
     }
     __syncthreads();
-    if (late) {  // the row's statistics by this workgroup alone
-        s = joined(running_stats(x, lead, a.vocabulary, 4 * threadIdx.x, lead + a.vocabulary, 4 * kWholeThreads, rate), rate, parts);
-    } else {
-        s = whole;
+    if (late) {
+        // every chunk's word by this workgroup alone, as its own would publish it: the
+        // same bits; then its own logits again
+#pragma unroll 1
+        for (uint32_t c = 0; c < a.chunks; ++c) {
+            s = joined(chunk_stats<ONCE>(x, lead, a.vocabulary, c * kWholeChunk + 4 * threadIdx.x, rate, q), rate, parts);
+            if (threadIdx.x == c) word = published(s, at);
+            __syncthreads();  // `parts` has been read
+        }
+        if (threadIdx.x < 64) join_words();
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kWholeFours; ++i)
+            q[i] = read4<ONCE>(x, lead, a.vocabulary, at0 + 4 * kWholeThreads * i, -INFINITY);
     }
+    s = whole;
     write_chunk(a, y, lead, at0, s, rate, q);
 }
 

@@ -378,9 +378,18 @@ charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_mat
         need(d.workspace, "workspace", 16);
         if (d.workspace_bytes < charlotte_hip_matmul_probabilities_workspace_bytes(d.rows, d.vocabulary))
             refuse("workspace shorter than probabilities_workspace_bytes");
+        a.looks = ctx->patience;
         a.stats = static_cast<chm::RowStats*>(d.workspace);
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
         return chm::launch_probabilities(a, static_cast<hipStream_t>(stream));
+    });
+}
+
+charlotte_hip_matmul_status charlotte_hip_matmul_set_patience(charlotte_hip_matmul_context* ctx, uint32_t looks) {
+    return guarded(ctx, "patience", [&] {
+        if (looks > CHARLOTTE_HIP_MATMUL_PATIENCE) refuse(std::to_string(looks) + " looks");
+        ctx->patience = looks;
+        return hipSuccess;
     });
 }
 

@@ -109,6 +109,7 @@ struct Probabilities {
     uint64_t logit_stride, output_stride;
     uint32_t rows, vocabulary, chunks;  // chunks a row: launch_probabilities'
     float temperature;
+    uint32_t looks;   // at a row's other chunks, before a workgroup reads the row itself
     RowStats* stats;  // [rows][chunks], or words of 8 bytes
 };
 

@@ -324,6 +324,7 @@ SIGNATURES = {
     "charlotte_hip_matmul_probabilities_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32]),
     "charlotte_hip_matmul_probabilities": (
         _c.c_int, [_c.c_void_p, _c.POINTER(_ProbabilitiesDesc), _c.c_void_p]),
+    "charlotte_hip_matmul_set_patience": (_c.c_int, [_c.c_void_p, _c.c_uint32]),
     "charlotte_hip_matmul_verify_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32, _c.c_uint32]),
     "charlotte_hip_matmul_verify": (
         _c.c_int, [_c.c_void_p, _c.POINTER(_VerifyDesc), _c.c_uint32, _c.c_uint32, _c.c_void_p]),
@@ -400,6 +401,10 @@ def repack_q6_k(stored: bytes, blocks: int):
     return [b.raw for b in bufs]
 
 
+# The most looks of Context.set_patience, and how many there are unless it is set (CHARLOTTE_HIP_MATMUL_PATIENCE).
+PATIENCE = 65536
+
+
 class Context:
     """One device (charlotte_hip_matmul_context)."""
 
@@ -429,6 +434,10 @@ class Context:
     def set_workspace(self, device_ptr, nbytes):
         """The matrix-core path's working memory (device pointer, bytes); 0, 0 unsets it."""
         self.check(lib.charlotte_hip_matmul_set_workspace(self.handle, device_ptr or None, nbytes))
+
+    def set_patience(self, looks):
+        """How often probabilities' workgroups look for each other's sums before they read a row themselves."""
+        self.check(lib.charlotte_hip_matmul_set_patience(self.handle, looks))
 
     def close(self):
         if self.handle:

@@ -604,6 +604,13 @@ uint64_t charlotte_hip_matmul_probabilities_workspace_bytes(uint32_t rows, uint3
 charlotte_hip_matmul_status charlotte_hip_matmul_probabilities(charlotte_hip_matmul_context* ctx,
                                                                const charlotte_hip_matmul_probabilities_desc* desc,
                                                                void* stream);
+/* Where many rows are read once, the workgroups of a row wait for each other's
+ * sums: each looks for them at most CHARLOTTE_HIP_MATMUL_PATIENCE times, some 0.1
+ * s (on a card that other work holds, they may not run together), then finds
+ * them itself. `looks` in place of that, 0 up to it, for the context's calls from
+ * now on; results are the same bits at any. */
+#define CHARLOTTE_HIP_MATMUL_PATIENCE 65536u
+charlotte_hip_matmul_status charlotte_hip_matmul_set_patience(charlotte_hip_matmul_context* ctx, uint32_t looks);
 
 /* Drafted tokens against the target's probabilities, from given uniform numbers
  * in [0, 1). A sequence's step holds `tokens` nodes (at most
