@@ -12,6 +12,7 @@ Activations are f32. charlotte_amd/speculative.py runs them together.
 
 import ctypes
 import enum
+import itertools
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -42,6 +43,18 @@ def rope_table(positions, rope_dims, base=10000.0, factors=None):
     return np.cos(angles).astype(np.float32), np.sin(angles).astype(np.float32)
 
 
+class _Call:
+    """A call's fields, whose C descriptor is built for the first call and after a field is set."""
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name != "_desc":
+            object.__setattr__(self, "_desc", None)
+
+
+_STAMPS = itertools.count()
+
+
 @dataclass
 class Heads:
     """The queries or the keys of a step: charlotte_hip_matmul_heads."""
@@ -53,9 +66,13 @@ class Heads:
     input_stride: int = 0
     output_stride: int = 0
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_stamp", next(_STAMPS))  # no other state of any Heads has it
+
 
 @dataclass
-class HeadNormRope:
+class HeadNormRope(_Call):
     """charlotte_hip_matmul_head_norm_rope_desc."""
 
     parts: Sequence[Heads]
@@ -77,12 +94,13 @@ class HeadNormRope:
         d.rope, d.rope_dims = int(self.rope), self.rope_dims
         d.cosines, d.sines, d.positions, d.table_rows = self.cosines, self.sines, self.positions, self.table_rows
         d.epsilon = self.epsilon
+        d.stamps = [p._stamp for p in self.parts]
         return d
 
 
 def head_norm_rope(ctx: Context, call: HeadNormRope, tokens: int, stream=None):
     """Each head normalised and rotated, queries and keys in one launch."""
-    if call._desc is None:
+    if call._desc is None or call._desc.stamps != [p._stamp for p in call.parts]:
         call._desc = call.desc()
     ctx.check(lib.charlotte_hip_matmul_head_norm_rope(ctx.handle, ctypes.byref(call._desc), tokens, stream))
 
@@ -131,7 +149,7 @@ class Cache:
 
 
 @dataclass
-class Attention:
+class Attention(_Call):
     """charlotte_hip_matmul_attention_desc."""
 
     cache: Cache
@@ -161,13 +179,13 @@ def attention_workspace_bytes(ctx: Context, cache: Cache, query_heads: int, toke
 
 def attention(ctx: Context, call: Attention, tokens: int, stream=None):
     """The step's tokens, already appended, over their sequences' caches."""
-    if call._desc is None:
+    if call._desc is None or not call.cache.handle:  # (a cache that was freed is refused)
         call._desc = call.desc()
     ctx.check(lib.charlotte_hip_matmul_attention(ctx.handle, ctypes.byref(call._desc), tokens, stream))
 
 
 @dataclass
-class Probabilities:
+class Probabilities(_Call):
     """charlotte_hip_matmul_probabilities_desc."""
 
     logits: int
@@ -198,7 +216,7 @@ def probabilities(ctx: Context, call: Probabilities, stream=None):
 
 
 @dataclass
-class Verify:
+class Verify(_Call):
     """charlotte_hip_matmul_verify_desc."""
 
     node_tokens: int

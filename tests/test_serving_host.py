@@ -70,3 +70,73 @@ def test_verify_reference():
     assert ref.verify([7, 1, 0], target, [0, 0, 0], draft, [0, 0.9, 0.0]) == ([0, 1], [1, 2])
     assert ref.verify([7, 1, 0], target, [0, 0, 0], draft, [0, 1.0, 0.0]) == ([0], [0])
     assert ref.verify([7, 1, 1], target, [0.6, 0.1, 0], parents=[-1, 0, 0]) == ([0, 1], [1, 2])
+
+
+class _Recorded:
+    """A library that keeps copies of the descriptors it is called with, and a context of it."""
+
+    handle = None
+
+    def __init__(self):
+        self.descs = []
+
+    def __getattr__(self, name):
+        def call(handle, desc, *rest):
+            self.descs.append(type(desc._obj).from_buffer_copy(desc._obj))
+            return 0
+        return call
+
+    def check(self, status):
+        assert status == 0
+
+
+class _CacheOf:
+    def __init__(self, handle):
+        self.handle = handle
+
+
+def test_a_field_set_between_calls_reaches_the_next(monkeypatch):
+    seen = _Recorded()
+    monkeypatch.setattr(sv, "lib", seen)
+
+    soft = sv.Probabilities(16, 32, 2, 100, temperature=1.0, workspace=48, workspace_bytes=64)
+    sv.probabilities(seen, soft)
+    kept = soft._desc
+    sv.probabilities(seen, soft)
+    assert soft._desc is kept  # built once while nothing changes
+    soft.temperature, soft.workspace = 0.5, 4096
+    sv.probabilities(seen, soft)
+    assert [(d.temperature, d.workspace) for d in seen.descs] == [(1.0, 48), (1.0, 48), (0.5, 4096)]
+
+    seen.descs.clear()
+    cache = _CacheOf(16)
+    attend = sv.Attention(cache, 16, 32, 4, 0.125, past=64)
+    sv.attention(seen, attend, 1)
+    attend.longest, attend.workspace_bytes = 300, 128
+    sv.attention(seen, attend, 1)
+    cache.handle = None  # freed
+    sv.attention(seen, attend, 1)
+    assert [(d.longest, d.workspace_bytes, d.cache) for d in seen.descs] == [(0, 0, 16), (300, 128, 16), (300, 128, None)]
+
+    seen.descs.clear()
+    check = sv.Verify(16, 32, 48, 100, 64, 80, 96)
+    sv.verify(seen, check, 1, 2)
+    check.draft, check.accepts = 112, 128
+    sv.verify(seen, check, 1, 2)
+    assert [(d.draft, d.accepts) for d in seen.descs] == [(None, None), (112, 128)]
+
+    seen.descs.clear()
+    q, k = sv.Heads(16, 32, 4), sv.Heads(48, 64, 2)
+    turn = sv.HeadNormRope([q], 64)
+    sv.head_norm_rope(seen, turn, 1)
+    turn.epsilon = 0.5
+    sv.head_norm_rope(seen, turn, 1)
+    q.input = 80
+    sv.head_norm_rope(seen, turn, 1)
+    turn.parts.append(k)
+    sv.head_norm_rope(seen, turn, 1)
+    turn.parts[0] = k
+    sv.head_norm_rope(seen, turn, 1)
+    sv.head_norm_rope(seen, turn, 1)
+    assert [(d.part_count, d.parts[0].input, d.epsilon) for d in seen.descs] == [
+        (1, 16, np.float32(1e-6)), (1, 16, 0.5), (1, 80, 0.5), (2, 80, 0.5), (2, 48, 0.5), (2, 48, 0.5)]
