@@ -78,6 +78,9 @@ class Decoder:
 
     def __init__(self, model, layers, sequences, capacity, most, cache_type):
         c, ctx, device = model.config, model.ctx, model.device
+        if capacity > model.cosines.shape[0]:
+            raise ValueError(f"a capacity of {capacity}, past the rotation's tables of {model.cosines.shape[0]} positions")
+        most = min(most, capacity)
         self.model, self.ctx, self.sequences, self.most, self.capacity = model, ctx, sequences, most, capacity
         rows = sequences * most
 
@@ -184,6 +187,8 @@ class Decoder:
 
     def read(self, prompt):
         """A prompt [sequences, tokens] into the caches, in blocks."""
+        if int(self.past.max()) + prompt.shape[1] > self.capacity:
+            raise ValueError(f"a prompt of {prompt.shape[1]} tokens passes the capacity of {self.capacity}")
         for at in range(0, prompt.shape[1], self.most):
             block = prompt[:, at:at + self.most]
             self.step(block, head=False)
@@ -199,7 +204,8 @@ class Speculative:
 
     def __init__(self, model, sequences, capacity, depth, width=0, temperature=0.0, cache_type=mm.TensorType.Q8_0,
                  seed=0, block=64):
-        most = max(block, 1 + depth * max(1, width))
+        self.nodes = 1 + depth * max(1, width)  # a round's
+        most = max(block, self.nodes)
         c = model.config
         self.target = Decoder(model, c.layers, sequences, capacity, most, cache_type)
         self.draft = Decoder(model, c.draft_layers, sequences, capacity, most, cache_type)
@@ -259,13 +265,15 @@ class Speculative:
 
     def generate(self, prompt, tokens):
         """At least `tokens` tokens after each prompt [sequences, length]; lists, and the number of rounds."""
+        if prompt.shape[1] - 1 + self.nodes > self.target.capacity:
+            raise ValueError(f"a prompt of {prompt.shape[1]} tokens and a round pass the capacity of {self.target.capacity}")
         for decoder in (self.target, self.draft):
             decoder.past.zero_()
             decoder.read(prompt[:, :-1])
         root = prompt[:, -1:].to(torch.int32)
         out, rounds = [[] for _ in range(self.sequences)], 0
         while min(map(len, out)) < tokens:
-            if int(self.target.past.max()) + self.target.most > self.target.capacity:
+            if int(self.target.past.max()) + self.nodes > self.target.capacity:
                 raise ValueError("the caches are full")
             emitted, count = self.round(root)
             root = emitted.gather(1, count[:, None].long() - 1)
@@ -281,6 +289,8 @@ class Speculative:
 
 def decode(model, prompt, tokens, temperature=0.0, cache_type=mm.TensorType.Q8_0, capacity=4096, seed=0, block=64):
     """The same without drafts: a token a step."""
+    if prompt.shape[1] - 1 + tokens > capacity:
+        raise ValueError(f"a prompt of {prompt.shape[1]} tokens and {tokens} after it pass the capacity of {capacity}")
     decoder = Decoder(model, model.config.layers, prompt.shape[0], capacity, block, cache_type)
     generator = torch.Generator(device=model.device)
     generator.manual_seed(seed)
@@ -311,7 +321,7 @@ def main():
     a = parser.parse_args()
     kind = mm.TensorType[a.cache.upper()]
     with mm.Context(0) as ctx:
-        model = Model(ctx)
+        model = Model(ctx, positions=a.capacity)
         prompt = torch.randint(model.config.vocabulary, (a.sequences, a.prompt), device=model.device, dtype=torch.int32)
         pair = Speculative(model, a.sequences, a.capacity, a.depth, a.width, a.temperature, kind)
         pair.generate(prompt, 2 * (a.depth + 1))  # the kernels loaded

@@ -62,7 +62,29 @@ def prompts(ctx):
     assert all(bool(torch.isfinite(y).all()) and (y - logits[0]).abs().max() <= 2e-3 * size for y in logits)
 
 
+def long(ctx):
+    """Positions past 4,096, up to the last slot; and one token more, refused."""
+    capacity = 4200
+    model = sp.Model(ctx, sp.Config(**CONFIG), seed=4, positions=capacity)
+    x = _prompt(model, 1, capacity - 20, seed=5)
+    want = sp.decode(model, x, 21, capacity=capacity)
+    pair = sp.Speculative(model, 1, capacity, 2)
+    got, _ = pair.generate(x, 18)  # a round of three tokens has to fit behind the last
+    pair.free()
+    print("long", want, got, flush=True)
+    assert got[0][:18] == want[0][:18]
+    decoder = sp.Decoder(model, model.config.layers, 1, capacity, 64, mm.TensorType.Q8_0)
+    decoder.read(x)
+    assert bool(torch.isfinite(decoder.step(x[:, -1:])).all())
+    decoder.free()
+    try:
+        sp.decode(model, x, 22, capacity=capacity)
+    except ValueError:
+        return
+    raise AssertionError("a step past the capacity")
+
+
 if __name__ == "__main__":
     with mm.Context(0) as context:
-        {"greedy": greedy, "itself": itself, "prompts": prompts}[sys.argv[1]](context, *sys.argv[2:])
+        {"greedy": greedy, "itself": itself, "prompts": prompts, "long": long}[sys.argv[1]](context, *sys.argv[2:])
     print("passed")

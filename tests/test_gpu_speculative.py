@@ -19,3 +19,7 @@ def test_speculative_decoding(check):
                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     print(run.stdout, flush=True)
     assert run.returncode == 0 and run.stdout.endswith("passed\n")
+
+
+def test_positions_past_the_default_tables():
+    test_speculative_decoding(["long"])
