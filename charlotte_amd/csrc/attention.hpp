@@ -45,17 +45,20 @@
 //
 // Bound and measured (8 key heads; a large copy moves 5.1 TB/s, a large binary16
 // product of the library's runs at 1.1 - 1.16 PFLOP/s):
-//   one token of 32 heads of 128 over 65,536 in Q8_0, by the cache's 142 MB: 30.2
-//   us, 4.7 TB/s, and 4.5 to join its 32 splits;
-//   16 heads over 911, by the latency of a launch and its reads: 6.4 and 3.2 us;
-//   a tree of 21 tokens of 32 heads of 64 over 8,191 in Q4_0, by the VALU - some
-//   500 instructions a tile of 32 rows: codes widened, the probabilities scaled
-//   and parted for each block of values: 15.6 and 4.0 us;
+//   one token of 32 heads of 128 over 65,536 in Q8_0, by the cache's 142 MB: 30.8
+//   us, 4.6 TB/s, and 4.6 to join its 32 splits; with half of its blocks 2^12 below
+//   the others, every tile wide, 44 in all where that is 34;
+//   16 heads over 911, by the latency of a launch and its reads: 6.6 and 3.4 us;
+//   a tree of 21 tokens of 32 heads of 64 over 8,191 in Q4_0, by latency: the VALU
+//   issues 42% of the time (some 500 instructions a tile of 32 rows: codes widened,
+//   the probabilities scaled and parted for each block of values), the matrix cores
+//   10%; the rest is the tree, read by every split, and 26 tiles over 8 waves: 16.6
+//   and 4.0 us;
 //   512 tokens of 32 heads of 128 over 15,873 in Q8_0 (attend_rows), by the matrix
 //   instructions: 339 GFLOP with queries, probabilities and values in parts (135
-//   by the formula), 320 - 340 us, 1.06 PFLOP/s; matrix cores busy 51% and the VALU
-//   44% of the time; priorities, operands read further ahead and the waves of a
-//   SIMD half a tile apart changed nothing or cost time.
+//   by the formula), 318 - 340 us, 1.04 PFLOP/s; matrix cores busy 50% and the VALU
+//   44% of the time; priorities and the waves of a SIMD half a tile apart changed
+//   nothing or cost time. Scales too far apart to lay out (attend_alone): 900 us.
 #pragma once
 
 #include "cache.hpp"
@@ -360,7 +363,8 @@ struct Rows {
     result_t out[kOuts];
     float largest, offset, sum;         // the raw maximum; exp2's offset; the lane's part of the sum
     int held;                           // outputs are over 2^held, the same in every lane
-    uint32_t scale_low, scale_high;     // the scales that it stays for, each twice in its dword: the least's bits less one; the largest's
+    // The scales that it stays for, each twice in its dword: the least's bits less one, and the largest's.
+    uint32_t scale_low, scale_high;
     Sight sight;
 
     // Where a lane's run of four output values stands in its row.

@@ -9,8 +9,8 @@ namespace chm {
 namespace {
 
 // Tiles a split takes at least: of wide binary16 heads two, but four once that
-// makes more than 64 splits (126 tiles of one head: 13.9 us in 63, 15.6 in 32; 501
-// tiles: 24.4 in 250, 20.8 in 126).
+// makes more than 64 splits (126 tiles of one head: 12.9 us in 63, 14.5 in 32; 501
+// tiles: 23.3 in 250, 19.3 in 126).
 uint64_t least_tiles(const CacheShape& cache, uint64_t tiles) {
     return cache.format == kF16 && cache.head_dim > 128 && tiles <= 128 ? 2 : 4;
 }
@@ -33,25 +33,26 @@ uint64_t splits_of(const CacheShape& cache, uint64_t row_groups, uint64_t tiles,
 // Workgroups of 16 rows (attend) have the shorter chain of products, and read
 // the cache once for every 16 rows; they are taken while load16 <= 24 and none
 // has to wait for another's compute unit. 8 key heads of 128, 20 rows over 8,000
-// in Q8_0: 16.0 us, by 32 rows 18.6; in binary16 over 500 10.2 and 15.3, 48 rows
-// over 8,000 (load16 = 24) 26.8 and 23.7; 128 rows of 8 sequences with none before
-// (twice as many workgroups as compute units) 13.6 and 10.5. Quantized
+// in Q8_0: 15.2 us, by 32 rows 16.8; in binary16 over 500 9.7 and 11.8, 48 rows
+// over 8,000 (load16 = 24) 23.4 and 21.2; 128 rows of 8 sequences with none before
+// (twice as many workgroups as compute units) 13.9 and 11.2. Quantized
 // heads past 64, whose codes cost more to widen than to read, up to 64: 84 rows
-// over 8,000 (48) 31.5 and 34.5, over 60,000 (352) 153 and 136.
+// over 8,000 (48) 28.2 and 32.5, over 60,000 (352) 140 and 140 - 145.
 //
 // A tile's codes laid out once for 128 or 256 rows (attend_rows) pay where each
 // compute unit has many products to feed: 1,024 rows of 8 key heads of 128 over
-// 16,000 in Q8_0 (load32 = 531) 182 us, by 32 rows 325; over 1,000 (47) 38.3 and
-// 39.9; over 400 (28) 32.5 and 29.1. Heads of 64, over 8,000 (266) 62 and 72,
-// 512 rows over 8,000 (129) 43.2 and 41.3. Heads of 256 hold 4 waves' rows, too
-// few to pay for laying codes out (Q8_0, 1,024 over 8,000: 396 and 321), but in
-// binary16 there is little to lay out: 328 and 609, 192 over 2,000 (13) 49 and 56.
+// 16,000 in Q8_0 (load32 = 531) 173 us, by 32 rows 325; over 1,400 (44) 39.3
+// and 41.2; over 1,000 (32) 34.2 and 31.1. Heads of 64, over 8,000 (250) 60 and 69,
+// 512 rows over 8,000 (125) 42 and 42. Heads of 256 hold 4 waves' rows, too
+// few to pay for laying codes out (Q8_0, 1,024 over 8,000: 387 and 308), but in
+// binary16 there is little to lay out: 184 and 408, 192 over 2,000 (11) 33 and 44,
+// 1,024 over 300 (10) 34 and 29.
 //
 // Few tiles are not split: the launch that joins them costs 2.5 us. One token, 2
-// rows of 8 heads, in one and in splits of four tiles: heads of 64, 19 tiles 8.1
-// and 8.9 us, 26 tiles 9.5 and 9.1; of 128, 11 tiles 7.9 and 9.0, 15 tiles 9.2
-// and 9.0; of 256, 8 tiles 14.0 and 13.0 (binary16 16.4 and 13.6, in splits of
-// two tiles 11.7). 512 tokens with none before, attend_rows: 46.5 and 28.3.
+// rows of 8 heads, in one and in splits of four tiles: heads of 64, 19 tiles 8.3
+// and 8.7 us, 26 tiles 9.5 and 8.7; of 128, 11 tiles 7.9 and 9.1, 15 tiles 9.4
+// and 9.2; of 256, 8 tiles 13.8 and 13.4 (binary16 14.6 and 13.2, in splits of
+// two tiles 11.3). 512 tokens with none before, attend_rows: 47.1 and 33.8.
 AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint32_t tokens, uint32_t longest,
                              uint32_t window, uint32_t compute_units) {
     const uint64_t rows = uint64_t{tokens} * (query_heads / cache.kv_heads);
@@ -63,7 +64,7 @@ AttentionPlan plan_attention(const CacheShape& cache, uint32_t query_heads, uint
     const uint64_t most16 = quantized && cache.head_dim > 64 ? 64 : 24;
     const uint64_t load16 = groups_of(rows, 16) * heads * tiles, load32 = groups_of(rows, 32) * heads * tiles;
     const uint32_t waves = row_waves(cache.head_dim);
-    const uint64_t least32 = cache.head_dim <= 64 ? 112 : cache.head_dim <= 128 ? 44 : quantized ? UINT64_MAX : 8;
+    const uint64_t least32 = cache.head_dim <= 64 ? 112 : cache.head_dim <= 128 ? 44 : quantized ? UINT64_MAX : 11;
     AttentionPlan plan{1, 1, 0, 0};
     if (rows > 16 * waves && load32 / compute_units >= least32)
         plan.octets = 2, plan.waves = waves;

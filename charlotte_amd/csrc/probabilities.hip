@@ -15,8 +15,8 @@
 // in the same order, so that none depends on when another runs. (That needs the logits as they were, so a
 // step in place takes the two passes.)
 //
-// Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 66 us (5.3 TB/s;
-// two passes 94), 1,024 x 131,072: 186 us (5.8 TB/s; 324); 6 x 151,936: passes of
+// Bound by bytes: 4 read and 4 written a logit. 168 x 262,144: 69.5 us (5.1 TB/s;
+// two passes 94), 1,024 x 131,072: 188 us (5.7 TB/s; 324); 6 x 151,936: passes of
 // 4.0 and 4.8 us, a launch's latency each.
 #include <algorithm>
 
@@ -120,12 +120,12 @@ constexpr uint32_t kWholeThreads = 512, kWholeFours = 8, kWholeChunk = 4 * kWhol
 // Logits past which rows are read once, their second read no longer all from
 // cache: of 151,936, 12 rows (7 MB) 10.6 us read once and 10.1 in two passes, 32
 // (19 MB) 14.9 and 14.0, 42 (26 MB) 15.7 and 16.9, 64 (39 MB) 18.9 and 23.5, 100 (61
-// MB) 25.7 and 33.5; of 262,144, 21 rows (22 MB) 15.4 and 15.6.
+// MB) 27.2 and 33.5; of 262,144, 21 rows (22 MB) 15.4 and 15.6.
 constexpr uint64_t kWholeBytes = 22ull << 20;
 // Logits past which, with as many probabilities, they leave the caches anyway and
-// are read without being kept there: 102 MB 42.4 us either way, 176 MB 66.0 and,
-// kept, 72.3 (the logits written before and their verification after: 171 and
-// 183); of 51 MB, which an earlier launch may have left there, 27.8 and 24.0.
+// are read without being kept there: 102 MB 42.4 us either way, 176 MB 69.5 and,
+// kept, 75.9, 537 MB 188 and 191 (176 MB with the logits written before and their
+// verification after: 171 and 183); of 51 MB, which an earlier launch may have left there, 27.8 and 24.0.
 // (Probabilities written past the caches would cost their reader more.)
 constexpr uint64_t kOnceBytes = 128ull << 20;
 // Rows from which a row of one to two chunks is one workgroup's, in one launch:

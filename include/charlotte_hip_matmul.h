@@ -629,8 +629,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_set_patience(charlotte_hip_matm
  *
  * A draw from row x with uniform number u (uniforms' of that node) is exact, in
  * whole numbers: weights floor(min(max(x, 0), 1) 2^44) (a NaN: 0), W their sum,
- * r = floor(u 2^31) within 0 .. 2^31 - 1, and the lowest index whose running sum
- * passes floor(W r / 2^31); with W = 0, index 0.
+ * r = floor(u 2^31) (a u outside 0 .. 1 - 2^-24 counts as the nearer end, a NaN
+ * as 0), and the lowest index whose running sum passes floor(W r / 2^31); with
+ * W = 0, index 0.
  *
  * path gets the accepted nodes, node 0 first, emitted the tokens after each of
  * them (the drafted ones accepted, then the one drawn): count of each, and -1
