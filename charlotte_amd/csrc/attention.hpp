@@ -303,6 +303,7 @@ struct Group {
     uint64_t sequence_head;
     uint32_t split;
 
+    Group() = default;
     // `rows` rows a workgroup, blockIdx.x = (head, row group, split).
     __device__ __forceinline__ Group(const Attention& a, uint32_t rows) {
         split = blockIdx.x % a.splits;

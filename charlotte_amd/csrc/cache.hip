@@ -20,6 +20,7 @@
 // 5.1 and 5.2, 4.7 and 7.0; read back 4.4 - 5.2 by units, 4.4 - 4.5 by tokens. Up to
 // 256 tokens of one sequence either is a launch's latency (3 us).
 #include "cache.hpp"
+#include "requests.hpp"
 
 namespace chm {
 
@@ -51,6 +52,25 @@ __device__ __forceinline__ Piece piece_of(const CacheRows& a) {
     p.sequence = p.live ? sequence : 0u;
     p.slot = static_cast<uint64_t>(a.first[p.sequence]) + row % a.tokens;
     p.live = p.live && p.slot < a.cache.capacity;
+    return p;
+}
+
+// The same of a pool: row r's slot is one of a page, which is the pool's sequence.
+__device__ __forceinline__ Piece paged_piece_of(const CacheRows& a) {
+    Piece p;
+    const uint32_t id = (blockIdx.x * 256 + threadIdx.x) / 8;
+    const uint32_t blocks = a.cache.head_dim / 32, row_blocks = blocks * a.cache.kv_heads;
+    p.lane = threadIdx.x & 7u;
+    p.values = blockIdx.y != 0;
+    const uint32_t in_row = id % row_blocks;
+    p.head = in_row / blocks;
+    p.block = in_row % blocks;
+    p.row = id / row_blocks;
+    p.live = p.row < a.tokens;
+    const uint32_t slot = p.live ? a.first[p.row] : 0u;
+    p.sequence = slot / a.cache.capacity;
+    p.slot = slot % a.cache.capacity;
+    p.live = p.live && p.sequence < a.cache.sequences;
     return p;
 }
 
@@ -137,8 +157,7 @@ __device__ __forceinline__ uint32_t quantize(const float4& v, uint32_t lane, boo
 }
 
 template <uint32_t F>
-__global__ __launch_bounds__(256) void cache_append(CacheRows a) {
-    const Piece p = piece_of(a);
+__device__ __forceinline__ void append_piece(const CacheRows& a, const Piece& p) {
     const uint32_t blocks = a.cache.head_dim / 32;
     const float* from = (p.values ? a.values + p.row * a.value_stride : a.keys + p.row * a.key_stride) +
                         static_cast<uint64_t>(p.head) * a.cache.head_dim + 32 * p.block + 4 * p.lane;
@@ -190,8 +209,7 @@ __global__ __launch_bounds__(256) void cache_append(CacheRows a) {
 }
 
 template <uint32_t F>
-__global__ __launch_bounds__(256) void cache_read(CacheRows a) {
-    const Piece p = piece_of(a);
+__device__ __forceinline__ void read_piece(const CacheRows& a, const Piece& p) {
     if (!p.live) return;
     const uint32_t blocks = a.cache.head_dim / 32;
     const uint8_t* record = record_of(a.cache, F, p.sequence, p.head, p.slot / kTile);
@@ -234,6 +252,23 @@ __global__ __launch_bounds__(256) void cache_read(CacheRows a) {
     float* to = const_cast<float*>(p.values ? a.values + p.row * a.value_stride : a.keys + p.row * a.key_stride) +
                 static_cast<uint64_t>(p.head) * a.cache.head_dim + 32 * p.block + 4 * p.lane;
     *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+template <uint32_t F>
+__global__ __launch_bounds__(256) void cache_append(CacheRows a) {
+    append_piece<F>(a, piece_of(a));
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void cache_read(CacheRows a) {
+    read_piece<F>(a, piece_of(a));
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void page_append(CacheRows a) {
+    append_piece<F>(a, paged_piece_of(a));
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void page_read(CacheRows a) {
+    read_piece<F>(a, paged_piece_of(a));
 }
 
 // ---- whole units ---------------------------------------------------------------
@@ -717,6 +752,29 @@ static hipError_t launch_rows(const CacheRows& a, bool read, hipStream_t stream)
 
 hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream) { return launch_rows(a, false, stream); }
 hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream) { return launch_rows(a, true, stream); }
+
+template <uint32_t F>
+static void launch_paged_rows(const CacheRows& a, bool read, hipStream_t stream) {
+    const uint64_t blocks = uint64_t{a.tokens} * a.cache.kv_heads * (a.cache.head_dim / 32);
+    const dim3 grid(static_cast<uint32_t>((blocks * 8 + 255) / 256), 2);
+    if (read)
+        hipLaunchKernelGGL(page_read<F>, grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(page_append<F>, grid, dim3(256), 0, stream, a);
+}
+
+static hipError_t launch_paged_rows(const CacheRows& a, bool read, hipStream_t stream) {
+    switch (a.cache.format) {
+        case kF16: launch_paged_rows<kF16>(a, read, stream); break;
+        case kQ4_0: launch_paged_rows<kQ4_0>(a, read, stream); break;
+        case kQ8_0: launch_paged_rows<kQ8_0>(a, read, stream); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_page_append(const CacheRows& a, hipStream_t stream) { return launch_paged_rows(a, false, stream); }
+hipError_t launch_page_read(const CacheRows& a, hipStream_t stream) { return launch_paged_rows(a, true, stream); }
 
 hipError_t launch_cache_keep(const CacheKeep& a, hipStream_t stream) {
     const dim3 grid(a.cache.sequences * a.cache.kv_heads);

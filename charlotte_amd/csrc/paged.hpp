@@ -1,0 +1,373 @@
+// Attention of several requests' new tokens over their pages (attention.hpp's
+// arithmetic, few rows' form: a workgroup has 16 or 32 rows of a key head, its
+// waves take the tiles in turn through LDS rings, and are joined in LDS).
+//
+// The requests' lengths are known to the device alone, and are anything: a
+// unit - 16 or 32 rows of a request and key head, over the tiles they see - may
+// be one tile or thousands. As many workgroups as the card holds lay all units
+// along a line, a key head after another, each by a running sum over the
+// requests, and take equal parts of it, so that each reads as many tiles as any
+// other; a unit that crosses parts is in pieces. Where all of it is less than
+// kLeastTiles a workgroup, units are cut in pieces of at most as many, which the
+// workgroups take in turn: a piece's fixed cost is then more than its tiles'.
+//
+// A unit's pieces leave their outputs, and their rows' offsets and sums, in the
+// workspace; the workgroup that finds itself the last of them (a counter, left
+// at 0) joins them, in the pieces' order.
+#pragma once
+
+#include "attention.hpp"
+#include "requests.hpp"
+
+namespace chm {
+
+// What a unit costs beside its tiles, in tiles.
+constexpr uint32_t kUnitTiles = 4;
+// Tiles a workgroup below which units are cut by length alone.
+constexpr uint32_t kLeastTiles = 12;
+
+// What is the same in every lane, as the compiler then knows.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return uint64_t{uniform(static_cast<uint32_t>(x >> 32))} << 32 | uniform(static_cast<uint32_t>(x));
+}
+
+struct NoTree {
+    uint32_t above[1][kTreeTokens / 32];
+    uint32_t depth[1];
+};
+
+// A request: its tokens, and the tiles that its rows see some of.
+struct Request {
+    uint32_t past, count, start;
+    uint32_t begin, tiles;  // the first, how many
+    uint32_t groups;        // units a key head
+    bool over;              // its tokens pass the table's row
+};
+
+template <uint32_t ROWS>
+__device__ __forceinline__ void place_request(const PagedAttention& a, Request& r) {
+    if (uint64_t{r.start} + r.count > a.rows) r.count = 0;
+    r.groups = (r.count * a.group + ROWS - 1) / ROWS;  // (rows * group is below 2^32)
+    const uint64_t end = uint64_t{r.past} + r.count;
+    r.over = end > uint64_t{a.table_stride} * a.pool.capacity;
+    if (r.over) {
+        r.begin = 0, r.tiles = 1;
+        return;
+    }
+    r.begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
+    r.tiles = (static_cast<uint32_t>(end) + kTile - 1) / kTile - r.begin;
+}
+
+// Line [0, length) in `parts` parts, the first ones a place longer.
+struct Parts {
+    uint64_t each, more;
+    __device__ __forceinline__ uint64_t begin(uint64_t part) const { return part * each + min(part, more); }
+    __device__ __forceinline__ uint32_t at(uint64_t place) const {
+        const uint64_t wide = more * (each + 1);
+        return static_cast<uint32_t>(place < wide ? place / (each + 1) : more + (place - wide) / each);
+    }
+};
+
+template <uint32_t F, uint32_t NB, uint32_t X>
+__global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_pages(PagedAttention a) {
+    using Shape = AttendShape<F, NB, X>;
+    constexpr uint32_t kRows = 16 * X, kRecord = Shape::kRecord, W = Shape::kWaves, D = Shape::kRing, T = 64 * W;
+    constexpr uint32_t kQuads = Rows<F, NB, X>::kQuads, kParts = kQuads * 64;  // float4s of a wave's outputs
+    __shared__ __align__(16) uint8_t space[sizeof(uint8_t[W][D][kRecord]) > sizeof(float4_t[W][kParts])
+                                               ? sizeof(uint8_t[W][D][kRecord])
+                                               : sizeof(float4_t[W][kParts])];
+    __shared__ float joined_offset[W][kRows], joined_sum[W][kRows];
+    // A thread's requests: the line's and the cut units' pieces before them, and the first of them.
+    __shared__ uint64_t line_before[T];
+    __shared__ uint32_t cut_before[T], request_past[T], request_count[T], request_start[T];
+    __shared__ uint64_t wave_tiles[W], wave_line[W], wave_cut[W];
+    __shared__ uint32_t last_piece;
+
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane % kRows;
+    // neighbours on the line on one XCD, whose cache then has the tiles that a request's units share
+    const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+    const uint32_t share = (a.requests + T - 1) / T, first_request = threadIdx.x * share;
+    const uint32_t last_request = min(first_request + share, a.requests);
+    const uint32_t tiles_a_page = a.pool.capacity / kTile;
+
+    auto request_of = [&](uint32_t i) {
+        Request r{a.past[i], a.counts[i], a.starts[i], 0, 0, 0, false};
+        place_request<kRows>(a, r);
+        return r;
+    };
+    // Over the threads before this one, in the wave and then all of them.
+    auto scan = [&](uint64_t x, uint64_t* of_waves) {
+        uint64_t sum = x;
+#pragma unroll
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint64_t other = __shfl_up(sum, o);
+            if (lane >= o) sum += other;
+        }
+        if (lane == 63) of_waves[wave] = sum;
+        return sum - x;
+    };
+    uint64_t tiles = 0;
+    for (uint32_t i = first_request; i < last_request; ++i) {
+        const Request r = request_of(i);
+        tiles += uint64_t{r.groups} * r.tiles;
+        if (i == first_request)
+            request_past[threadIdx.x] = r.past, request_count[threadIdx.x] = r.count, request_start[threadIdx.x] = r.start;
+    }
+    scan(tiles, wave_tiles);
+    __syncthreads();
+    uint64_t all_tiles = 0;
+    for (uint32_t w = 0; w < W; ++w) all_tiles += wave_tiles[w];
+    // Equal parts of the line, or pieces in turn.
+    const bool even = uniform(all_tiles) * a.pool.kv_heads >= uint64_t{gridDim.x} * kLeastTiles;
+    auto pieces_of = [&](const Request& r) { return (r.tiles + kLeastTiles - 1) / kLeastTiles; };
+    auto length_of = [&](const Request& r) { return even ? r.tiles + kUnitTiles : pieces_of(r); };
+    uint64_t line = 0, cut = 0;
+    for (uint32_t i = first_request; i < last_request; ++i) {
+        const Request r = request_of(i);
+        line += uint64_t{r.groups} * length_of(r);
+        if (!even && pieces_of(r) > 1) cut += r.groups * pieces_of(r);
+    }
+    line = scan(line, wave_line), cut = scan(cut, wave_cut);
+    __syncthreads();
+    uint64_t head_line = 0, head_cut = 0;
+    for (uint32_t w = 0; w < W; ++w) {
+        if (w < wave) line += wave_line[w], cut += wave_cut[w];
+        head_line += wave_line[w], head_cut += wave_cut[w];
+    }
+    line_before[threadIdx.x] = line, cut_before[threadIdx.x] = static_cast<uint32_t>(cut);
+    __syncthreads();
+    head_line = uniform(head_line), head_cut = uniform(head_cut);
+
+    const uint64_t length = head_line * a.pool.kv_heads;
+    const Parts parts{length / gridDim.x, length % gridDim.x};
+    uint64_t place = even ? parts.begin(part) : part;
+    const uint64_t end = even ? parts.begin(uint64_t{part} + 1) : length;
+    const uint32_t scanned = min(T, (a.requests + share - 1) / share);
+
+    Attention b{};
+    b.queries = a.queries, b.output = a.output;
+    b.query_stride = a.query_stride, b.output_stride = a.output_stride;
+    b.tokens = 1, b.group = a.group, b.window = a.window, b.scale = a.scale, b.splits = 1;
+    const NoTree tree{};
+
+    while (place < end) {
+        // The unit: its request, the last whose part of the head's line does not begin past the place.
+        const uint32_t head = static_cast<uint32_t>(place / head_line);
+        const uint64_t on_head = place - head * head_line;
+        uint32_t low = 0, high = scanned;
+        while (high - low > 1) {
+            const uint32_t middle = (low + high) / 2;
+            if (line_before[middle] <= on_head)
+                low = middle;
+            else
+                high = middle;
+        }
+        low = uniform(low);
+        uint64_t before = uniform(line_before[low]);
+        uint32_t cut_at = uniform(cut_before[low]), at = low * share;
+        Request r{uniform(request_past[low]), uniform(request_count[low]), uniform(request_start[low]), 0, 0, 0, false};
+        place_request<kRows>(a, r);
+        while (before + uint64_t{r.groups} * length_of(r) <= on_head) {
+            before += uint64_t{r.groups} * length_of(r);
+            if (!even && pieces_of(r) > 1) cut_at += r.groups * pieces_of(r);
+            ++at;
+            r.past = uniform(a.past[at]), r.count = uniform(a.counts[at]), r.start = uniform(a.starts[at]);
+            place_request<kRows>(a, r);
+        }
+        const uint32_t unit_length = length_of(r);
+        const uint32_t unit = static_cast<uint32_t>((on_head - before) / unit_length);
+        const uint64_t unit_begin = head * head_line + before + uint64_t{unit} * unit_length, unit_end = unit_begin + unit_length;
+
+        // The piece: its tiles of the unit's, its number among the unit's, where it is kept.
+        uint32_t tile_begin = 0, tile_end = r.tiles, pieces = 1, piece = 0, kept = 0, counter = 0;
+        if (even) {
+            const uint32_t from = parts.at(unit_begin), to = parts.at(unit_end - 1);
+            pieces = to - from + 1, piece = part - from;
+            kept = 2 * part + (piece == 0), counter = 2 * from + 1;
+            const uint64_t mine = max(parts.begin(part), unit_begin), until = min(end, unit_end);
+            tile_begin = mine > unit_begin + kUnitTiles ? static_cast<uint32_t>(mine - unit_begin) - kUnitTiles : 0;
+            tile_end = until > unit_begin + kUnitTiles ? static_cast<uint32_t>(until - unit_begin) - kUnitTiles : 0;
+            place = until;
+        } else {
+            pieces = unit_length, piece = static_cast<uint32_t>(place - unit_begin);
+            counter = head * static_cast<uint32_t>(head_cut) + cut_at + unit * pieces, kept = counter + piece;
+            tile_begin = static_cast<uint32_t>(uint64_t{r.tiles} * piece / pieces);
+            tile_end = static_cast<uint32_t>(uint64_t{r.tiles} * (piece + 1) / pieces);
+            place += gridDim.x;
+        }
+
+        Group group;
+        group.sequence = r.start, group.head = head, group.past = r.past, group.latest = r.past + r.count;
+        group.row0 = unit * kRows, group.row_end = min(group.row0 + kRows, r.count * a.group);
+        group.token0 = group.row0 / a.group, group.token_end = (group.row_end - 1) / a.group + 1;
+        group.all_begin = a.window && group.latest > a.window ? group.latest - a.window : 0u;
+        // of the tiles, those that its rows see
+        const uint32_t sees_from = a.window && r.past + group.token0 + 1 > a.window ? r.past + group.token0 + 1 - a.window : 0u;
+        group.tile_begin = max(r.begin + tile_begin, sees_from / kTile);
+        group.tile_end = min(r.begin + tile_end, (r.past + group.token_end + kTile - 1) / kTile);
+        if (r.over) group.tile_end = group.tile_begin;
+
+        // A tile's record: its page is read from the table by scalar loads, an iteration ahead of its copy.
+        typedef const __attribute__((address_space(4))) uint32_t* scalar_pointer;
+        const auto entries = (scalar_pointer)(a.table + uint64_t{at} * a.table_stride);
+        const uint32_t first = group.tile_begin + wave;
+        const uint32_t count = first < group.tile_end ? (group.tile_end - first + W - 1) / W : 0;  // the wave's tiles
+        uint8_t* ring = space + wave * (D * kRecord);
+        uint32_t gone = 0;  // a bit a place of the ring: its page is none of the pool's
+        auto page_of = [&](uint32_t j) { return entries[__builtin_amdgcn_readfirstlane((first + j * W) / tiles_a_page)]; };
+        auto copy = [&](uint32_t j, uint32_t page) {
+            const uint32_t tile = first + j * W, bit = 1u << (j % D);
+            const bool there = page < a.pool.sequences;
+            gone = there ? gone & ~bit : gone | bit;
+            const uint64_t record = (uint64_t{there ? page : 0u} * a.pool.kv_heads + head) * tiles_a_page + tile % tiles_a_page;
+            copy_record<kRecord>(a.pool.base + record * kRecord, ring + j % D * kRecord);
+        };
+#pragma unroll
+        for (uint32_t j = 0; j + 1 < D; ++j)
+            if (j < count) copy(j, page_of(j));
+        uint32_t ahead = D - 1 < count ? page_of(D - 1) : 0;
+        typename Rows<F, NB, X>::Queries queries;
+        Rows<F, NB, X>::fetch(b, group, group.row0, queries);
+        Rows<F, NB, X> rows;
+        rows.begin(b, group, tree, group.row0, queries);
+        if (r.over) rows.sum = __builtin_nanf("");
+        for (uint32_t j = 0; j < count; ++j) {
+            if (j + D - 1 < count) {
+                copy(j + D - 1, ahead);
+                if (j + D < count) ahead = page_of(j + D);
+                wait_loads<(D - 1) * Shape::kCopies>();
+            } else {
+                wait_loads<0>();
+            }
+            const uint32_t slot0 = (first + j * W) * kTile;
+            if (__builtin_expect(gone >> (j % D) & 1u, 0)) {
+                if (rows.sees(b, group, tree, slot0) != 0) rows.sum = __builtin_nanf("");
+            } else {
+                const Record<F, NB, X> record{ring + j % D * kRecord, slot0, group.latest};
+                rows.template tile<kCodes>(b, group, tree, slot0, record);
+            }
+            __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");  // the record's reads, before its place is copied to
+        }
+        rows.end();
+        __syncthreads();
+
+        // The waves joined, as attend joins them.
+        float4_t(*joined)[kParts] = reinterpret_cast<float4_t(*)[kParts]>(space);
+        const float mine = sum_of_row<X>(rows.sum);
+        if (lane < kRows) joined_offset[wave][n] = rows.offset, joined_sum[wave][n] = mine;
+#pragma unroll
+        for (uint32_t t = 0; t < kQuads; ++t) joined[wave][t * 64 + lane] = rows.quad(t);
+        __syncthreads();
+        auto output_of = [&](uint32_t row, uint32_t value) {
+            return a.output + (uint64_t{r.start} + row / a.group) * a.output_stride +
+                   (uint64_t{head} * a.group + row % a.group) * (32 * NB) + value;
+        };
+        for (uint32_t i = threadIdx.x; i < kParts; i += T) {
+            if (group.row0 + n >= group.row_end) continue;
+            float least = INFINITY, total = 0.0f;
+            float4_t out = float4_t(0.0f);
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+                const float theirs = joined_offset[w][n];
+                least = theirs < least || theirs != theirs ? theirs : least;
+            }
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+                const float theirs = joined_offset[w][n];
+                const float factor = theirs == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(least - theirs);
+                total = __builtin_fmaf(joined_sum[w][n], factor, total);
+                out += joined[w][i] * factor;
+            }
+            const bool empty = least == INFINITY && total == 0.0f;
+            const uint32_t value = Rows<F, NB, X>::quad_at(i / 64);
+            if (pieces == 1) {
+                *reinterpret_cast<float4_t*>(output_of(group.row0 + n, value)) = empty ? float4_t(0.0f) : out * (1.0f / total);
+            } else {
+                *reinterpret_cast<float4_t*>(a.partial + (uint64_t{kept} * kRows + n) * (32 * NB) + value) = out;
+                if (i < kRows) a.stats[uint64_t{kept} * kRows + n] = make_float2(total != total ? total : least, total);
+            }
+        }
+        wait_loads<0>();
+        __syncthreads();  // the LDS is read, and what was written has left the waves
+        if (pieces == 1) continue;
+        if (threadIdx.x == 0) {
+            __threadfence();
+            last_piece = atomicInc(a.counters + counter, pieces - 1) == pieces - 1;
+            __threadfence();
+        }
+        __syncthreads();
+        if (!last_piece) continue;
+
+        // The pieces joined: a thread four values of a row, over its share of the pieces; then over the shares.
+        const uint32_t quads = 8 * NB, work = (group.row_end - group.row0) * quads;
+        const uint32_t shares = max(1u, T / work);
+        auto kept_of = [&](uint32_t p) { return even ? 2 * (part - piece + p) + (p == 0) : counter + p; };
+        float4_t* sums = reinterpret_cast<float4_t*>(space);
+        float2* sides = reinterpret_cast<float2*>(space + T * sizeof(float4_t));
+        for (uint32_t i0 = 0; i0 < work; i0 += T) {
+            const uint32_t i = i0 + threadIdx.x % min(work, T), mine_of = work <= T ? threadIdx.x / work : 0;
+            const bool live = i < work && mine_of < shares;
+            const uint32_t row = i / quads, value = i % quads * 4;
+            float least = INFINITY, total = 0.0f;
+            float4_t out = float4_t(0.0f);
+            if (live)
+#pragma unroll 4
+                for (uint32_t p = mine_of; p < pieces; p += shares) {
+                    const uint64_t from = uint64_t{kept_of(p)} * kRows + row;
+                    const float2 st = a.stats[from];
+                    const float4_t theirs = *reinterpret_cast<const float4_t*>(a.partial + from * (32 * NB) + value);
+                    const float lower = st.x < least || st.x != st.x ? st.x : least;
+                    const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
+                    const float factor = st.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - st.x);
+                    total = total * down + st.y * factor;
+                    out = out * down + theirs * factor;
+                    least = lower;
+                }
+            if (shares > 1) {
+                sums[threadIdx.x] = out, sides[threadIdx.x] = make_float2(least, total);
+                __syncthreads();
+                if (live && mine_of == 0)
+                    for (uint32_t x = 1; x < shares; ++x) {
+                        const float2 st = sides[threadIdx.x + x * work];
+                        const float lower = st.x < least || st.x != st.x ? st.x : least;
+                        const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
+                        const float factor = st.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - st.x);
+                        total = total * down + st.y * factor;
+                        out = out * down + sums[threadIdx.x + x * work] * factor;
+                        least = lower;
+                    }
+            }
+            if (live && mine_of == 0)
+                *reinterpret_cast<float4_t*>(output_of(group.row0 + row, value)) =
+                    least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
+        }
+        __syncthreads();
+    }
+}
+
+template <uint32_t F, uint32_t NB>
+static hipError_t launch_paged_blocks(const PagedAttention& a, uint32_t octets, hipStream_t stream) {
+    if (octets == 2)
+        hipLaunchKernelGGL((attend_pages<F, NB, 2>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attend_pages<F, NB, 1>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 1>::kWaves), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <uint32_t F>
+static hipError_t launch_paged(const PagedAttention& a, uint32_t octets, hipStream_t stream) {
+    switch (a.pool.head_dim / 32) {
+        case 1: return launch_paged_blocks<F, 1>(a, octets, stream);
+        case 2: return launch_paged_blocks<F, 2>(a, octets, stream);
+        case 3: return launch_paged_blocks<F, 3>(a, octets, stream);
+        case 4: return launch_paged_blocks<F, 4>(a, octets, stream);
+        case 5: return launch_paged_blocks<F, 5>(a, octets, stream);
+        case 6: return launch_paged_blocks<F, 6>(a, octets, stream);
+        case 7: return launch_paged_blocks<F, 7>(a, octets, stream);
+        case 8: return launch_paged_blocks<F, 8>(a, octets, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace chm

@@ -4,7 +4,7 @@
 // every value a kernel holds in 32 is checked first.
 #include <cmath>
 
-#include "context.hpp"
+#include "checks.hpp"
 #include "formats.hpp"
 #include "serving.hpp"
 
@@ -17,60 +17,13 @@ struct charlotte_hip_matmul_cache {
 
 namespace {
 
-using chm::fail;
-using chm::hip_fail;
-using chm::ok;
-using Status = charlotte_hip_matmul_status;
-
-constexpr uint64_t kGrid = 0x7FFFFFull;  // workgroups a launch may have: of up to 512 threads, below 2^32 of them
-
-// A failed check, thrown to `guarded` within this file alone.
-struct Refused {
-    Status status;
-    std::string message;
-};
-
-[[noreturn]] void refuse(std::string message, Status status = CHARLOTTE_HIP_MATMUL_INVALID_ARGUMENT) {
-    throw Refused{status, std::move(message)};
-}
-
-// Runs `body`, whose every failure becomes a status and a message beginning
-// with `who`: nothing is thrown across the ABI.
-template <typename Body>
-Status guarded(charlotte_hip_matmul_context* ctx, const char* who, Body body) noexcept {
-    if (!ctx) return CHARLOTTE_HIP_MATMUL_INVALID_ARGUMENT;
-    try {
-        try {
-            const hipError_t e = body();
-            return e == hipSuccess ? ok(ctx) : hip_fail(ctx, e, who);
-        } catch (const Refused& r) {
-            return fail(ctx, r.status, std::string(who) + ": " + r.message);
-        }
-    } catch (...) {  // no memory for a message
-        return CHARLOTTE_HIP_MATMUL_OUT_OF_MEMORY;
-    }
-}
-
-bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-
-// A required device pointer.
-void need(const void* p, const char* name, uintptr_t to) {
-    if (!p) refuse(std::string("no ") + name);
-    if (!aligned(p, to)) refuse(std::string(name) + " not " + std::to_string(to) + "-byte aligned");
-}
-
-// A row stride in floats: 0 means `width`; else at least it, in whole `step`s.
-uint64_t stride_of(uint64_t stride, uint64_t width, uint64_t step, const char* name) {
-    if (stride == 0) stride = width;
-    if (stride < width) refuse(std::string(name) + " below a row's " + std::to_string(width) + " floats");
-    if (stride % step != 0) refuse(std::string(name) + " not whole " + std::to_string(step) + "s");
-    if (stride > (1ull << 40)) refuse(std::string(name) + " past 2^40");
-    return stride;
-}
-
-void need_grid(uint64_t workgroups) {
-    if (workgroups > kGrid) refuse("too many rows a step");
-}
+using chm::aligned;
+using chm::guarded;
+using chm::need;
+using chm::need_grid;
+using chm::refuse;
+using chm::Status;
+using chm::stride_of;
 
 bool cache_type(uint32_t type) {
     return type == CHARLOTTE_HIP_MATMUL_F16 || type == CHARLOTTE_HIP_MATMUL_Q4_0 || type == CHARLOTTE_HIP_MATMUL_Q8_0;
@@ -135,7 +88,7 @@ chm::CacheRows rows_of(const charlotte_hip_matmul_context* ctx, const charlotte_
 uint64_t rows_a_head(const chm::CacheShape& c, uint32_t query_heads, uint32_t tokens) {
     if (query_heads == 0 || query_heads % c.kv_heads != 0 || tokens == 0 || tokens > c.capacity) return 0;
     const uint64_t rows = uint64_t{tokens} * (query_heads / c.kv_heads);
-    return rows * c.sequences * c.kv_heads <= 16 * kGrid ? rows : 0;
+    return rows * c.sequences * c.kv_heads <= 16 * chm::kGrid ? rows : 0;
 }
 
 }  // namespace

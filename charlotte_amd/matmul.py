@@ -236,6 +236,45 @@ class _VerifyDesc(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_uint64)]
 
 
+class _PagePlanDesc(ctypes.Structure):
+    _fields_ = [("past", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("held", ctypes.c_void_p),
+                ("held_after", ctypes.c_void_p), ("table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p), ("free_count_after", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("granted", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("requests", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("table_stride", ctypes.c_uint32), ("pages", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class _PagedAttentionDesc(ctypes.Structure):
+    _fields_ = [("pool", ctypes.c_void_p), ("queries", ctypes.c_void_p), ("output", ctypes.c_void_p),
+                ("query_stride", ctypes.c_uint64), ("output_stride", ctypes.c_uint64),
+                ("query_heads", ctypes.c_uint32), ("window", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("requests", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("most", ctypes.c_uint32),
+                ("past", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _ResidualNormDesc(ctypes.Structure):
+    _fields_ = [("residual", ctypes.c_void_p), ("branch", ctypes.c_void_p), ("branch_weight", ctypes.c_void_p),
+                ("gate", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("residual_out", ctypes.c_void_p),
+                ("normed", ctypes.c_void_p), ("residual_stride", ctypes.c_uint64),
+                ("branch_stride", ctypes.c_uint64), ("gate_stride", ctypes.c_uint64),
+                ("residual_out_stride", ctypes.c_uint64), ("normed_stride", ctypes.c_uint64),
+                ("width", ctypes.c_uint32), ("epsilon", ctypes.c_float), ("residual_scale", ctypes.c_float),
+                ("branch_scale", ctypes.c_float)]
+
+
+class _SampleDesc(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("logit_stride", ctypes.c_uint64), ("uniforms", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("chances", ctypes.c_void_p), ("temperatures", ctypes.c_void_p),
+                ("top_ks", ctypes.c_void_p), ("top_ps", ctypes.c_void_p), ("min_ps", ctypes.c_void_p),
+                ("rows", ctypes.c_uint32), ("vocabulary", ctypes.c_uint32), ("temperature", ctypes.c_float),
+                ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 class _GgufTensor(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char_p),
@@ -328,6 +367,37 @@ SIGNATURES = {
     "charlotte_hip_matmul_verify_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32, _c.c_uint32]),
     "charlotte_hip_matmul_verify": (
         _c.c_int, [_c.c_void_p, _c.POINTER(_VerifyDesc), _c.c_uint32, _c.c_uint32, _c.c_void_p]),
+    "charlotte_hip_matmul_page_pool_bytes": (
+        _c.c_uint64, [_c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_page_pool_create": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.POINTER(_c.c_void_p)],
+    ),
+    "charlotte_hip_matmul_page_pool_wrap": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_uint32, _c.c_void_p, _c.c_uint64,
+         _c.POINTER(_c.c_void_p)],
+    ),
+    "charlotte_hip_matmul_page_pool_free": (_c.c_int, [_c.c_void_p]),
+    "charlotte_hip_matmul_page_plan": (_c.c_int, [_c.c_void_p, _c.POINTER(_PagePlanDesc), _c.c_void_p]),
+    "charlotte_hip_matmul_page_append": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint64, _c.c_uint64, _c.c_void_p, _c.c_uint32,
+         _c.c_void_p],
+    ),
+    "charlotte_hip_matmul_page_read": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint64, _c.c_uint64, _c.c_void_p, _c.c_uint32,
+         _c.c_void_p],
+    ),
+    "charlotte_hip_matmul_paged_attention_workspace_bytes": (
+        _c.c_uint64, [_c.c_void_p, _c.c_void_p, _c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_paged_attention": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_PagedAttentionDesc), _c.c_void_p]),
+    "charlotte_hip_matmul_residual_norm": (
+        _c.c_int, [_c.c_void_p, _c.POINTER(_ResidualNormDesc), _c.c_uint32, _c.c_void_p]),
+    "charlotte_hip_matmul_sample_workspace_bytes": (_c.c_uint64, [_c.c_uint32, _c.c_uint32]),
+    "charlotte_hip_matmul_sample": (_c.c_int, [_c.c_void_p, _c.POINTER(_SampleDesc), _c.c_void_p]),
     "charlotte_hip_matmul_gguf_open": (_c.c_int, [_c.c_char_p, _c.POINTER(_c.c_void_p), _c.POINTER(_c.c_uint32)]),
     "charlotte_hip_matmul_gguf_read": (
         _c.c_int,

@@ -2,12 +2,15 @@
 C ABI (include/charlotte_hip_matmul.h): norms of queries and keys with the
 position rotation, the quantized cache, attention over it for one token, a
 chain or a tree of drafted ones, softmax of the head's logits, and the
-verification of drafted tokens.
+verification of drafted tokens. For a step of several requests of any lengths:
+a pool of cache pages and its tables, attention over it, norms of the residual
+stream, and sampling.
 
 As in charlotte_amd.matmul, calls take device pointers (ints), run on a HIP
-stream, allocate nothing (a Cache aside) and raise ``MatmulError``. Lengths and
-positions are device memory, so a captured step can be replayed as they grow.
-Activations are f32. charlotte_amd/speculative.py runs them together.
+stream, allocate nothing (a Cache or a PagePool aside) and raise
+``MatmulError``. Lengths and positions are device memory, so a captured step can
+be replayed as they grow. Activations are f32. charlotte_amd/speculative.py and
+charlotte_amd/batching.py run them together.
 """
 
 import ctypes
@@ -17,7 +20,8 @@ from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
 from charlotte_amd.matmul import (
-    Context, TensorType, _AttentionDesc, _Heads, _HeadNormRopeDesc, _ProbabilitiesDesc, _VerifyDesc, lib)
+    Context, TensorType, _AttentionDesc, _Heads, _HeadNormRopeDesc, _PagedAttentionDesc, _PagePlanDesc,
+    _ProbabilitiesDesc, _ResidualNormDesc, _SampleDesc, _VerifyDesc, lib)
 
 # The most tokens of a sequence a step with parents may hold.
 TREE_TOKENS = 256
@@ -251,3 +255,198 @@ def verify(ctx: Context, call: Verify, sequences: int, tokens: int, stream=None)
     if call._desc is None:
         call._desc = call.desc()
     ctx.check(lib.charlotte_hip_matmul_verify(ctx.handle, ctypes.byref(call._desc), sequences, tokens, stream))
+
+
+# ---- a step of several requests -------------------------------------------------
+
+
+def page_pool_bytes(gguf_type, pages, page_tokens, kv_heads, head_dim):
+    return lib.charlotte_hip_matmul_page_pool_bytes(int(gguf_type), pages, page_tokens, kv_heads, head_dim)
+
+
+class PagePool:
+    """Keys and values of `pages` pages of `page_tokens` tokens, in Q8_0, Q4_0 or F16
+    (charlotte_hip_matmul_page_pool); in memory of its own, or in `device` (nbytes of it), borrowed."""
+
+    def __init__(self, ctx: Context, gguf_type, pages, page_tokens, kv_heads, head_dim, device=None, nbytes=0):
+        self.handle = None
+        h = ctypes.c_void_p()
+        shape = (int(gguf_type), pages, page_tokens, kv_heads, head_dim)
+        if device is None:
+            ctx.check(lib.charlotte_hip_matmul_page_pool_create(ctx.handle, *shape, ctypes.byref(h)))
+        else:
+            ctx.check(lib.charlotte_hip_matmul_page_pool_wrap(ctx.handle, *shape, device, nbytes, ctypes.byref(h)))
+        self.ctx, self.handle, self.type = ctx, h, TensorType(gguf_type)
+        self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
+
+    def append(self, keys, values, slots, rows, key_stride=0, value_stride=0, stream=None):
+        """Row i's keys and values, quantized, into slot slots[i]."""
+        self.ctx.check(lib.charlotte_hip_matmul_page_append(self.ctx.handle, self.handle, keys, values, key_stride,
+                                                            value_stride, slots, rows, stream))
+
+    def read(self, keys, values, slots, rows, key_stride=0, value_stride=0, stream=None):
+        """The f32 values that slots slots[i] stand for, into row i."""
+        self.ctx.check(lib.charlotte_hip_matmul_page_read(self.ctx.handle, self.handle, keys, values, key_stride,
+                                                          value_stride, slots, rows, stream))
+
+    def free(self):
+        if self.handle and lib:
+            lib.charlotte_hip_matmul_page_pool_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        self.free()
+
+
+@dataclass
+class PagePlan(_Call):
+    """charlotte_hip_matmul_page_plan_desc."""
+
+    requests: int
+    rows: int
+    pages: int
+    page_tokens: int
+    past: int
+    counts: int
+    table: int
+    table_stride: int
+    held: int
+    held_after: int
+    free_pages: int
+    free_count: int
+    free_count_after: int
+    starts: int
+    granted: int
+    slots: int
+    positions: int = 0
+    _desc: Optional[_PagePlanDesc] = field(default=None, repr=False)
+
+    def desc(self):
+        return _PagePlanDesc(self.past, self.counts, self.held, self.held_after, self.table, self.free_pages,
+                             self.free_count, self.free_count_after, self.starts, self.granted, self.slots,
+                             self.positions, self.requests, self.rows, self.table_stride, self.pages, self.page_tokens, 0)
+
+
+def page_plan(ctx: Context, call: PagePlan, stream=None):
+    """Pages given back and taken as the requests' lengths need, and each row's slot and position."""
+    if call._desc is None:
+        call._desc = call.desc()
+    ctx.check(lib.charlotte_hip_matmul_page_plan(ctx.handle, ctypes.byref(call._desc), stream))
+
+
+@dataclass
+class PagedAttention(_Call):
+    """charlotte_hip_matmul_paged_attention_desc."""
+
+    pool: PagePool
+    queries: int
+    output: int
+    query_heads: int
+    scale: float
+    requests: int
+    rows: int
+    past: int
+    counts: int
+    starts: int
+    table: int
+    table_stride: int
+    window: int = 0
+    most: int = 1
+    query_stride: int = 0
+    output_stride: int = 0
+    workspace: int = 0
+    workspace_bytes: int = 0
+    _desc: Optional[_PagedAttentionDesc] = field(default=None, repr=False)
+
+    def desc(self):
+        return _PagedAttentionDesc(self.pool.handle, self.queries, self.output, self.query_stride, self.output_stride,
+                                   self.query_heads, self.window, self.scale, self.requests, self.rows, self.most,
+                                   self.past, self.counts, self.starts, self.table, self.table_stride, 0, self.workspace,
+                                   self.workspace_bytes)
+
+
+def paged_attention_workspace_bytes(ctx: Context, pool: PagePool, query_heads: int, most: int = 1):
+    return lib.charlotte_hip_matmul_paged_attention_workspace_bytes(ctx.handle, pool.handle, query_heads, most)
+
+
+def paged_attention(ctx: Context, call: PagedAttention, stream=None):
+    """The requests' new tokens, already appended, over their pages."""
+    if call._desc is None or not call.pool.handle:  # (a pool that was freed is refused)
+        call._desc = call.desc()
+    ctx.check(lib.charlotte_hip_matmul_paged_attention(ctx.handle, ctypes.byref(call._desc), stream))
+
+
+@dataclass
+class ResidualNorm(_Call):
+    """charlotte_hip_matmul_residual_norm_desc."""
+
+    width: int
+    residual: int
+    branch: int = 0
+    residual_out: int = 0
+    normed: int = 0
+    weight: int = 0
+    branch_weight: int = 0
+    gate: int = 0
+    residual_scale: float = 1.0
+    branch_scale: float = 1.0
+    epsilon: float = 1e-6
+    residual_stride: int = 0
+    branch_stride: int = 0
+    gate_stride: int = 0
+    residual_out_stride: int = 0
+    normed_stride: int = 0
+    _desc: Optional[_ResidualNormDesc] = field(default=None, repr=False)
+
+    def desc(self):
+        return _ResidualNormDesc(self.residual, self.branch, self.branch_weight, self.gate, self.weight, self.residual_out,
+                                 self.normed, self.residual_stride, self.branch_stride, self.gate_stride,
+                                 self.residual_out_stride, self.normed_stride, self.width, self.epsilon,
+                                 self.residual_scale, self.branch_scale)
+
+
+def residual_norm(ctx: Context, call: ResidualNorm, rows: int, stream=None):
+    """A block's output normalised, gated and added to the residual stream, and the stream normalised for the next."""
+    if call._desc is None:
+        call._desc = call.desc()
+    ctx.check(lib.charlotte_hip_matmul_residual_norm(ctx.handle, ctypes.byref(call._desc), rows, stream))
+
+
+@dataclass
+class Sample(_Call):
+    """charlotte_hip_matmul_sample_desc. A setting is the call's, or each row's own where its array is given."""
+
+    logits: int
+    tokens: int
+    rows: int
+    vocabulary: int
+    uniforms: int
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    temperatures: int = 0
+    top_ks: int = 0
+    top_ps: int = 0
+    min_ps: int = 0
+    chances: int = 0
+    logit_stride: int = 0
+    workspace: int = 0
+    workspace_bytes: int = 0
+    _desc: Optional[_SampleDesc] = field(default=None, repr=False)
+
+    def desc(self):
+        return _SampleDesc(self.logits, self.logit_stride, self.uniforms, self.tokens, self.chances, self.temperatures,
+                           self.top_ks, self.top_ps, self.min_ps, self.rows, self.vocabulary, self.temperature, self.top_k,
+                           self.top_p, self.min_p, self.workspace, self.workspace_bytes)
+
+
+def sample_workspace_bytes(rows: int, vocabulary: int):
+    return lib.charlotte_hip_matmul_sample_workspace_bytes(rows, vocabulary)
+
+
+def sample(ctx: Context, call: Sample, stream=None):
+    """A token drawn from each row of logits."""
+    if call._desc is None:
+        call._desc = call.desc()
+    ctx.check(lib.charlotte_hip_matmul_sample(ctx.handle, ctypes.byref(call._desc), stream))

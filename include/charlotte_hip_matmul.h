@@ -10,7 +10,9 @@
  * bound by HBM), more tokens the prefill form (a tiled matrix product). The
  * embedding gather decodes table rows through the same formats. Between the
  * products: norms and rotation of heads, a quantized cache, attention over it;
- * after the head: probabilities, and drafted tokens verified.
+ * after the head: probabilities, and drafted tokens verified. For a step of
+ * several requests: a pool of cache pages, its tables, attention over it, norms of
+ * the residual stream, sampling.
  *
  * What each part replaces in the reference (paths relative to its root):
  *   charlotte_hip_matmul_desc       kernels::MatmulLaunch  src/core/kernels/matmul/matmul.h:602-632
@@ -660,6 +662,216 @@ uint64_t charlotte_hip_matmul_verify_workspace_bytes(uint32_t sequences, uint32_
 charlotte_hip_matmul_status charlotte_hip_matmul_verify(charlotte_hip_matmul_context* ctx,
                                                         const charlotte_hip_matmul_verify_desc* desc,
                                                         uint32_t sequences, uint32_t tokens, void* stream);
+
+/* ---- a step of several requests ---------------------------------------------------- */
+
+/* What a decoder step runs for requests of any lengths at once, each with new
+ * tokens of its own: page_plan, which gives their tokens pages of a pool; around
+ * every block residual_norm; after the QKV product head_norm_rope over all rows,
+ * page_append and paged_attention; after the head sample. A step's rows are the
+ * requests' new tokens, request after request. Lengths, counts and tables are
+ * device memory, so a captured step replays as requests come, grow and end. The
+ * pool aside nothing here allocates. Results are the same bits for the same call. */
+
+/* Keys and values of `pages` pages of `page_tokens` tokens (whole 32s), in a
+ * cache's format and records; a request's tokens are in the pages that its row of
+ * a table names, token t in page table[t / page_tokens]. A slot is page *
+ * page_tokens + t % page_tokens. A page may stand in several requests' rows.
+ * Calls on one pool are ordered by the caller (one stream, or events). */
+typedef struct charlotte_hip_matmul_page_pool charlotte_hip_matmul_page_pool;
+
+/* Bytes the pages take; 0 for a format or sizes a pool cannot have (pages *
+ * page_tokens is below 2^31). */
+uint64_t charlotte_hip_matmul_page_pool_bytes(uint32_t gguf_type, uint32_t pages, uint32_t page_tokens,
+                                              uint32_t kv_heads, uint32_t head_dim);
+/* A pool in memory of the library's (cleared), or in the caller's: `device`
+ * 16-byte aligned, any contents, borrowed until freed. Both allocate some words
+ * more that paged_attention counts in, and are synchronous. */
+charlotte_hip_matmul_status charlotte_hip_matmul_page_pool_create(charlotte_hip_matmul_context* ctx, uint32_t gguf_type,
+                                                                  uint32_t pages, uint32_t page_tokens,
+                                                                  uint32_t kv_heads, uint32_t head_dim,
+                                                                  charlotte_hip_matmul_page_pool** out);
+charlotte_hip_matmul_status charlotte_hip_matmul_page_pool_wrap(charlotte_hip_matmul_context* ctx, uint32_t gguf_type,
+                                                                uint32_t pages, uint32_t page_tokens,
+                                                                uint32_t kv_heads, uint32_t head_dim, void* device,
+                                                                uint64_t bytes, charlotte_hip_matmul_page_pool** out);
+charlotte_hip_matmul_status charlotte_hip_matmul_page_pool_free(charlotte_hip_matmul_page_pool* pool);
+
+/* Block tables and slot maps from the requests' lengths. Request r has past[r]
+ * tokens that stay, and counts[r] new ones; its table row names held[r] pages.
+ * It needs ceil((past + counts) / page_tokens): a request that holds more gives
+ * the rest back (one that has ended: past and counts 0), one that holds fewer
+ * takes more. free_pages is a stack, its first free_count entries the free pages.
+ * All pages given back go onto it first, requests and their entries in rising
+ * order; then the requests take theirs off its top, in that order too. They are
+ * served while the running sum of what they take is at most what is there: from
+ * the first that is not, requests that need pages get none, others are served.
+ * Served neither is a request that needs more than table_stride pages, or has
+ * new tokens past row `rows` of the step (it neither gives nor takes).
+ *
+ *   held_after[r]     pages of the request now: held[r] where it was not served
+ *   free_count_after  entries of free_pages that are free now
+ *   starts[r]         its first row: the sum of the counts before it; starts[requests]: of all
+ *   granted[r]        counts[r], or 0 where it was not served
+ *   slots[i]          row i's slot in the pool; 0xFFFFFFFF where it has none
+ *   positions[i]      past[r] plus the row's place among its request's; 0 for rows of no request
+ * Entries of the table and of the stack that the step neither gives nor takes
+ * are left as they are. held_after may be held, free_count_after free_count (or,
+ * to run a step again, memory apart); the rest is apart from each other. */
+typedef struct {
+    const uint32_t* past;         /* device: a word a request, as the next three */
+    const uint32_t* counts;
+    const uint32_t* held;
+    uint32_t* held_after;
+    uint32_t* table;              /* device: requests rows of table_stride */
+    uint32_t* free_pages;         /* device: `pages` words */
+    const uint32_t* free_count;   /* device: a word */
+    uint32_t* free_count_after;
+    uint32_t* starts;             /* device: requests + 1 */
+    uint32_t* granted;            /* device: requests */
+    uint32_t* slots;              /* device: rows */
+    uint32_t* positions;          /* device: rows, or NULL */
+    uint32_t requests;            /* 1 .. 65,536 */
+    uint32_t rows;                /* the step's, at least 1; rows past the requests' have no slot */
+    uint32_t table_stride;
+    uint32_t pages;               /* the pool's */
+    uint32_t page_tokens;
+    uint32_t reserved;            /* 0 */
+} charlotte_hip_matmul_page_plan_desc;
+
+charlotte_hip_matmul_status charlotte_hip_matmul_page_plan(charlotte_hip_matmul_context* ctx,
+                                                           const charlotte_hip_matmul_page_plan_desc* desc, void* stream);
+
+/* Row i's keys and values (as cache_append's: strides, alignment, rounding) into
+ * slot slots[i], for i = 0 .. rows - 1; a row whose slot the pool does not have is
+ * not written. No two rows have one slot. */
+charlotte_hip_matmul_status charlotte_hip_matmul_page_append(charlotte_hip_matmul_context* ctx,
+                                                             charlotte_hip_matmul_page_pool* pool, const float* keys,
+                                                             const float* values, uint64_t key_stride,
+                                                             uint64_t value_stride, const uint32_t* slots,
+                                                             uint32_t rows, void* stream);
+/* The reverse: the values that the slots stand for. A row whose slot the pool does
+ * not have is left as it is. */
+charlotte_hip_matmul_status charlotte_hip_matmul_page_read(charlotte_hip_matmul_context* ctx,
+                                                           const charlotte_hip_matmul_page_pool* pool, float* keys,
+                                                           float* values, uint64_t key_stride, uint64_t value_stride,
+                                                           const uint32_t* slots, uint32_t rows, void* stream);
+
+/* Attention of each request's new tokens, already appended at places past[r] ..
+ * past[r] + counts[r] - 1, over its pages: as charlotte_hip_matmul_attention's of
+ * a chain, each token seeing those before it and itself, with a window w > 0 the
+ * last w of them. Row starts[r] + t is request r's token t (page_plan's starts; its
+ * granted are the counts: a request not granted sees nothing and its rows are left
+ * as they are, as rows of no request are). A request whose rows pass `rows` is
+ * left out. A token in a page that the pool does not have makes the outputs of the
+ * rows that see it NaN, tokens past the table's row those of all of the request's.
+ * The work is shared among the card's compute units by the tokens that are there,
+ * whatever the requests' lengths. */
+typedef struct {
+    const charlotte_hip_matmul_page_pool* pool;
+    const float* queries;     /* device, 16-byte aligned: row i's heads at queries + i * query_stride */
+    float* output;            /* device, 16-byte aligned, apart from queries: rows of query_heads * head_dim */
+    uint64_t query_stride;    /* floats, whole 4s; 0: query_heads * head_dim */
+    uint64_t output_stride;
+    uint32_t query_heads;     /* a multiple of the pool's kv_heads */
+    uint32_t window;          /* 0: none */
+    float scale;              /* finite */
+    uint32_t requests;        /* 1 .. 65,536 */
+    uint32_t rows;            /* the step's, 1 .. 2^20 */
+    /* The most new tokens of a request, for the choice of a kernel alone (0: 1): any value gives a right answer. */
+    uint32_t most;
+    const uint32_t* past;     /* device: a word a request */
+    const uint32_t* counts;
+    const uint32_t* starts;
+    const uint32_t* table;    /* device: requests rows of table_stride */
+    uint32_t table_stride;    /* at least 1; table_stride * page_tokens below 2^31 */
+    uint32_t reserved;        /* 0 */
+    void* workspace;          /* device, 16-byte aligned: paged_attention_workspace_bytes */
+    uint64_t workspace_bytes;
+} charlotte_hip_matmul_paged_attention_desc;
+
+/* Bytes of workspace that serve every step whose `most` is at most this one; 0
+ * for sizes the launch refuses. The contents need no care; launches that share a
+ * workspace must be ordered on one stream. */
+uint64_t charlotte_hip_matmul_paged_attention_workspace_bytes(const charlotte_hip_matmul_context* ctx,
+                                                              const charlotte_hip_matmul_page_pool* pool,
+                                                              uint32_t query_heads, uint32_t most);
+charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_matmul_context* ctx,
+                                                                 const charlotte_hip_matmul_paged_attention_desc* desc,
+                                                                 void* stream);
+
+/* Between two blocks, for each row of the residual stream x and a block's output y:
+ *   z = y, or with branch_weight y / sqrt(mean(y^2) + epsilon) * branch_weight
+ *   r = residual_scale x + branch_scale gate z       (no gate: one; no branch: no such term)
+ *   n = r / sqrt(mean(r^2) + epsilon) * weight
+ * r goes to residual_out, n to normed, either of which may be NULL. Sums are f32.
+ * An output may be an input's memory with its stride, or memory apart from all. */
+typedef struct {
+    const float* residual;        /* device: rows of `width`, residual_stride apart */
+    const float* branch;          /* device, or NULL */
+    const float* branch_weight;   /* device: `width`, or NULL */
+    const float* gate;            /* device: `width` a row, gate_stride apart, or NULL */
+    const float* weight;          /* device: `width`; with normed */
+    float* residual_out;          /* device, or NULL */
+    float* normed;                /* device, or NULL */
+    uint64_t residual_stride;     /* floats; 0: width */
+    uint64_t branch_stride;
+    uint64_t gate_stride;         /* floats; 0: one gate for every row */
+    uint64_t residual_out_stride;
+    uint64_t normed_stride;
+    uint32_t width;               /* 1 .. 32,768 */
+    float epsilon;                /* finite, not negative */
+    float residual_scale;         /* finite */
+    float branch_scale;           /* finite */
+} charlotte_hip_matmul_residual_norm_desc;
+
+charlotte_hip_matmul_status charlotte_hip_matmul_residual_norm(charlotte_hip_matmul_context* ctx,
+                                                               const charlotte_hip_matmul_residual_norm_desc* desc,
+                                                               uint32_t rows, void* stream);
+
+/* A token drawn from each row of logits l. Its tokens stand in the order of their
+ * logits, the largest first, of equals the lowest index; a NaN counts as -inf. The
+ * weight of a token is the whole number floor(2^40 exp((l - m) / temperature)), m
+ * the row's largest (a row with +inf: 2^40 for those, 0 for the rest; -inf: 0).
+ * Kept are, each of the ones before it:
+ *   top_k > 0    the first top_k tokens
+ *   top_p < 1    the shortest run of the first tokens whose weights' sum is at
+ *                least ceil(top_p * that of all kept so far)
+ *   min_p > 0    the tokens whose weight is at least ceil(min_p * 2^40)
+ * and always the first. At a temperature below 1e-6 (or one that is a NaN) it alone.
+ * top_p is taken within 0 .. 1, a NaN as 1; min_p within 0 .. 1, a NaN as 0. With W
+ * the kept tokens' sum and r = floor(u 2^31) (u as verify takes it: one outside 0
+ * .. 1 - 2^-24 as the nearer end, a NaN as 0), the token drawn is the first whose
+ * running sum passes floor(W r / 2^31): in whole numbers, but for the exponential
+ * (in f64, within a unit of its last place).
+ *
+ * tokens gets the token, -1 for a row of nothing but -inf; chances, if given, its
+ * weight over W (such a row: 0). The settings are a row's own where their array is
+ * given (device, a word a row), else the call's. */
+typedef struct {
+    const float* logits;          /* device, 4-byte aligned: row i at logits + i * logit_stride */
+    uint64_t logit_stride;        /* floats; 0: vocabulary */
+    const float* uniforms;        /* device: rows */
+    int32_t* tokens;              /* device: rows */
+    float* chances;               /* device: rows, or NULL */
+    const float* temperatures;    /* device: rows, or NULL; likewise the next three */
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    uint32_t rows;
+    uint32_t vocabulary;          /* at most 2^18 */
+    float temperature;            /* without temperatures: not negative; likewise the next three */
+    int32_t top_k;                /* 0 and below: all */
+    float top_p;
+    float min_p;
+    void* workspace;              /* device, 16-byte aligned: sample_workspace_bytes */
+    uint64_t workspace_bytes;
+} charlotte_hip_matmul_sample_desc;
+
+/* The contents need no care; launches that share a workspace must be ordered on one stream. */
+uint64_t charlotte_hip_matmul_sample_workspace_bytes(uint32_t rows, uint32_t vocabulary);
+charlotte_hip_matmul_status charlotte_hip_matmul_sample(charlotte_hip_matmul_context* ctx,
+                                                        const charlotte_hip_matmul_sample_desc* desc, void* stream);
 
 /* ---- GGUF files (gguf::read_index, src/core/gguf/reader.cpp) -------------------- */
 
