@@ -8,18 +8,25 @@
 // a number? It is answered without sorting the row, in three launches over chunks
 // of the rows:
 //   row_largest   each chunk's largest logit;
-//   row_bins      the weights and counts of kBins equal steps of (m - l) / T, down
-//                 to where a weight is 0. The workgroup that ends a row last finds
-//                 the bins that the cuts and the draw may fall into: a cut's bin
-//                 bounds what is kept, that the bins of the cuts after it;
-//   row_draw      the tokens of those bins, few hundreds, gathered. The last
-//                 workgroup of a row sorts them, and answers exactly.
+//   row_bins      counts, and weights to within known bounds (f32's exponential, in
+//                 whole units of 2^-26), of kBins equal steps of (m - l) / T, down to
+//                 where a weight is 0; a bin's two sums in one word. The workgroup
+//                 that ends a row last finds the bins that the cuts and the draw may
+//                 fall into: a cut's bins bound what is kept, that the next one's;
+//   row_draw      the exact weights: those before each run of such bins summed, the
+//                 tokens in them, some hundreds, gathered. The last workgroup of a
+//                 row sorts them by finer bins, and answers.
 // Where those bins hold more than kList tokens (many equal logits, a temperature
 // that makes them so) or the largest is +inf, one workgroup answers by descent:
 // weights and counts of the logits' leading bits (as keys that rise with them)
 // summed in LDS, the part that holds the answer opened by its next bits; tokens of
 // one key have one weight, so the place among them is a division.
 // Sums are of whole numbers, so that atomics may add them in any order.
+//
+// What a row's workgroups leave for the last of them goes past the caches that
+// they do not share, by atomics and by loads and stores of the device's scope:
+// each workgroup waits for its own to arrive, then counts itself; no cache is
+// written back or cleared for it.
 #include <algorithm>
 #include <cstddef>
 
@@ -38,6 +45,7 @@ constexpr double kWhole = 1099511627776.0;  // 2^40
 // A row's settings, as its kernels use them.
 struct Settings {
     double rate;       // 1 / temperature
+    double octaves;    // log2(e) / temperature
     uint64_t top_k;    // tokens
     double top_p;      // 1: all
     uint64_t least;    // min_p's weight
@@ -53,6 +61,7 @@ __device__ __forceinline__ Settings settings_of(const Sample& a, uint32_t row) {
     Settings s;
     s.greedy = !(t >= 1e-6f) || k == 1;
     s.rate = s.greedy ? 1.0 : 1.0 / static_cast<double>(t);
+    s.octaves = s.rate * 1.44269504088896340736;
     s.top_k = k > 0 && static_cast<uint32_t>(k) < a.vocabulary ? static_cast<uint32_t>(k) : a.vocabulary;
     s.top_p = p < 1.0f ? fmax(static_cast<double>(p), 0.0) : 1.0;  // (a NaN: 1)
     s.least = static_cast<uint64_t>(ceil((m > 0.0f ? fmin(static_cast<double>(m), 1.0) : 0.0) * kWhole));
@@ -70,10 +79,30 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-__device__ __forceinline__ uint64_t weight_of(float l, float most, double rate) {
+// floor(2^40 exp((l - m) rate)), `octaves` = rate log2(e): 2^z by its series, z within
+// half of a whole number (the 12th term is below 2^-47), all of it within 2^-46.
+__device__ __forceinline__ uint64_t weight_of(float l, float most, double octaves) {
     if (l == most) return 1ull << 40;
     if (l == -INFINITY || most == INFINITY) return 0;
-    return static_cast<uint64_t>(exp((static_cast<double>(l) - static_cast<double>(most)) * rate) * kWhole);
+    const double y = (static_cast<double>(l) - static_cast<double>(most)) * octaves;
+    if (y < -41.0) return 0;
+    const double whole = rint(y), z = (y - whole) * 0.693147180559945309417;
+    double p = 1.0 / 39916800;
+    p = __builtin_fma(p, z, 1.0 / 3628800);
+    p = __builtin_fma(p, z, 1.0 / 362880);
+    p = __builtin_fma(p, z, 1.0 / 40320);
+    p = __builtin_fma(p, z, 1.0 / 5040);
+    p = __builtin_fma(p, z, 1.0 / 720);
+    p = __builtin_fma(p, z, 1.0 / 120);
+    p = __builtin_fma(p, z, 1.0 / 24);
+    p = __builtin_fma(p, z, 1.0 / 6);
+    p = __builtin_fma(p, z, 0.5);
+    p = __builtin_fma(p, z, 1.0);
+    p = __builtin_fma(p, z, 1.0);
+    // at most 2^40, in two parts that 32 bits hold
+    const double w = ldexp(p, static_cast<int>(whole) + 40);
+    const uint32_t high = static_cast<uint32_t>(w * 0x1p-20), low = static_cast<uint32_t>(__builtin_fma(high, -0x1p20, w));
+    return (uint64_t{high} << 20) + low;
 }
 
 // The sum over the workgroup's threads before this one, and of all. `parts`: a word a wave.
@@ -103,7 +132,7 @@ struct DrawRow {
     const float* x;
     uint32_t lead, vocabulary;
     float most;
-    double rate;
+    double octaves;
 
     // f(logit, index) for each of the row's tokens.
     template <typename F>
@@ -148,7 +177,7 @@ __device__ Place descend(const DrawRow& row, uint64_t target, Descent& d) {
             const uint32_t key = key_of(l);
             if (level > 0 && key >> above != prefix) return;
             const uint32_t bin = key >> shift & (kBins - 1) & ((1u << (above - shift)) - 1);
-            const uint64_t w = weight_of(l, row.most, row.rate);
+            const uint64_t w = weight_of(l, row.most, row.octaves);
             if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&d.weights[bin]), static_cast<unsigned long long>(w));
             if (COUNT) atomicAdd(&d.counts[bin], 1u);
         });
@@ -175,7 +204,7 @@ __device__ Place descend(const DrawRow& row, uint64_t target, Descent& d) {
     Place p;
     p.key = prefix;
     p.before = before_weight;
-    p.weight = weight_of(logit_of(prefix), row.most, row.rate);
+    p.weight = weight_of(logit_of(prefix), row.most, row.octaves);
     p.rank = COUNT ? target - before_count : (target - before_weight) / p.weight;
     return p;
 }
@@ -221,12 +250,12 @@ __device__ __forceinline__ void write_draw(const Sample& a, uint32_t row, uint32
 
 // A row by one workgroup, by descent.
 __device__ void draw_alone(const Sample& a, uint32_t r, const Settings& s, float most, Descent& d) {
-    DrawRow row{a.logits + r * a.logit_stride, 0, a.vocabulary, most, s.rate};
+    DrawRow row{a.logits + r * a.logit_stride, 0, a.vocabulary, most, s.octaves};
     row.lead = lead_of(row.x);
     // All weights, and those that min_p leaves.
     uint64_t all = 0, some = 0;
     row.each([&](float l, uint32_t) {
-        const uint64_t w = weight_of(l, row.most, row.rate);
+        const uint64_t w = weight_of(l, row.most, row.octaves);
         all += w;
         if (w >= s.least) some += w;
     });
@@ -249,31 +278,41 @@ __device__ void draw_alone(const Sample& a, uint32_t r, const Settings& s, float
 
 // ---- by bins -----------------------------------------------------------------
 
-// Runs of bins whose tokens are gathered, in order and apart; what lies before each.
-struct Run {
-    uint32_t first, last;
-    uint64_t weight, count;
-    uint32_t start;         // its first token's place in the list
-    uint32_t reserved;
-};
-struct DrawPlan {
-    uint64_t likely;            // the weight that min_p leaves
-    uint64_t kept;              // without a cut: what top_k leaves
-    uint32_t binned, gathered;  // workgroups of row_bins, of row_draw, that have ended
-    uint32_t listed;            // tokens gathered
-    uint32_t runs, alone;       // runs; or by descent
-    uint32_t cut;               // top_k's last token is in a run
-    Run run[3];
-};
+// What a row's workgroups share, at the device's scope.
+template <typename T>
+__device__ __forceinline__ T get(const T& x) {
+    return __hip_atomic_load(&x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ void put(T& x, T value) {
+    __hip_atomic_store(&x, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T add(T& x, T value) {
+    return __hip_atomic_fetch_add(&x, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
+// Bins whose tokens are gathered: `first` .. `last`, of `count` tokens, those before
+// them `before`; the first token's place in the list.
+struct Run {
+    uint32_t first, last, count, before, start, reserved;
+};
+constexpr uint32_t kRuns = 3;
 // A row's part of the workspace.
 struct DrawRoom {
-    uint64_t weights[kBins];
-    uint32_t counts[kBins];
-    DrawPlan plan;          // (cleared with the bins by row_largest)
-    uint64_t list[kList];   // key, and the index's complement: the first token is the largest
+    uint64_t bins[kBins];        // a count, and under it weights in 2^-26
+    uint64_t sums[2 + kRuns];    // exact weights: of all tokens, of those that min_p leaves, and of those before a run
+    uint32_t binned, gathered;   // workgroups of row_bins, of row_draw, that have ended
+    uint32_t listed;             // tokens gathered
+    uint32_t runs, alone;        // runs; or by descent
+    uint32_t cut;                // top_k's last token is in a run
+    Run run[kRuns];
+    uint64_t list[kList];        // key, and the index's complement: the first token is the largest
 };
-constexpr uint32_t kCleared = (offsetof(DrawRoom, list) + 3) / 4;
+constexpr uint32_t kCleared = offsetof(DrawRoom, list) / 8;
+static_assert(offsetof(DrawRoom, list) % 8 == 0, "words of 8 bytes");
+constexpr uint32_t kWeightBits = 45;  // 2^26 of each of 2^18 tokens, and 2^18 above them
+constexpr float kUnit = 0x1p26f;
 
 struct DrawChunks {
     DrawRoom* rooms;
@@ -305,7 +344,7 @@ __device__ __forceinline__ uint64_t most_of_wave(uint64_t x) {
 __global__ __launch_bounds__(kDrawThreads) void row_largest(Sample a, DrawChunks c) {
     __shared__ uint64_t parts[kDrawThreads / 64];
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
-    uint32_t* room = reinterpret_cast<uint32_t*>(c.rooms + row);
+    uint64_t* room = reinterpret_cast<uint64_t*>(c.rooms + row);
     for (uint32_t i = chunk * kDrawThreads + threadIdx.x; i < kCleared; i += c.chunks * kDrawThreads) room[i] = 0;
     uint64_t most = 0;
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) { most = max(most, uint64_t{key_of(l)} << 32 | ~i); });
@@ -325,175 +364,245 @@ __device__ __forceinline__ uint64_t largest_of(const DrawChunks& c, uint32_t row
     return most_of_wave(most);
 }
 
-// The bin of a logit: it does not fall as the logit does.
-__device__ __forceinline__ uint32_t bin_of(float l, float most, float steps) {
-    return static_cast<uint32_t>(fminf((most - l) * steps, static_cast<float>(kBins - 1)));
+// A logit's place among the bins: it does not fall as the logit does.
+__device__ __forceinline__ float place_of(float l, float most, float steps) {
+    return fminf((most - l) * steps, static_cast<float>(kBins - 1));
 }
 __device__ __forceinline__ float steps_of(const Settings& s) {
     return static_cast<float>(s.rate * (static_cast<double>(kBins - 1) / kReach));
 }
 
-// Whether this is the last of a row's workgroups to come here; then it sees what they wrote.
-__device__ __forceinline__ bool last_of(uint32_t* counter, uint32_t workgroups, uint32_t* flag) {
-    __builtin_amdgcn_s_waitcnt(0);  // each wave's writes are out
+// Whether this is the last of a row's workgroups to come here.
+__device__ __forceinline__ bool last_of(uint32_t& counter, uint32_t workgroups, uint32_t* flag) {
+    __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");  // what each wave wrote has arrived
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        *flag = atomicAdd(counter, 1u) == workgroups - 1;
-        __threadfence();
-    }
+    if (threadIdx.x == 0) *flag = add(counter, 1u) == workgroups - 1;
     __syncthreads();
     return *flag != 0;
 }
 
+// Bounds of a weight, in units of 2^-40, of which `sum` is the binned one, in 2^-26,
+// of `count` tokens: a token's was cut to a whole unit, and f32's exponential is
+// within 2^-16 of it (its argument, below 41, within 3 times 2^-24 of itself); the
+// exact one is cut to a whole 2^-40. Twice that, and the sums' own roundings.
+__device__ __forceinline__ uint64_t at_least(uint64_t sum, uint64_t count) {
+    const uint64_t off = (sum >> 15) + (count >> 14) + 8;
+    return sum > off ? (sum - off) << 14 : 0;
+}
+__device__ __forceinline__ uint64_t at_most(uint64_t sum, uint64_t count) { return (sum + (sum >> 15) + count + 8) << 14; }
+
+struct Planning {
+    uint64_t sums[kBins + 1];    // binned weights before a bin
+    uint32_t counts[kBins + 1];
+    uint64_t parts[kDrawThreads / 64];
+};
+
 // The bins that the row's cuts and its draw may fall into, by the last of its workgroups.
-__device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Descent& d) {
+__device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Planning& d) {
     constexpr uint32_t kMine = kBins / kDrawThreads;
-    uint64_t w[kMine], c[kMine], weight = 0, count = 0, total, tokens;
+    uint64_t word[kMine], sum = 0, all;
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) word[i] = get(room.bins[kMine * threadIdx.x + i]);
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) sum += word[i];
+    // both sums of a word at once: neither passes its bits
+    uint64_t before = sum_before(sum, d.parts, &all);
 #pragma unroll
     for (uint32_t i = 0; i < kMine; ++i) {
         const uint32_t bin = kMine * threadIdx.x + i;
-        w[i] = room.weights[bin], c[i] = room.counts[bin];
-        weight += w[i], count += c[i];
+        d.sums[bin] = before & ((1ull << kWeightBits) - 1), d.counts[bin] = static_cast<uint32_t>(before >> kWeightBits);
+        before += word[i];
     }
-    weight = sum_before(weight, d.parts, &total);
-    count = sum_before(count, d.parts, &tokens);
+    if (threadIdx.x == 0) d.sums[kBins] = all & ((1ull << kWeightBits) - 1), d.counts[kBins] = static_cast<uint32_t>(all >> kWeightBits);
     __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-        const uint32_t bin = kMine * threadIdx.x + i;
-        d.weights[bin] = weight, d.counts[bin] = static_cast<uint32_t>(count);  // before the bin
-        weight += w[i], count += c[i];
-    }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    auto after = [&](uint32_t bin) { return bin + 1 < kBins ? d.weights[bin + 1] : total; };
-    auto counted = [&](uint32_t bin) { return bin + 1 < kBins ? uint64_t{d.counts[bin + 1]} : tokens; };
-    // the bin whose running weight passes `target`
-    auto bin_at = [&](uint64_t target) {
-        uint32_t low = 0, high = kBins;
-        while (high - low > 1) {
-            const uint32_t middle = (low + high) / 2;
-            (d.weights[middle] <= target ? low : high) = middle;
-        }
-        return low;
+    if (threadIdx.x >= 64) return;
+    // By one wave: the first bin (of kBins) of which `passed` is true, as it is of all after it.
+    const uint32_t lane = threadIdx.x;
+    auto first_bin = [&](auto passed) {
+        const uint32_t block = __popcll(__ballot(!passed(kBins / 64 * lane + kBins / 64 - 1)));
+        if (block == 64) return kBins - 1;
+        const uint32_t in = __popcll(__ballot(lane < kBins / 64 && !passed(kBins / 64 * block + lane % (kBins / 64))));
+        return kBins / 64 * block + in;
     };
-    __shared__ Run run[3];  // (indexed by thread 0 alone)
-    uint32_t runs = 0;
-    uint64_t low = total, high = total;  // what is kept weighs no less and no more
+    // a question's bins, its target between `low` and `high`
+    auto run_of = [&](uint64_t low, uint64_t high) {
+        Run r{};
+        r.first = first_bin([&](uint32_t bin) { return at_most(d.sums[bin + 1], d.counts[bin + 1]) > low; });
+        r.last = first_bin([&](uint32_t bin) { return at_least(d.sums[bin + 1], d.counts[bin + 1]) > high; });
+        r.last = min(r.last, kBins - 2);  // the last bin's tokens weigh nothing
+        return r;
+    };
+    Run none{kBins, kBins, 0, 0, 0, 0}, top_k = none, top_p = none;
+    uint64_t low = at_least(d.sums[kBins], d.counts[kBins]), high = at_most(d.sums[kBins], d.counts[kBins]);  // of what is kept
     if (s.top_k < a.vocabulary) {
-        uint32_t from = 0, to = kBins;
-        while (to - from > 1) {
-            const uint32_t middle = (from + to) / 2;
-            (d.counts[middle] < s.top_k ? from : to) = middle;
+        const uint32_t bin = first_bin([&](uint32_t b) { return d.counts[b + 1] >= s.top_k; });
+        if (bin < kBins - 1) {
+            top_k.first = top_k.last = bin;
+            low = at_least(d.sums[bin], d.counts[bin]), high = at_most(d.sums[bin + 1], d.counts[bin + 1]);
         }
-        low = d.weights[from], high = after(from);
-        if (counted(from) == s.top_k) low = high;
-        if (low != high) run[runs++] = {from, from, 0, 0, 0, 0};
     }
-    room.plan.cut = low != high, room.plan.kept = low;
+    low = max(low, 1ull << 40), high = max(high, 1ull << 40);  // the first token is always kept
     if (s.top_p < 1.0) {
-        const uint32_t from = bin_at(passed_by(s, low)), to = bin_at(passed_by(s, high));
-        run[runs++] = {from, to, 0, 0, 0, 0};
-        low = d.weights[from], high = after(to);
+        top_p = run_of(passed_by(s, low), passed_by(s, high));
+        low = max(at_least(d.sums[top_p.first], d.counts[top_p.first]), 1ull << 40);
+        high = min(high, max(at_most(d.sums[top_p.last + 1], d.counts[top_p.last + 1]), 1ull << 40));
     }
-    const uint64_t likely = max(room.plan.likely, 1ull << 40);
-    low = max(min(low, likely), 1ull), high = min(high, likely);
-    run[runs++] = {bin_at(drawn_at(s, low)), bin_at(drawn_at(s, high)), 0, 0, 0, 0};
+    if (s.least > 0) {
+        // min_p's last token is in the bin of its distance or, by rounding, one beside it
+        const double at = -log(static_cast<double>(s.least) / kWhole) * (static_cast<double>(kBins - 1) / kReach);
+        const uint32_t bin = static_cast<uint32_t>(fmin(at, static_cast<double>(kBins - 1)));
+        const uint32_t from = bin > 1 ? bin - 1 : 0, to = min(bin + 2, kBins);
+        low = min(low, max(at_least(d.sums[from], d.counts[from]), 1ull << 40));
+        high = min(high, max(at_most(d.sums[to], d.counts[to]), 1ull << 40));
+    }
+    const Run draw = run_of(drawn_at(s, low), drawn_at(s, high));
+    if (lane != 0) return;
     // in order, and those that meet as one
-    for (uint32_t i = 1; i < runs; ++i)
-        for (uint32_t j = i; j > 0 && run[j].first < run[j - 1].first; --j) {
-            const Run t = run[j];
-            run[j] = run[j - 1], run[j - 1] = t;
+    Run x = draw, y = top_k, z = top_p;
+    auto order = [](Run& u, Run& v) {
+        if (v.first < u.first) {
+            const Run t = u;
+            u = v, v = t;
         }
-    uint32_t merged = 0;
-    for (uint32_t i = 1; i < runs; ++i)
-        if (run[i].first <= run[merged].last + 1)
-            run[merged].last = max(run[merged].last, run[i].last);
-        else
-            run[++merged] = run[i];
-    uint64_t listed = 0;
-    for (uint32_t i = 0; i <= merged; ++i) {
-        run[i].weight = d.weights[run[i].first], run[i].count = d.counts[run[i].first];
-        run[i].start = static_cast<uint32_t>(listed);
-        listed += counted(run[i].last) - run[i].count;
-        room.plan.run[i] = run[i];
+    };
+    order(x, y), order(y, z), order(x, y);
+    uint32_t runs = 0, listed = 0;
+    auto keep = [&](Run r) {
+        r.before = d.counts[r.first], r.count = d.counts[r.last + 1] - r.before, r.start = listed;
+        listed += r.count;
+        room.run[runs++] = r;
+    };
+    auto meet = [](const Run& u, const Run& v) { return v.first < kBins && v.first <= u.last + 1; };
+    if (meet(y, z)) y.last = max(y.last, z.last), z = none;
+    if (meet(x, y)) {
+        x.last = max(x.last, y.last), y = z, z = none;
+        if (meet(x, y)) x.last = max(x.last, y.last), y = none;
     }
-    room.plan.runs = merged + 1;
-    room.plan.alone = listed > kList;
+    keep(x);
+    if (y.first < kBins) keep(y);
+    if (z.first < kBins) keep(z);
+    room.runs = runs, room.cut = top_k.first < kBins, room.alone = listed > kList;
 }
 
 __global__ __launch_bounds__(kDrawThreads) void row_bins(Sample a, DrawChunks c) {
-    __shared__ Descent d;
+    __shared__ union {
+        uint64_t bins[kBins];
+        Planning planning;
+    } space;
     __shared__ uint32_t last;
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
+    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads) space.bins[i] = 0;
     const Settings s = settings_of(a, row);
     const float most = logit_of(static_cast<uint32_t>(largest_of(c, row) >> 32));
     if (s.greedy || fabsf(most) == INFINITY) return;
     DrawRoom& room = c.rooms[row];
-    const float steps = steps_of(s);
-    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads) d.weights[i] = 0, d.counts[i] = 0;
+    const float steps = steps_of(s), octaves = static_cast<float>(s.octaves);
     __syncthreads();
-    uint64_t likely = 0;
     uint32_t rest = 0;
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t) {
-        const uint32_t bin = bin_of(l, most, steps);
+        const uint32_t bin = static_cast<uint32_t>(place_of(l, most, steps));
         if (bin == kBins - 1) {
             ++rest;
             return;
         }
-        const uint64_t w = weight_of(l, most, s.rate);
-        if (w >= s.least) likely += w;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&d.weights[bin]), static_cast<unsigned long long>(w));
-        atomicAdd(&d.counts[bin], 1u);
+        const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_exp2f((l - most) * octaves) * kUnit);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&space.bins[bin]), 1ull << kWeightBits | w);
     });
 #pragma unroll
-    for (uint32_t o = 32; o > 0; o >>= 1) likely += __shfl_xor(likely, o), rest += __shfl_xor(rest, o);
-    if ((threadIdx.x & 63u) == 0) {
-        if (rest) atomicAdd(&d.counts[kBins - 1], rest);
-        if (likely) atomicAdd(reinterpret_cast<unsigned long long*>(&room.plan.likely), static_cast<unsigned long long>(likely));
-    }
+    for (uint32_t o = 32; o > 0; o >>= 1) rest += __shfl_xor(rest, o);
+    if ((threadIdx.x & 63u) == 0 && rest > 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&space.bins[kBins - 1]), static_cast<unsigned long long>(rest) << kWeightBits);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads) {
-        if (d.counts[i] == 0) continue;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&room.weights[i]), static_cast<unsigned long long>(d.weights[i]));
-        atomicAdd(&room.counts[i], d.counts[i]);
-    }
-    if (last_of(&room.plan.binned, c.chunks, &last)) plan_row(a, s, room, d);
+    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads)
+        if (space.bins[i] != 0) add(room.bins[i], space.bins[i]);
+    if (last_of(room.binned, c.chunks, &last)) plan_row(a, s, room, space.planning);
 }
 
 // The row's list sorted, and its questions answered, by the last of its workgroups.
 struct Sorting {
-    uint64_t list[kList];
-    uint64_t before[kList];  // the list's weight before a token
+    uint64_t list[kList], sorted[kList];
+    uint64_t before[kList];        // the list's weight before a token
+    uint32_t buckets[kList + 1];   // tokens, then those before
     uint64_t parts[kDrawThreads / 64];
     uint64_t passed, own;
     uint32_t token;
 };
 
 __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, float most, const DrawRoom& room, Sorting& t) {
-    const uint32_t n = min(room.plan.listed, kList);
-    uint32_t size = 64;
-    while (size < n) size *= 2;
-    for (uint32_t i = threadIdx.x; i < size; i += kDrawThreads) t.list[i] = i < n ? room.list[i] : 0;
-    // bitonic, falling; the places past the list, zeros, come last
-    for (uint32_t k = 2; k <= size; k *= 2)
-        for (uint32_t j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < size / 2; i += kDrawThreads) {
-                const uint32_t x = 2 * i - (i & (j - 1)), y = x + j;
-                const uint64_t u = t.list[x], v = t.list[y];
-                if ((u < v) == ((x & k) == 0)) t.list[x] = v, t.list[y] = u;
-            }
-        }
+    constexpr uint32_t kMine = kList / kDrawThreads;
+    const float steps = steps_of(s);
+    Run run[kRuns];
+    uint64_t run_before[kRuns];
+    const uint32_t runs = room.runs;
+    uint32_t n = 0, bins = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < kRuns; ++q) {
+        run[q] = q < runs ? room.run[q] : Run{kBins, kBins, 0, 0, kList, 0};
+        run_before[q] = get(room.sums[2 + q]);
+        if (q < runs) n += run[q].count, bins += run[q].last - run[q].first + 1;
+    }
+    // Buckets: each bin in as many equal parts, which rise as the logits fall.
+    const uint32_t each = max(kList / bins, 1u);
+    uint64_t token[kMine];
+    uint32_t bucket[kMine], slot[kMine];
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) {
+        const uint32_t i = kDrawThreads * e + threadIdx.x;
+        token[e] = i < n ? get(room.list[i]) : 0;
+        t.buckets[i] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) {
+        if (kDrawThreads * e + threadIdx.x >= n) continue;
+        const float place = place_of(logit_of(static_cast<uint32_t>(token[e] >> 32)), most, steps);
+        uint32_t q = 0, from = 0;
+#pragma unroll
+        for (uint32_t x = 1; x < kRuns; ++x)
+            if (x < runs && place >= static_cast<float>(run[x].first)) q = x;
+#pragma unroll
+        for (uint32_t x = 0; x + 1 < kRuns; ++x)
+            if (x < q) from += run[x].last - run[x].first + 1;
+        Run r = run[0];
+#pragma unroll
+        for (uint32_t x = 1; x < kRuns; ++x)
+            if (q == x) r = run[x];
+        const uint32_t part = static_cast<uint32_t>((place - static_cast<float>(r.first)) * static_cast<float>(each));
+        bucket[e] = min(from * each + min(part, (r.last - r.first + 1) * each - 1), kList - 1);
+        slot[e] = atomicAdd(&t.buckets[bucket[e]], 1u);
+    }
+    __syncthreads();
+    uint64_t sum = 0, all;
+    uint32_t size[kMine];
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) size[e] = t.buckets[kMine * threadIdx.x + e], sum += size[e];
+    sum = sum_before(sum, t.parts, &all);
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) t.buckets[kMine * threadIdx.x + e] = static_cast<uint32_t>(sum), sum += size[e];
+    if (threadIdx.x == 0) t.buckets[kList] = n;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e)
+        if (kDrawThreads * e + threadIdx.x < n) t.list[t.buckets[bucket[e]] + slot[e]] = token[e];
+    __syncthreads();
+    // within a bucket, mostly of one or two, by counting
+#pragma unroll
+    for (uint32_t e = 0; e < kMine; ++e) {
+        if (kDrawThreads * e + threadIdx.x >= n) continue;
+        const uint32_t first = t.buckets[bucket[e]], end = t.buckets[bucket[e] + 1];
+        uint32_t rank = 0;
+        for (uint32_t j = first; j < end; ++j) rank += t.list[j] > token[e];
+        t.sorted[first + rank] = token[e];
+    }
     __syncthreads();
     // a thread's tokens: their weights, and the row's weight and count before them
-    constexpr uint32_t kMine = kList / kDrawThreads;
-    uint64_t own[kMine], before[kMine], count[kMine], sum = 0, all;
+    uint64_t own[kMine], before[kMine];
+    uint32_t count[kMine];
+    sum = 0;
 #pragma unroll
     for (uint32_t e = 0; e < kMine; ++e) {
         const uint32_t i = kMine * threadIdx.x + e;
-        own[e] = i < n ? weight_of(logit_of(static_cast<uint32_t>(t.list[i] >> 32)), most, s.rate) : 0;
+        own[e] = i < n ? weight_of(logit_of(static_cast<uint32_t>(t.sorted[i] >> 32)), most, s.octaves) : 0;
         before[e] = sum, sum += own[e];
     }
     sum = sum_before(sum, t.parts, &all);
@@ -503,11 +612,13 @@ __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, flo
 #pragma unroll
     for (uint32_t e = 0; e < kMine; ++e) {
         const uint32_t i = kMine * threadIdx.x + e;
-        Run run = room.plan.run[0];
-        for (uint32_t q = 1; q < room.plan.runs; ++q)
-            if (room.plan.run[q].start <= i) run = room.plan.run[q];
-        count[e] = run.count + (i - run.start);
-        before[e] = run.weight + (before[e] - t.before[run.start]);
+        Run r = run[0];
+        uint64_t ahead = run_before[0];
+#pragma unroll
+        for (uint32_t q = 1; q < kRuns; ++q)
+            if (q < runs && run[q].start <= i) r = run[q], ahead = run_before[q];
+        count[e] = r.before + (i - r.start);
+        before[e] = ahead + (before[e] - t.before[r.start]);
     }
     // The weight up to the token at which the row's running count or weight passes `target`, its own in t.own.
     auto passed_at = [&](bool by_count, uint64_t target) {
@@ -516,15 +627,16 @@ __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, flo
         for (uint32_t e = 0; e < kMine; ++e) {
             const uint32_t i = kMine * threadIdx.x + e;
             if (i < n && (by_count ? count[e] == target : before[e] <= target && target < before[e] + own[e]))
-                t.passed = before[e] + own[e], t.own = own[e], t.token = ~static_cast<uint32_t>(t.list[i]);
+                t.passed = before[e] + own[e], t.own = own[e], t.token = ~static_cast<uint32_t>(t.sorted[i]);
         }
         __syncthreads();
         return t.passed;
     };
-    uint64_t kept = room.plan.kept;
-    if (room.plan.cut) kept = passed_at(true, s.top_k - 1);
+    uint64_t kept = get(room.sums[0]);
+    const uint64_t likely = get(room.sums[1]);
+    if (room.cut) kept = passed_at(true, s.top_k - 1);
     if (s.top_p < 1.0) kept = passed_at(false, passed_by(s, kept));
-    kept = min(kept, max(room.plan.likely, 1ull << 40));
+    kept = min(kept, likely);
     passed_at(false, drawn_at(s, kept));
     if (threadIdx.x == 0) write_draw(a, row, t.token, t.own, kept);
 }
@@ -533,7 +645,9 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
     __shared__ union {
         Descent descent;
         Sorting sorting;
+        uint64_t list[kList];
     } space;
+    __shared__ uint64_t sums[2 + kRuns];
     __shared__ uint32_t last, listed, base;
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
     const Settings s = settings_of(a, row);
@@ -549,32 +663,53 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
         return;
     }
     DrawRoom& room = c.rooms[row];
-    if (most == INFINITY || room.plan.alone) {
+    if (most == INFINITY || room.alone) {
         if (chunk == 0) draw_alone(a, row, s, most, space.descent);
         return;
     }
+    if (threadIdx.x < 2 + kRuns) sums[threadIdx.x] = 0;
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
     const float steps = steps_of(s);
-    uint32_t first[3], width[3];  // a run that is not there holds no bin
+    uint32_t first[kRuns], width[kRuns];  // a run that is not there holds no bin
 #pragma unroll
-    for (uint32_t q = 0; q < 3; ++q) {
-        const bool there = q < room.plan.runs;
-        first[q] = there ? room.plan.run[q].first : kBins, width[q] = there ? room.plan.run[q].last - first[q] : 0;
+    for (uint32_t q = 0; q < kRuns; ++q) {
+        const bool there = q < room.runs;
+        first[q] = there ? room.run[q].first : kBins, width[q] = there ? room.run[q].last - first[q] : 0;
     }
+    // all weights, those that min_p leaves, and those before a run
+    uint64_t mine[2 + kRuns] = {};
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) {
-        const uint32_t bin = bin_of(l, most, steps);
-        if (bin - first[0] > width[0] && bin - first[1] > width[1] && bin - first[2] > width[2]) return;
-        const uint32_t at = atomicAdd(&listed, 1u);
-        if (at < kList) space.sorting.list[at] = uint64_t{key_of(l)} << 32 | ~i;
+        const uint32_t bin = static_cast<uint32_t>(place_of(l, most, steps));
+        const uint64_t w = weight_of(l, most, s.octaves);
+        mine[0] += w;
+        if (w >= s.least) mine[1] += w;
+        bool in = false;
+#pragma unroll
+        for (uint32_t q = 0; q < kRuns; ++q) {
+            if (bin < first[q]) mine[2 + q] += w;
+            in |= bin - first[q] <= width[q];
+        }
+        if (in) {
+            const uint32_t at = atomicAdd(&listed, 1u);
+            if (at < kList) space.list[at] = uint64_t{key_of(l)} << 32 | ~i;
+        }
     });
+#pragma unroll
+    for (uint32_t q = 0; q < 2 + kRuns; ++q) {
+#pragma unroll
+        for (uint32_t o = 32; o > 0; o >>= 1) mine[q] += __shfl_xor(mine[q], o);
+        if ((threadIdx.x & 63u) == 0)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sums[q]), static_cast<unsigned long long>(mine[q]));
+    }
     __syncthreads();
-    const uint32_t mine = min(listed, kList);
-    if (threadIdx.x == 0 && mine > 0) base = atomicAdd(&room.plan.listed, mine);
+    const uint32_t here = min(listed, kList);
+    if (threadIdx.x < 2 + kRuns && sums[threadIdx.x] > 0) add(room.sums[threadIdx.x], sums[threadIdx.x]);
+    if (threadIdx.x == 0 && here > 0) base = add(room.listed, here);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < mine; i += kDrawThreads)
-        if (base + i < kList) room.list[base + i] = space.sorting.list[i];
-    if (last_of(&room.plan.gathered, c.chunks, &last)) answer_row(a, row, s, most, room, space.sorting);
+    for (uint32_t i = threadIdx.x; i < here; i += kDrawThreads)
+        if (base + i < kList) put(room.list[base + i], space.list[i]);
+    if (last_of(room.gathered, c.chunks, &last)) answer_row(a, row, s, most, room, space.sorting);
 }
 
 // About a thousand workgroups, a chunk of at least two fours a thread; of whole fours.
