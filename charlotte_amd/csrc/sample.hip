@@ -69,23 +69,22 @@ __device__ __forceinline__ Settings settings_of(const Sample& a, uint32_t row) {
     return s;
 }
 
-// A logit as a word that rises with it; a NaN as -inf, and one zero.
-__device__ __forceinline__ float clean(float l) { return l == l ? l + 0.0f : -INFINITY; }
+// A logit that is a NaN counts as -inf.
+__device__ __forceinline__ float clean(float l) { return fmaxf(l, -INFINITY); }
+// A logit as a word that rises with it; both zeros as one.
 __device__ __forceinline__ uint32_t key_of(float l) {
-    const uint32_t bits = __float_as_uint(l);
+    const uint32_t bits = __float_as_uint(l + 0.0f);
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// floor(2^40 exp((l - m) rate)), `octaves` = rate log2(e): 2^z by its series, z within
-// half of a whole number (the 12th term is below 2^-47), all of it within 2^-46.
-__device__ __forceinline__ uint64_t weight_of(float l, float most, double octaves) {
-    if (l == most) return 1ull << 40;
-    if (l == -INFINITY || most == INFINITY) return 0;
-    const double y = (static_cast<double>(l) - static_cast<double>(most)) * octaves;
-    if (y < -41.0) return 0;
+// floor(2^40 exp((l - m) rate)), `octaves` = rate log2(e), of a finite m: 2^z by its
+// series, z within half of a whole number (the 12th term is below 2^-47), all of it
+// within 2^-46. A whole number that f64 holds.
+__device__ __forceinline__ double whole_weight(float l, double most, double octaves) {
+    const double y = fmax((static_cast<double>(l) - most) * octaves, -64.0);
     const double whole = rint(y), z = (y - whole) * 0.693147180559945309417;
     double p = 1.0 / 39916800;
     p = __builtin_fma(p, z, 1.0 / 3628800);
@@ -99,10 +98,13 @@ __device__ __forceinline__ uint64_t weight_of(float l, float most, double octave
     p = __builtin_fma(p, z, 0.5);
     p = __builtin_fma(p, z, 1.0);
     p = __builtin_fma(p, z, 1.0);
-    // at most 2^40, in two parts that 32 bits hold
-    const double w = ldexp(p, static_cast<int>(whole) + 40);
-    const uint32_t high = static_cast<uint32_t>(w * 0x1p-20), low = static_cast<uint32_t>(__builtin_fma(high, -0x1p20, w));
-    return (uint64_t{high} << 20) + low;
+    return floor(ldexp(p, static_cast<int>(whole) + 40));
+}
+
+__device__ __forceinline__ uint64_t weight_of(float l, float most, double octaves) {
+    if (l == most) return 1ull << 40;
+    if (l == -INFINITY || most == INFINITY) return 0;
+    return static_cast<uint64_t>(whole_weight(l, most, octaves));
 }
 
 // The sum over the workgroup's threads before this one, and of all. `parts`: a word a wave.
@@ -320,7 +322,8 @@ struct DrawChunks {
     uint32_t chunks, share;
 };
 
-// f(logit, index) for each token of a workgroup's chunk.
+// f(logit, index) for each token of a workgroup's chunk; in the fours at the row's
+// ends also for what is no token, at -inf.
 template <typename F>
 __device__ __forceinline__ void each_of_chunk(const Sample& a, const DrawChunks& c, uint32_t row, uint32_t chunk, F f) {
     const float* x = a.logits + row * a.logit_stride;
@@ -328,10 +331,7 @@ __device__ __forceinline__ void each_of_chunk(const Sample& a, const DrawChunks&
 #pragma unroll 2
     for (uint32_t at = chunk * c.share + 4 * threadIdx.x; at < end; at += 4 * kDrawThreads) {
         const float4 q = read4(x, lead, a.vocabulary, at, -INFINITY);
-        const float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-            if (at + e >= lead && at + e < lead + a.vocabulary) f(clean(v[e]), at + e - lead);
+        f(clean(q.x), at - lead), f(clean(q.y), at + 1 - lead), f(clean(q.z), at + 2 - lead), f(clean(q.w), at + 3 - lead);
     }
 }
 
@@ -520,8 +520,11 @@ __global__ __launch_bounds__(kDrawThreads) void row_bins(Sample a, DrawChunks c)
 
 // The row's list sorted, and its questions answered, by the last of its workgroups.
 struct Sorting {
-    uint64_t list[kList], sorted[kList];
-    uint64_t before[kList];        // the list's weight before a token
+    union {
+        uint64_t list[kList];
+        uint64_t before[kList];    // the list's weight before a token, once it is sorted
+    };
+    uint64_t sorted[kList];
     uint32_t buckets[kList + 1];   // tokens, then those before
     uint64_t parts[kDrawThreads / 64];
     uint64_t passed, own;
@@ -633,7 +636,7 @@ __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, flo
         return t.passed;
     };
     uint64_t kept = get(room.sums[0]);
-    const uint64_t likely = get(room.sums[1]);
+    const uint64_t likely = s.least > 0 ? get(room.sums[1]) : kept;
     if (room.cut) kept = passed_at(true, s.top_k - 1);
     if (s.top_p < 1.0) kept = passed_at(false, passed_by(s, kept));
     kept = min(kept, likely);
@@ -677,17 +680,21 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
         const bool there = q < room.runs;
         first[q] = there ? room.run[q].first : kBins, width[q] = there ? room.run[q].last - first[q] : 0;
     }
-    // all weights, those that min_p leaves, and those before a run
-    uint64_t mine[2 + kRuns] = {};
+    // all weights, those that min_p leaves, and those before a run: whole numbers, of a
+    // thread's few tokens below 2^53
+    double mine[2 + kRuns] = {};
+    const double least = static_cast<double>(s.least);
+    const uint32_t runs = room.runs;
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) {
         const uint32_t bin = static_cast<uint32_t>(place_of(l, most, steps));
-        const uint64_t w = weight_of(l, most, s.octaves);
+        const double w = whole_weight(l, most, s.octaves);
         mine[0] += w;
-        if (w >= s.least) mine[1] += w;
+        if (s.least > 0) mine[1] += w >= least ? w : 0.0;
         bool in = false;
 #pragma unroll
         for (uint32_t q = 0; q < kRuns; ++q) {
-            if (bin < first[q]) mine[2 + q] += w;
+            if (q > 0 && q >= runs) break;
+            mine[2 + q] += bin < first[q] ? w : 0.0;
             in |= bin - first[q] <= width[q];
         }
         if (in) {
@@ -697,10 +704,11 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
     });
 #pragma unroll
     for (uint32_t q = 0; q < 2 + kRuns; ++q) {
+        if (q == 1 ? s.least == 0 : q > 2 && q - 2 >= runs) continue;
+        uint64_t sum = static_cast<uint64_t>(mine[q]);
 #pragma unroll
-        for (uint32_t o = 32; o > 0; o >>= 1) mine[q] += __shfl_xor(mine[q], o);
-        if ((threadIdx.x & 63u) == 0)
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sums[q]), static_cast<unsigned long long>(mine[q]));
+        for (uint32_t o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if ((threadIdx.x & 63u) == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[q]), static_cast<unsigned long long>(sum));
     }
     __syncthreads();
     const uint32_t here = min(listed, kList);
@@ -714,8 +722,8 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
 
 // About a thousand workgroups, a chunk of at least two fours a thread; of whole fours.
 static uint32_t draw_chunks(uint32_t rows, uint32_t vocabulary) {
-    const uint32_t most = (vocabulary + 3 + 8 * kDrawThreads - 1) / (8 * kDrawThreads);
-    return std::max(1u, std::min((1024 + rows - 1) / rows, most));
+    const uint32_t most = (vocabulary + 3 + 4 * kDrawThreads - 1) / (4 * kDrawThreads);
+    return std::max(1u, std::min((512 + rows - 1) / rows, most));
 }
 
 uint64_t sample_bytes(uint32_t rows, uint32_t vocabulary) {
