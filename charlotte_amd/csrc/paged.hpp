@@ -4,16 +4,18 @@
 //
 // The requests' lengths are known to the device alone, and are anything: a
 // unit - 16 or 32 rows of a request and key head, over the tiles they see - may
-// be one tile or thousands. As many workgroups as the card holds lay all units
-// along a line, a key head after another, each by a running sum over the
-// requests, and take equal parts of it, so that each reads as many tiles as any
-// other; a unit that crosses parts is in pieces. Where all of it is less than
-// kLeastTiles a workgroup, units are cut in pieces of at most as many, which the
-// workgroups take in turn: a piece's fixed cost is then more than its tiles'.
+// be one tile or thousands. Each workgroup finds its work from all the lengths,
+// by sums over the requests, with no launch ahead of it. Where units are fewer than
+// workgroups, each is cut in pieces of equal length, a workgroup a piece. Where
+// that would leave some with much more than others, the units are laid along a line,
+// a key head after another, and each workgroup takes an equal part of it: a long
+// unit that crosses parts is in pieces, a short one is its first part's.
 //
 // A unit's pieces leave their outputs, and their rows' offsets and sums, in the
-// workspace; the workgroup that finds itself the last of them (a counter, left
-// at 0) joins them, in the pieces' order.
+// workspace, past the caches that the workgroups do not share (loads and stores of
+// the device's scope); each waits for its own to arrive, then counts itself, and
+// the one that finds itself the last (the counter is left at 0) joins them, in the
+// pieces' order. No cache is written back or cleared for it.
 #pragma once
 
 #include "attention.hpp"
@@ -21,15 +23,43 @@
 
 namespace chm {
 
-// What a unit costs beside its tiles, in tiles.
-constexpr uint32_t kUnitTiles = 4;
-// Tiles a workgroup below which units are cut by length alone.
-constexpr uint32_t kLeastTiles = 12;
+// What a unit costs beside its tiles, in tiles, and up to what length it is whole
+// on the line.
+constexpr uint32_t kUnitTiles = 8, kWholeTiles = 16;
+// Tiles more than on the line that a workgroup may have for units cut in pieces:
+// about what a unit's ends cost that the line leaves in two workgroups.
+constexpr uint32_t kPieceTiles = 24;
 
 // What is the same in every lane, as the compiler then knows.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uniform(uint64_t x) {
     return uint64_t{uniform(static_cast<uint32_t>(x >> 32))} << 32 | uniform(static_cast<uint32_t>(x));
+}
+// A quotient; lines are rarely past 32 bits.
+__device__ __forceinline__ uint64_t over(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? x / y : static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+}
+
+// Four floats at the device's scope.
+__device__ __forceinline__ void put(float* to, const float4_t& x) {
+    auto* words = reinterpret_cast<uint64_t*>(to);
+    const auto pair = __builtin_bit_cast(uint64_t __attribute__((ext_vector_type(2))), x);
+    __hip_atomic_store(words, pair.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(words + 1, pair.y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float4_t get(const float* from) {
+    const auto* words = reinterpret_cast<const uint64_t*>(from);
+    uint64_t __attribute__((ext_vector_type(2))) pair;
+    pair.x = __hip_atomic_load(words, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    pair.y = __hip_atomic_load(words + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return __builtin_bit_cast(float4_t, pair);
+}
+// A row's offset and sum.
+__device__ __forceinline__ void put(float2* to, float2 x) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get(const float2* from) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 struct NoTree {
@@ -65,7 +95,7 @@ struct Parts {
     __device__ __forceinline__ uint64_t begin(uint64_t part) const { return part * each + min(part, more); }
     __device__ __forceinline__ uint32_t at(uint64_t place) const {
         const uint64_t wide = more * (each + 1);
-        return static_cast<uint32_t>(place < wide ? place / (each + 1) : more + (place - wide) / each);
+        return static_cast<uint32_t>(place < wide ? over(place, each + 1) : more + over(place - wide, each));
     }
 };
 
@@ -78,11 +108,11 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
                                                ? sizeof(uint8_t[W][D][kRecord])
                                                : sizeof(float4_t[W][kParts])];
     __shared__ float joined_offset[W][kRows], joined_sum[W][kRows];
-    // A thread's requests: the line's and the cut units' pieces before them, and the first of them.
+    // A thread's requests: the line before them, and the first of them.
     __shared__ uint64_t line_before[T];
-    __shared__ uint32_t cut_before[T], request_past[T], request_count[T], request_start[T];
-    __shared__ uint64_t wave_tiles[W], wave_line[W], wave_cut[W];
-    __shared__ uint32_t last_piece;
+    __shared__ uint32_t request_past[T], request_count[T], request_start[T];
+    __shared__ uint64_t wave_tiles[W], wave_line[W];
+    __shared__ uint32_t wave_units[W], wave_longest[W], last_piece;
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane % kRows;
     // neighbours on the line on one XCD, whose cache then has the tiles that a request's units share
@@ -96,53 +126,70 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         place_request<kRows>(a, r);
         return r;
     };
-    // Over the threads before this one, in the wave and then all of them.
-    auto scan = [&](uint64_t x, uint64_t* of_waves) {
-        uint64_t sum = x;
+    Request mine{};
+    if (first_request < last_request) mine = request_of(first_request);
+    request_past[threadIdx.x] = mine.past, request_count[threadIdx.x] = mine.count, request_start[threadIdx.x] = mine.start;
+    uint64_t tiles = uint64_t{mine.groups} * mine.tiles;
+    uint32_t units = mine.groups, longest = mine.groups ? mine.tiles : 0;
+    for (uint32_t i = first_request + 1; i < last_request; ++i) {
+        const Request r = request_of(i);
+        tiles += uint64_t{r.groups} * r.tiles;
+        units += r.groups;
+        if (r.groups) longest = max(longest, r.tiles);
+    }
+#pragma unroll
+    for (uint32_t o = 32; o > 0; o >>= 1) {
+        tiles += __shfl_xor(tiles, o), units += __shfl_xor(units, o);
+        longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, o)));
+    }
+    if (lane == 0) wave_tiles[wave] = tiles, wave_units[wave] = units, wave_longest[wave] = longest;
+    __syncthreads();
+    tiles = 0, units = 0, longest = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w)
+        tiles += wave_tiles[w], units += wave_units[w], longest = max(longest, wave_longest[w]);
+    const uint64_t all_tiles = uniform(tiles) * a.pool.kv_heads, all_units = uint64_t{uniform(units)} * a.pool.kv_heads;
+
+    // Pieces of at most `piece_tiles`, which are no more than the workgroups; or equal parts of the line.
+    const uint64_t even_tiles = over(all_tiles, gridDim.x);
+    uint64_t piece_tiles = 0;
+    if (all_units < gridDim.x) piece_tiles = max(over(all_tiles, gridDim.x - all_units) + 1, uint64_t{W});
+    const bool even = all_units >= gridDim.x || min(piece_tiles, uint64_t{uniform(longest)}) > even_tiles + kPieceTiles;
+    auto length_of = [&](const Request& r) {
+        return even ? r.tiles + kUnitTiles : (r.tiles + static_cast<uint32_t>(piece_tiles) - 1) / static_cast<uint32_t>(piece_tiles);
+    };
+    uint64_t line = mine.groups ? uint64_t{mine.groups} * length_of(mine) : 0;
+    for (uint32_t i = first_request + 1; i < last_request; ++i) {
+        const Request r = request_of(i);
+        line += uint64_t{r.groups} * length_of(r);
+    }
+    {
+        // what is before the thread, in its wave and then in all
+        uint64_t sum = line;
 #pragma unroll
         for (uint32_t o = 1; o < 64; o <<= 1) {
             const uint64_t other = __shfl_up(sum, o);
             if (lane >= o) sum += other;
         }
-        if (lane == 63) of_waves[wave] = sum;
-        return sum - x;
-    };
-    uint64_t tiles = 0;
-    for (uint32_t i = first_request; i < last_request; ++i) {
-        const Request r = request_of(i);
-        tiles += uint64_t{r.groups} * r.tiles;
-        if (i == first_request)
-            request_past[threadIdx.x] = r.past, request_count[threadIdx.x] = r.count, request_start[threadIdx.x] = r.start;
+        if (lane == 63) wave_line[wave] = sum;
+        line = sum - line;
     }
-    scan(tiles, wave_tiles);
     __syncthreads();
-    uint64_t all_tiles = 0;
-    for (uint32_t w = 0; w < W; ++w) all_tiles += wave_tiles[w];
-    // Equal parts of the line, or pieces in turn.
-    const bool even = uniform(all_tiles) * a.pool.kv_heads >= uint64_t{gridDim.x} * kLeastTiles;
-    auto pieces_of = [&](const Request& r) { return (r.tiles + kLeastTiles - 1) / kLeastTiles; };
-    auto length_of = [&](const Request& r) { return even ? r.tiles + kUnitTiles : pieces_of(r); };
-    uint64_t line = 0, cut = 0;
-    for (uint32_t i = first_request; i < last_request; ++i) {
-        const Request r = request_of(i);
-        line += uint64_t{r.groups} * length_of(r);
-        if (!even && pieces_of(r) > 1) cut += r.groups * pieces_of(r);
-    }
-    line = scan(line, wave_line), cut = scan(cut, wave_cut);
-    __syncthreads();
-    uint64_t head_line = 0, head_cut = 0;
+    uint64_t head_line = 0;
+#pragma unroll
     for (uint32_t w = 0; w < W; ++w) {
-        if (w < wave) line += wave_line[w], cut += wave_cut[w];
-        head_line += wave_line[w], head_cut += wave_cut[w];
+        if (w < wave) line += wave_line[w];
+        head_line += wave_line[w];
     }
-    line_before[threadIdx.x] = line, cut_before[threadIdx.x] = static_cast<uint32_t>(cut);
+    line_before[threadIdx.x] = line;
     __syncthreads();
-    head_line = uniform(head_line), head_cut = uniform(head_cut);
+    head_line = uniform(head_line);
 
     const uint64_t length = head_line * a.pool.kv_heads;
-    const Parts parts{length / gridDim.x, length % gridDim.x};
+    const uint64_t part_length = over(length, gridDim.x);
+    const Parts parts{part_length, length - part_length * gridDim.x};
     uint64_t place = even ? parts.begin(part) : part;
-    const uint64_t end = even ? parts.begin(uint64_t{part} + 1) : length;
+    const uint64_t end = even ? parts.begin(uint64_t{part} + 1) : min(length, uint64_t{part} + 1);
     const uint32_t scanned = min(T, (a.requests + share - 1) / share);
 
     Attention b{};
@@ -153,7 +200,7 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
     while (place < end) {
         // The unit: its request, the last whose part of the head's line does not begin past the place.
-        const uint32_t head = static_cast<uint32_t>(place / head_line);
+        const uint32_t head = static_cast<uint32_t>(over(place, head_line));
         const uint64_t on_head = place - head * head_line;
         uint32_t low = 0, high = scanned;
         while (high - low > 1) {
@@ -165,36 +212,41 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         }
         low = uniform(low);
         uint64_t before = uniform(line_before[low]);
-        uint32_t cut_at = uniform(cut_before[low]), at = low * share;
+        uint32_t at = low * share;
         Request r{uniform(request_past[low]), uniform(request_count[low]), uniform(request_start[low]), 0, 0, 0, false};
         place_request<kRows>(a, r);
         while (before + uint64_t{r.groups} * length_of(r) <= on_head) {
             before += uint64_t{r.groups} * length_of(r);
-            if (!even && pieces_of(r) > 1) cut_at += r.groups * pieces_of(r);
             ++at;
             r.past = uniform(a.past[at]), r.count = uniform(a.counts[at]), r.start = uniform(a.starts[at]);
             place_request<kRows>(a, r);
         }
         const uint32_t unit_length = length_of(r);
-        const uint32_t unit = static_cast<uint32_t>((on_head - before) / unit_length);
+        const uint32_t unit = static_cast<uint32_t>(over(on_head - before, unit_length));
         const uint64_t unit_begin = head * head_line + before + uint64_t{unit} * unit_length, unit_end = unit_begin + unit_length;
 
-        // The piece: its tiles of the unit's, its number among the unit's, where it is kept.
+        // The piece: its tiles of the unit's, its number among the unit's, where it is
+        // kept. (On the line a part keeps at most the end of one unit and the begin of
+        // another.)
         uint32_t tile_begin = 0, tile_end = r.tiles, pieces = 1, piece = 0, kept = 0, counter = 0;
-        if (even) {
+        if (!even) {
+            pieces = unit_length, piece = static_cast<uint32_t>(place - unit_begin);
+            kept = part, counter = part - piece;
+            tile_begin = static_cast<uint32_t>(over(uint64_t{r.tiles} * piece, pieces));
+            tile_end = static_cast<uint32_t>(over(uint64_t{r.tiles} * (piece + 1), pieces));
+            place = end;
+        } else if (unit_length <= kUnitTiles + kWholeTiles) {
+            const bool earlier = unit_begin < parts.begin(part);
+            place = unit_end;
+            if (earlier) continue;
+        } else {
             const uint32_t from = parts.at(unit_begin), to = parts.at(unit_end - 1);
             pieces = to - from + 1, piece = part - from;
             kept = 2 * part + (piece == 0), counter = 2 * from + 1;
-            const uint64_t mine = max(parts.begin(part), unit_begin), until = min(end, unit_end);
-            tile_begin = mine > unit_begin + kUnitTiles ? static_cast<uint32_t>(mine - unit_begin) - kUnitTiles : 0;
+            const uint64_t begin = max(parts.begin(part), unit_begin), until = min(end, unit_end);
+            tile_begin = begin > unit_begin + kUnitTiles ? static_cast<uint32_t>(begin - unit_begin) - kUnitTiles : 0;
             tile_end = until > unit_begin + kUnitTiles ? static_cast<uint32_t>(until - unit_begin) - kUnitTiles : 0;
             place = until;
-        } else {
-            pieces = unit_length, piece = static_cast<uint32_t>(place - unit_begin);
-            counter = head * static_cast<uint32_t>(head_cut) + cut_at + unit * pieces, kept = counter + piece;
-            tile_begin = static_cast<uint32_t>(uint64_t{r.tiles} * piece / pieces);
-            tile_end = static_cast<uint32_t>(uint64_t{r.tiles} * (piece + 1) / pieces);
-            place += gridDim.x;
         }
 
         Group group;
@@ -254,8 +306,8 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
         // The waves joined, as attend joins them.
         float4_t(*joined)[kParts] = reinterpret_cast<float4_t(*)[kParts]>(space);
-        const float mine = sum_of_row<X>(rows.sum);
-        if (lane < kRows) joined_offset[wave][n] = rows.offset, joined_sum[wave][n] = mine;
+        const float row_sum = sum_of_row<X>(rows.sum);
+        if (lane < kRows) joined_offset[wave][n] = rows.offset, joined_sum[wave][n] = row_sum;
 #pragma unroll
         for (uint32_t t = 0; t < kQuads; ++t) joined[wave][t * 64 + lane] = rows.quad(t);
         __syncthreads();
@@ -284,18 +336,14 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
             if (pieces == 1) {
                 *reinterpret_cast<float4_t*>(output_of(group.row0 + n, value)) = empty ? float4_t(0.0f) : out * (1.0f / total);
             } else {
-                *reinterpret_cast<float4_t*>(a.partial + (uint64_t{kept} * kRows + n) * (32 * NB) + value) = out;
-                if (i < kRows) a.stats[uint64_t{kept} * kRows + n] = make_float2(total != total ? total : least, total);
+                put(a.partial + (uint64_t{kept} * kRows + n) * (32 * NB) + value, out);
+                if (i < kRows) put(a.stats + uint64_t{kept} * kRows + n, make_float2(total != total ? total : least, total));
             }
         }
         wait_loads<0>();
-        __syncthreads();  // the LDS is read, and what was written has left the waves
+        __syncthreads();  // the LDS is read, and what was written has arrived
         if (pieces == 1) continue;
-        if (threadIdx.x == 0) {
-            __threadfence();
-            last_piece = atomicInc(a.counters + counter, pieces - 1) == pieces - 1;
-            __threadfence();
-        }
+        if (threadIdx.x == 0) last_piece = atomicInc(a.counters + counter, pieces - 1) == pieces - 1;
         __syncthreads();
         if (!last_piece) continue;
 
@@ -315,8 +363,8 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 #pragma unroll 4
                 for (uint32_t p = mine_of; p < pieces; p += shares) {
                     const uint64_t from = uint64_t{kept_of(p)} * kRows + row;
-                    const float2 st = a.stats[from];
-                    const float4_t theirs = *reinterpret_cast<const float4_t*>(a.partial + from * (32 * NB) + value);
+                    const float2 st = get(a.stats + from);
+                    const float4_t theirs = get(a.partial + from * (32 * NB) + value);
                     const float lower = st.x < least || st.x != st.x ? st.x : least;
                     const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
                     const float factor = st.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - st.x);

@@ -12,7 +12,7 @@ struct charlotte_hip_matmul_page_pool {
     const charlotte_hip_matmul_context* ctx = nullptr;  // compared, never followed: it may be gone before the pool
     int device = 0;
     chm::CacheShape shape{};
-    uint32_t* counters = nullptr;  // two words a compute unit, 0 between launches
+    uint32_t* counters = nullptr;  // kPieces words a compute unit, 0 between launches
     bool owned = false;
 };
 
@@ -49,7 +49,7 @@ void check_pool(uint32_t type, uint32_t pages, uint32_t page_tokens, uint32_t kv
 hipError_t make_pool(charlotte_hip_matmul_context* ctx, uint32_t type, uint32_t pages, uint32_t page_tokens,
                      uint32_t kv_heads, uint32_t head_dim, void* device, charlotte_hip_matmul_page_pool** out) {
     const uint64_t bytes = chm::cache_bytes(type, pages, kv_heads, head_dim, page_tokens);
-    const uint64_t counted = uint64_t{ctx->compute_units} * 2 * sizeof(uint32_t);
+    const uint64_t counted = uint64_t{ctx->compute_units} * chm::kPieces * sizeof(uint32_t);
     if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
     const bool owned = device == nullptr;
     void* counters = nullptr;
@@ -110,7 +110,7 @@ void check_table(uint32_t requests, uint32_t table_stride, uint32_t page_tokens)
 
 // Bytes of a step's pieces of units of 16 * octets rows: outputs, then offsets and sums.
 uint64_t piece_bytes(const charlotte_hip_matmul_context* ctx, const chm::CacheShape& c, uint32_t octets) {
-    return uint64_t{ctx->compute_units} * 2 * 16 * octets * (uint64_t{c.head_dim} * 4 + 8);
+    return uint64_t{ctx->compute_units} * chm::kPieces * 16 * octets * (uint64_t{c.head_dim} * 4 + 8);
 }
 
 // An output that is an input's memory has its stride.
@@ -259,7 +259,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         need(d.workspace, "workspace", 16);
         if (d.workspace_bytes < bytes) refuse("needs a workspace of " + std::to_string(bytes) + " bytes");
         a.partial = static_cast<float*>(d.workspace);
-        a.stats = reinterpret_cast<float2*>(a.partial + uint64_t{ctx->compute_units} * 2 * 16 * octets * c.head_dim);
+        a.stats = reinterpret_cast<float2*>(a.partial + uint64_t{ctx->compute_units} * chm::kPieces * 16 * octets * c.head_dim);
         a.counters = d.pool->counters;
         a.parts = ctx->compute_units;
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;

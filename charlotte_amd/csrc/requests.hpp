@@ -51,6 +51,8 @@ struct PagedAttention {
     float scale;
 };
 
+// Pieces of units that a step may leave, a workgroup.
+constexpr uint32_t kPieces = 2;
 // Rows a workgroup: 16, or 32 where requests bring more.
 inline uint32_t paged_octets(uint32_t group, uint32_t most) { return uint64_t{group} * most > 16 ? 2 : 1; }
 hipError_t launch_paged_f16(const PagedAttention& a, uint32_t octets, hipStream_t stream);
