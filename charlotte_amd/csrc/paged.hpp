@@ -4,8 +4,8 @@
 //
 // The requests' lengths are known to the device alone, and are anything: a
 // unit - 16 or 32 rows of a request and key head, over the tiles they see - may
-// be one tile or thousands. Each workgroup finds its work from all the lengths,
-// by sums over the requests, with no launch ahead of it. Where units are fewer than
+// be one tile or thousands. Each wave finds its workgroup's work from all the
+// lengths, by sums over the requests, some a lane, with no launch ahead of it. Where units are fewer than
 // workgroups, each is cut in pieces of equal length, a workgroup a piece. Where
 // that would leave some with much more than others, the units are laid along a line,
 // a key head after another, and each workgroup takes an equal part of it: a long
@@ -34,6 +34,11 @@ constexpr uint32_t kPieceTiles = 24;
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uniform(uint64_t x) {
     return uint64_t{uniform(static_cast<uint32_t>(x >> 32))} << 32 | uniform(static_cast<uint32_t>(x));
+}
+// A lane's.
+__device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, uint32_t lane) {
+    return uint64_t{of_lane(static_cast<uint32_t>(x >> 32), lane)} << 32 | of_lane(static_cast<uint32_t>(x), lane);
 }
 // A quotient; lines are rarely past 32 bits.
 __device__ __forceinline__ uint64_t over(uint64_t x, uint64_t y) {
@@ -108,16 +113,12 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
                                                ? sizeof(uint8_t[W][D][kRecord])
                                                : sizeof(float4_t[W][kParts])];
     __shared__ float joined_offset[W][kRows], joined_sum[W][kRows];
-    // A thread's requests: the line before them, and the first of them.
-    __shared__ uint64_t line_before[T];
-    __shared__ uint32_t request_past[T], request_count[T], request_start[T];
-    __shared__ uint64_t wave_tiles[W], wave_line[W];
-    __shared__ uint32_t wave_units[W], wave_longest[W], last_piece;
+    __shared__ uint32_t last_piece;
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane % kRows;
     // neighbours on the line on one XCD, whose cache then has the tiles that a request's units share
     const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-    const uint32_t share = (a.requests + T - 1) / T, first_request = threadIdx.x * share;
+    const uint32_t share = (a.requests + 63) / 64, first_request = lane * share;
     const uint32_t last_request = min(first_request + share, a.requests);
     const uint32_t tiles_a_page = a.pool.capacity / kTile;
 
@@ -128,7 +129,6 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
     };
     Request mine{};
     if (first_request < last_request) mine = request_of(first_request);
-    request_past[threadIdx.x] = mine.past, request_count[threadIdx.x] = mine.count, request_start[threadIdx.x] = mine.start;
     uint64_t tiles = uint64_t{mine.groups} * mine.tiles;
     uint32_t units = mine.groups, longest = mine.groups ? mine.tiles : 0;
     for (uint32_t i = first_request + 1; i < last_request; ++i) {
@@ -142,12 +142,6 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         tiles += __shfl_xor(tiles, o), units += __shfl_xor(units, o);
         longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, o)));
     }
-    if (lane == 0) wave_tiles[wave] = tiles, wave_units[wave] = units, wave_longest[wave] = longest;
-    __syncthreads();
-    tiles = 0, units = 0, longest = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < W; ++w)
-        tiles += wave_tiles[w], units += wave_units[w], longest = max(longest, wave_longest[w]);
     const uint64_t all_tiles = uniform(tiles) * a.pool.kv_heads, all_units = uint64_t{uniform(units)} * a.pool.kv_heads;
 
     // Pieces of at most `piece_tiles`, which are no more than the workgroups; or equal parts of the line.
@@ -163,34 +157,21 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         const Request r = request_of(i);
         line += uint64_t{r.groups} * length_of(r);
     }
-    {
-        // what is before the thread, in its wave and then in all
-        uint64_t sum = line;
+    // what is before the lane
+    uint64_t line_before = line;
 #pragma unroll
-        for (uint32_t o = 1; o < 64; o <<= 1) {
-            const uint64_t other = __shfl_up(sum, o);
-            if (lane >= o) sum += other;
-        }
-        if (lane == 63) wave_line[wave] = sum;
-        line = sum - line;
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint64_t other = __shfl_up(line_before, o);
+        if (lane >= o) line_before += other;
     }
-    __syncthreads();
-    uint64_t head_line = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < W; ++w) {
-        if (w < wave) line += wave_line[w];
-        head_line += wave_line[w];
-    }
-    line_before[threadIdx.x] = line;
-    __syncthreads();
-    head_line = uniform(head_line);
+    const uint64_t head_line = of_lane(line_before, 63u);
+    line_before -= line;
 
     const uint64_t length = head_line * a.pool.kv_heads;
     const uint64_t part_length = over(length, gridDim.x);
     const Parts parts{part_length, length - part_length * gridDim.x};
     uint64_t place = even ? parts.begin(part) : part;
     const uint64_t end = even ? parts.begin(uint64_t{part} + 1) : min(length, uint64_t{part} + 1);
-    const uint32_t scanned = min(T, (a.requests + share - 1) / share);
 
     Attention b{};
     b.queries = a.queries, b.output = a.output;
@@ -199,21 +180,13 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
     const NoTree tree{};
 
     while (place < end) {
-        // The unit: its request, the last whose part of the head's line does not begin past the place.
+        // The unit: its request, of those of the last lane whose line does not begin past the place.
         const uint32_t head = static_cast<uint32_t>(over(place, head_line));
         const uint64_t on_head = place - head * head_line;
-        uint32_t low = 0, high = scanned;
-        while (high - low > 1) {
-            const uint32_t middle = (low + high) / 2;
-            if (line_before[middle] <= on_head)
-                low = middle;
-            else
-                high = middle;
-        }
-        low = uniform(low);
-        uint64_t before = uniform(line_before[low]);
+        const uint32_t low = 63u - __builtin_clzll(__ballot(first_request < a.requests && line_before <= on_head));
+        uint64_t before = of_lane(line_before, low);
         uint32_t at = low * share;
-        Request r{uniform(request_past[low]), uniform(request_count[low]), uniform(request_start[low]), 0, 0, 0, false};
+        Request r{of_lane(mine.past, low), of_lane(mine.count, low), of_lane(mine.start, low), 0, 0, 0, false};
         place_request<kRows>(a, r);
         while (before + uint64_t{r.groups} * length_of(r) <= on_head) {
             before += uint64_t{r.groups} * length_of(r);
