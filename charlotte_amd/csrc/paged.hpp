@@ -30,20 +30,18 @@ constexpr uint32_t kUnitTiles = 8, kWholeTiles = 16;
 // about what a unit's ends cost that the line leaves in two workgroups.
 constexpr uint32_t kPieceTiles = 24;
 
-// What is the same in every lane, as the compiler then knows.
+// What is the same in every lane, as the compiler then knows; a lane's.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {
-    return uint64_t{uniform(static_cast<uint32_t>(x >> 32))} << 32 | uniform(static_cast<uint32_t>(x));
-}
-// A lane's.
 __device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
-__device__ __forceinline__ uint64_t of_lane(uint64_t x, uint32_t lane) {
-    return uint64_t{of_lane(static_cast<uint32_t>(x >> 32), lane)} << 32 | of_lane(static_cast<uint32_t>(x), lane);
+
+// What does not fit in 32 bits stays at kTooMuch: of a step's own lengths none does
+// (the host refuses one that may not), of starts and counts that are none's it may.
+constexpr uint32_t kTooMuch = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t times(uint32_t x, uint32_t y) {
+    const uint64_t product = uint64_t{x} * y;
+    return product >> 32 ? kTooMuch : static_cast<uint32_t>(product);
 }
-// A quotient; lines are rarely past 32 bits.
-__device__ __forceinline__ uint64_t over(uint64_t x, uint64_t y) {
-    return (x | y) >> 32 ? x / y : static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
-}
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return x + y < x ? kTooMuch : x + y; }
 
 // Four floats at the device's scope.
 __device__ __forceinline__ void put(float* to, const float4_t& x) {
@@ -65,6 +63,16 @@ __device__ __forceinline__ void put(float2* to, float2 x) {
 }
 __device__ __forceinline__ float2 get(const float2* from) {
     return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Another piece's offset and sum, and its outputs, to those so far.
+__device__ __forceinline__ void join(float2 side, const float4_t& theirs, float& least, float& total, float4_t& out) {
+    const float lower = side.x < least || side.x != side.x ? side.x : least;
+    const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
+    const float factor = side.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - side.x);
+    total = total * down + side.y * factor;
+    out = out * down + theirs * factor;
+    least = lower;
 }
 
 struct NoTree {
@@ -94,13 +102,13 @@ __device__ __forceinline__ void place_request(const PagedAttention& a, Request& 
     r.tiles = (static_cast<uint32_t>(end) + kTile - 1) / kTile - r.begin;
 }
 
-// Line [0, length) in `parts` parts, the first ones a place longer.
+// A line in equal parts, the first ones a place longer.
 struct Parts {
-    uint64_t each, more;
-    __device__ __forceinline__ uint64_t begin(uint64_t part) const { return part * each + min(part, more); }
-    __device__ __forceinline__ uint32_t at(uint64_t place) const {
-        const uint64_t wide = more * (each + 1);
-        return static_cast<uint32_t>(place < wide ? over(place, each + 1) : more + over(place - wide, each));
+    uint32_t each, more;
+    __device__ __forceinline__ uint32_t begin(uint32_t part) const { return part * each + min(part, more); }
+    __device__ __forceinline__ uint32_t at(uint32_t place) const {
+        const uint32_t wide = more * (each + 1);
+        return place < wide ? place / (each + 1) : more + (place - wide) / each;
     }
 };
 
@@ -121,6 +129,8 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
     const uint32_t share = (a.requests + 63) / 64, first_request = lane * share;
     const uint32_t last_request = min(first_request + share, a.requests);
     const uint32_t tiles_a_page = a.pool.capacity / kTile;
+    // a tile's page, exact: tiles are below 2^26, pages of at most 64
+    auto page_at = [&](uint32_t tile) { return tiles_a_page == 1 ? tile : __umulhi(tile, a.page_inverse); };
 
     auto request_of = [&](uint32_t i) {
         Request r{a.past[i], a.counts[i], a.starts[i], 0, 0, 0, false};
@@ -129,49 +139,49 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
     };
     Request mine{};
     if (first_request < last_request) mine = request_of(first_request);
-    uint64_t tiles = uint64_t{mine.groups} * mine.tiles;
+    uint32_t tiles = times(mine.groups, mine.tiles);
     uint32_t units = mine.groups, longest = mine.groups ? mine.tiles : 0;
     for (uint32_t i = first_request + 1; i < last_request; ++i) {
         const Request r = request_of(i);
-        tiles += uint64_t{r.groups} * r.tiles;
-        units += r.groups;
+        tiles = plus(tiles, times(r.groups, r.tiles)), units = plus(units, r.groups);
         if (r.groups) longest = max(longest, r.tiles);
     }
 #pragma unroll
     for (uint32_t o = 32; o > 0; o >>= 1) {
-        tiles += __shfl_xor(tiles, o), units += __shfl_xor(units, o);
+        tiles = plus(tiles, __shfl_xor(tiles, o)), units = plus(units, __shfl_xor(units, o));
         longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, o)));
     }
-    const uint64_t all_tiles = uniform(tiles) * a.pool.kv_heads, all_units = uint64_t{uniform(units)} * a.pool.kv_heads;
+    const uint32_t all_tiles = times(uniform(tiles), a.pool.kv_heads), all_units = times(uniform(units), a.pool.kv_heads);
+    if (all_tiles == kTooMuch || all_units == kTooMuch) return;
 
     // Pieces of at most `piece_tiles`, which are no more than the workgroups; or equal parts of the line.
-    const uint64_t even_tiles = over(all_tiles, gridDim.x);
-    uint64_t piece_tiles = 0;
-    if (all_units < gridDim.x) piece_tiles = max(over(all_tiles, gridDim.x - all_units) + 1, uint64_t{W});
-    const bool even = all_units >= gridDim.x || min(piece_tiles, uint64_t{uniform(longest)}) > even_tiles + kPieceTiles;
+    const uint32_t even_tiles = all_tiles / gridDim.x;
+    uint32_t piece_tiles = 0;
+    if (all_units < gridDim.x) piece_tiles = max(all_tiles / (gridDim.x - all_units) + 1, W);
+    const bool even = all_units >= gridDim.x || min(piece_tiles, uniform(longest)) > even_tiles + kPieceTiles;
     auto length_of = [&](const Request& r) {
-        return even ? r.tiles + kUnitTiles : (r.tiles + static_cast<uint32_t>(piece_tiles) - 1) / static_cast<uint32_t>(piece_tiles);
+        return even ? r.tiles + kUnitTiles : (r.tiles + piece_tiles - 1) / piece_tiles;
     };
-    uint64_t line = mine.groups ? uint64_t{mine.groups} * length_of(mine) : 0;
+    uint32_t line = mine.groups ? times(mine.groups, length_of(mine)) : 0;
     for (uint32_t i = first_request + 1; i < last_request; ++i) {
         const Request r = request_of(i);
-        line += uint64_t{r.groups} * length_of(r);
+        line = plus(line, times(r.groups, length_of(r)));
     }
     // what is before the lane
-    uint64_t line_before = line;
+    uint32_t line_before = line;
 #pragma unroll
     for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint64_t other = __shfl_up(line_before, o);
-        if (lane >= o) line_before += other;
+        const uint32_t other = __shfl_up(line_before, o);
+        if (lane >= o) line_before = plus(line_before, other);
     }
-    const uint64_t head_line = of_lane(line_before, 63u);
+    const uint32_t head_line = of_lane(line_before, 63u);
     line_before -= line;
 
-    const uint64_t length = head_line * a.pool.kv_heads;
-    const uint64_t part_length = over(length, gridDim.x);
-    const Parts parts{part_length, length - part_length * gridDim.x};
-    uint64_t place = even ? parts.begin(part) : part;
-    const uint64_t end = even ? parts.begin(uint64_t{part} + 1) : min(length, uint64_t{part} + 1);
+    const uint32_t length = times(head_line, a.pool.kv_heads);
+    if (length == kTooMuch) return;
+    const Parts parts{length / gridDim.x, length % gridDim.x};
+    uint32_t place = even ? parts.begin(part) : part;
+    const uint32_t end = even ? parts.begin(part + 1) : min(length, part + 1);
 
     Attention b{};
     b.queries = a.queries, b.output = a.output;
@@ -181,32 +191,33 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
     while (place < end) {
         // The unit: its request, of those of the last lane whose line does not begin past the place.
-        const uint32_t head = static_cast<uint32_t>(over(place, head_line));
-        const uint64_t on_head = place - head * head_line;
+        const uint32_t head = place / head_line;
+        const uint32_t on_head = place - head * head_line;
         const uint32_t low = 63u - __builtin_clzll(__ballot(first_request < a.requests && line_before <= on_head));
-        uint64_t before = of_lane(line_before, low);
+        uint32_t before = of_lane(line_before, low);
         uint32_t at = low * share;
         Request r{of_lane(mine.past, low), of_lane(mine.count, low), of_lane(mine.start, low), 0, 0, 0, false};
         place_request<kRows>(a, r);
-        while (before + uint64_t{r.groups} * length_of(r) <= on_head) {
-            before += uint64_t{r.groups} * length_of(r);
+        while (before + r.groups * length_of(r) <= on_head) {
+            before += r.groups * length_of(r);
             ++at;
             r.past = uniform(a.past[at]), r.count = uniform(a.counts[at]), r.start = uniform(a.starts[at]);
             place_request<kRows>(a, r);
         }
         const uint32_t unit_length = length_of(r);
-        const uint32_t unit = static_cast<uint32_t>(over(on_head - before, unit_length));
-        const uint64_t unit_begin = head * head_line + before + uint64_t{unit} * unit_length, unit_end = unit_begin + unit_length;
+        const uint32_t unit = (on_head - before) / unit_length;
+        const uint32_t unit_begin = head * head_line + before + unit * unit_length, unit_end = unit_begin + unit_length;
 
         // The piece: its tiles of the unit's, its number among the unit's, where it is
         // kept. (On the line a part keeps at most the end of one unit and the begin of
         // another.)
         uint32_t tile_begin = 0, tile_end = r.tiles, pieces = 1, piece = 0, kept = 0, counter = 0;
         if (!even) {
-            pieces = unit_length, piece = static_cast<uint32_t>(place - unit_begin);
+            pieces = unit_length, piece = place - unit_begin;
             kept = part, counter = part - piece;
-            tile_begin = static_cast<uint32_t>(over(uint64_t{r.tiles} * piece, pieces));
-            tile_end = static_cast<uint32_t>(over(uint64_t{r.tiles} * (piece + 1), pieces));
+            // equal but for one tile: the first ones have it
+            const uint32_t each = r.tiles / pieces, more = r.tiles % pieces;
+            tile_begin = piece * each + min(piece, more), tile_end = tile_begin + each + (piece < more);
             place = end;
         } else if (unit_length <= kUnitTiles + kWholeTiles) {
             const bool earlier = unit_begin < parts.begin(part);
@@ -216,9 +227,9 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
             const uint32_t from = parts.at(unit_begin), to = parts.at(unit_end - 1);
             pieces = to - from + 1, piece = part - from;
             kept = 2 * part + (piece == 0), counter = 2 * from + 1;
-            const uint64_t begin = max(parts.begin(part), unit_begin), until = min(end, unit_end);
-            tile_begin = begin > unit_begin + kUnitTiles ? static_cast<uint32_t>(begin - unit_begin) - kUnitTiles : 0;
-            tile_end = until > unit_begin + kUnitTiles ? static_cast<uint32_t>(until - unit_begin) - kUnitTiles : 0;
+            const uint32_t begin = max(parts.begin(part), unit_begin), until = min(end, unit_end);
+            tile_begin = max(begin - unit_begin, kUnitTiles) - kUnitTiles;
+            tile_end = max(until - unit_begin, kUnitTiles) - kUnitTiles;
             place = until;
         }
 
@@ -240,12 +251,13 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         const uint32_t count = first < group.tile_end ? (group.tile_end - first + W - 1) / W : 0;  // the wave's tiles
         uint8_t* ring = space + wave * (D * kRecord);
         uint32_t gone = 0;  // a bit a place of the ring: its page is none of the pool's
-        auto page_of = [&](uint32_t j) { return entries[__builtin_amdgcn_readfirstlane((first + j * W) / tiles_a_page)]; };
+        auto page_of = [&](uint32_t j) { return entries[page_at(first + j * W)]; };
         auto copy = [&](uint32_t j, uint32_t page) {
             const uint32_t tile = first + j * W, bit = 1u << (j % D);
             const bool there = page < a.pool.sequences;
             gone = there ? gone & ~bit : gone | bit;
-            const uint64_t record = (uint64_t{there ? page : 0u} * a.pool.kv_heads + head) * tiles_a_page + tile % tiles_a_page;
+            const uint64_t record = (uint64_t{there ? page : 0u} * a.pool.kv_heads + head) * tiles_a_page +
+                                    (tile - page_at(tile) * tiles_a_page);
             copy_record<kRecord>(a.pool.base + record * kRecord, ring + j % D * kRecord);
         };
 #pragma unroll
@@ -332,32 +344,27 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
             const uint32_t row = i / quads, value = i % quads * 4;
             float least = INFINITY, total = 0.0f;
             float4_t out = float4_t(0.0f);
-            if (live)
-#pragma unroll 4
-                for (uint32_t p = mine_of; p < pieces; p += shares) {
+            constexpr uint32_t kBatch = 8;  // on their way together
+            for (uint32_t p0 = mine_of; live && p0 < pieces; p0 += kBatch * shares) {
+                float2 side[kBatch];
+                float4_t theirs[kBatch];
+#pragma unroll
+                for (uint32_t x = 0; x < kBatch; ++x) {
+                    const uint32_t p = p0 + x * shares;
+                    side[x] = make_float2(INFINITY, 0.0f), theirs[x] = float4_t(0.0f);
+                    if (p >= pieces) continue;
                     const uint64_t from = uint64_t{kept_of(p)} * kRows + row;
-                    const float2 st = get(a.stats + from);
-                    const float4_t theirs = get(a.partial + from * (32 * NB) + value);
-                    const float lower = st.x < least || st.x != st.x ? st.x : least;
-                    const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
-                    const float factor = st.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - st.x);
-                    total = total * down + st.y * factor;
-                    out = out * down + theirs * factor;
-                    least = lower;
+                    side[x] = get(a.stats + from), theirs[x] = get(a.partial + from * (32 * NB) + value);
                 }
+#pragma unroll
+                for (uint32_t x = 0; x < kBatch; ++x) join(side[x], theirs[x], least, total, out);
+            }
             if (shares > 1) {
                 sums[threadIdx.x] = out, sides[threadIdx.x] = make_float2(least, total);
                 __syncthreads();
                 if (live && mine_of == 0)
-                    for (uint32_t x = 1; x < shares; ++x) {
-                        const float2 st = sides[threadIdx.x + x * work];
-                        const float lower = st.x < least || st.x != st.x ? st.x : least;
-                        const float down = least == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - least);
-                        const float factor = st.x == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lower - st.x);
-                        total = total * down + st.y * factor;
-                        out = out * down + sums[threadIdx.x + x * work] * factor;
-                        least = lower;
-                    }
+                    for (uint32_t x = 1; x < shares; ++x)
+                        join(sides[threadIdx.x + x * work], sums[threadIdx.x + x * work], least, total, out);
             }
             if (live && mine_of == 0)
                 *reinterpret_cast<float4_t*>(output_of(group.row0 + row, value)) =

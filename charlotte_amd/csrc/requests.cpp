@@ -237,7 +237,11 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         if (d.query_heads == 0 || d.query_heads % c.kv_heads != 0)
             refuse("query heads " + std::to_string(d.query_heads) + " over " + std::to_string(c.kv_heads) + " key heads");
         const uint32_t group = d.query_heads / c.kv_heads;
-        if (uint64_t{d.rows} * group >= (1ull << 28)) refuse("too many rows a step");
+        const uint32_t octets = chm::paged_octets(group, d.most);
+        // all units, each of all the tiles that a table's row holds
+        const uint64_t units = (uint64_t{d.rows} * group / (16 * octets) + d.requests) * c.kv_heads;
+        if (uint64_t{d.rows} * group >= (1ull << 28) || units * (uint64_t{d.table_stride} * (c.capacity / 32) + 16) >= (1ull << 32))
+            refuse("too many rows a step for tables so long");
         if (!std::isfinite(d.scale)) refuse("scale not finite");
         need(d.queries, "queries", 16);
         need(d.output, "output", 16);
@@ -254,7 +258,6 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         a.past = d.past, a.counts = d.counts, a.starts = d.starts, a.table = d.table;
         a.requests = d.requests, a.rows = d.rows, a.table_stride = d.table_stride;
         a.group = group, a.window = d.window, a.scale = d.scale;
-        const uint32_t octets = chm::paged_octets(group, d.most);
         const uint64_t bytes = piece_bytes(ctx, c, octets);
         need(d.workspace, "workspace", 16);
         if (d.workspace_bytes < bytes) refuse("needs a workspace of " + std::to_string(bytes) + " bytes");
@@ -262,6 +265,8 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         a.stats = reinterpret_cast<float2*>(a.partial + uint64_t{ctx->compute_units} * chm::kPieces * 16 * octets * c.head_dim);
         a.counters = d.pool->counters;
         a.parts = ctx->compute_units;
+        const uint32_t page_tiles = c.capacity / 32;
+        a.page_inverse = page_tiles > 1 ? static_cast<uint32_t>(((1ull << 32) + page_tiles - 1) / page_tiles) : 0;
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
         const auto s = static_cast<hipStream_t>(stream);
         return c.format == chm::kF16    ? chm::launch_paged_f16(a, octets, s)

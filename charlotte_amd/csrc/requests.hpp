@@ -48,6 +48,7 @@ struct PagedAttention {
     float2* stats;       // its rows' offsets and sums, [piece][row]
     uint32_t* counters;  // pieces of a unit that are done; 0 between launches
     uint32_t requests, rows, table_stride, group, window, parts;
+    uint32_t page_inverse;  // of a page's tiles, where they are two and more: 2^32 over them, rounded up
     float scale;
 };
 

@@ -766,7 +766,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_page_read(charlotte_hip_matmul_
  * left out. A token in a page that the pool does not have makes the outputs of the
  * rows that see it NaN, tokens past the table's row those of all of the request's.
  * The work is shared among the card's compute units by the tokens that are there,
- * whatever the requests' lengths. */
+ * whatever the requests' lengths. Refused is a step of so many rows over tables so
+ * long that (rows * query_heads / 16 + requests * kv_heads) * (table_stride *
+ * page_tokens / 32 + 16) may pass 2^32. */
 typedef struct {
     const charlotte_hip_matmul_page_pool* pool;
     const float* queries;     /* device, 16-byte aligned: row i's heads at queries + i * query_stride */

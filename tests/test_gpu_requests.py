@@ -405,6 +405,27 @@ def test_pages_that_the_pool_does_not_have(ctx, dev):
     pool.pool.free()
 
 
+def test_starts_and_counts_that_are_no_steps(ctx, dev):
+    """Requests whose counts together pass every bound: nothing past the output is written, and the call ends."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+
+    rows, requests = 4096, 65536
+    pool = _Pool(dev, "q4_0", 4, 2048, 1, 32).pool
+    need = sv.paged_attention_workspace_bytes(ctx, pool, 16)
+    work, _ = dev.room(need, np.uint8)
+    q = dev.put(np.ones((rows, 16 * 32), np.float32))
+    out, read = dev.room(rows * 16 * 32 + 4096)
+    full = {n: dev.put(np.full(requests, v, np.uint32)) for n, v in (("past", 3000), ("counts", rows), ("starts", 0), ("none", 0xFFFFFFFF))}
+    table = dev.put(np.zeros((requests, 60), np.uint32))
+    for past, counts, starts in (("past", "counts", "starts"), ("none", "none", "none"), ("past", "none", "starts")):
+        sv.paged_attention(ctx, sv.PagedAttention(pool, q, out, 16, 0.1, requests, rows, full[past], full[counts], full[starts],
+                                                  table, 60, workspace=work, workspace_bytes=need))
+        hx.sync()
+        assert (read()[rows * 16 * 32:].view(np.uint32) == NOWHERE).all()
+    pool.free()
+
+
 def test_pool_offsets_past_32_bits(ctx, dev):
     """A pool of more than 4 GiB, its last pages."""
     from charlotte_amd import harness as hx
