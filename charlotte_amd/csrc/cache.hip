@@ -342,6 +342,17 @@ struct Unit {
         first = const_cast<float*>(VALUES ? a.values : a.keys) + row * static_cast<int64_t>(stride) +
                 static_cast<uint64_t>(head) * a.cache.head_dim + 32 * block + (VALUES ? lane & 15u : 4 * (lane >> 4));
     }
+    // The whole tile of a pool whose tokens are the step's rows from `row0` on, from `slot` on.
+    __device__ __forceinline__ Unit(const CacheRows& a, uint32_t head_, uint32_t block_, uint32_t row0, uint32_t slot) {
+        lane = threadIdx.x & 63u;
+        head = head_, block = block_;
+        sequence = slot / a.cache.capacity, tile = slot % a.cache.capacity / kTile;
+        ahead = 0, limit = kTile, live = whole = true;
+        stride = VALUES ? a.value_stride : a.key_stride;
+        const uint64_t row = row0 + (VALUES ? 4 * (lane >> 4) : lane & 15u);
+        first = const_cast<float*>(VALUES ? a.values : a.keys) + row * stride + static_cast<uint64_t>(head) * a.cache.head_dim +
+                32 * block + (VALUES ? lane & 15u : 4 * (lane >> 4));
+    }
     // a token of the tile: past the lane's first one
     __device__ __forceinline__ static uint32_t token(uint32_t part, uint32_t e) { return VALUES ? 16 * (e >> 2) + (e & 3) : 16 * part; }
     __device__ __forceinline__ bool inside(uint32_t part, uint32_t e) const {
@@ -439,8 +450,7 @@ __device__ __forceinline__ void store_unit(uint8_t* unit, uint32_t lane, const u
 }
 
 template <uint32_t F, bool VALUES>
-__device__ __forceinline__ void append_unit(const CacheRows& a, uint32_t tiles) {
-    const Unit<VALUES> u(a, tiles);
+__device__ __forceinline__ void append_unit(const CacheRows& a, const Unit<VALUES>& u) {
     if (!u.live) return;
     float x[2][8];
 #pragma unroll
@@ -557,8 +567,7 @@ __device__ __forceinline__ void append_unit(const CacheRows& a, uint32_t tiles) 
 }
 
 template <uint32_t F, bool VALUES>
-__device__ __forceinline__ void read_unit(const CacheRows& a, uint32_t tiles) {
-    const Unit<VALUES> u(a, tiles);
+__device__ __forceinline__ void read_unit(const CacheRows& a, const Unit<VALUES>& u) {
     if (!u.live) return;
     const uint32_t blocks = a.cache.head_dim / 32;
     const uint8_t* record = record_of(a.cache, F, u.sequence, u.head, u.tile);
@@ -600,16 +609,101 @@ __device__ __forceinline__ void read_unit(const CacheRows& a, uint32_t tiles) {
 template <uint32_t F>
 __global__ __launch_bounds__(256) void append_units(CacheRows a, uint32_t tiles) {
     if (blockIdx.y == 0)
-        append_unit<F, false>(a, tiles);
+        append_unit<F, false>(a, Unit<false>(a, tiles));
     else
-        append_unit<F, true>(a, tiles);
+        append_unit<F, true>(a, Unit<true>(a, tiles));
 }
 template <uint32_t F>
 __global__ __launch_bounds__(256) void read_units(CacheRows a, uint32_t tiles) {
     if (blockIdx.y == 0)
-        read_unit<F, false>(a, tiles);
+        read_unit<F, false>(a, Unit<false>(a, tiles));
     else
-        read_unit<F, true>(a, tiles);
+        read_unit<F, true>(a, Unit<true>(a, tiles));
+}
+
+// Rows of a pool: a wave has 32 rows' block of a head. Where 32 rows from one of
+// them on have the slots of a whole tile in turn - a prompt's, from its first whole
+// tile on - they are a unit, and theirs alone (the slots between are not a tile's
+// first); the rows left, 8 lanes each, are 8 at a time.
+template <bool VALUES>
+struct Window {
+    uint32_t row0, head, block;
+    uint32_t from, slot;  // the row, of 32, at which a tile begins (32: none), and its slot
+    uint32_t left;        // rows of no tile, as bits
+
+    // Lanes' slots: the first of 32 lanes from which on 32 have a tile's.
+    __device__ __forceinline__ static uint32_t tile_of(uint32_t slot, bool there, uint32_t* first) {
+        const uint32_t lane = threadIdx.x & 63u;
+        uint64_t begins = __ballot(there && slot % kTile == 0) & 0xFFFFFFFFull;
+        while (begins) {
+            const uint32_t at = __builtin_ctzll(begins);
+            *first = __builtin_amdgcn_readlane(slot, at);
+            if ((__ballot(there && slot - *first == lane - at) >> at & 0xFFFFFFFFull) == 0xFFFFFFFFull) return at;
+            begins &= begins - 1;
+        }
+        return 32;
+    }
+    __device__ __forceinline__ explicit Window(const CacheRows& a) {
+        const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t id = blockIdx.x * 4 + wave, blocks = a.cache.head_dim / 32, units = blocks * a.cache.kv_heads;
+        row0 = id / units * 32, head = id % units / blocks, block = id % blocks;
+        auto slot_at = [&](uint32_t row, bool* there) {
+            const uint32_t s = row < a.tokens ? a.first[row] : 0u;
+            *there = row < a.tokens && s / a.cache.capacity < a.cache.sequences;
+            return s;
+        };
+        // this window's rows and the next one's; the one's before and this one's
+        bool there, there_before;
+        const uint32_t mine = slot_at(row0 + lane, &there), before = slot_at(row0 + lane - 32, &there_before);
+        from = tile_of(mine, there, &slot);
+        uint32_t unused;
+        const uint32_t into = tile_of(before, there_before, &unused);  // a tile of the window before has rows up to this one
+        left = static_cast<uint32_t>(__ballot(there));
+        if (into < 32) left &= ~((1u << into) - 1);
+        if (from < 32) left &= (1u << from) - 1;
+    }
+    // f(piece) with eight rows' pieces at a time
+    template <typename FN>
+    __device__ __forceinline__ void each_left(const CacheRows& a, FN f) const {
+#pragma unroll 1
+        for (uint32_t k = 0; k < 4; ++k) {
+            if ((left >> (8 * k) & 0xFFu) == 0) continue;
+            Piece p;
+            const uint32_t at = 8 * k + (threadIdx.x & 63u) / 8;
+            p.row = row0 + at, p.head = head, p.block = block, p.lane = threadIdx.x & 7u, p.values = VALUES;
+            p.live = left >> at & 1u;
+            const uint32_t s = p.live ? a.first[p.row] : 0u;
+            p.sequence = s / a.cache.capacity, p.slot = s % a.cache.capacity;
+            f(p);
+        }
+    }
+};
+
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void append_window(const CacheRows& a) {
+    const Window<VALUES> w(a);
+    if (w.from < 32) append_unit<F, VALUES>(a, Unit<VALUES>(a, w.head, w.block, w.row0 + w.from, w.slot));
+    w.each_left(a, [&](const Piece& p) { append_piece<F>(a, p); });
+}
+template <uint32_t F, bool VALUES>
+__device__ __forceinline__ void read_window(const CacheRows& a) {
+    const Window<VALUES> w(a);
+    if (w.from < 32) read_unit<F, VALUES>(a, Unit<VALUES>(a, w.head, w.block, w.row0 + w.from, w.slot));
+    w.each_left(a, [&](const Piece& p) { read_piece<F>(a, p); });
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void page_append_windows(CacheRows a) {
+    if (blockIdx.y == 0)
+        append_window<F, false>(a);
+    else
+        append_window<F, true>(a);
+}
+template <uint32_t F>
+__global__ __launch_bounds__(256) void page_read_windows(CacheRows a) {
+    if (blockIdx.y == 0)
+        read_window<F, false>(a);
+    else
+        read_window<F, true>(a);
 }
 
 // keep: a workgroup a head of a sequence, a thread a byte run of a token
@@ -753,8 +847,20 @@ static hipError_t launch_rows(const CacheRows& a, bool read, hipStream_t stream)
 hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream) { return launch_rows(a, false, stream); }
 hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream) { return launch_rows(a, true, stream); }
 
+// Rows from which a step of a pool looks for tiles among them.
+constexpr uint32_t kWindowRows = 64;
+
 template <uint32_t F>
 static void launch_paged_rows(const CacheRows& a, bool read, hipStream_t stream) {
+    if (a.tokens >= kWindowRows) {
+        const uint64_t units = (uint64_t{a.tokens} + 31) / 32 * a.cache.kv_heads * (a.cache.head_dim / 32);
+        const dim3 grid(static_cast<uint32_t>((units + 3) / 4), 2);
+        if (read)
+            hipLaunchKernelGGL(page_read_windows<F>, grid, dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL(page_append_windows<F>, grid, dim3(256), 0, stream, a);
+        return;
+    }
     const uint64_t blocks = uint64_t{a.tokens} * a.cache.kv_heads * (a.cache.head_dim / 32);
     const dim3 grid(static_cast<uint32_t>((blocks * 8 + 255) / 256), 2);
     if (read)

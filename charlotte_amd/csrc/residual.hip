@@ -133,7 +133,7 @@ static hipError_t launch_fours(const ResidualNorm& a, uint32_t threads, hipStrea
 hipError_t launch_residual_norm(const ResidualNorm& a, hipStream_t stream) {
     const uint32_t fours = (a.width + 3) / 4;
     auto threads = [&](uint32_t each) { return (fours + 64 * each - 1) / (64 * each) * 64; };
-    if (threads(1) <= 256) return launch_fours<1>(a, threads(1), stream);
+    if (threads(1) <= 256 || (threads(1) <= 64 * kMostWaves && a.rows <= 512)) return launch_fours<1>(a, threads(1), stream);
     if (threads(4) <= 64 * kMostWaves) return launch_fours<4>(a, threads(4), stream);
     return launch_fours<8>(a, threads(8), stream);
 }
