@@ -246,6 +246,7 @@ __device__ __forceinline__ uint32_t kept_scale(uint32_t scale, uint32_t kept) {
 constexpr uint32_t kUnused = 0xFFFFFFFFu;
 template <uint32_t TOKENS>
 struct Tree {
+    static constexpr bool kTrees = true;
     int32_t parents[kTreeTokens];
     uint32_t above[TOKENS][kTreeTokens / 32];
     uint32_t depth[TOKENS];
@@ -992,23 +993,30 @@ struct Stage {
 // Waves of 32 rows a workgroup: two a SIMD where their registers allow.
 constexpr uint32_t row_waves(uint32_t blocks) { return blocks <= 4 ? 8 : 4; }
 
-// A wave's rows, their last tile done.
-template <uint32_t F, uint32_t NB, uint32_t X>
-__device__ __forceinline__ void write_rows(const Attention& a, const Group& group, Rows<F, NB, X>& rows, uint32_t row0) {
+// A wave's rows, their last tile done: `write` takes what `finish` does.
+template <uint32_t F, uint32_t NB, uint32_t X, typename WRITE>
+__device__ __forceinline__ void write_rows(const Group& group, Rows<F, NB, X>& rows, uint32_t row0, const WRITE& write) {
     rows.end();
     const uint32_t lane = threadIdx.x & 63u, row = row0 + lane % (16 * X);
     const float total = sum_of_row<X>(rows.sum);
     if (row >= group.row_end) return;
 #pragma unroll
     for (uint32_t t = 0; t < Rows<F, NB, X>::kQuads; ++t)
-        finish<NB>(a, group, row, rows.sight.live, Rows<F, NB, X>::quad_at(t), rows.quad(t), total, rows.offset,
-                   t == 0 && lane < 16 * X);
+        write(row, rows.sight.live, Rows<F, NB, X>::quad_at(t), rows.quad(t), total, rows.offset, t == 0 && lane < 16 * X);
 }
 
+// A sequence's records, one after the other: record t.
+struct Records {
+    static constexpr bool kGaps = false;  // none is missing
+    const uint8_t* base;
+    uint32_t bytes;
+    __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const { return base + static_cast<uint64_t>(t) * bytes; }
+};
+
 // A wave's 32 rows by themselves, straight from the records, 16 at a time.
-template <uint32_t F, uint32_t NB, typename TREE>
-__device__ __forceinline__ void attend_alone(const Attention& a, const Group& group, const TREE& tree, const uint8_t* base,
-                                             uint32_t row0) {
+template <uint32_t F, uint32_t NB, typename TREE, typename RECORDS, typename WRITE>
+__device__ __forceinline__ void attend_alone(const Attention& a, const Group& group, const TREE& tree, const RECORDS& records,
+                                             uint32_t row0, const WRITE& write) {
 #pragma unroll 1
     for (uint32_t first = row0; first < min(row0 + 32, group.row_end); first += 16) {
         typename Rows<F, NB, 1>::Queries queries;
@@ -1017,27 +1025,45 @@ __device__ __forceinline__ void attend_alone(const Attention& a, const Group& gr
         rows.begin(a, group, tree, first, queries);
 #pragma unroll 1
         for (uint32_t t = group.tile_begin; t < group.tile_end; ++t) {
-            const Record<F, NB, 1> record{base + static_cast<uint64_t>(t) * cache_record(F, NB), t * kTile, group.latest};
+            const uint8_t* at = records(t);
+            if constexpr (RECORDS::kGaps)
+                if (!at) {  // NaNs for the rows that see it
+                    if (rows.sees(a, group, tree, t * kTile) != 0) rows.sum = __builtin_nanf("");
+                    continue;
+                }
+            const Record<F, NB, 1> record{at, t * kTile, group.latest};
             rows.template tile<kCodes>(a, group, tree, t * kTile, record);
         }
-        write_rows(a, group, rows, first);
+        write_rows(group, rows, first, write);
     }
 }
 
+// A workgroup's LDS for them.
 template <uint32_t F, uint32_t NB>
-__global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
-    constexpr uint32_t W = row_waves(NB), kRows = 32 * W, kRecord = cache_record(F, NB), kUnit = cache_unit(F);
-    constexpr uint32_t kTiles = NB <= 4 ? 2 : 1;                                // a stage's
+struct RowsShape {
+    static constexpr uint32_t W = row_waves(NB), kRows = 32 * W;
+    static constexpr uint32_t kTiles = NB <= 4 ? 2 : 1;  // a stage's
+};
+template <uint32_t F, uint32_t NB>
+struct RowsSpace {
+    Stage<F, NB> stages[2][RowsShape<F, NB>::kTiles];
+    uint32_t wave_most[row_waves(NB)], wave_least[row_waves(NB)], wave_spoilt[row_waves(NB)];
+};
+
+// A workgroup's rows over its split's tiles; `alone`: some record is missing.
+template <uint32_t F, uint32_t NB, typename TREE, typename RECORDS, typename WRITE>
+__device__ __forceinline__ void attend_group(const Attention& a, const Group& group, TREE& tree, RowsSpace<F, NB>& space,
+                                             const RECORDS& records, const WRITE& write, bool alone) {
+    using Shape = RowsShape<F, NB>;
+    constexpr uint32_t W = Shape::W, kUnit = cache_unit(F), kTiles = Shape::kTiles;
     constexpr uint32_t kUnits = 2 * NB * kTiles, kMine = (kUnits + W - 1) / W;  // units of a stage; a wave's, at most
     constexpr uint32_t kScaleWords = (key_scales(F) ? 32 : 16) * NB;            // a tile's
     constexpr uint32_t kLoads = kUnit / 1024 + (kUnit < 1024 ? 1 : 0);          // 16-byte (Q4_0: 8-byte) loads a lane a unit
     static_assert(kScaleWords * kTiles <= 64 * W, "a thread a dword");
-    __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
-    __shared__ Stage<F, NB> stages[2][kTiles];
-    __shared__ uint32_t wave_most[W], wave_least[W], wave_spoilt[W];
+    auto& stages = space.stages;
+    auto &wave_most = space.wave_most, &wave_least = space.wave_least, &wave_spoilt = space.wave_spoilt;
 
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Group group(a, kRows);
     const uint32_t row0 = group.row0 + 32 * wave;
     const bool mine = row0 < group.row_end;  // a wave without rows still lays out its share
     typename Rows<F, NB, 2>::Queries queries;
@@ -1045,7 +1071,11 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     // a chain's wave sees nothing past its last row's token
     const uint32_t sees_to =
         a.parents ? group.latest : group.past + (min(row0 + 32, group.row_end) - 1) / a.group + 1;
-    const uint8_t* base = record_of(a.cache, F, group.sequence, group.head, 0);
+    if constexpr (RECORDS::kGaps)
+        if (alone) {
+            attend_alone<F, NB>(a, group, tree, records, row0, write);
+            return;
+        }
 
     // All the tiles' value scales, once: how far they reach, and whether any is a NaN (F16: other than one).
     Scales reach;
@@ -1054,7 +1084,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     for (uint32_t x = threadIdx.x; x < (group.tile_end - group.tile_begin) * 16 * NB; x += 64 * W) {
         const uint32_t t = group.tile_begin + x / (16 * NB), w = x % (16 * NB);
         const uint32_t word = kept_scale<F>(
-            reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord + value_scales_at(F, NB))[w],
+            reinterpret_cast<const uint32_t*>(records(t) + value_scales_at(F, NB))[w],
             kept_of(t * kTile, w / 4 & 3u, w & 3u, group.latest));
         if constexpr (F == kF16)
             spoilt |= word ^ 0x3C003C00u;
@@ -1064,9 +1094,10 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     reach.join();
     spoilt = F == kF16 ? __any(spoilt != 0) : reach.nan;
     if (lane == 0) wave_most[wave] = reach.most, wave_least[wave] = reach.least, wave_spoilt[wave] = spoilt;
-    if (a.parents)
-        read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
-                  group.token_end - group.token0, a.window);
+    if constexpr (TREE::kTrees)
+        if (a.parents)
+            read_tree(tree, a.parents + static_cast<uint64_t>(group.sequence) * a.tokens, a.tokens, group.token0,
+                      group.token_end - group.token0, a.window);
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w)
@@ -1078,7 +1109,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     if constexpr (F != kF16)
         if (__builtin_amdgcn_readfirstlane(reach.least) < power_bits(exponent + kCodeTop - kSplitSpread)) {
             // scales further apart than a layout is made for
-            attend_alone<F, NB>(a, group, tree, base, row0);
+            attend_alone<F, NB>(a, group, tree, records, row0, write);
             return;
         }
     Rows<F, NB, 2> rows;
@@ -1097,7 +1128,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
         for (uint32_t j = 0; j < kMine; ++j) {
             const uint32_t u = wave + W * j, t = tile0 + u / (2 * NB);
             if (u >= kUnits || t >= group.tile_end) continue;
-            const uint8_t* record = base + static_cast<uint64_t>(t) * kRecord;
+            const uint8_t* record = records(t);
             const uint8_t* unit = record + u % (2 * NB) * kUnit;
             if constexpr (F == kQ4_0) {
                 const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * lane);
@@ -1111,8 +1142,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
         }
         const uint32_t t = tile0 + threadIdx.x / kScaleWords;
         if (threadIdx.x < kScaleWords * kTiles && t < group.tile_end)
-            scale_word = reinterpret_cast<const uint32_t*>(base + static_cast<uint64_t>(t) * kRecord +
-                                                           key_scales_at(F, NB))[threadIdx.x % kScaleWords];
+            scale_word = reinterpret_cast<const uint32_t*>(records(t) + key_scales_at(F, NB))[threadIdx.x % kScaleWords];
     };
     auto lay = [&](uint32_t tile0, Stage<F, NB>* stage) {
         const uint32_t quarter = lane >> 4, column = lane & 15u;
@@ -1207,7 +1237,20 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
         if (more) lay(tile0 + kTiles, stages[turn ^ 1]);
         __syncthreads();
     }
-    if (mine) write_rows(a, group, rows, row0);
+    if (mine) write_rows(group, rows, row0, write);
+}
+
+template <uint32_t F, uint32_t NB>
+__global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
+    constexpr uint32_t kRows = RowsShape<F, NB>::kRows;
+    __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
+    __shared__ RowsSpace<F, NB> space;
+    const Group group(a, kRows);
+    const Records records{record_of(a.cache, F, group.sequence, group.head, 0), cache_record(F, NB)};
+    auto write = [&](uint32_t row, bool live, uint32_t at, float4_t out, float total, float least, bool stats) {
+        finish<NB>(a, group, row, live, at, out, total, least, stats);
+    };
+    attend_group<F, NB>(a, group, tree, space, records, write, false);
 }
 
 template <uint32_t F, uint32_t NB>

@@ -1,6 +1,8 @@
 // Attention of several requests' new tokens over their pages (attention.hpp's
-// arithmetic, few rows' form: a workgroup has 16 or 32 rows of a key head, its
-// waves take the tiles in turn through LDS rings, and are joined in LDS).
+// arithmetic): attend_pages with few rows a workgroup, 16 or 32 of a key head, its
+// waves taking the tiles in turn through LDS rings and joined in LDS;
+// attend_page_rows, for the requests of a step that bring kManyRows and more,
+// with 128 or 256, a tile laid out once for all of them.
 //
 // The requests' lengths are known to the device alone, and are anything: a
 // unit - 16 or 32 rows of a request and key head, over the tiles they see - may
@@ -76,6 +78,7 @@ __device__ __forceinline__ void join(float2 side, const float4_t& theirs, float&
 }
 
 struct NoTree {
+    static constexpr bool kTrees = false;
     uint32_t above[1][kTreeTokens / 32];
     uint32_t depth[1];
 };
@@ -91,13 +94,14 @@ struct Request {
 template <uint32_t ROWS>
 __device__ __forceinline__ void place_request(const PagedAttention& a, Request& r) {
     if (uint64_t{r.start} + r.count > a.rows) r.count = 0;
-    r.groups = (r.count * a.group + ROWS - 1) / ROWS;  // (rows * group is below 2^32)
+    r.groups = (r.count * a.group + ROWS - 1) / ROWS;  // (rows * group is below 2^28)
     const uint64_t end = uint64_t{r.past} + r.count;
     r.over = end > uint64_t{a.table_stride} * a.pool.capacity;
     if (r.over) {
         r.begin = 0, r.tiles = 1;
         return;
     }
+    if (r.count * a.group > a.few) r.groups = 0;  // the other kernel's
     r.begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
     r.tiles = (static_cast<uint32_t>(end) + kTile - 1) / kTile - r.begin;
 }
@@ -111,6 +115,47 @@ struct Parts {
         return place < wide ? place / (each + 1) : more + (place - wide) / each;
     }
 };
+
+// A unit's pieces joined, by a thread four values of a row over its share of the
+// pieces; then over the shares. `space`: T float4s and T float2s of LDS.
+template <uint32_t NB, uint32_t T, typename KEPT, typename OUTPUT>
+__device__ __forceinline__ void join_pieces(const PagedAttention& a, uint32_t unit_rows, uint32_t rows, uint32_t pieces,
+                                            const KEPT& kept_of, const OUTPUT& output_of, uint8_t* space) {
+    const uint32_t quads = 8 * NB, work = rows * quads, shares = max(1u, T / work);
+    float4_t* sums = reinterpret_cast<float4_t*>(space);
+    float2* sides = reinterpret_cast<float2*>(space + T * sizeof(float4_t));
+    for (uint32_t i0 = 0; i0 < work; i0 += T) {
+        const uint32_t i = i0 + threadIdx.x % min(work, T), mine = work <= T ? threadIdx.x / work : 0;
+        const bool live = i < work && mine < shares;
+        const uint32_t row = i / quads, value = i % quads * 4;
+        float least = INFINITY, total = 0.0f;
+        float4_t out = float4_t(0.0f);
+        constexpr uint32_t kBatch = 8;  // on their way together
+        for (uint32_t p0 = mine; live && p0 < pieces; p0 += kBatch * shares) {
+            float2 side[kBatch];
+            float4_t theirs[kBatch];
+#pragma unroll
+            for (uint32_t x = 0; x < kBatch; ++x) {
+                const uint32_t p = p0 + x * shares;
+                side[x] = make_float2(INFINITY, 0.0f), theirs[x] = float4_t(0.0f);
+                if (p >= pieces) continue;
+                const uint64_t from = uint64_t{kept_of(p)} * unit_rows + row;
+                side[x] = get(a.stats + from), theirs[x] = get(a.partial + from * (32 * NB) + value);
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < kBatch; ++x) join(side[x], theirs[x], least, total, out);
+        }
+        if (shares > 1) {
+            sums[threadIdx.x] = out, sides[threadIdx.x] = make_float2(least, total);
+            __syncthreads();
+            if (live && mine == 0)
+                for (uint32_t x = 1; x < shares; ++x)
+                    join(sides[threadIdx.x + x * work], sums[threadIdx.x + x * work], least, total, out);
+        }
+        if (live && mine == 0)
+            *reinterpret_cast<float4_t*>(output_of(row, value)) = least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
+    }
+}
 
 template <uint32_t F, uint32_t NB, uint32_t X>
 __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_pages(PagedAttention a) {
@@ -332,51 +377,175 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         __syncthreads();
         if (!last_piece) continue;
 
-        // The pieces joined: a thread four values of a row, over its share of the pieces; then over the shares.
-        const uint32_t quads = 8 * NB, work = (group.row_end - group.row0) * quads;
-        const uint32_t shares = max(1u, T / work);
-        auto kept_of = [&](uint32_t p) { return even ? 2 * (part - piece + p) + (p == 0) : counter + p; };
-        float4_t* sums = reinterpret_cast<float4_t*>(space);
-        float2* sides = reinterpret_cast<float2*>(space + T * sizeof(float4_t));
-        for (uint32_t i0 = 0; i0 < work; i0 += T) {
-            const uint32_t i = i0 + threadIdx.x % min(work, T), mine_of = work <= T ? threadIdx.x / work : 0;
-            const bool live = i < work && mine_of < shares;
-            const uint32_t row = i / quads, value = i % quads * 4;
-            float least = INFINITY, total = 0.0f;
-            float4_t out = float4_t(0.0f);
-            constexpr uint32_t kBatch = 8;  // on their way together
-            for (uint32_t p0 = mine_of; live && p0 < pieces; p0 += kBatch * shares) {
-                float2 side[kBatch];
-                float4_t theirs[kBatch];
+        join_pieces<NB, T>(a, kRows, group.row_end - group.row0, pieces,
+                           [&](uint32_t p) { return even ? 2 * (part - piece + p) + (p == 0) : counter + p; },
+                           [&](uint32_t row, uint32_t value) { return output_of(group.row0 + row, value); }, space);
+        __syncthreads();
+    }
+}
+
+// ---- requests of many rows -----------------------------------------------------
+
+// What a unit of many rows costs beside its tiles, and the least tiles of a part.
+constexpr uint32_t kManyUnitTiles = 2, kManyPartTiles = 8;
+// Pages of a piece whose table is kept in LDS; what is past them is read where it is.
+constexpr uint32_t kKeptPages = 1024;
+
+// A request's records through its pages; null where the page is none of the pool's.
+struct PagedRecords {
+    static constexpr bool kGaps = true;
+    const uint8_t* base;
+    const uint32_t* table;  // the request's row
+    const uint32_t* kept;   // LDS: its pages from `first` on
+    uint32_t first, record, tiles_a_page, page_inverse, kv_heads, head, pages;
+
+    __device__ __forceinline__ uint32_t place_of(uint32_t t) const { return tiles_a_page == 1 ? t : __umulhi(t, page_inverse); }
+    __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const {
+        const uint32_t place = place_of(t), page = place - first < kKeptPages ? kept[place - first] : table[place];
+        if (page >= pages) return nullptr;
+        return base + ((uint64_t{page} * kv_heads + head) * tiles_a_page + (t - place * tiles_a_page)) * record;
+    }
+};
+
+template <uint32_t F, uint32_t NB>
+__global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAttention a) {
+    constexpr uint32_t kRows = RowsShape<F, NB>::kRows, T = 64 * row_waves(NB);
+    static_assert(sizeof(RowsSpace<F, NB>) >= T * 24, "join_pieces' LDS");
+    __shared__ __align__(16) RowsSpace<F, NB> space;
+    __shared__ uint32_t kept_pages[kKeptPages], last_piece, missing;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t share = (a.requests + 63) / 64, first_request = lane * share;
+    const uint32_t last_request = min(first_request + share, a.requests);
+
+    // Request i, if it is of many rows: its rows a unit each kRows, and the tiles that a unit's see.
+    struct Many {
+        uint32_t past, count, start, groups;
+    };
+    auto many_of = [&](uint32_t i) {
+        Many m{a.past[i], a.counts[i], a.starts[i], 0};
+        const bool mine = uint64_t{m.start} + m.count <= a.rows && m.count * a.group > a.few &&
+                          uint64_t{m.past} + m.count <= uint64_t{a.table_stride} * a.pool.capacity;
+        if (mine) m.groups = (m.count * a.group + kRows - 1) / kRows;
+        return m;
+    };
+    auto begin_of = [&](const Many& m, uint32_t unit) {
+        const uint32_t place = m.past + unit * kRows / a.group + 1;
+        return a.window && place > a.window ? (place - a.window) / kTile : 0u;
+    };
+    auto end_of = [&](const Many& m, uint32_t unit) {
+        const uint32_t rows = min((unit + 1) * kRows, m.count * a.group);
+        return (m.past + (rows - 1) / a.group + kTile) / kTile;
+    };
+    auto length_of = [&](const Many& m, uint32_t unit) { return end_of(m, unit) - begin_of(m, unit) + kManyUnitTiles; };
+    uint32_t line = 0;
+    for (uint32_t i = first_request; i < last_request; ++i) {
+        const Many m = many_of(i);
+        for (uint32_t g = 0; g < m.groups; ++g) line = plus(line, length_of(m, g));
+    }
+    uint32_t line_before = line;
 #pragma unroll
-                for (uint32_t x = 0; x < kBatch; ++x) {
-                    const uint32_t p = p0 + x * shares;
-                    side[x] = make_float2(INFINITY, 0.0f), theirs[x] = float4_t(0.0f);
-                    if (p >= pieces) continue;
-                    const uint64_t from = uint64_t{kept_of(p)} * kRows + row;
-                    side[x] = get(a.stats + from), theirs[x] = get(a.partial + from * (32 * NB) + value);
-                }
-#pragma unroll
-                for (uint32_t x = 0; x < kBatch; ++x) join(side[x], theirs[x], least, total, out);
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t other = __shfl_up(line_before, o);
+        if (lane >= o) line_before = plus(line_before, other);
+    }
+    const uint32_t head_line = of_lane(line_before, 63u), length = times(head_line, a.pool.kv_heads);
+    if (length == kTooMuch || length == 0) return;
+    line_before -= line;
+    const uint32_t count = min(gridDim.x, max(length / kManyPartTiles, 1u));
+    // neighbours on the line on one XCD
+    const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+    if (part >= count) return;
+    const Parts parts{length / count, length % count};
+    uint32_t place = parts.begin(part);
+    const uint32_t end = parts.begin(part + 1);
+
+    Attention b{};
+    b.queries = a.queries, b.output = a.output;
+    b.query_stride = a.query_stride, b.output_stride = a.output_stride;
+    b.tokens = 1, b.group = a.group, b.window = a.window, b.scale = a.scale, b.splits = 1;
+    NoTree tree{};
+
+    while (place < end) {
+        // The unit at the place: among those of the last lane whose line does not begin past it.
+        const uint32_t head = place / head_line, on_head = place - head * head_line;
+        const uint32_t low = 63u - __builtin_clzll(__ballot(first_request < a.requests && line_before <= on_head));
+        uint32_t before = of_lane(line_before, low), at = low * share, unit = 0;
+        Many m = many_of(at);
+        for (;;) {
+            if (unit < m.groups) {
+                const uint32_t next = before + length_of(m, unit);
+                if (next > on_head) break;
+                before = next, ++unit;
+            } else {
+                m = many_of(++at), unit = 0;
             }
-            if (shares > 1) {
-                sums[threadIdx.x] = out, sides[threadIdx.x] = make_float2(least, total);
-                __syncthreads();
-                if (live && mine_of == 0)
-                    for (uint32_t x = 1; x < shares; ++x)
-                        join(sides[threadIdx.x + x * work], sums[threadIdx.x + x * work], least, total, out);
-            }
-            if (live && mine_of == 0)
-                *reinterpret_cast<float4_t*>(output_of(group.row0 + row, value)) =
-                    least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
         }
+        at = uniform(at), unit = uniform(unit);
+        m = Many{uniform(m.past), uniform(m.count), uniform(m.start), uniform(m.groups)};
+        const uint32_t unit_begin = head * head_line + uniform(before), unit_end = unit_begin + length_of(m, unit);
+        const uint32_t from = parts.at(unit_begin), pieces = parts.at(unit_end - 1) - from + 1, piece = part - from;
+        const uint32_t kept = 2 * part + (piece == 0), counter = 2 * from + 1;
+        const uint32_t begin = max(parts.begin(part), unit_begin), until = min(end, unit_end);
+        place = until;
+
+        Group group;
+        group.sequence = m.start, group.head = head, group.past = m.past, group.latest = m.past + m.count;
+        group.row0 = unit * kRows, group.row_end = min(group.row0 + kRows, m.count * a.group);
+        group.token0 = group.row0 / a.group, group.token_end = (group.row_end - 1) / a.group + 1;
+        group.all_begin = a.window && group.latest > a.window ? group.latest - a.window : 0u;
+        group.tile_begin = begin_of(m, unit) + max(begin - unit_begin, kManyUnitTiles) - kManyUnitTiles;
+        group.tile_end = begin_of(m, unit) + max(until - unit_begin, kManyUnitTiles) - kManyUnitTiles;
+
+        // The piece's pages, and whether one is none of the pool's.
+        PagedRecords records{a.pool.base, a.table + uint64_t{at} * a.table_stride, kept_pages, 0, cache_record(F, NB),
+                             a.pool.capacity / kTile, a.page_inverse, a.pool.kv_heads, head, a.pool.sequences};
+        records.first = records.place_of(group.tile_begin);
+        const uint32_t places = group.tile_begin < group.tile_end ? records.place_of(group.tile_end - 1) - records.first + 1 : 0;
+        if (threadIdx.x == 0) missing = 0;
+        __syncthreads();
+        bool gone = false;
+        for (uint32_t i = threadIdx.x; i < places; i += T) {
+            const uint32_t page = records.table[records.first + i];
+            if (i < kKeptPages) kept_pages[i] = page;
+            gone |= page >= a.pool.sequences;
+        }
+        if (gone) missing = 1;
+        __syncthreads();
+        auto write = [&](uint32_t row, bool live, uint32_t value, float4_t out, float total, float least, bool stats) {
+            if (pieces == 1) {
+                finish<NB>(b, group, row, live, value, out, total, least, false);
+                return;
+            }
+            const bool empty = !live || (least == INFINITY && total == 0.0f);
+            const uint64_t to = uint64_t{kept} * kRows + (row - group.row0);
+            put(a.partial + to * (32 * NB) + value, empty ? float4_t(0.0f) : out);
+            if (stats) put(a.stats + to, make_float2(empty ? INFINITY : total != total ? total : least, empty ? 0.0f : total));
+        };
+        attend_group<F, NB>(b, group, tree, space, records, write, uniform(missing) != 0);
+        wait_loads<0>();
+        __syncthreads();  // the LDS is read, and what was written has arrived
+        if (pieces == 1) continue;
+        if (threadIdx.x == 0) last_piece = atomicInc(a.counters + counter, pieces - 1) == pieces - 1;
+        __syncthreads();
+        if (!last_piece) continue;
+        join_pieces<NB, T>(
+            a, kRows, group.row_end - group.row0, pieces, [&](uint32_t p) { return 2 * (from + p) + (p == 0); },
+            [&](uint32_t row, uint32_t value) {
+                const uint32_t of = group.row0 + row;
+                return a.output + (uint64_t{m.start} + of / a.group) * a.output_stride +
+                       (uint64_t{head} * a.group + of % a.group) * (32 * NB) + value;
+            },
+            reinterpret_cast<uint8_t*>(&space));
         __syncthreads();
     }
 }
 
 template <uint32_t F, uint32_t NB>
 static hipError_t launch_paged_blocks(const PagedAttention& a, uint32_t octets, hipStream_t stream) {
-    if (octets == 2)
+    if (octets == 0) {
+        if constexpr (many_rows_of(F, 32 * NB))
+            hipLaunchKernelGGL((attend_page_rows<F, NB>), dim3(a.parts), dim3(64 * row_waves(NB)), 0, stream, a);
+    } else if (octets == 2)
         hipLaunchKernelGGL((attend_pages<F, NB, 2>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
     else
         hipLaunchKernelGGL((attend_pages<F, NB, 1>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 1>::kWaves), 0, stream, a);

@@ -2,6 +2,7 @@
 // (include/charlotte_hip_matmul.h): their checks, on the host and before any
 // kernel launches, and their launches. Lengths and tables are device memory, and
 // what they hold is checked by the kernels.
+#include <algorithm>
 #include <cmath>
 
 #include "checks.hpp"
@@ -108,9 +109,24 @@ void check_table(uint32_t requests, uint32_t table_stride, uint32_t page_tokens)
         refuse("table stride " + std::to_string(table_stride));
 }
 
-// Bytes of a step's pieces of units of 16 * octets rows: outputs, then offsets and sums.
-uint64_t piece_bytes(const charlotte_hip_matmul_context* ctx, const chm::CacheShape& c, uint32_t octets) {
-    return uint64_t{ctx->compute_units} * chm::kPieces * 16 * octets * (uint64_t{c.head_dim} * 4 + 8);
+// How a step of attention runs: the rows of a unit of attend_pages, in 16s; the
+// rows of one of attend_page_rows, 0 where that does not run.
+struct PagedPlan {
+    uint32_t octets, many;
+};
+PagedPlan paged_plan(const chm::CacheShape& c, uint32_t group, uint32_t most) {
+    // (what many rows bring has its own kernel: the others are mostly single tokens')
+    if (uint64_t{group} * most >= chm::kManyRows && chm::many_rows_of(c.format, c.head_dim))
+        return {chm::paged_octets(group, 1), c.head_dim <= 128 ? 256u : 128u};
+    return {chm::paged_octets(group, most), 0};
+}
+
+// Pieces' places, outputs and then offsets and sums, of units of `rows` rows.
+uint64_t piece_rows(const charlotte_hip_matmul_context* ctx, uint32_t rows) {
+    return uint64_t{ctx->compute_units} * chm::kPieces * rows;
+}
+uint64_t piece_bytes(const charlotte_hip_matmul_context* ctx, const chm::CacheShape& c, const PagedPlan& plan) {
+    return piece_rows(ctx, std::max(16 * plan.octets, plan.many)) * (uint64_t{c.head_dim} * 4 + 8);
 }
 
 // An output that is an input's memory has its stride.
@@ -221,7 +237,10 @@ uint64_t charlotte_hip_matmul_paged_attention_workspace_bytes(const charlotte_hi
                                                               const charlotte_hip_matmul_page_pool* pool,
                                                               uint32_t query_heads, uint32_t most) {
     if (!ctx || !pool || query_heads == 0 || query_heads % pool->shape.kv_heads != 0) return 0;
-    return piece_bytes(ctx, pool->shape, chm::paged_octets(query_heads / pool->shape.kv_heads, most));
+    // a smaller step may have units of 32 rows where this one has them of 16
+    const uint32_t group = query_heads / pool->shape.kv_heads;
+    return std::max(piece_bytes(ctx, pool->shape, paged_plan(pool->shape, group, most)),
+                    piece_bytes(ctx, pool->shape, {chm::paged_octets(group, most), 0}));
 }
 
 charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_matmul_context* ctx,
@@ -237,9 +256,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         if (d.query_heads == 0 || d.query_heads % c.kv_heads != 0)
             refuse("query heads " + std::to_string(d.query_heads) + " over " + std::to_string(c.kv_heads) + " key heads");
         const uint32_t group = d.query_heads / c.kv_heads;
-        const uint32_t octets = chm::paged_octets(group, d.most);
+        const PagedPlan plan = paged_plan(c, group, d.most);
         // all units, each of all the tiles that a table's row holds
-        const uint64_t units = (uint64_t{d.rows} * group / (16 * octets) + d.requests) * c.kv_heads;
+        const uint64_t units = (uint64_t{d.rows} * group / (16 * plan.octets) + d.requests) * c.kv_heads;
         if (uint64_t{d.rows} * group >= (1ull << 28) || units * (uint64_t{d.table_stride} * (c.capacity / 32) + 16) >= (1ull << 32))
             refuse("too many rows a step for tables so long");
         if (!std::isfinite(d.scale)) refuse("scale not finite");
@@ -258,20 +277,26 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         a.past = d.past, a.counts = d.counts, a.starts = d.starts, a.table = d.table;
         a.requests = d.requests, a.rows = d.rows, a.table_stride = d.table_stride;
         a.group = group, a.window = d.window, a.scale = d.scale;
-        const uint64_t bytes = piece_bytes(ctx, c, octets);
+        const uint64_t bytes = piece_bytes(ctx, c, plan);
         need(d.workspace, "workspace", 16);
         if (d.workspace_bytes < bytes) refuse("needs a workspace of " + std::to_string(bytes) + " bytes");
         a.partial = static_cast<float*>(d.workspace);
-        a.stats = reinterpret_cast<float2*>(a.partial + uint64_t{ctx->compute_units} * chm::kPieces * 16 * octets * c.head_dim);
         a.counters = d.pool->counters;
         a.parts = ctx->compute_units;
         const uint32_t page_tiles = c.capacity / 32;
         a.page_inverse = page_tiles > 1 ? static_cast<uint32_t>(((1ull << 32) + page_tiles - 1) / page_tiles) : 0;
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
-        const auto s = static_cast<hipStream_t>(stream);
-        return c.format == chm::kF16    ? chm::launch_paged_f16(a, octets, s)
-               : c.format == chm::kQ4_0 ? chm::launch_paged_q4_0(a, octets, s)
-                                        : chm::launch_paged_q8_0(a, octets, s);
+        auto run = [&](uint32_t rows, uint32_t octets) {
+            a.stats = reinterpret_cast<float2*>(a.partial + piece_rows(ctx, rows) * c.head_dim);
+            const auto s = static_cast<hipStream_t>(stream);
+            return c.format == chm::kF16    ? chm::launch_paged_f16(a, octets, s)
+                   : c.format == chm::kQ4_0 ? chm::launch_paged_q4_0(a, octets, s)
+                                            : chm::launch_paged_q8_0(a, octets, s);
+        };
+        a.few = plan.many ? chm::kManyRows - 1 : 0xFFFFFFFFu;
+        if (plan.many)
+            if (hipError_t e = run(plan.many, 0); e != hipSuccess) return e;
+        return run(16 * plan.octets, plan.octets);
     });
 }
 

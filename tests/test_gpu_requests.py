@@ -253,7 +253,7 @@ def test_a_pool_reads_back_what_its_format_holds(ctx, dev, format_, heads, dim, 
 
 
 def _check_paged(dev, format_, requests, heads, kv_heads, dim, page_tokens=32, window=0, seed=0, most=None, rows=None,
-                 granted=None, scale=None, spread=1.0, query_stride=0, output_stride=0, stride=None, twice=False):
+                 granted=None, scale=None, spread=1.0, query_stride=0, output_stride=0, stride=None, twice=False, grow=0):
     """requests: (past, count) each. Every row of theirs against the restatement, others left as they were."""
     from charlotte_amd import harness as hx
     from charlotte_amd import serving as sv
@@ -277,6 +277,8 @@ def _check_paged(dev, format_, requests, heads, kv_heads, dim, page_tokens=32, w
         n = p + c
         k = rng.standard_normal((n, kv_heads, dim)).astype(np.float32)
         v = (rng.standard_normal((n, kv_heads, dim)) * spread).astype(np.float32)
+        if grow:  # in octaves, a token's values less or more than another's
+            v *= (2.0 ** -rng.integers(0, grow, (n, 1, 1))).astype(np.float32) * np.float32(2.0 ** (grow // 2))
         keys.append(k)
         values.append(v)
     slots = [int(table[r, t // page_tokens]) * page_tokens + t % page_tokens
@@ -312,8 +314,10 @@ def _check_paged(dev, format_, requests, heads, kv_heads, dim, page_tokens=32, w
         touched[at] = True
         want, weight, size = ref.attention(q[at], ref.stored(keys[r], format_), ref.stored(values[r], format_), past, scale,
                                            window=window)
-        # as attention's, and once more for each piece that is joined
-        assert (np.abs(got[at] - want) <= ref.attention_bound(weight, size, past + count + 32 * 256, dim)).all(), r
+        # as attention's, and once more for each piece that is joined; NaNs where a block is not held
+        none = np.isnan(want)
+        assert np.array_equal(np.isnan(got[at]), none), r
+        assert (np.abs(got[at] - want) <= ref.attention_bound(weight, size, past + count + 32 * 256, dim))[~none].all(), r
     assert (got[~touched].view(np.uint32) == NOWHERE).all()
     pool.pool.free()
     return got
@@ -341,6 +345,62 @@ def test_paged_attention_of_requests_of_any_lengths(ctx, dev, format_, requests,
 def test_paged_attention_shares_its_work_evenly(ctx, dev, dim, heads, kv_heads, lengths):
     """Lines of several parts: units in many pieces, many units in one part, more requests than threads."""
     _check_paged(dev, "q8_0", [(n, 1) for n in lengths], heads, kv_heads, dim, seed=len(lengths), twice=True)
+
+
+@pytest.mark.parametrize("format_", FORMATS)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 256])
+def test_paged_attention_of_many_rows(ctx, dev, format_, dim):
+    """Requests that bring 256 rows of a key head and more, beside others: workgroups of many rows, in pieces and whole."""
+    _check_paged(dev, format_, [(150, 91), (40, 1), (700, 86), (0, 85)], 3, 1, dim, page_tokens=64, seed=dim, twice=True)
+
+
+@pytest.mark.parametrize("requests,heads,kv_heads,page_tokens,window", [
+    ([(0, 700)], 2, 2, 32, 0), ([(3000, 300)], 2, 1, 96, 0), ([(33000, 130)], 2, 1, 32, 0),   # more pages than LDS keeps
+    ([(500, 256), (10, 255), (20, 257), (0, 1)], 1, 1, 32, 0), ([(500, 300), (0, 260)], 4, 2, 32, 70),
+    ([(900, 280), (77, 1)], 1, 1, 32, 1), ([(100, 300), (4000, 300)], 8, 8, 128, 1000)])
+def test_paged_attention_of_many_rows_in_pieces(ctx, dev, requests, heads, kv_heads, page_tokens, window):
+    _check_paged(dev, "q8_0", requests, heads, kv_heads, 64, page_tokens=page_tokens, window=window, seed=heads, twice=True)
+    _check_paged(dev, "f16", requests, heads, kv_heads, 32, page_tokens=page_tokens, window=window, seed=heads, spread=100.0)
+
+
+def test_many_rows_of_scales_far_apart(ctx, dev):
+    """Values whose scales a layout is not made for; the largest are past what Q4_0's scales hold."""
+    _check_paged(dev, "q8_0", [(300, 130), (64, 1)], 2, 1, 64, seed=3, grow=40)
+    _check_paged(dev, "q4_0", [(300, 130), (64, 1)], 2, 1, 64, seed=3, grow=28)
+    _check_paged(dev, "q4_0", [(300, 130), (64, 1)], 2, 1, 64, seed=3, grow=40)
+
+
+def test_pages_that_the_pool_does_not_have_of_many_rows(ctx, dev):
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(15)
+    pool = _Pool(dev, "q8_0", 12, 32, 1, 32)
+    k, v = (rng.standard_normal((12 * 32, 32)).astype(np.float32) for _ in range(2))
+    pool.write(k, v, np.arange(384))
+    table = _words([[3, 4, 5, 6, 12, 8, 9, 10, 11], [0, 1, 2, 3, 4, 5, 6, 7, 8], [0, 1, 2, 3, 4, 5, 6, 7, 8]])
+    past, counts, starts = [20, 20, 40], [260, 260, 260], [0, 260, 520, 780]  # the last passes nine pages
+    q = rng.standard_normal((780, 1, 32)).astype(np.float32)
+    need = sv.paged_attention_workspace_bytes(ctx, pool.pool, 1, 260)
+    work, _ = dev.room(need, np.uint8)
+    for window in (0, 40):
+        out, read = dev.room(780 * 32)
+        sv.paged_attention(ctx, sv.PagedAttention(pool.pool, dev.put(q), out, 1, 0.2, 3, 780, dev.put(_words(past)),
+                                                  dev.put(_words(counts)), dev.put(_words(starts)), dev.put(table), 9, window, 260,
+                                                  workspace=work, workspace_bytes=need))
+        hx.sync()
+        got = read().reshape(780, 1, 32)
+        # page 4 has places 128 .. 159; token t stands at 20 + t
+        t = np.arange(260) + 20
+        sees = (t >= 128) & ((window == 0) | (t - window + 1 <= 159))
+        assert np.isnan(got[:260][sees]).all() and np.isfinite(got[:260][~sees]).all()
+        assert np.isnan(got[520:]).all()
+        of = [int(table[1][i // 32]) * 32 + i % 32 for i in range(280)]
+        want, weight, size = ref.attention(q[260:520], ref.stored(k, "q8_0")[of][:, None], ref.stored(v, "q8_0")[of][:, None], 20, 0.2,
+                                           window=window)
+        assert (np.abs(got[260:520] - want) <= ref.attention_bound(weight, size, 400, 32)).all()
+    pool.pool.free()
 
 
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
