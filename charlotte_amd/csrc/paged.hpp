@@ -91,19 +91,41 @@ struct Request {
     bool over;              // its tokens pass the table's row
 };
 
+// `many`: requests of kManyRows rows and more are the other kernel's.
 template <uint32_t ROWS>
-__device__ __forceinline__ void place_request(const PagedAttention& a, Request& r) {
+__device__ __forceinline__ void place_request(const PagedAttention& a, Request& r, bool many) {
     if (uint64_t{r.start} + r.count > a.rows) r.count = 0;
-    r.groups = (r.count * a.group + ROWS - 1) / ROWS;  // (rows * group is below 2^28)
+    const uint32_t rows = r.count * a.group;  // below 2^28
+    r.groups = rows > a.above && rows <= a.upto ? (rows + ROWS - 1) / ROWS : 0;
     const uint64_t end = uint64_t{r.past} + r.count;
     r.over = end > uint64_t{a.table_stride} * a.pool.capacity;
     if (r.over) {
         r.begin = 0, r.tiles = 1;
         return;
     }
-    if (r.count * a.group > a.few) r.groups = 0;  // the other kernel's
+    if (many && rows >= kManyRows) r.groups = 0;
     r.begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
     r.tiles = (static_cast<uint32_t>(end) + kTile - 1) / kTile - r.begin;
+}
+
+// Whether the requests of kManyRows rows and more are worth their own kernel: 32 rows by
+// a tile of theirs number a.many_load a workgroup and more. The same in every kernel
+// of the step.
+__device__ __forceinline__ bool many_rows(const PagedAttention& a) {
+    if (a.many_load == 0) return false;
+    const uint32_t lane = threadIdx.x & 63u, share = (a.requests + 63) / 64;
+    uint32_t load = 0;
+    for (uint32_t i = lane * share; i < min((lane + 1) * share, a.requests); ++i) {
+        Request r{a.past[i], a.counts[i], a.starts[i], 0, 0, 0, false};
+        if (uint64_t{r.start} + r.count > a.rows || r.count * a.group < kManyRows) continue;
+        const uint64_t end = uint64_t{r.past} + r.count;
+        if (end > uint64_t{a.table_stride} * a.pool.capacity) continue;
+        const uint32_t begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
+        load = plus(load, times((r.count * a.group + 31) / 32, (static_cast<uint32_t>(end) + kTile - 1) / kTile - begin));
+    }
+#pragma unroll
+    for (uint32_t o = 32; o > 0; o >>= 1) load = plus(load, __shfl_xor(load, o));
+    return times(uniform(load), a.pool.kv_heads) >= a.many_load * a.parts;
 }
 
 // A line in equal parts, the first ones a place longer.
@@ -177,9 +199,10 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
     // a tile's page, exact: tiles are below 2^26, pages of at most 64
     auto page_at = [&](uint32_t tile) { return tiles_a_page == 1 ? tile : __umulhi(tile, a.page_inverse); };
 
+    const bool many = many_rows(a);
     auto request_of = [&](uint32_t i) {
         Request r{a.past[i], a.counts[i], a.starts[i], 0, 0, 0, false};
-        place_request<kRows>(a, r);
+        place_request<kRows>(a, r, many);
         return r;
     };
     Request mine{};
@@ -197,12 +220,23 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         longest = max(longest, static_cast<uint32_t>(__shfl_xor(longest, o)));
     }
     const uint32_t all_tiles = times(uniform(tiles), a.pool.kv_heads), all_units = times(uniform(units), a.pool.kv_heads);
-    if (all_tiles == kTooMuch || all_units == kTooMuch) return;
+    if (all_units == 0 || all_tiles == kTooMuch || all_units == kTooMuch) return;
 
     // Pieces of at most `piece_tiles`, which are no more than the workgroups; or equal parts of the line.
     const uint32_t even_tiles = all_tiles / gridDim.x;
     uint32_t piece_tiles = 0;
-    if (all_units < gridDim.x) piece_tiles = max(all_tiles / (gridDim.x - all_units) + 1, W);
+    if (all_units < gridDim.x) {
+        // as many workgroups as there are have it evenly, if the units' own ends leave them enough
+        piece_tiles = max((all_tiles + gridDim.x - 1) / gridDim.x, W);
+        uint32_t pieces = 0;
+        for (uint32_t i = first_request; i < last_request; ++i) {
+            const Request r = i == first_request ? mine : request_of(i);
+            pieces += r.groups * ((r.tiles + piece_tiles - 1) / piece_tiles);
+        }
+#pragma unroll
+        for (uint32_t o = 32; o > 0; o >>= 1) pieces += __shfl_xor(pieces, o);
+        if (uniform(pieces) * a.pool.kv_heads > gridDim.x) piece_tiles = max(all_tiles / (gridDim.x - all_units) + 1, W);
+    }
     const bool even = all_units >= gridDim.x || min(piece_tiles, uniform(longest)) > even_tiles + kPieceTiles;
     auto length_of = [&](const Request& r) {
         return even ? r.tiles + kUnitTiles : (r.tiles + piece_tiles - 1) / piece_tiles;
@@ -242,12 +276,12 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
         uint32_t before = of_lane(line_before, low);
         uint32_t at = low * share;
         Request r{of_lane(mine.past, low), of_lane(mine.count, low), of_lane(mine.start, low), 0, 0, 0, false};
-        place_request<kRows>(a, r);
+        place_request<kRows>(a, r, many);
         while (before + r.groups * length_of(r) <= on_head) {
             before += r.groups * length_of(r);
             ++at;
             r.past = uniform(a.past[at]), r.count = uniform(a.counts[at]), r.start = uniform(a.starts[at]);
-            place_request<kRows>(a, r);
+            place_request<kRows>(a, r, many);
         }
         const uint32_t unit_length = length_of(r);
         const uint32_t unit = (on_head - before) / unit_length;
@@ -407,68 +441,65 @@ struct PagedRecords {
     }
 };
 
-template <uint32_t F, uint32_t NB>
-__global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAttention a) {
-    constexpr uint32_t kRows = RowsShape<F, NB>::kRows, T = 64 * row_waves(NB);
-    static_assert(sizeof(RowsSpace<F, NB>) >= T * 24, "join_pieces' LDS");
-    __shared__ __align__(16) RowsSpace<F, NB> space;
-    __shared__ uint32_t kept_pages[kKeptPages], last_piece, missing;
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t share = (a.requests + 63) / 64, first_request = lane * share;
-    const uint32_t last_request = min(first_request + share, a.requests);
+// Where piece p of the unit that begins in part `first` is kept.
+__device__ __forceinline__ uint64_t kept_at(uint32_t first, uint32_t p) { return 2 * (first + p) + (p == 0); }
 
-    // Request i, if it is of many rows: its rows a unit each kRows, and the tiles that a unit's see.
-    struct Many {
-        uint32_t past, count, start, groups;
-    };
-    auto many_of = [&](uint32_t i) {
-        Many m{a.past[i], a.counts[i], a.starts[i], 0};
-        const bool mine = uint64_t{m.start} + m.count <= a.rows && m.count * a.group > a.few &&
+// Request i, if it is of many rows: a unit each ROWS of them.
+struct Many {
+    uint32_t at, past, count, start, groups;
+};
+// Their units on a line, each as long as the tiles that its rows see and kManyUnitTiles.
+template <uint32_t ROWS>
+struct ManyLine {
+    const PagedAttention& a;
+    uint32_t share, line_before, head_line, count;
+    Parts parts;
+
+    __device__ __forceinline__ Many many_of(uint32_t i) const {
+        Many m{i, a.past[i], a.counts[i], a.starts[i], 0};
+        const bool mine = uint64_t{m.start} + m.count <= a.rows && m.count * a.group >= kManyRows &&
                           uint64_t{m.past} + m.count <= uint64_t{a.table_stride} * a.pool.capacity;
-        if (mine) m.groups = (m.count * a.group + kRows - 1) / kRows;
+        if (mine) m.groups = (m.count * a.group + ROWS - 1) / ROWS;
         return m;
-    };
-    auto begin_of = [&](const Many& m, uint32_t unit) {
-        const uint32_t place = m.past + unit * kRows / a.group + 1;
+    }
+    __device__ __forceinline__ uint32_t begin_of(const Many& m, uint32_t unit) const {
+        const uint32_t place = m.past + unit * ROWS / a.group + 1;
         return a.window && place > a.window ? (place - a.window) / kTile : 0u;
-    };
-    auto end_of = [&](const Many& m, uint32_t unit) {
-        const uint32_t rows = min((unit + 1) * kRows, m.count * a.group);
-        return (m.past + (rows - 1) / a.group + kTile) / kTile;
-    };
-    auto length_of = [&](const Many& m, uint32_t unit) { return end_of(m, unit) - begin_of(m, unit) + kManyUnitTiles; };
-    uint32_t line = 0;
-    for (uint32_t i = first_request; i < last_request; ++i) {
-        const Many m = many_of(i);
-        for (uint32_t g = 0; g < m.groups; ++g) line = plus(line, length_of(m, g));
     }
-    uint32_t line_before = line;
+    __device__ __forceinline__ uint32_t length_of(const Many& m, uint32_t unit) const {
+        const uint32_t rows = min((unit + 1) * ROWS, m.count * a.group);
+        return (m.past + (rows - 1) / a.group + kTile) / kTile - begin_of(m, unit) + kManyUnitTiles;
+    }
+    // Laid out by each wave; no parts where there is nothing, or too much.
+    __device__ __forceinline__ explicit ManyLine(const PagedAttention& a_) : a(a_), share((a_.requests + 63) / 64), count(0) {
+        const uint32_t lane = threadIdx.x & 63u, first = lane * share;
+        uint32_t line = 0;
+        for (uint32_t i = first; i < min(first + share, a.requests); ++i) {
+            const Many m = many_of(i);
+            for (uint32_t g = 0; g < m.groups; ++g) line = plus(line, length_of(m, g));
+        }
+        line_before = line;
 #pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint32_t other = __shfl_up(line_before, o);
-        if (lane >= o) line_before = plus(line_before, other);
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint32_t other = __shfl_up(line_before, o);
+            if (lane >= o) line_before = plus(line_before, other);
+        }
+        head_line = of_lane(line_before, 63u);
+        line_before -= line;
+        const uint32_t length = times(head_line, a.pool.kv_heads);
+        if (length == kTooMuch || length == 0) return;
+        count = min(a.parts, max(length / kManyPartTiles, 1u));
+        parts = {length / count, length % count};
     }
-    const uint32_t head_line = of_lane(line_before, 63u), length = times(head_line, a.pool.kv_heads);
-    if (length == kTooMuch || length == 0) return;
-    line_before -= line;
-    const uint32_t count = min(gridDim.x, max(length / kManyPartTiles, 1u));
-    // neighbours on the line on one XCD
-    const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-    if (part >= count) return;
-    const Parts parts{length / count, length % count};
-    uint32_t place = parts.begin(part);
-    const uint32_t end = parts.begin(part + 1);
-
-    Attention b{};
-    b.queries = a.queries, b.output = a.output;
-    b.query_stride = a.query_stride, b.output_stride = a.output_stride;
-    b.tokens = 1, b.group = a.group, b.window = a.window, b.scale = a.scale, b.splits = 1;
-    NoTree tree{};
-
-    while (place < end) {
-        // The unit at the place: among those of the last lane whose line does not begin past it.
-        const uint32_t head = place / head_line, on_head = place - head * head_line;
-        const uint32_t low = 63u - __builtin_clzll(__ballot(first_request < a.requests && line_before <= on_head));
+    // The unit at a place: of those of the last lane whose line does not begin past it.
+    struct Unit {
+        Many m;
+        uint32_t head, unit, begin, end;  // on the line
+        uint32_t first, pieces;           // its first part, its parts
+    };
+    __device__ __forceinline__ Unit unit_at(uint32_t place) const {
+        const uint32_t lane = threadIdx.x & 63u, head = place / head_line, on_head = place - head * head_line;
+        const uint32_t low = 63u - __builtin_clzll(__ballot(lane * share < a.requests && line_before <= on_head));
         uint32_t before = of_lane(line_before, low), at = low * share, unit = 0;
         Many m = many_of(at);
         for (;;) {
@@ -480,25 +511,53 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
                 m = many_of(++at), unit = 0;
             }
         }
-        at = uniform(at), unit = uniform(unit);
-        m = Many{uniform(m.past), uniform(m.count), uniform(m.start), uniform(m.groups)};
-        const uint32_t unit_begin = head * head_line + uniform(before), unit_end = unit_begin + length_of(m, unit);
-        const uint32_t from = parts.at(unit_begin), pieces = parts.at(unit_end - 1) - from + 1, piece = part - from;
-        const uint32_t kept = 2 * part + (piece == 0), counter = 2 * from + 1;
-        const uint32_t begin = max(parts.begin(part), unit_begin), until = min(end, unit_end);
+        unit = uniform(unit);
+        m = Many{uniform(m.at), uniform(m.past), uniform(m.count), uniform(m.start), uniform(m.groups)};
+        Unit u{m, head, unit, head * head_line + uniform(before), 0, 0, 0};
+        u.end = u.begin + length_of(m, unit);
+        u.first = parts.at(u.begin), u.pieces = parts.at(u.end - 1) - u.first + 1;
+        return u;
+    }
+    // Where piece p of a unit is kept: a part has at most the end of one unit and the begin of another.
+    __device__ __forceinline__ static uint64_t kept_of(const Unit& u, uint32_t p) { return kept_at(u.first, p); }
+};
+
+template <uint32_t F, uint32_t NB>
+__global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAttention a) {
+    constexpr uint32_t kRows = RowsShape<F, NB>::kRows, T = 64 * row_waves(NB);
+    __shared__ RowsSpace<F, NB> space;
+    __shared__ uint32_t kept_pages[kKeptPages], missing;
+    // neighbours on the line on one XCD
+    const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+    if (threadIdx.x == 0) a.joins[part].pieces = 0;
+    if (!many_rows(a)) return;
+    const ManyLine<kRows> line(a);
+    if (part >= line.count) return;
+    uint32_t place = line.parts.begin(part);
+    const uint32_t end = line.parts.begin(part + 1);
+
+    Attention b{};
+    b.queries = a.queries, b.output = a.output;
+    b.query_stride = a.query_stride, b.output_stride = a.output_stride;
+    b.tokens = 1, b.group = a.group, b.window = a.window, b.scale = a.scale, b.splits = 1;
+    NoTree tree{};
+
+    while (place < end) {
+        const auto u = line.unit_at(place);
+        const uint32_t begin = max(line.parts.begin(part), u.begin), until = min(end, u.end);
         place = until;
 
         Group group;
-        group.sequence = m.start, group.head = head, group.past = m.past, group.latest = m.past + m.count;
-        group.row0 = unit * kRows, group.row_end = min(group.row0 + kRows, m.count * a.group);
+        group.sequence = u.m.start, group.head = u.head, group.past = u.m.past, group.latest = u.m.past + u.m.count;
+        group.row0 = u.unit * kRows, group.row_end = min(group.row0 + kRows, u.m.count * a.group);
         group.token0 = group.row0 / a.group, group.token_end = (group.row_end - 1) / a.group + 1;
         group.all_begin = a.window && group.latest > a.window ? group.latest - a.window : 0u;
-        group.tile_begin = begin_of(m, unit) + max(begin - unit_begin, kManyUnitTiles) - kManyUnitTiles;
-        group.tile_end = begin_of(m, unit) + max(until - unit_begin, kManyUnitTiles) - kManyUnitTiles;
+        group.tile_begin = line.begin_of(u.m, u.unit) + max(begin - u.begin, kManyUnitTiles) - kManyUnitTiles;
+        group.tile_end = line.begin_of(u.m, u.unit) + max(until - u.begin, kManyUnitTiles) - kManyUnitTiles;
 
         // The piece's pages, and whether one is none of the pool's.
-        PagedRecords records{a.pool.base, a.table + uint64_t{at} * a.table_stride, kept_pages, 0, cache_record(F, NB),
-                             a.pool.capacity / kTile, a.page_inverse, a.pool.kv_heads, head, a.pool.sequences};
+        PagedRecords records{a.pool.base, a.table + uint64_t{u.m.at} * a.table_stride, kept_pages, 0, cache_record(F, NB),
+                             a.pool.capacity / kTile, a.page_inverse, a.pool.kv_heads, u.head, a.pool.sequences};
         records.first = records.place_of(group.tile_begin);
         const uint32_t places = group.tile_begin < group.tile_end ? records.place_of(group.tile_end - 1) - records.first + 1 : 0;
         if (threadIdx.x == 0) missing = 0;
@@ -511,40 +570,68 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
         }
         if (gone) missing = 1;
         __syncthreads();
+        // (the part's one unit that goes on past it)
+        if (threadIdx.x == 0 && u.pieces > 1 && u.first == part)
+            a.joins[part] = {u.m.start, u.head, group.row0, group.row_end - group.row0, u.pieces, 0};
+        const uint64_t kept = line.kept_of(u, part - u.first) * kRows;
         auto write = [&](uint32_t row, bool live, uint32_t value, float4_t out, float total, float least, bool stats) {
-            if (pieces == 1) {
+            if (u.pieces == 1) {
                 finish<NB>(b, group, row, live, value, out, total, least, false);
                 return;
             }
             const bool empty = !live || (least == INFINITY && total == 0.0f);
-            const uint64_t to = uint64_t{kept} * kRows + (row - group.row0);
-            put(a.partial + to * (32 * NB) + value, empty ? float4_t(0.0f) : out);
-            if (stats) put(a.stats + to, make_float2(empty ? INFINITY : total != total ? total : least, empty ? 0.0f : total));
+            const uint64_t to = kept + (row - group.row0);
+            *reinterpret_cast<float4_t*>(a.partial + to * (32 * NB) + value) = empty ? float4_t(0.0f) : out;
+            if (stats) a.stats[to] = make_float2(empty ? INFINITY : total != total ? total : least, empty ? 0.0f : total);
         };
         attend_group<F, NB>(b, group, tree, space, records, write, uniform(missing) != 0);
-        wait_loads<0>();
-        __syncthreads();  // the LDS is read, and what was written has arrived
-        if (pieces == 1) continue;
-        if (threadIdx.x == 0) last_piece = atomicInc(a.counters + counter, pieces - 1) == pieces - 1;
-        __syncthreads();
-        if (!last_piece) continue;
-        join_pieces<NB, T>(
-            a, kRows, group.row_end - group.row0, pieces, [&](uint32_t p) { return 2 * (from + p) + (p == 0); },
-            [&](uint32_t row, uint32_t value) {
-                const uint32_t of = group.row0 + row;
-                return a.output + (uint64_t{m.start} + of / a.group) * a.output_stride +
-                       (uint64_t{head} * a.group + of % a.group) * (32 * NB) + value;
-            },
-            reinterpret_cast<uint8_t*>(&space));
-        __syncthreads();
+        __syncthreads();  // the LDS is read
+    }
+}
+
+// The units in pieces joined, in a launch of its own: a workgroup 16 rows of the unit
+// that begins in a part and goes on past it.
+template <uint32_t NB, uint32_t ROWS>
+__global__ __launch_bounds__(256) void join_page_rows(PagedAttention a) {
+    constexpr uint32_t kMine = 16, kShares = ROWS / kMine, kQuads = 8 * NB;
+    const uint32_t part = blockIdx.x / kShares, row0 = blockIdx.x % kShares * kMine;
+    const PagedJoin u = a.joins[part];
+    for (uint32_t i = threadIdx.x; u.pieces > 1 && i < kMine * kQuads; i += 256) {
+        const uint32_t row = row0 + i / kQuads, value = i % kQuads * 4;
+        if (row >= u.rows) break;
+        float least = INFINITY, total = 0.0f;
+        float4_t out = float4_t(0.0f);
+        constexpr uint32_t kBatch = 8;  // on their way together
+        for (uint32_t p0 = 0; p0 < u.pieces; p0 += kBatch) {
+            float2 side[kBatch];
+            float4_t theirs[kBatch];
+#pragma unroll
+            for (uint32_t x = 0; x < kBatch; ++x) {
+                side[x] = make_float2(INFINITY, 0.0f), theirs[x] = float4_t(0.0f);
+                if (p0 + x >= u.pieces) continue;
+                const uint64_t from = kept_at(part, p0 + x) * ROWS + row;
+                side[x] = a.stats[from];
+                theirs[x] = *reinterpret_cast<const float4_t*>(a.partial + from * (32 * NB) + value);
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < kBatch; ++x) join(side[x], theirs[x], least, total, out);
+        }
+        const uint32_t of = u.row0 + row;
+        float* to = a.output + (uint64_t{u.start} + of / a.group) * a.output_stride +
+                    (uint64_t{u.head} * a.group + of % a.group) * (32 * NB) + value;
+        *reinterpret_cast<float4_t*>(to) = least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
     }
 }
 
 template <uint32_t F, uint32_t NB>
 static hipError_t launch_paged_blocks(const PagedAttention& a, uint32_t octets, hipStream_t stream) {
     if (octets == 0) {
-        if constexpr (many_rows_of(F, 32 * NB))
+        if constexpr (many_rows_of(F, 32 * NB)) {
             hipLaunchKernelGGL((attend_page_rows<F, NB>), dim3(a.parts), dim3(64 * row_waves(NB)), 0, stream, a);
+            if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            constexpr uint32_t kRows = RowsShape<F, NB>::kRows;
+            hipLaunchKernelGGL((join_page_rows<NB, kRows>), dim3(a.parts * (kRows / 16)), dim3(256), 0, stream, a);
+        }
     } else if (octets == 2)
         hipLaunchKernelGGL((attend_pages<F, NB, 2>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
     else

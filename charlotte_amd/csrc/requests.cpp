@@ -109,16 +109,23 @@ void check_table(uint32_t requests, uint32_t table_stride, uint32_t page_tokens)
         refuse("table stride " + std::to_string(table_stride));
 }
 
-// How a step of attention runs: the rows of a unit of attend_pages, in 16s; the
-// rows of one of attend_page_rows, 0 where that does not run.
+// How a step of attention runs: requests of up to 16 rows of a key head by units of
+// 16, of more by units of 32, of kManyRows and more, where they are load enough, by
+// units of `many`; each in launches of its own. One request, which is of one kind,
+// and groups past 16 have no launch of units of 16.
 struct PagedPlan {
-    uint32_t octets, many;
+    bool ones, twos;
+    uint32_t many, many_load;  // 0: none
 };
-PagedPlan paged_plan(const chm::CacheShape& c, uint32_t group, uint32_t most) {
-    // (what many rows bring has its own kernel: the others are mostly single tokens')
-    if (uint64_t{group} * most >= chm::kManyRows && chm::many_rows_of(c.format, c.head_dim))
-        return {chm::paged_octets(group, 1), c.head_dim <= 128 ? 256u : 128u};
-    return {chm::paged_octets(group, most), 0};
+PagedPlan paged_plan(const chm::CacheShape& c, uint32_t group, uint32_t most, uint32_t requests, uint64_t most_load) {
+    const uint64_t rows = uint64_t{group} * std::max(most, 1u);
+    if (rows <= 16) return {true, false, 0, 0};
+    PagedPlan plan{requests > 1 && group <= 16, true, 0, 0};
+    // the loads at which attention takes its form of many rows (attention_plan.cpp)
+    const uint32_t load = c.head_dim <= 64 ? 112 : c.head_dim <= 128 ? 44 : 11;
+    if (rows >= chm::kManyRows && chm::many_rows_of(c.format, c.head_dim) && most_load >= load)
+        plan.many = c.head_dim <= 128 ? 256 : 128, plan.many_load = load;
+    return plan;
 }
 
 // Pieces' places, outputs and then offsets and sums, of units of `rows` rows.
@@ -126,7 +133,8 @@ uint64_t piece_rows(const charlotte_hip_matmul_context* ctx, uint32_t rows) {
     return uint64_t{ctx->compute_units} * chm::kPieces * rows;
 }
 uint64_t piece_bytes(const charlotte_hip_matmul_context* ctx, const chm::CacheShape& c, const PagedPlan& plan) {
-    return piece_rows(ctx, std::max(16 * plan.octets, plan.many)) * (uint64_t{c.head_dim} * 4 + 8);
+    return piece_rows(ctx, std::max(plan.twos ? 32u : 16u, plan.many)) * (uint64_t{c.head_dim} * 4 + 8) +
+           (plan.many ? ctx->compute_units * sizeof(chm::PagedJoin) : 0);
 }
 
 // An output that is an input's memory has its stride.
@@ -237,10 +245,7 @@ uint64_t charlotte_hip_matmul_paged_attention_workspace_bytes(const charlotte_hi
                                                               const charlotte_hip_matmul_page_pool* pool,
                                                               uint32_t query_heads, uint32_t most) {
     if (!ctx || !pool || query_heads == 0 || query_heads % pool->shape.kv_heads != 0) return 0;
-    // a smaller step may have units of 32 rows where this one has them of 16
-    const uint32_t group = query_heads / pool->shape.kv_heads;
-    return std::max(piece_bytes(ctx, pool->shape, paged_plan(pool->shape, group, most)),
-                    piece_bytes(ctx, pool->shape, {chm::paged_octets(group, most), 0}));
+    return piece_bytes(ctx, pool->shape, paged_plan(pool->shape, query_heads / pool->shape.kv_heads, most, 2, UINT64_MAX));
 }
 
 charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_matmul_context* ctx,
@@ -256,9 +261,12 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         if (d.query_heads == 0 || d.query_heads % c.kv_heads != 0)
             refuse("query heads " + std::to_string(d.query_heads) + " over " + std::to_string(c.kv_heads) + " key heads");
         const uint32_t group = d.query_heads / c.kv_heads;
-        const PagedPlan plan = paged_plan(c, group, d.most);
+        // 32 rows by a tile, for each compute unit, if every row were to see the longest request
+        const uint64_t reach = uint64_t{d.table_stride} * c.capacity, longest = d.longest ? std::min<uint64_t>(d.longest, reach) : reach;
+        const uint64_t load = (uint64_t{d.rows} * group + 31) / 32 * c.kv_heads * ((longest + 31) / 32) / ctx->compute_units;
+        const PagedPlan plan = paged_plan(c, group, d.most, d.requests, load);
         // all units, each of all the tiles that a table's row holds
-        const uint64_t units = (uint64_t{d.rows} * group / (16 * plan.octets) + d.requests) * c.kv_heads;
+        const uint64_t units = (uint64_t{d.rows} * group / (plan.twos ? 32 : 16) + d.requests) * c.kv_heads;
         if (uint64_t{d.rows} * group >= (1ull << 28) || units * (uint64_t{d.table_stride} * (c.capacity / 32) + 16) >= (1ull << 32))
             refuse("too many rows a step for tables so long");
         if (!std::isfinite(d.scale)) refuse("scale not finite");
@@ -288,15 +296,22 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
         if (hipError_t e = hipSetDevice(ctx->device); e != hipSuccess) return e;
         auto run = [&](uint32_t rows, uint32_t octets) {
             a.stats = reinterpret_cast<float2*>(a.partial + piece_rows(ctx, rows) * c.head_dim);
+            a.joins = reinterpret_cast<chm::PagedJoin*>(a.stats + piece_rows(ctx, rows));
             const auto s = static_cast<hipStream_t>(stream);
             return c.format == chm::kF16    ? chm::launch_paged_f16(a, octets, s)
                    : c.format == chm::kQ4_0 ? chm::launch_paged_q4_0(a, octets, s)
                                             : chm::launch_paged_q8_0(a, octets, s);
         };
-        a.few = plan.many ? chm::kManyRows - 1 : 0xFFFFFFFFu;
+        a.many_load = plan.many_load;
+        a.above = 0, a.upto = 0xFFFFFFFFu;
         if (plan.many)
             if (hipError_t e = run(plan.many, 0); e != hipSuccess) return e;
-        return run(16 * plan.octets, plan.octets);
+        if (plan.twos) {
+            a.above = plan.ones ? 16 : 0;
+            if (hipError_t e = run(32, 2); e != hipSuccess || !plan.ones) return e;
+        }
+        a.above = 0, a.upto = plan.twos ? 16 : 0xFFFFFFFFu;
+        return run(16, 1);
     });
 }
 

@@ -35,6 +35,11 @@ hipError_t launch_page_read(const CacheRows& a, hipStream_t stream);
 
 // ---- paged attention (paged.hpp, paged_*.hip) ----
 
+// A unit of many rows in pieces, of which the first is a part's.
+struct PagedJoin {
+    uint32_t start, head, row0, rows, pieces, reserved;
+};
+
 struct PagedAttention {
     CacheShape pool;
     const float* queries;
@@ -46,22 +51,24 @@ struct PagedAttention {
     const uint32_t* table;
     float* partial;      // a piece's outputs, [piece][row][head_dim]
     float2* stats;       // its rows' offsets and sums, [piece][row]
+    PagedJoin* joins;    // many rows: a part's unit in pieces
     uint32_t* counters;  // pieces of a unit that are done; 0 between launches
     uint32_t requests, rows, table_stride, group, window, parts;
-    uint32_t few;           // the most rows of a key head that a request of attend_pages has; the others are attend_page_rows'
+    // attend_pages has the requests of more rows of a key head than `above`, up to
+    // `upto`; but those of kManyRows and more are attend_page_rows' where their load
+    // is many_load and more (0: never).
+    uint32_t above, upto, many_load;
     uint32_t page_inverse;  // of a page's tiles, where they are two and more: 2^32 over them, rounded up
     float scale;
 };
 
 // Pieces of units that a step may leave, a workgroup.
 constexpr uint32_t kPieces = 2;
-// Rows a workgroup: 16, or 32 where requests bring more.
-inline uint32_t paged_octets(uint32_t group, uint32_t most) { return uint64_t{group} * most > 16 ? 2 : 1; }
 // Rows of a key head from which a request has workgroups of many rows, in the
 // formats and widths that attention has them for (attention_plan.cpp).
 constexpr uint32_t kManyRows = 256;
 constexpr bool many_rows_of(uint32_t format, uint32_t head_dim) { return format == 1 /* F16 */ || head_dim <= 128; }
-// `octets`: 1 or 2 of attend_pages; 0: attend_page_rows.
+// `octets`: 1 or 2 of attend_pages; 0: attend_page_rows, and what joins its pieces.
 hipError_t launch_paged_f16(const PagedAttention& a, uint32_t octets, hipStream_t stream);
 hipError_t launch_paged_q4_0(const PagedAttention& a, uint32_t octets, hipStream_t stream);
 hipError_t launch_paged_q8_0(const PagedAttention& a, uint32_t octets, hipStream_t stream);

@@ -252,7 +252,7 @@ class _PagedAttentionDesc(ctypes.Structure):
                 ("query_heads", ctypes.c_uint32), ("window", ctypes.c_uint32), ("scale", ctypes.c_float),
                 ("requests", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("most", ctypes.c_uint32),
                 ("past", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("starts", ctypes.c_void_p),
-                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32), ("longest", ctypes.c_uint32),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 

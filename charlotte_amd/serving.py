@@ -356,12 +356,14 @@ class PagedAttention(_Call):
     output_stride: int = 0
     workspace: int = 0
     workspace_bytes: int = 0
+    longest: int = 0
     _desc: Optional[_PagedAttentionDesc] = field(default=None, repr=False)
 
     def desc(self):
         return _PagedAttentionDesc(self.pool.handle, self.queries, self.output, self.query_stride, self.output_stride,
                                    self.query_heads, self.window, self.scale, self.requests, self.rows, self.most,
-                                   self.past, self.counts, self.starts, self.table, self.table_stride, 0, self.workspace,
+                                   self.past, self.counts, self.starts, self.table, self.table_stride, self.longest,
+                                   self.workspace,
                                    self.workspace_bytes)
 
 

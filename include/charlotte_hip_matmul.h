@@ -787,7 +787,8 @@ typedef struct {
     const uint32_t* starts;
     const uint32_t* table;    /* device: requests rows of table_stride */
     uint32_t table_stride;    /* at least 1; table_stride * page_tokens below 2^31 */
-    uint32_t reserved;        /* 0 */
+    /* The most past + counts of a request, likewise for the choice alone (0: what a table's row holds). */
+    uint32_t longest;
     void* workspace;          /* device, 16-byte aligned: paged_attention_workspace_bytes */
     uint64_t workspace_bytes;
 } charlotte_hip_matmul_paged_attention_desc;
