@@ -1006,11 +1006,11 @@ __device__ __forceinline__ void write_rows(const Group& group, Rows<F, NB, X>& r
 }
 
 // A sequence's records, one after the other: record t.
+template <uint32_t BYTES>
 struct Records {
     static constexpr bool kGaps = false;  // none is missing
     const uint8_t* base;
-    uint32_t bytes;
-    __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const { return base + static_cast<uint64_t>(t) * bytes; }
+    __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const { return base + static_cast<uint64_t>(t) * BYTES; }
 };
 
 // A wave's 32 rows by themselves, straight from the records, 16 at a time.
@@ -1052,8 +1052,8 @@ struct RowsSpace {
 
 // A workgroup's rows over its split's tiles; `alone`: some record is missing.
 template <uint32_t F, uint32_t NB, typename TREE, typename RECORDS, typename WRITE>
-__device__ __forceinline__ void attend_group(const Attention& a, const Group& group, TREE& tree, RowsSpace<F, NB>& space,
-                                             const RECORDS& records, const WRITE& write, bool alone) {
+__device__ __forceinline__ void attend_group(Attention a, Group group, TREE& tree, RowsSpace<F, NB>& space,
+                                             RECORDS records, WRITE write, bool alone) {
     using Shape = RowsShape<F, NB>;
     constexpr uint32_t W = Shape::W, kUnit = cache_unit(F), kTiles = Shape::kTiles;
     constexpr uint32_t kUnits = 2 * NB * kTiles, kMine = (kUnits + W - 1) / W;  // units of a stage; a wave's, at most
@@ -1246,7 +1246,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_rows(Attention a) {
     __shared__ Tree<kRows < kTreeTokens ? kRows : kTreeTokens> tree;
     __shared__ RowsSpace<F, NB> space;
     const Group group(a, kRows);
-    const Records records{record_of(a.cache, F, group.sequence, group.head, 0), cache_record(F, NB)};
+    const Records<cache_record(F, NB)> records{record_of(a.cache, F, group.sequence, group.head, 0)};
     auto write = [&](uint32_t row, bool live, uint32_t at, float4_t out, float total, float least, bool stats) {
         finish<NB>(a, group, row, live, at, out, total, least, stats);
     };

@@ -420,8 +420,8 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
 // ---- requests of many rows -----------------------------------------------------
 
-// What a unit of many rows costs beside its tiles, and the least tiles of a part.
-constexpr uint32_t kManyUnitTiles = 2, kManyPartTiles = 8;
+// What a unit of many rows costs beside its tiles, and the least tiles of a part or a piece.
+constexpr uint32_t kManyUnitTiles = 2, kManyPartTiles = 8, kManyPieceTiles = 4;
 // Pages of a piece whose table is kept in LDS; what is past them is read where it is.
 constexpr uint32_t kKeptPages = 1024;
 
@@ -448,11 +448,14 @@ __device__ __forceinline__ uint64_t kept_at(uint32_t first, uint32_t p) { return
 struct Many {
     uint32_t at, past, count, start, groups;
 };
-// Their units on a line, each as long as the tiles that its rows see and kManyUnitTiles.
+// Their units on a line, each as long as the tiles that its rows see and
+// kManyUnitTiles; or, where as many pieces of equal length as there are workgroups
+// hold all of them, as long as its pieces, a part each.
 template <uint32_t ROWS>
 struct ManyLine {
     const PagedAttention& a;
     uint32_t share, line_before, head_line, count;
+    uint32_t piece_tiles;  // 0: by tiles
     Parts parts;
 
     __device__ __forceinline__ Many many_of(uint32_t i) const {
@@ -466,18 +469,50 @@ struct ManyLine {
         const uint32_t place = m.past + unit * ROWS / a.group + 1;
         return a.window && place > a.window ? (place - a.window) / kTile : 0u;
     }
-    __device__ __forceinline__ uint32_t length_of(const Many& m, uint32_t unit) const {
+    __device__ __forceinline__ uint32_t tiles_of(const Many& m, uint32_t unit) const {
         const uint32_t rows = min((unit + 1) * ROWS, m.count * a.group);
-        return (m.past + (rows - 1) / a.group + kTile) / kTile - begin_of(m, unit) + kManyUnitTiles;
+        return (m.past + (rows - 1) / a.group + kTile) / kTile - begin_of(m, unit);
     }
-    // Laid out by each wave; no parts where there is nothing, or too much.
-    __device__ __forceinline__ explicit ManyLine(const PagedAttention& a_) : a(a_), share((a_.requests + 63) / 64), count(0) {
-        const uint32_t lane = threadIdx.x & 63u, first = lane * share;
-        uint32_t line = 0;
+    __device__ __forceinline__ uint32_t length_of(const Many& m, uint32_t unit) const {
+        const uint32_t tiles = tiles_of(m, unit);
+        return piece_tiles ? (tiles + piece_tiles - 1) / piece_tiles : tiles + kManyUnitTiles;
+    }
+    // All units of the lane's requests, summed up.
+    template <typename FN>
+    __device__ __forceinline__ uint32_t sum_units(FN f) const {
+        const uint32_t first = (threadIdx.x & 63u) * share;
+        uint32_t sum = 0;
         for (uint32_t i = first; i < min(first + share, a.requests); ++i) {
             const Many m = many_of(i);
-            for (uint32_t g = 0; g < m.groups; ++g) line = plus(line, length_of(m, g));
+            for (uint32_t g = 0; g < m.groups; ++g) sum = plus(sum, f(m, g));
         }
+        return sum;
+    }
+    __device__ __forceinline__ static uint32_t of_wave(uint32_t sum) {
+#pragma unroll
+        for (uint32_t o = 32; o > 0; o >>= 1) sum = plus(sum, __shfl_xor(sum, o));
+        return uniform(sum);
+    }
+    // Piece `part` of a unit that is in pieces, or its part of the line: tiles of the unit's.
+    template <typename UNIT>
+    __device__ __forceinline__ void tiles_at(const UNIT& u, uint32_t part, uint32_t* from, uint32_t* to) const {
+        if (piece_tiles) {
+            const uint32_t tiles = tiles_of(u.m, u.unit), piece = part - u.first, each = tiles / u.pieces, more = tiles % u.pieces;
+            *from = piece * each + min(piece, more), *to = *from + each + (piece < more);
+        } else {
+            *from = max(max(parts.begin(part), u.begin) - u.begin, kManyUnitTiles) - kManyUnitTiles;
+            *to = max(min(parts.begin(part + 1), u.end) - u.begin, kManyUnitTiles) - kManyUnitTiles;
+        }
+    }
+    // Laid out by each wave; no parts where there is nothing, or too much.
+    __device__ __forceinline__ explicit ManyLine(const PagedAttention& a_) : a(a_), share((a_.requests + 63) / 64), count(0), piece_tiles(0) {
+        const uint32_t lane = threadIdx.x & 63u;
+        const uint32_t all = times(of_wave(sum_units([&](const Many& m, uint32_t g) { return tiles_of(m, g); })), a.pool.kv_heads);
+        if (all == kTooMuch || all == 0) return;
+        const uint32_t even = max((all + a.parts - 1) / a.parts, kManyPieceTiles);
+        const uint32_t pieces = of_wave(sum_units([&](const Many& m, uint32_t g) { return (tiles_of(m, g) + even - 1) / even; }));
+        if (times(pieces, a.pool.kv_heads) <= a.parts) piece_tiles = even;
+        const uint32_t line = sum_units([&](const Many& m, uint32_t g) { return length_of(m, g); });
         line_before = line;
 #pragma unroll
         for (uint32_t o = 1; o < 64; o <<= 1) {
@@ -488,7 +523,7 @@ struct ManyLine {
         line_before -= line;
         const uint32_t length = times(head_line, a.pool.kv_heads);
         if (length == kTooMuch || length == 0) return;
-        count = min(a.parts, max(length / kManyPartTiles, 1u));
+        count = piece_tiles ? length : min(a.parts, max(length / kManyPartTiles, 1u));
         parts = {length / count, length % count};
     }
     // The unit at a place: of those of the last lane whose line does not begin past it.
@@ -544,16 +579,15 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
 
     while (place < end) {
         const auto u = line.unit_at(place);
-        const uint32_t begin = max(line.parts.begin(part), u.begin), until = min(end, u.end);
-        place = until;
+        place = min(end, u.end);
 
         Group group;
         group.sequence = u.m.start, group.head = u.head, group.past = u.m.past, group.latest = u.m.past + u.m.count;
         group.row0 = u.unit * kRows, group.row_end = min(group.row0 + kRows, u.m.count * a.group);
         group.token0 = group.row0 / a.group, group.token_end = (group.row_end - 1) / a.group + 1;
         group.all_begin = a.window && group.latest > a.window ? group.latest - a.window : 0u;
-        group.tile_begin = line.begin_of(u.m, u.unit) + max(begin - u.begin, kManyUnitTiles) - kManyUnitTiles;
-        group.tile_end = line.begin_of(u.m, u.unit) + max(until - u.begin, kManyUnitTiles) - kManyUnitTiles;
+        line.tiles_at(u, part, &group.tile_begin, &group.tile_end);
+        group.tile_begin += line.begin_of(u.m, u.unit), group.tile_end += line.begin_of(u.m, u.unit);
 
         // The piece's pages, and whether one is none of the pool's.
         PagedRecords records{a.pool.base, a.table + uint64_t{u.m.at} * a.table_stride, kept_pages, 0, cache_record(F, NB),
