@@ -1011,6 +1011,7 @@ struct Records {
     static constexpr bool kGaps = false;  // none is missing
     const uint8_t* base;
     __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const { return base + static_cast<uint64_t>(t) * BYTES; }
+    __device__ __forceinline__ const uint8_t* of_wave(uint32_t t) const { return (*this)(t); }  // a t that is the wave's
 };
 
 // A wave's 32 rows by themselves, straight from the records, 16 at a time.
@@ -1128,7 +1129,7 @@ __device__ __forceinline__ void attend_group(Attention a, Group group, TREE& tre
         for (uint32_t j = 0; j < kMine; ++j) {
             const uint32_t u = wave + W * j, t = tile0 + u / (2 * NB);
             if (u >= kUnits || t >= group.tile_end) continue;
-            const uint8_t* record = records(t);
+            const uint8_t* record = records.of_wave(t);
             const uint8_t* unit = record + u % (2 * NB) * kUnit;
             if constexpr (F == kQ4_0) {
                 const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * lane);
@@ -1142,7 +1143,8 @@ __device__ __forceinline__ void attend_group(Attention a, Group group, TREE& tre
         }
         const uint32_t t = tile0 + threadIdx.x / kScaleWords;
         if (threadIdx.x < kScaleWords * kTiles && t < group.tile_end)
-            scale_word = reinterpret_cast<const uint32_t*>(records(t) + key_scales_at(F, NB))[threadIdx.x % kScaleWords];
+            scale_word = reinterpret_cast<const uint32_t*>((kScaleWords % 64 ? records(t) : records.of_wave(t)) +
+                                                           key_scales_at(F, NB))[threadIdx.x % kScaleWords];
     };
     auto lay = [&](uint32_t tile0, Stage<F, NB>* stage) {
         const uint32_t quarter = lane >> 4, column = lane & 15u;

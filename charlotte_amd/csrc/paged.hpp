@@ -420,24 +420,36 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
 // ---- requests of many rows -----------------------------------------------------
 
-// What a unit of many rows costs beside its tiles, and the least tiles of a part or a piece.
-constexpr uint32_t kManyUnitTiles = 2, kManyPartTiles = 8, kManyPieceTiles = 4;
-// Pages of a piece whose table is kept in LDS; what is past them is read where it is.
-constexpr uint32_t kKeptPages = 1024;
+// What a unit of many rows costs beside its tiles, and the least tiles of a part.
+constexpr uint32_t kManyUnitTiles = 4, kManyPartTiles = 8;
+// Tiles of a piece whose records' places are kept in LDS; past them they are found anew.
+constexpr uint32_t kKeptTiles = 1024;
 
-// A request's records through its pages; null where the page is none of the pool's.
+// Where a request's tile is in its pool; kNoRecord where its page is none of the pool's.
+constexpr uint64_t kNoRecord = ~0ull;
+struct PagePlaces {
+    const uint32_t* table;  // the request's row
+    uint32_t tiles_a_page, page_inverse, kv_heads, head, pages, record;
+    __device__ __forceinline__ uint64_t operator()(uint32_t t) const {
+        const uint32_t place = tiles_a_page == 1 ? t : __umulhi(t, page_inverse), page = table[place];
+        return page < pages ? ((uint64_t{page} * kv_heads + head) * tiles_a_page + (t - place * tiles_a_page)) * record : kNoRecord;
+    }
+};
+// A piece's records, from its tile `first` on.
 struct PagedRecords {
     static constexpr bool kGaps = true;
     const uint8_t* base;
-    const uint32_t* table;  // the request's row
-    const uint32_t* kept;   // LDS: its pages from `first` on
-    uint32_t first, record, tiles_a_page, page_inverse, kv_heads, head, pages;
-
-    __device__ __forceinline__ uint32_t place_of(uint32_t t) const { return tiles_a_page == 1 ? t : __umulhi(t, page_inverse); }
+    const uint64_t* kept;  // LDS
+    const PagePlaces* far; // LDS
+    uint32_t first;
     __device__ __forceinline__ const uint8_t* operator()(uint32_t t) const {
-        const uint32_t place = place_of(t), page = place - first < kKeptPages ? kept[place - first] : table[place];
-        if (page >= pages) return nullptr;
-        return base + ((uint64_t{page} * kv_heads + head) * tiles_a_page + (t - place * tiles_a_page)) * record;
+        const uint64_t at = __builtin_expect(t - first < kKeptTiles, true) ? kept[t - first] : (*far)(t);
+        return at != kNoRecord ? base + at : nullptr;
+    }
+    // The wave's t, of a unit that misses no page: an address that is the same in every lane.
+    __device__ __forceinline__ const uint8_t* of_wave(uint32_t t) const {
+        const uint64_t at = __builtin_expect(t - first < kKeptTiles, true) ? kept[t - first] : (*far)(t);
+        return base + (uint64_t{uniform(static_cast<uint32_t>(at >> 32))} << 32 | uniform(static_cast<uint32_t>(at)));
     }
 };
 
@@ -448,14 +460,11 @@ __device__ __forceinline__ uint64_t kept_at(uint32_t first, uint32_t p) { return
 struct Many {
     uint32_t at, past, count, start, groups;
 };
-// Their units on a line, each as long as the tiles that its rows see and
-// kManyUnitTiles; or, where as many pieces of equal length as there are workgroups
-// hold all of them, as long as its pieces, a part each.
+// Their units on a line, each as long as the tiles that its rows see and kManyUnitTiles.
 template <uint32_t ROWS>
 struct ManyLine {
     const PagedAttention& a;
     uint32_t share, line_before, head_line, count;
-    uint32_t piece_tiles;  // 0: by tiles
     Parts parts;
 
     __device__ __forceinline__ Many many_of(uint32_t i) const {
@@ -474,8 +483,7 @@ struct ManyLine {
         return (m.past + (rows - 1) / a.group + kTile) / kTile - begin_of(m, unit);
     }
     __device__ __forceinline__ uint32_t length_of(const Many& m, uint32_t unit) const {
-        const uint32_t tiles = tiles_of(m, unit);
-        return piece_tiles ? (tiles + piece_tiles - 1) / piece_tiles : tiles + kManyUnitTiles;
+        return tiles_of(m, unit) + kManyUnitTiles;
     }
     // All units of the lane's requests, summed up.
     template <typename FN>
@@ -488,30 +496,15 @@ struct ManyLine {
         }
         return sum;
     }
-    __device__ __forceinline__ static uint32_t of_wave(uint32_t sum) {
-#pragma unroll
-        for (uint32_t o = 32; o > 0; o >>= 1) sum = plus(sum, __shfl_xor(sum, o));
-        return uniform(sum);
-    }
-    // Piece `part` of a unit that is in pieces, or its part of the line: tiles of the unit's.
+    // A part's tiles of a unit: of the unit's.
     template <typename UNIT>
     __device__ __forceinline__ void tiles_at(const UNIT& u, uint32_t part, uint32_t* from, uint32_t* to) const {
-        if (piece_tiles) {
-            const uint32_t tiles = tiles_of(u.m, u.unit), piece = part - u.first, each = tiles / u.pieces, more = tiles % u.pieces;
-            *from = piece * each + min(piece, more), *to = *from + each + (piece < more);
-        } else {
-            *from = max(max(parts.begin(part), u.begin) - u.begin, kManyUnitTiles) - kManyUnitTiles;
-            *to = max(min(parts.begin(part + 1), u.end) - u.begin, kManyUnitTiles) - kManyUnitTiles;
-        }
+        *from = max(max(parts.begin(part), u.begin) - u.begin, kManyUnitTiles) - kManyUnitTiles;
+        *to = max(min(parts.begin(part + 1), u.end) - u.begin, kManyUnitTiles) - kManyUnitTiles;
     }
     // Laid out by each wave; no parts where there is nothing, or too much.
-    __device__ __forceinline__ explicit ManyLine(const PagedAttention& a_) : a(a_), share((a_.requests + 63) / 64), count(0), piece_tiles(0) {
+    __device__ __forceinline__ explicit ManyLine(const PagedAttention& a_) : a(a_), share((a_.requests + 63) / 64), count(0) {
         const uint32_t lane = threadIdx.x & 63u;
-        const uint32_t all = times(of_wave(sum_units([&](const Many& m, uint32_t g) { return tiles_of(m, g); })), a.pool.kv_heads);
-        if (all == kTooMuch || all == 0) return;
-        const uint32_t even = max((all + a.parts - 1) / a.parts, kManyPieceTiles);
-        const uint32_t pieces = of_wave(sum_units([&](const Many& m, uint32_t g) { return (tiles_of(m, g) + even - 1) / even; }));
-        if (times(pieces, a.pool.kv_heads) <= a.parts) piece_tiles = even;
         const uint32_t line = sum_units([&](const Many& m, uint32_t g) { return length_of(m, g); });
         line_before = line;
 #pragma unroll
@@ -523,7 +516,7 @@ struct ManyLine {
         line_before -= line;
         const uint32_t length = times(head_line, a.pool.kv_heads);
         if (length == kTooMuch || length == 0) return;
-        count = piece_tiles ? length : min(a.parts, max(length / kManyPartTiles, 1u));
+        count = min(a.parts, max(length / kManyPartTiles, 1u));
         parts = {length / count, length % count};
     }
     // The unit at a place: of those of the last lane whose line does not begin past it.
@@ -561,13 +554,17 @@ template <uint32_t F, uint32_t NB>
 __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAttention a) {
     constexpr uint32_t kRows = RowsShape<F, NB>::kRows, T = 64 * row_waves(NB);
     __shared__ RowsSpace<F, NB> space;
-    __shared__ uint32_t kept_pages[kKeptPages], missing;
+    __shared__ uint64_t kept_places[kKeptTiles];
+    __shared__ PagePlaces far;
+    __shared__ uint32_t missing, line_before[64];
     // neighbours on the line on one XCD
     const uint32_t part = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
     if (threadIdx.x == 0) a.joins[part].pieces = 0;
     if (!many_rows(a)) return;
-    const ManyLine<kRows> line(a);
+    ManyLine<kRows> line(a);
     if (part >= line.count) return;
+    if (threadIdx.x < 64) line_before[threadIdx.x] = line.line_before;
+    __syncthreads();
     uint32_t place = line.parts.begin(part);
     const uint32_t end = line.parts.begin(part + 1);
 
@@ -578,6 +575,7 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
     NoTree tree{};
 
     while (place < end) {
+        line.line_before = line_before[threadIdx.x & 63u];  // no register over the tiles
         const auto u = line.unit_at(place);
         place = min(end, u.end);
 
@@ -589,21 +587,20 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
         line.tiles_at(u, part, &group.tile_begin, &group.tile_end);
         group.tile_begin += line.begin_of(u.m, u.unit), group.tile_end += line.begin_of(u.m, u.unit);
 
-        // The piece's pages, and whether one is none of the pool's.
-        PagedRecords records{a.pool.base, a.table + uint64_t{u.m.at} * a.table_stride, kept_pages, 0, cache_record(F, NB),
-                             a.pool.capacity / kTile, a.page_inverse, a.pool.kv_heads, u.head, a.pool.sequences};
-        records.first = records.place_of(group.tile_begin);
-        const uint32_t places = group.tile_begin < group.tile_end ? records.place_of(group.tile_end - 1) - records.first + 1 : 0;
-        if (threadIdx.x == 0) missing = 0;
+        // The piece's records, and whether one has a page that is none of the pool's.
+        const PagePlaces places{a.table + uint64_t{u.m.at} * a.table_stride, a.pool.capacity / kTile, a.page_inverse,
+                                a.pool.kv_heads, u.head, a.pool.sequences, cache_record(F, NB)};
+        if (threadIdx.x == 0) missing = 0, far = places;
         __syncthreads();
         bool gone = false;
-        for (uint32_t i = threadIdx.x; i < places; i += T) {
-            const uint32_t page = records.table[records.first + i];
-            if (i < kKeptPages) kept_pages[i] = page;
-            gone |= page >= a.pool.sequences;
+        for (uint32_t t = group.tile_begin + threadIdx.x; t < group.tile_end; t += T) {
+            const uint64_t at = places(t);
+            if (t - group.tile_begin < kKeptTiles) kept_places[t - group.tile_begin] = at;
+            gone |= at == kNoRecord;
         }
         if (gone) missing = 1;
         __syncthreads();
+        const PagedRecords records{a.pool.base, kept_places, &far, group.tile_begin};
         // (the part's one unit that goes on past it)
         if (threadIdx.x == 0 && u.pieces > 1 && u.first == part)
             a.joins[part] = {u.m.start, u.head, group.row0, group.row_end - group.row0, u.pieces, 0};
@@ -623,37 +620,54 @@ __global__ __launch_bounds__(64 * row_waves(NB)) void attend_page_rows(PagedAtte
     }
 }
 
-// The units in pieces joined, in a launch of its own: a workgroup 16 rows of the unit
-// that begins in a part and goes on past it.
+// The units in pieces joined, in a launch of its own, by all its threads: each finds
+// all units (that which begins in a part and goes on past it), and a thread takes
+// four values of a row of theirs at a time.
+constexpr uint32_t kJoinThreads = 256;
 template <uint32_t NB, uint32_t ROWS>
-__global__ __launch_bounds__(256) void join_page_rows(PagedAttention a) {
-    constexpr uint32_t kMine = 16, kShares = ROWS / kMine, kQuads = 8 * NB;
-    const uint32_t part = blockIdx.x / kShares, row0 = blockIdx.x % kShares * kMine;
-    const PagedJoin u = a.joins[part];
-    for (uint32_t i = threadIdx.x; u.pieces > 1 && i < kMine * kQuads; i += 256) {
-        const uint32_t row = row0 + i / kQuads, value = i % kQuads * 4;
-        if (row >= u.rows) break;
-        float least = INFINITY, total = 0.0f;
-        float4_t out = float4_t(0.0f);
-        constexpr uint32_t kBatch = 8;  // on their way together
-        for (uint32_t p0 = 0; p0 < u.pieces; p0 += kBatch) {
-            float2 side[kBatch];
-            float4_t theirs[kBatch];
-#pragma unroll
-            for (uint32_t x = 0; x < kBatch; ++x) {
-                side[x] = make_float2(INFINITY, 0.0f), theirs[x] = float4_t(0.0f);
-                if (p0 + x >= u.pieces) continue;
-                const uint64_t from = kept_at(part, p0 + x) * ROWS + row;
-                side[x] = a.stats[from];
-                theirs[x] = *reinterpret_cast<const float4_t*>(a.partial + from * (32 * NB) + value);
-            }
-#pragma unroll
-            for (uint32_t x = 0; x < kBatch; ++x) join(side[x], theirs[x], least, total, out);
+__global__ __launch_bounds__(kJoinThreads) void join_page_rows(PagedAttention a) {
+    constexpr uint32_t kQuads = 8 * NB;
+    __shared__ uint32_t unit_parts[kJoinThreads], wave_units[kJoinThreads / 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    for (uint32_t part0 = 0; part0 < a.parts; part0 += kJoinThreads) {
+        const uint32_t mine = part0 + threadIdx.x;
+        const bool in_pieces = mine < a.parts && a.joins[mine].pieces > 1;
+        const uint64_t theirs = __ballot(in_pieces);
+        if (lane == 0) wave_units[wave] = __builtin_popcountll(theirs);
+        __syncthreads();
+        uint32_t units = 0, at = 0;
+        for (uint32_t w = 0; w < kJoinThreads / 64; ++w) {
+            if (w == wave) at = units;
+            units += wave_units[w];
         }
-        const uint32_t of = u.row0 + row;
-        float* to = a.output + (uint64_t{u.start} + of / a.group) * a.output_stride +
-                    (uint64_t{u.head} * a.group + of % a.group) * (32 * NB) + value;
-        *reinterpret_cast<float4_t*>(to) = least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
+        if (in_pieces) unit_parts[at + __builtin_popcountll(theirs & ((1ull << lane) - 1))] = mine;
+        __syncthreads();
+        for (uint32_t i = blockIdx.x * kJoinThreads + threadIdx.x; i < units * ROWS * kQuads; i += gridDim.x * kJoinThreads) {
+            const uint32_t part = unit_parts[i / (ROWS * kQuads)], row = i / kQuads % ROWS, value = i % kQuads * 4;
+            const PagedJoin u = a.joins[part];
+            if (row >= u.rows) continue;
+            float least = INFINITY, total = 0.0f;
+            float4_t out = float4_t(0.0f);
+            constexpr uint32_t kBatch = 8;  // on their way together
+            for (uint32_t p0 = 0; p0 < u.pieces; p0 += kBatch) {
+                float2 side[kBatch];
+                float4_t theirs[kBatch];
+#pragma unroll
+                for (uint32_t x = 0; x < kBatch; ++x) {
+                    const uint64_t from = kept_at(part, min(p0 + x, u.pieces - 1)) * ROWS + row;
+                    side[x] = a.stats[from];
+                    theirs[x] = *reinterpret_cast<const float4_t*>(a.partial + from * (32 * NB) + value);
+                }
+#pragma unroll
+                for (uint32_t x = 0; x < kBatch; ++x)
+                    if (p0 + x < u.pieces) join(side[x], theirs[x], least, total, out);
+            }
+            const uint32_t of = u.row0 + row;
+            float* to = a.output + (uint64_t{u.start} + of / a.group) * a.output_stride +
+                        (uint64_t{u.head} * a.group + of % a.group) * (32 * NB) + value;
+            *reinterpret_cast<float4_t*>(to) = least == INFINITY ? float4_t(0.0f) : out * (1.0f / total);
+        }
+        __syncthreads();  // the list is read
     }
 }
 
@@ -664,7 +678,7 @@ static hipError_t launch_paged_blocks(const PagedAttention& a, uint32_t octets, 
             hipLaunchKernelGGL((attend_page_rows<F, NB>), dim3(a.parts), dim3(64 * row_waves(NB)), 0, stream, a);
             if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
             constexpr uint32_t kRows = RowsShape<F, NB>::kRows;
-            hipLaunchKernelGGL((join_page_rows<NB, kRows>), dim3(a.parts * (kRows / 16)), dim3(256), 0, stream, a);
+            hipLaunchKernelGGL((join_page_rows<NB, kRows>), dim3(4 * a.parts), dim3(kJoinThreads), 0, stream, a);
         }
     } else if (octets == 2)
         hipLaunchKernelGGL((attend_pages<F, NB, 2>), dim3(a.parts), dim3(64 * AttendShape<F, NB, 2>::kWaves), 0, stream, a);
