@@ -19,6 +19,12 @@
 // 23.3 (a copy of as many bytes 6.5 - 7.3). 32 sequences of 16 tokens: 4.9 and 5.7,
 // 5.1 and 5.2, 4.7 and 7.0; read back 4.4 - 5.2 by units, 4.4 - 4.5 by tokens. Up to
 // 256 tokens of one sequence either is a launch's latency (3 us).
+//
+// A pool's rows go through a slot map: by tokens as above (page_append, page_read), or,
+// of many, a wave 32 rows' block of a head (page_append_windows, page_read_windows),
+// units where the slots are a whole tile's. 64 requests with two prompts of 2,048 tokens, 8
+// heads of 128 in Q4_0 (39 MB each way): 12.6 - 14.1 and 11.2 - 11.9 us; 24 requests' 23
+// tokens 3.3 and 2.6, latency.
 #include "cache.hpp"
 #include "requests.hpp"
 
@@ -847,12 +853,16 @@ static hipError_t launch_rows(const CacheRows& a, bool read, hipStream_t stream)
 hipError_t launch_cache_append(const CacheRows& a, hipStream_t stream) { return launch_rows(a, false, stream); }
 hipError_t launch_cache_read(const CacheRows& a, hipStream_t stream) { return launch_rows(a, true, stream); }
 
-// Rows from which a step of a pool looks for tiles among them.
-constexpr uint32_t kWindowRows = 64;
+// Values of a step's keys from which a step of a pool looks for tiles among its rows.
+// A prompt of 2,048 tokens, 8 heads of 128 in Q8_0, append and read: 7.3 and 7.2 us by
+// windows, 13.9 and 9.0 by tokens; 1,024 6.2 and 5.6, 9.4 and 5.7; 512 5.6 and 4.8, 6.0 and 4.6;
+// 256 5.4 and 4.6, 4.3 and 3.3. Rows of which none make a tile: 1,100 requests' 10.4
+// and 8.0, 9.8 and 7.5.
+constexpr uint64_t kWindowValues = 1u << 19;
 
 template <uint32_t F>
 static void launch_paged_rows(const CacheRows& a, bool read, hipStream_t stream) {
-    if (a.tokens >= kWindowRows) {
+    if (uint64_t{a.tokens} * a.cache.kv_heads * a.cache.head_dim >= kWindowValues) {
         const uint64_t units = (uint64_t{a.tokens} + 31) / 32 * a.cache.kv_heads * (a.cache.head_dim / 32);
         const dim3 grid(static_cast<uint32_t>((units + 3) / 4), 2);
         if (read)

@@ -10,14 +10,31 @@
 // lengths, by sums over the requests, some a lane, with no launch ahead of it. Where units are fewer than
 // workgroups, each is cut in pieces of equal length, a workgroup a piece. Where
 // that would leave some with much more than others, the units are laid along a line,
-// a key head after another, and each workgroup takes an equal part of it: a long
-// unit that crosses parts is in pieces, a short one is its first part's.
+// a key head after another, and each workgroup takes an equal part of it: a
+// unit that crosses parts is in pieces.
 //
 // A unit's pieces leave their outputs, and their rows' offsets and sums, in the
 // workspace, past the caches that the workgroups do not share (loads and stores of
 // the device's scope); each waits for its own to arrive, then counts itself, and
 // the one that finds itself the last (the counter is left at 0) joins them, in the
-// pieces' order. No cache is written back or cleared for it.
+// pieces' order. No cache is written back or cleared for it: the write-back that a
+// release at the device's scope asks for took 4 us. Of many rows, whose pieces are
+// MBs, a launch of its own joins them.
+//
+// Few rows are bound by the cache's bytes: 64 requests of 50 - 32,768 tokens, 8 key
+// heads of 128 in Q8_0 (731 MB), 140 - 141 us, 5.2 TB/s, as a large copy. One token over
+// 65,536, 8 heads of 64 in Q4_0 (38 MB): 23.8 us, of which 4.5 go before the first tile,
+// 11 over the tiles (the VALU: 4-bit codes widened for four rows of 16) and 8 from a
+// workgroup's last tile to the units' join. 3 requests of up to 911 tokens: 15 us, of the
+// same parts. Many rows are bound by the VALU and the matrix cores in turn (two prompts of
+// 512 tokens over up to 8,000, 8 key heads of 64: 197 us of 212 in attend_page_rows, matrix
+// cores 35% busy, VALU 48%, at attend_rows' rate for such heads); their requests in units
+// of 32 rows took 293.
+//
+// Against one sequence's contiguous cache (attention.hpp), Q8_0, 8 key heads of 128, us:
+// 512 tokens over 15,873 368 beside 341, over 2,000 82 and 71, over none 37 and 36; 2,048 over
+// 2,048 312 and 314; one over 65,536 39 and 33; F16, one key head of 256, 512 over 8,000
+// 87 and 68 (more registers than 256: some of the tile's are spilled).
 #pragma once
 
 #include "attention.hpp"
@@ -25,11 +42,13 @@
 
 namespace chm {
 
-// What a unit costs beside its tiles, in tiles, and up to what length it is whole
-// on the line.
-constexpr uint32_t kUnitTiles = 8, kWholeTiles = 16;
+// What a unit costs beside its tiles, in tiles (its queries, its waves' join). One token
+// each of 64 requests of 50 - 32,768 tokens, 8 key heads of 128 in Q8_0: 181 us at none,
+// 163 - 169 at 8, 156 at 16, 160 at 24; of 200 requests of 50 - 2,000 115, 92, 92 and 92.
+constexpr uint32_t kUnitTiles = 16;
 // Tiles more than on the line that a workgroup may have for units cut in pieces:
-// about what a unit's ends cost that the line leaves in two workgroups.
+// about what a unit's ends cost that the line leaves in two workgroups. 8 requests of
+// 4,000 tokens 25.5 us in pieces, 28.6 on the line; 30 of 50 - 32,768 340 and 81.
 constexpr uint32_t kPieceTiles = 24;
 
 // What is the same in every lane, as the compiler then knows; a lane's.
@@ -298,10 +317,6 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
             const uint32_t each = r.tiles / pieces, more = r.tiles % pieces;
             tile_begin = piece * each + min(piece, more), tile_end = tile_begin + each + (piece < more);
             place = end;
-        } else if (unit_length <= kUnitTiles + kWholeTiles) {
-            const bool earlier = unit_begin < parts.begin(part);
-            place = unit_end;
-            if (earlier) continue;
         } else {
             const uint32_t from = parts.at(unit_begin), to = parts.at(unit_end - 1);
             pieces = to - from + 1, piece = part - from;
@@ -420,7 +435,9 @@ __global__ __launch_bounds__((64 * AttendShape<F, NB, X>::kWaves)) void attend_p
 
 // ---- requests of many rows -----------------------------------------------------
 
-// What a unit of many rows costs beside its tiles, and the least tiles of a part.
+// What a unit of many rows costs beside its tiles, and the least tiles of a part. 512
+// tokens over 2,000 (8 key heads of 128, Q8_0) 86 us at a cost of 2, 82 at 4, 89 at 6; over
+// 8,000 (one of 256, F16) 91, 87 and 89.
 constexpr uint32_t kManyUnitTiles = 4, kManyPartTiles = 8;
 // Tiles of a piece whose records' places are kept in LDS; past them they are found anew.
 constexpr uint32_t kKeptTiles = 1024;

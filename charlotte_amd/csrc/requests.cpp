@@ -111,8 +111,9 @@ void check_table(uint32_t requests, uint32_t table_stride, uint32_t page_tokens)
 
 // How a step of attention runs: requests of up to 16 rows of a key head by units of
 // 16, of more by units of 32, of kManyRows and more, where they are load enough, by
-// units of `many`; each in launches of its own. One request, which is of one kind,
-// and groups past 16 have no launch of units of 16.
+// units of `many`; each in launches of its own, of which one that finds no request of
+// its kind takes 4 - 5 us. One request, which is of one kind, and groups past 16 have no
+// launch of units of 16.
 struct PagedPlan {
     bool ones, twos;
     uint32_t many, many_load;  // 0: none
@@ -342,6 +343,8 @@ charlotte_hip_matmul_status charlotte_hip_matmul_residual_norm(charlotte_hip_mat
         a.residual_out_stride = stride_of(d.residual_out_stride, d.width, 1, "residual_out stride");
         a.normed_stride = stride_of(d.normed_stride, d.width, 1, "normed stride");
         if (d.residual_out && d.residual_out == d.normed) refuse("two results in one place");
+        for (const float* shared : {d.branch_weight, d.weight})  // other rows read it
+            if (shared && (shared == d.residual_out || shared == d.normed)) refuse("a result over a weight");
         for (const float* input : {d.residual, d.branch, d.gate}) {
             const uint64_t stride = input == d.residual ? a.residual_stride : input == d.branch ? a.branch_stride : a.gate_stride;
             in_place(d.residual_out, a.residual_out_stride, input, stride);

@@ -676,7 +676,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_verify(charlotte_hip_matmul_con
 /* Keys and values of `pages` pages of `page_tokens` tokens (whole 32s), in a
  * cache's format and records; a request's tokens are in the pages that its row of
  * a table names, token t in page table[t / page_tokens]. A slot is page *
- * page_tokens + t % page_tokens. A page may stand in several requests' rows.
+ * page_tokens + t % page_tokens. A page may stand in several requests' rows
+ * (page_plan then gives it back once for each: a caller that shares pages keeps
+ * them out of what it gives back until the last).
  * Calls on one pool are ordered by the caller (one stream, or events). */
 typedef struct charlotte_hip_matmul_page_pool charlotte_hip_matmul_page_pool;
 
@@ -808,7 +810,8 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
  *   r = residual_scale x + branch_scale gate z       (no gate: one; no branch: no such term)
  *   n = r / sqrt(mean(r^2) + epsilon) * weight
  * r goes to residual_out, n to normed, either of which may be NULL. Sums are f32.
- * An output may be an input's memory with its stride, or memory apart from all. */
+ * An output may be the memory of residual, branch or a gate a row, with its stride,
+ * or memory apart from all. */
 typedef struct {
     const float* residual;        /* device: rows of `width`, residual_stride apart */
     const float* branch;          /* device, or NULL */

@@ -249,11 +249,43 @@ def test_a_pool_reads_back_what_its_format_holds(ctx, dev, format_, heads, dim, 
     pool.pool.free()
 
 
+@pytest.mark.parametrize("format_,heads,dim,page_tokens,lengths", [
+    ("q8_0", 8, 128, 64, (530, 1, 1, 97, 1)), ("q4_0", 4, 256, 32, (1, 31, 32, 33, 300, 250)), ("f16", 8, 128, 2048, (700,)),
+    ("q8_0", 1, 32, 128, (9000, 1, 7400, 1, 5)), ("f16", 2, 224, 96, (640, 640))])
+def test_a_pool_of_many_rows(ctx, dev, format_, heads, dim, page_tokens, lengths):
+    """Prompts of any lengths, each from the middle of a page on, over pages in any order."""
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(dim + len(lengths))
+    print("page_append", format_, heads, dim, page_tokens, lengths, flush=True)
+    width, slots = heads * dim, []
+    pages = sum(n // page_tokens + 2 for n in lengths)
+    order = rng.permutation(pages).tolist()
+    for n in lengths:
+        past = int(rng.integers(page_tokens))
+        held = [order.pop() for _ in range(-(-(past + n) // page_tokens))]
+        slots += [held[t // page_tokens] * page_tokens + t % page_tokens for t in range(past, past + n)]
+    slots = np.array(slots)
+    k, v = (rng.standard_normal((len(slots), width)).astype(np.float32) for _ in range(2))
+    pool = _Pool(dev, format_, pages, page_tokens, heads, dim, byte=0)
+    bad = rng.random(len(slots)) < 0.01
+    given = np.where(bad, NOWHERE, slots)
+    rest = np.setdiff1d(np.arange(pages * page_tokens), given[~bad])
+    before = pool.read(rest, width)
+    pool.write(k, v, given)
+    for got, x in zip(pool.read(given, width), (k, v)):
+        want = ref.stored(x.reshape(-1, heads, dim), format_).reshape(x.shape)
+        assert np.array_equal(got, np.where(bad[:, None], np.float32(5), want))
+    for got, old in zip(pool.read(rest, width), before):
+        assert np.array_equal(got, old)
+    pool.pool.free()
+
+
 # ---- paged attention --------------------------------------------------------------
 
 
 def _check_paged(dev, format_, requests, heads, kv_heads, dim, page_tokens=32, window=0, seed=0, most=None, rows=None,
-                 granted=None, scale=None, spread=1.0, query_stride=0, output_stride=0, stride=None, twice=False, grow=0):
+                 granted=None, scale=None, spread=1.0, query_stride=0, output_stride=0, stride=None, twice=False, grow=0, longest=0):
     """requests: (past, count) each. Every row of theirs against the restatement, others left as they were."""
     from charlotte_amd import harness as hx
     from charlotte_amd import serving as sv
@@ -296,7 +328,7 @@ def _check_paged(dev, format_, requests, heads, kv_heads, dim, page_tokens=32, w
     out, read = dev.room(rows * out_width)
     call = sv.PagedAttention(pool.pool, dev.put(given), out, heads, scale, len(requests), rows,
                              dev.put(_words([p for p, _ in requests])), dev.put(_words(granted)), dev.put(_words(starts)),
-                             dev.put(_words(table)), width, window, most, query_stride, output_stride, work, need)
+                             dev.put(_words(table)), width, window, most, query_stride, output_stride, work, need, longest)
     sv.paged_attention(dev.ctx, call)
     hx.sync()
     got = read().reshape(rows, out_width)
@@ -411,6 +443,42 @@ def test_paged_attention_in_a_window(ctx, dev, window):
 @pytest.mark.parametrize("most", [0, 1, 7, 1000])
 def test_the_most_tokens_named_change_no_answer(ctx, dev, most):
     _check_paged(dev, "q4_0", [(200, 9), (63, 1), (150, 20)], 8, 4, 64, most=most, seed=1)
+
+
+@pytest.mark.parametrize("longest", [1, 300, 1 << 30])
+def test_the_longest_named_changes_no_answer(ctx, dev, longest):
+    _check_paged(dev, "q8_0", [(4000, 90), (17, 1), (0, 260), (3000, 3)], 8, 1, 64, page_tokens=64, longest=longest, seed=3)
+
+
+def test_requests_that_share_pages(ctx, dev):
+    """Two continuations of one prompt, whose pages stand in both rows."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(8)
+    heads, kv_heads, dim, shared = 8, 2, 64, 5 * 32
+    pool = _Pool(dev, "q8_0", 9, 32, kv_heads, dim)
+    past, counts = [shared + 3, shared + 7], [2, 1]
+    table = np.array([[8, 0, 7, 2, 5, 1], [8, 0, 7, 2, 5, 6]])
+    slots = [table[0, t // 32] * 32 + t % 32 for t in range(shared + 5)] + [6 * 32 + t for t in range(8)]
+    k, v = (rng.standard_normal((len(slots), kv_heads, dim)).astype(np.float32) for _ in range(2))
+    pool.write(k.reshape(len(slots), -1), v.reshape(len(slots), -1), slots)
+    q = rng.standard_normal((3, heads, dim)).astype(np.float32)
+    need = sv.paged_attention_workspace_bytes(ctx, pool.pool, heads, 2)
+    work, _ = dev.room(need, np.uint8)
+    out, read = dev.room(3 * heads * dim)
+    sv.paged_attention(ctx, sv.PagedAttention(pool.pool, dev.put(q), out, heads, 0.1, 2, 3, dev.put(_words(past)),
+                                              dev.put(_words(counts)), dev.put(_words([0, 2, 3])), dev.put(_words(table)), 6, most=2,
+                                              workspace=work, workspace_bytes=need))
+    hx.sync()
+    got = read().reshape(3, heads, dim)
+    own = [slice(shared, shared + 5), slice(shared + 5, shared + 13)]
+    for at, p, mine in zip((slice(0, 2), slice(2, 3)), past, own):
+        kv = [ref.stored(np.concatenate([x[:shared], x[mine]]), "q8_0") for x in (k, v)]
+        want, weight, size = ref.attention(q[at], *kv, p, 0.1)
+        assert (np.abs(got[at] - want) <= ref.attention_bound(weight, size, shared + 8 + 32 * 256, dim)).all()
+    pool.pool.free()
 
 
 def test_rows_of_no_request_are_left_as_they_were(ctx, dev):
@@ -798,6 +866,75 @@ def test_a_captured_step_replays_as_requests_grow(ctx, dev, format_, heads, kv_h
         side.pool.free()
 
 
+def test_steps_on_two_streams_at_once(ctx, dev):
+    """Two pools, each with a workspace and a stream of its own, and the same calls one after the other; then two graphs that
+    share a workspace on one stream."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+
+    rng = np.random.default_rng(12)
+    heads, kv_heads, dim, vocabulary = 8, 2, 64, 20001
+    past, counts = [700, 0, 31, 4000], [1, 120, 1, 2]
+    starts, rows = np.concatenate([[0], np.cumsum(counts)]), sum(counts)
+    held = [-(-(p + c) // 64) for p, c in zip(past, counts)]
+    stride = max(held)
+    uniforms = dev.put(rng.random(rows, np.float32))
+
+    class Side:
+        def __init__(self):
+            pages = sum(held) + 1
+            order = rng.permutation(pages).tolist()
+            table = np.full((4, stride), NOWHERE, np.uint64)
+            for r, n in enumerate(held):
+                table[r, :n] = [order.pop() for _ in range(n)]
+            self.pool = _Pool(dev, "q8_0", pages, 64, kv_heads, dim)
+            slots = [int(table[r, t // 64]) * 64 + t % 64 for r in range(4) for t in range(past[r] + counts[r])]
+            k, v = (rng.standard_normal((len(slots), kv_heads * dim)).astype(np.float32) for _ in range(2))
+            self.pool.write(k, v, slots)
+            q, logits = (dev.put(rng.standard_normal((rows, n)).astype(np.float32)) for n in (heads * dim, vocabulary))
+            self.need = max(sv.paged_attention_workspace_bytes(ctx, self.pool.pool, heads, 120),
+                            sv.sample_workspace_bytes(rows, vocabulary))
+            work, _ = dev.room(self.need, np.uint8)
+            (out, self.read_out), (tokens, self.read_tokens) = dev.room(rows * heads * dim), dev.room(rows, np.int32)
+            self.attend = sv.PagedAttention(self.pool.pool, q, out, heads, 0.1, 4, rows, dev.put(_words(past)),
+                                            dev.put(_words(counts)), dev.put(_words(starts)), dev.put(_words(table)), stride, most=120,
+                                            workspace=work, workspace_bytes=self.need)
+            self.draw = sv.Sample(logits, tokens, rows, vocabulary, uniforms, 0.9, 0, 0.9, workspace=work, workspace_bytes=self.need)
+
+        def run(self, stream):
+            sv.paged_attention(ctx, self.attend, stream=stream)
+            sv.sample(ctx, self.draw, stream=stream)
+
+        def all(self):
+            return [self.read_out().view(np.uint32), self.read_tokens()]
+
+    sides, streams, want = [Side(), Side()], [hx.Stream(), hx.Stream()], []
+    for side in sides:
+        side.run(None)
+        hx.sync()
+        want.append(side.all())
+    for _ in range(10):
+        for side, stream in zip(sides, streams):
+            side.run(stream.handle)
+        for stream in streams:
+            stream.sync()
+        for side, w in zip(sides, want):
+            assert all(np.array_equal(a, b) for a, b in zip(side.all(), w))
+    for call in (sides[1].attend, sides[1].draw):
+        call.workspace = sides[0].attend.workspace
+    graphs = [hx.Graph(streams[0], lambda: side.run(streams[0].handle), global_mode=True) for side in sides]
+    for turn in range(6):
+        for graph in graphs[::1 if turn % 2 else -1]:
+            graph.launch()
+        streams[0].sync()
+        for side, w in zip(sides, want):
+            assert all(np.array_equal(a, b) for a, b in zip(side.all(), w)), turn
+    for x in (*graphs, *streams):
+        x.destroy()
+    for side in sides:
+        side.pool.pool.free()
+
+
 # ---- refusals -------------------------------------------------------------------------
 
 
@@ -891,7 +1028,8 @@ def test_residual_norm_and_sample_refuse(ctx, dev):
                    {"epsilon": -1.0}, {"epsilon": float("inf")}, {"residual_scale": float("nan")}, {"branch_scale": float("inf")},
                    {"residual_stride": 63}, {"branch_stride": 1}, {"gate": x, "gate_stride": 7}, {"residual_out_stride": 5},
                    {"normed_stride": 5}, {"residual_out": x, "residual_out_stride": 80}, {"normed": x + 512},
-                   {"normed": x + 256, "normed_stride": 72}, {"gate": x + 2048, "normed": x + 2048}):
+                   {"normed": x + 256, "normed_stride": 72}, {"gate": x + 2048, "normed": x + 2048}, {"normed": x + 1024},
+                   {"branch_weight": x + 512}):
         _refused(lambda: sv.residual_norm(ctx, sv.ResidualNorm(**{**good, **change}), 1), bad)
     for rows in (0, 0xFFFFFFFF):
         _refused(lambda: sv.residual_norm(ctx, sv.ResidualNorm(**good), rows), bad)
