@@ -7,17 +7,15 @@
 // itself are one question: at which token does the running count or weight pass
 // a number? It is answered without sorting the row, in three launches over chunks
 // of the rows:
-//   row_largest   each chunk's largest logit;
-//   row_bins      counts, and weights to within known bounds (f32's exponential, in
-//                 whole units of 2^-26), of kBins equal steps of (m - l) / T, down to
-//                 where a weight is 0; a bin's two sums in one word. The workgroup
-//                 that ends a row last finds the bins that the cuts and the draw may
-//                 fall into: a cut's bins bound what is kept, that the next one's;
-//   row_draw      the exact weights: those before each run of such bins summed, the
-//                 tokens in them, some hundreds, gathered. The last workgroup of a
-//                 row sorts them by finer bins, and answers.
-// Where those bins hold more than kList tokens (many equal logits, a temperature
-// that makes them so) or the largest is +inf, one workgroup answers by descent:
+//   row_largest   each chunk's largest logit, and its smallest;
+//   row_bins      counts and weights of kBins equal steps of m - l, down to where a
+//                 weight is 0 or the logits end. The workgroup that ends a row last finds
+//                 the bins that the cuts and the draw may fall into: a cut's bins bound
+//                 what is kept, that the next one's;
+//   row_draw      the tokens in those bins, some hundreds, gathered. The last workgroup
+//                 of a row sorts them by finer bins, and answers.
+// Where those bins hold more than kList tokens (many equal logits) or the logits'
+// distances pass f32, one workgroup answers by descent:
 // weights and counts of the logits' leading bits (as keys that rise with them)
 // summed in LDS, the part that holds the answer opened by its next bits; tokens of
 // one key have one weight, so the place among them is a division.
@@ -28,11 +26,13 @@
 // each workgroup waits for its own to arrive, then counts itself; no cache is
 // written back or cleared for it.
 //
-// Bound by f64 arithmetic and by the chain of each row's last workgroup: 1 x 151,936 logits
-// 22 us (2.9 + 8.5 + 10.5: launches of a chunk a workgroup, then a row's bins searched and
-// its list sorted); 64 x 128,256, settings a row, 51 (7.8, read at 4.2 TB/s, + 16.8, of
-// which adds to LDS bins, + 28.2: 30 operations of f64 a logit, 7 us at their full rate,
-// and the sort); 24 x 262,144 by temperature alone 50.
+// Bound by f64 arithmetic and by the chains of each row's last workgroups: 1 x 151,936 logits
+// 22 us (3.4 + 10.4 + 9.3: a chunk a workgroup, then the bins searched, then the list
+// sorted); 64 x 128,256, settings a row, 51 (7.3, read at 4.5 TB/s, + 25.2: 30 operations
+// of f64 a logit, 7 us at their full rate, two adds to LDS, the bins added up + 17.9);
+// 24 x 262,144 by temperature alone 50. Weights of f32's exponential in the bins, with
+// bounds, and the exact ones summed in row_draw took as long where few tokens lay within
+// the bounds, and 200 - 600 us where a draw near the end of a flat row had thousands.
 #include <algorithm>
 #include <cstddef>
 
@@ -301,30 +301,32 @@ __device__ __forceinline__ T add(T& x, T value) {
 }
 
 // Bins whose tokens are gathered: `first` .. `last`, of `count` tokens, those before
-// them `before`; the first token's place in the list.
+// them `before` and their weight `ahead`; the first token's place in the list.
 struct Run {
     uint32_t first, last, count, before, start, reserved;
+    uint64_t ahead;
 };
 constexpr uint32_t kRuns = 3;
 // A row's part of the workspace.
 struct DrawRoom {
-    uint64_t bins[kBins];        // a count, and under it weights in 2^-26
-    uint64_t sums[2 + kRuns];    // exact weights: of all tokens, of those that min_p leaves, and of those before a run
+    uint64_t weights[kBins];     // the bins' weights
+    uint64_t counts[kBins / 2];  // and tokens, two bins' in a word
+    uint64_t likely;             // weight that min_p leaves of the bins of its end
     uint32_t binned, gathered;   // workgroups of row_bins, of row_draw, that have ended
     uint32_t listed;             // tokens gathered
     uint32_t runs, alone;        // runs; or by descent
     uint32_t cut;                // top_k's last token is in a run
+    uint32_t end_first, end_past;  // the bins that min_p's end may be in
+    uint64_t all, end_ahead;     // weight of all tokens; of those before these bins
     Run run[kRuns];
     uint64_t list[kList];        // key, and the index's complement: the first token is the largest
 };
 constexpr uint32_t kCleared = offsetof(DrawRoom, list) / 8;
 static_assert(offsetof(DrawRoom, list) % 8 == 0, "words of 8 bytes");
-constexpr uint32_t kWeightBits = 45;  // 2^26 of each of 2^18 tokens, and 2^18 above them
-constexpr float kUnit = 0x1p26f;
-
 struct DrawChunks {
     DrawRoom* rooms;
     uint64_t* largest;  // [rows][chunks]: key, and the index's complement
+    float* smallest;    // [rows][chunks], of what is finite
     uint32_t chunks, share;
 };
 
@@ -346,36 +348,60 @@ __device__ __forceinline__ uint64_t most_of_wave(uint64_t x) {
     for (uint32_t o = 32; o > 0; o >>= 1) x = max(x, static_cast<uint64_t>(__shfl_xor(x, o)));
     return x;
 }
+__device__ __forceinline__ float least_of_wave(float x) {
+#pragma unroll
+    for (uint32_t o = 32; o > 0; o >>= 1) x = fminf(x, __shfl_xor(x, o));
+    return x;
+}
 
 __global__ __launch_bounds__(kDrawThreads) void row_largest(Sample a, DrawChunks c) {
     __shared__ uint64_t parts[kDrawThreads / 64];
+    __shared__ float least_parts[kDrawThreads / 64];
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
     uint64_t* room = reinterpret_cast<uint64_t*>(c.rooms + row);
     for (uint32_t i = chunk * kDrawThreads + threadIdx.x; i < kCleared; i += c.chunks * kDrawThreads) room[i] = 0;
     uint64_t most = 0;
-    each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) { most = max(most, uint64_t{key_of(l)} << 32 | ~i); });
-    most = most_of_wave(most);
-    if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = most;
+    float least = INFINITY;
+    each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) {
+        most = max(most, uint64_t{key_of(l)} << 32 | ~i);
+        least = fminf(least, l == -INFINITY ? INFINITY : l);
+    });
+    most = most_of_wave(most), least = least_of_wave(least);
+    if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = most, least_parts[threadIdx.x >> 6] = least;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < kDrawThreads / 64; ++w) most = max(most, parts[w]);
-        c.largest[blockIdx.x] = most;
+        for (uint32_t w = 1; w < kDrawThreads / 64; ++w) most = max(most, parts[w]), least = fminf(least, least_parts[w]);
+        c.largest[blockIdx.x] = most, c.smallest[blockIdx.x] = least;
     }
 }
 
-// The row's largest: its key, and its index's complement; in every thread.
-__device__ __forceinline__ uint64_t largest_of(const DrawChunks& c, uint32_t row) {
-    uint64_t most = 0;
-    for (uint32_t i = threadIdx.x & 63u; i < c.chunks; i += 64) most = max(most, c.largest[uint64_t{row} * c.chunks + i]);
-    return most_of_wave(most);
+// The row's largest, its key and its index's complement, and its smallest that is finite; in every thread.
+struct Ends {
+    uint64_t largest;
+    float smallest;
+};
+__device__ __forceinline__ Ends ends_of(const DrawChunks& c, uint32_t row) {
+    Ends e{0, INFINITY};
+    for (uint32_t i = threadIdx.x & 63u; i < c.chunks; i += 64) {
+        e.largest = max(e.largest, c.largest[uint64_t{row} * c.chunks + i]);
+        e.smallest = fminf(e.smallest, c.smallest[uint64_t{row} * c.chunks + i]);
+    }
+    return {most_of_wave(e.largest), least_of_wave(e.smallest)};
 }
+
+// An infinite logit, or two whose distance f32 does not hold: the row has no bins.
+__device__ __forceinline__ bool too_far(float most, float smallest) { return most - smallest == INFINITY; }
 
 // A logit's place among the bins: it does not fall as the logit does.
 __device__ __forceinline__ float place_of(float l, float most, float steps) {
     return fminf((most - l) * steps, static_cast<float>(kBins - 1));
 }
-__device__ __forceinline__ float steps_of(const Settings& s) {
-    return static_cast<float>(s.rate * (static_cast<double>(kBins - 1) / kReach));
+// Bins a unit of a logit: over what weighs anything, or over the row's logits where
+// they reach less far, so that no bin has much more of them than another (one that
+// has more than kList is answered by descent); all that weigh before the last bin.
+__device__ __forceinline__ float steps_of(const Settings& s, float most, float smallest) {
+    const double range = static_cast<double>(most) - static_cast<double>(smallest);
+    return static_cast<float>(fmin(fmax(s.rate * (static_cast<double>(kBins - 1) / kReach), (kBins - 3) / range), 1e30));
 }
 
 // Whether this is the last of a row's workgroups to come here.
@@ -387,39 +413,33 @@ __device__ __forceinline__ bool last_of(uint32_t& counter, uint32_t workgroups, 
     return *flag != 0;
 }
 
-// Bounds of a weight, in units of 2^-40, of which `sum` is the binned one, in 2^-26,
-// of `count` tokens: a token's was cut to a whole unit, and f32's exponential is
-// within 2^-16 of it (its argument, below 41, within 3 times 2^-24 of itself); the
-// exact one is cut to a whole 2^-40. Twice that, and the sums' own roundings.
-__device__ __forceinline__ uint64_t at_least(uint64_t sum, uint64_t count) {
-    const uint64_t off = (sum >> 15) + (count >> 14) + 8;
-    return sum > off ? (sum - off) << 14 : 0;
-}
-__device__ __forceinline__ uint64_t at_most(uint64_t sum, uint64_t count) { return (sum + (sum >> 15) + count + 8) << 14; }
-
 struct Planning {
-    uint64_t sums[kBins + 1];    // binned weights before a bin
+    uint64_t sums[kBins + 1];    // weights before a bin
     uint32_t counts[kBins + 1];
     uint64_t parts[kDrawThreads / 64];
 };
 
 // The bins that the row's cuts and its draw may fall into, by the last of its workgroups.
-__device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Planning& d) {
+__device__ void plan_row(const Sample& a, const Settings& s, float steps, DrawRoom& room, Planning& d) {
     constexpr uint32_t kMine = kBins / kDrawThreads;
-    uint64_t word[kMine], sum = 0, all;
+    static_assert(kMine % 2 == 0, "whole words of counts");
+    uint64_t weight[kMine], pair[kMine / 2], sum = 0, tokens = 0, all, all_tokens;
 #pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) word[i] = get(room.bins[kMine * threadIdx.x + i]);
+    for (uint32_t i = 0; i < kMine; ++i) weight[i] = get(room.weights[kMine * threadIdx.x + i]), sum += weight[i];
 #pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) sum += word[i];
-    // both sums of a word at once: neither passes its bits
+    for (uint32_t i = 0; i < kMine / 2; ++i) {
+        pair[i] = get(room.counts[kMine / 2 * threadIdx.x + i]);
+        tokens += (pair[i] & 0xFFFFFFFFull) + (pair[i] >> 32);
+    }
     uint64_t before = sum_before(sum, d.parts, &all);
+    uint32_t before_tokens = static_cast<uint32_t>(sum_before(tokens, d.parts, &all_tokens));
 #pragma unroll
     for (uint32_t i = 0; i < kMine; ++i) {
         const uint32_t bin = kMine * threadIdx.x + i;
-        d.sums[bin] = before & ((1ull << kWeightBits) - 1), d.counts[bin] = static_cast<uint32_t>(before >> kWeightBits);
-        before += word[i];
+        d.sums[bin] = before, d.counts[bin] = before_tokens;
+        before += weight[i], before_tokens += static_cast<uint32_t>(pair[i / 2] >> (i % 2 * 32));
     }
-    if (threadIdx.x == 0) d.sums[kBins] = all & ((1ull << kWeightBits) - 1), d.counts[kBins] = static_cast<uint32_t>(all >> kWeightBits);
+    if (threadIdx.x == 0) d.sums[kBins] = all, d.counts[kBins] = static_cast<uint32_t>(all_tokens);
     __syncthreads();
     if (threadIdx.x >= 64) return;
     // By one wave: the first bin (of kBins) of which `passed` is true, as it is of all after it.
@@ -433,33 +453,31 @@ __device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Pla
     // a question's bins, its target between `low` and `high`
     auto run_of = [&](uint64_t low, uint64_t high) {
         Run r{};
-        r.first = first_bin([&](uint32_t bin) { return at_most(d.sums[bin + 1], d.counts[bin + 1]) > low; });
-        r.last = first_bin([&](uint32_t bin) { return at_least(d.sums[bin + 1], d.counts[bin + 1]) > high; });
+        r.first = first_bin([&](uint32_t bin) { return d.sums[bin + 1] > low; });
+        r.last = first_bin([&](uint32_t bin) { return d.sums[bin + 1] > high; });
         r.last = min(r.last, kBins - 2);  // the last bin's tokens weigh nothing
         return r;
     };
-    Run none{kBins, kBins, 0, 0, 0, 0}, top_k = none, top_p = none;
-    uint64_t low = at_least(d.sums[kBins], d.counts[kBins]), high = at_most(d.sums[kBins], d.counts[kBins]);  // of what is kept
+    Run none{kBins, kBins, 0, 0, 0, 0, 0}, top_k = none, top_p = none;
+    uint64_t low = d.sums[kBins], high = low;  // of what is kept
     if (s.top_k < a.vocabulary) {
         const uint32_t bin = first_bin([&](uint32_t b) { return d.counts[b + 1] >= s.top_k; });
         if (bin < kBins - 1) {
             top_k.first = top_k.last = bin;
-            low = at_least(d.sums[bin], d.counts[bin]), high = at_most(d.sums[bin + 1], d.counts[bin + 1]);
+            low = max(d.sums[bin], 1ull << 40), high = d.sums[bin + 1];  // the first token is always kept
         }
     }
-    low = max(low, 1ull << 40), high = max(high, 1ull << 40);  // the first token is always kept
     if (s.top_p < 1.0) {
         top_p = run_of(passed_by(s, low), passed_by(s, high));
-        low = max(at_least(d.sums[top_p.first], d.counts[top_p.first]), 1ull << 40);
-        high = min(high, max(at_most(d.sums[top_p.last + 1], d.counts[top_p.last + 1]), 1ull << 40));
+        low = max(d.sums[top_p.first], 1ull << 40), high = min(high, d.sums[top_p.last + 1]);
     }
     if (s.least > 0) {
         // min_p's last token is in the bin of its distance or, by rounding, one beside it
-        const double at = -log(static_cast<double>(s.least) / kWhole) * (static_cast<double>(kBins - 1) / kReach);
+        const double at = -log(static_cast<double>(s.least) / kWhole) / s.rate * static_cast<double>(steps);
         const uint32_t bin = static_cast<uint32_t>(fmin(at, static_cast<double>(kBins - 1)));
         const uint32_t from = bin > 1 ? bin - 1 : 0, to = min(bin + 2, kBins);
-        low = min(low, max(at_least(d.sums[from], d.counts[from]), 1ull << 40));
-        high = min(high, max(at_most(d.sums[to], d.counts[to]), 1ull << 40));
+        low = min(low, max(d.sums[from], 1ull << 40)), high = min(high, d.sums[to]);
+        if (lane == 0) room.end_first = from, room.end_past = to, room.end_ahead = d.sums[from];
     }
     const Run draw = run_of(drawn_at(s, low), drawn_at(s, high));
     if (lane != 0) return;
@@ -475,6 +493,7 @@ __device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Pla
     uint32_t runs = 0, listed = 0;
     auto keep = [&](Run r) {
         r.before = d.counts[r.first], r.count = d.counts[r.last + 1] - r.before, r.start = listed;
+        r.ahead = d.sums[r.first];
         listed += r.count;
         room.run[runs++] = r;
     };
@@ -488,21 +507,26 @@ __device__ void plan_row(const Sample& a, const Settings& s, DrawRoom& room, Pla
     if (y.first < kBins) keep(y);
     if (z.first < kBins) keep(z);
     room.runs = runs, room.cut = top_k.first < kBins, room.alone = listed > kList;
+    room.all = d.sums[kBins];
 }
 
 __global__ __launch_bounds__(kDrawThreads) void row_bins(Sample a, DrawChunks c) {
     __shared__ union {
-        uint64_t bins[kBins];
+        struct {
+            uint64_t weights[kBins];
+            uint32_t counts[kBins];
+        } bins;
         Planning planning;
     } space;
     __shared__ uint32_t last;
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
-    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads) space.bins[i] = 0;
+    for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads) space.bins.weights[i] = 0, space.bins.counts[i] = 0;
     const Settings s = settings_of(a, row);
-    const float most = logit_of(static_cast<uint32_t>(largest_of(c, row) >> 32));
-    if (s.greedy || fabsf(most) == INFINITY) return;
+    const Ends ends = ends_of(c, row);
+    const float most = logit_of(static_cast<uint32_t>(ends.largest >> 32));
+    if (s.greedy || most == -INFINITY || too_far(most, ends.smallest)) return;
     DrawRoom& room = c.rooms[row];
-    const float steps = steps_of(s), octaves = static_cast<float>(s.octaves);
+    const float steps = steps_of(s, most, ends.smallest);
     __syncthreads();
     uint32_t rest = 0;
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t) {
@@ -511,17 +535,20 @@ __global__ __launch_bounds__(kDrawThreads) void row_bins(Sample a, DrawChunks c)
             ++rest;
             return;
         }
-        const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_exp2f((l - most) * octaves) * kUnit);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&space.bins[bin]), 1ull << kWeightBits | w);
+        // a whole number below 2^52 in its bits
+        const double w = whole_weight(l, most, s.octaves) + 0x1p52;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&space.bins.weights[bin]), __builtin_bit_cast(unsigned long long, w) & ((1ull << 52) - 1));
+        atomicAdd(&space.bins.counts[bin], 1u);
     });
 #pragma unroll
     for (uint32_t o = 32; o > 0; o >>= 1) rest += __shfl_xor(rest, o);
-    if ((threadIdx.x & 63u) == 0 && rest > 0)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&space.bins[kBins - 1]), static_cast<unsigned long long>(rest) << kWeightBits);
+    if ((threadIdx.x & 63u) == 0 && rest > 0) atomicAdd(&space.bins.counts[kBins - 1], rest);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kBins; i += kDrawThreads)
-        if (space.bins[i] != 0) add(room.bins[i], space.bins[i]);
-    if (last_of(room.binned, c.chunks, &last)) plan_row(a, s, room, space.planning);
+        if (space.bins.weights[i] != 0) add(room.weights[i], space.bins.weights[i]);
+    for (uint32_t i = threadIdx.x; i < kBins / 2; i += kDrawThreads)
+        if (const uint64_t pair = space.bins.counts[2 * i] | uint64_t{space.bins.counts[2 * i + 1]} << 32) add(room.counts[i], pair);
+    if (last_of(room.binned, c.chunks, &last)) plan_row(a, s, steps, room, space.planning);
 }
 
 // The row's list sorted, and its questions answered, by the last of its workgroups.
@@ -537,17 +564,15 @@ struct Sorting {
     uint32_t token;
 };
 
-__device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, float most, const DrawRoom& room, Sorting& t) {
+__device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, float most, float steps, const DrawRoom& room,
+                           Sorting& t) {
     constexpr uint32_t kMine = kList / kDrawThreads;
-    const float steps = steps_of(s);
     Run run[kRuns];
-    uint64_t run_before[kRuns];
     const uint32_t runs = room.runs;
     uint32_t n = 0, bins = 0;
 #pragma unroll
     for (uint32_t q = 0; q < kRuns; ++q) {
-        run[q] = q < runs ? room.run[q] : Run{kBins, kBins, 0, 0, kList, 0};
-        run_before[q] = get(room.sums[2 + q]);
+        run[q] = q < runs ? room.run[q] : Run{kBins, kBins, 0, 0, kList, 0, 0};
         if (q < runs) n += run[q].count, bins += run[q].last - run[q].first + 1;
     }
     // Buckets: each bin in as many equal parts, which rise as the logits fall.
@@ -622,12 +647,11 @@ __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, flo
     for (uint32_t e = 0; e < kMine; ++e) {
         const uint32_t i = kMine * threadIdx.x + e;
         Run r = run[0];
-        uint64_t ahead = run_before[0];
 #pragma unroll
         for (uint32_t q = 1; q < kRuns; ++q)
-            if (q < runs && run[q].start <= i) r = run[q], ahead = run_before[q];
+            if (q < runs && run[q].start <= i) r = run[q];
         count[e] = r.before + (i - r.start);
-        before[e] = ahead + (before[e] - t.before[r.start]);
+        before[e] = r.ahead + (before[e] - t.before[r.start]);
     }
     // The weight up to the token at which the row's running count or weight passes `target`, its own in t.own.
     auto passed_at = [&](bool by_count, uint64_t target) {
@@ -641,8 +665,8 @@ __device__ void answer_row(const Sample& a, uint32_t row, const Settings& s, flo
         __syncthreads();
         return t.passed;
     };
-    uint64_t kept = get(room.sums[0]);
-    const uint64_t likely = s.least > 0 ? get(room.sums[1]) : kept;
+    uint64_t kept = room.all;
+    const uint64_t likely = s.least > 0 ? room.end_ahead + get(room.likely) : kept;
     if (room.cut) kept = passed_at(true, s.top_k - 1);
     if (s.top_p < 1.0) kept = passed_at(false, passed_by(s, kept));
     kept = min(kept, likely);
@@ -656,74 +680,65 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
         Sorting sorting;
         uint64_t list[kList];
     } space;
-    __shared__ uint64_t sums[2 + kRuns];
+    __shared__ uint64_t likely;
     __shared__ uint32_t last, listed, base;
     const uint32_t row = blockIdx.x / c.chunks, chunk = blockIdx.x % c.chunks;
     const Settings s = settings_of(a, row);
-    const uint64_t largest = largest_of(c, row);
-    const float most = logit_of(static_cast<uint32_t>(largest >> 32));
+    const Ends ends = ends_of(c, row);
+    const float most = logit_of(static_cast<uint32_t>(ends.largest >> 32));
     if (s.greedy || most == -INFINITY) {
         if (chunk == 0 && threadIdx.x == 0) {
             if (most == -INFINITY)
                 write_draw(a, row, 0xFFFFFFFFu, 0, 1);
             else
-                write_draw(a, row, ~static_cast<uint32_t>(largest), 1, 1);
+                write_draw(a, row, ~static_cast<uint32_t>(ends.largest), 1, 1);
         }
         return;
     }
     DrawRoom& room = c.rooms[row];
-    if (most == INFINITY || room.alone) {
+    if (too_far(most, ends.smallest) || room.alone) {
         if (chunk == 0) draw_alone(a, row, s, most, space.descent);
         return;
     }
-    if (threadIdx.x < 2 + kRuns) sums[threadIdx.x] = 0;
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) listed = 0, likely = 0;
     __syncthreads();
-    const float steps = steps_of(s);
+    const float steps = steps_of(s, most, ends.smallest);
     uint32_t first[kRuns], width[kRuns];  // a run that is not there holds no bin
 #pragma unroll
     for (uint32_t q = 0; q < kRuns; ++q) {
         const bool there = q < room.runs;
         first[q] = there ? room.run[q].first : kBins, width[q] = there ? room.run[q].last - first[q] : 0;
     }
-    // all weights, those that min_p leaves, and those before a run: whole numbers, of a
-    // thread's few tokens below 2^53
-    double mine[2 + kRuns] = {};
-    const double least = static_cast<double>(s.least);
-    const uint32_t runs = room.runs;
+    // the bins that min_p's end may be in: none without it
+    const uint32_t end_first = s.least > 0 ? room.end_first : kBins, end_bins = s.least > 0 ? room.end_past - end_first : 0;
+    uint64_t mine = 0;
     each_of_chunk(a, c, row, chunk, [&](float l, uint32_t i) {
         const uint32_t bin = static_cast<uint32_t>(place_of(l, most, steps));
-        const double w = whole_weight(l, most, s.octaves);
-        mine[0] += w;
-        if (s.least > 0) mine[1] += w >= least ? w : 0.0;
+        if (bin - end_first < end_bins) {
+            const uint64_t w = weight_of(l, most, s.octaves);
+            mine += w >= s.least ? w : 0;
+        }
         bool in = false;
 #pragma unroll
-        for (uint32_t q = 0; q < kRuns; ++q) {
-            if (q > 0 && q >= runs) break;
-            mine[2 + q] += bin < first[q] ? w : 0.0;
-            in |= bin - first[q] <= width[q];
-        }
-        if (in) {
+        for (uint32_t q = 0; q < kRuns; ++q) in |= bin - first[q] <= width[q];
+        if (in && l != -INFINITY) {
             const uint32_t at = atomicAdd(&listed, 1u);
             if (at < kList) space.list[at] = uint64_t{key_of(l)} << 32 | ~i;
         }
     });
+    if (s.least > 0) {
 #pragma unroll
-    for (uint32_t q = 0; q < 2 + kRuns; ++q) {
-        if (q == 1 ? s.least == 0 : q > 2 && q - 2 >= runs) continue;
-        uint64_t sum = static_cast<uint64_t>(mine[q]);
-#pragma unroll
-        for (uint32_t o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        if ((threadIdx.x & 63u) == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[q]), static_cast<unsigned long long>(sum));
+        for (uint32_t o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
+        if ((threadIdx.x & 63u) == 0 && mine > 0) atomicAdd(reinterpret_cast<unsigned long long*>(&likely), static_cast<unsigned long long>(mine));
     }
     __syncthreads();
     const uint32_t here = min(listed, kList);
-    if (threadIdx.x < 2 + kRuns && sums[threadIdx.x] > 0) add(room.sums[threadIdx.x], sums[threadIdx.x]);
+    if (threadIdx.x == 0 && likely > 0) add(room.likely, likely);
     if (threadIdx.x == 0 && here > 0) base = add(room.listed, here);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < here; i += kDrawThreads)
         if (base + i < kList) put(room.list[base + i], space.list[i]);
-    if (last_of(room.gathered, c.chunks, &last)) answer_row(a, row, s, most, room, space.sorting);
+    if (last_of(room.gathered, c.chunks, &last)) answer_row(a, row, s, most, steps, room, space.sorting);
 }
 
 // About 512 workgroups, two a CU, a chunk of at least a four a thread; of whole fours.
@@ -735,7 +750,7 @@ static uint32_t draw_chunks(uint32_t rows, uint32_t vocabulary) {
 }
 
 uint64_t sample_bytes(uint32_t rows, uint32_t vocabulary) {
-    return rows * (sizeof(DrawRoom) + uint64_t{draw_chunks(rows, vocabulary)} * 8);
+    return rows * (sizeof(DrawRoom) + uint64_t{draw_chunks(rows, vocabulary)} * 12);
 }
 
 hipError_t launch_sample(const Sample& a, hipStream_t stream) {
@@ -744,6 +759,7 @@ hipError_t launch_sample(const Sample& a, hipStream_t stream) {
     c.largest = reinterpret_cast<uint64_t*>(c.rooms + a.rows);
     c.chunks = draw_chunks(a.rows, a.vocabulary);
     c.share = ((a.vocabulary + 3 + c.chunks - 1) / c.chunks + 3) / 4 * 4;
+    c.smallest = reinterpret_cast<float*>(c.largest + uint64_t{a.rows} * c.chunks);
     const dim3 grid(a.rows * c.chunks);
     hipLaunchKernelGGL(row_largest, grid, dim3(kDrawThreads), 0, stream, a, c);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;

@@ -763,6 +763,23 @@ def test_sample_settings_at_their_ends(ctx, dev, vocabulary):
         _check_sample(ctx, dev, rng.standard_normal((len(ends), vocabulary)).astype(np.float32), [(*e, u) for e in ends])
 
 
+@pytest.mark.parametrize("temperature", [0.3, 1.0, 5.0, 1e4, float("inf")])
+def test_sample_where_many_tokens_are_alike(ctx, dev, temperature):
+    """Draws from where a row's tokens lie closest, one of them past what is kept."""
+    rng = np.random.default_rng(23)
+    logits = (rng.standard_normal((9, 262144)) * np.array([1, 1, 1, 0.01, 1e-6, 1e-30, 3, 1, 1])[:, None]).astype(np.float32)
+    logits[7] = np.round(logits[7])  # many equal ones
+    logits[8, 1000:] = -np.inf
+    settings = [(temperature, 0, 1.0, 0.0, u) for u in (0.02, 0.5, 0.98, 0.5, 0.3, 0.7, 0.9)]
+    settings += [(temperature, 100000, 0.9, 1e-7, 0.6), (temperature, 900, 0.5, 0.5, 0.9)]
+    _check_sample(ctx, dev, logits, settings)
+
+
+def test_sample_logits_as_far_apart_as_f32_has_them(ctx, dev):
+    logits = np.array([[-3e38, 3e38, 0.0, 1e38, -1e38] * 40, [3.4e38, -3.4e38, 1.0, 2.0, -np.inf] * 40], np.float32)
+    _check_sample(ctx, dev, logits, [(1e38, 0, 1.0, 0.0, 0.97), (2e38, 90, 1.0, 0.01, 0.999)])
+
+
 def test_samples_follow_the_weights(ctx, dev):
     """Every token's share of many draws over a grid of uniform numbers, to one draw."""
     from tests.support import requests_ref as ref
