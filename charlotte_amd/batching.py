@@ -2,7 +2,7 @@
 products of charlotte_amd.matmul and, of charlotte_amd.serving, what runs
 between them for a step of several requests, as a program would run them.
 
-    python -m charlotte_amd.batching [--requests 48] [--together 16] [--pages 400] [--temperature 0.8] ...
+    python -m charlotte_amd.batching [--requests 40] [--together 16] [--pages 400] [--temperature 0.8] ...
 
 A step has a token of every request that is generating and blocks of the
 prompts of those that came last. page_plan gives the new tokens pages and every
@@ -229,7 +229,7 @@ def _before(request):
 
 def main():
     parser = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
-    parser.add_argument("--requests", type=int, default=48)
+    parser.add_argument("--requests", type=int, default=40)
     parser.add_argument("--together", type=int, default=16)
     parser.add_argument("--prompt", type=int, default=300, help="the longest prompt")
     parser.add_argument("--tokens", type=int, default=64)

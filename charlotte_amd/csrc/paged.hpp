@@ -27,9 +27,9 @@
 // 11 over the tiles (the VALU: 4-bit codes widened for four rows of 16) and 8 from a
 // workgroup's last tile to the units' join. 3 requests of up to 911 tokens: 15 us, of the
 // same parts. Many rows are bound by the VALU and the matrix cores in turn (two prompts of
-// 512 tokens over up to 8,000, 8 key heads of 64: 197 us of 212 in attend_page_rows, matrix
-// cores 35% busy, VALU 48%, at attend_rows' rate for such heads); their requests in units
-// of 32 rows took 293.
+// 512 tokens over up to 8,000, 8 key heads of 64: 212 us; traced 217 in attend_page_rows,
+// matrix cores 35% busy, VALU 48%, beside 32 in the other launches); their requests in
+// units of 32 rows took 293.
 //
 // Against one sequence's contiguous cache (attention.hpp), Q8_0, 8 key heads of 128, us:
 // 512 tokens over 15,873 368 beside 341, over 2,000 82 and 71, over none 37 and 36; 2,048 over

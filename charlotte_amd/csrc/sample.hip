@@ -742,8 +742,8 @@ __global__ __launch_bounds__(kDrawThreads) void row_draw(Sample a, DrawChunks c)
 }
 
 // About 512 workgroups, two a CU, a chunk of at least a four a thread; of whole fours.
-// 64 x 128,256 logits 53 us; 58 by 256 workgroups, 63 by 1,024 (a row's bins are cleared,
-// added up and counted a workgroup); 24 x 262,144 51, 53 and 61.
+// 64 x 128,256 logits 52 us; 57 by 256 workgroups, 62 by 1,024 (a row's bins are cleared,
+// added up and counted a workgroup); 24 x 262,144 52, 55 and 56.
 static uint32_t draw_chunks(uint32_t rows, uint32_t vocabulary) {
     const uint32_t most = (vocabulary + 3 + 4 * kDrawThreads - 1) / (4 * kDrawThreads);
     return std::max(1u, std::min((512 + rows - 1) / rows, most));

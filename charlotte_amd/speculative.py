@@ -12,10 +12,10 @@ layers, as a chain (drawn from their probabilities) or, with a width, as a tree
 (the likeliest first tokens, each continued with the likeliest); the accepted
 path's slots are moved together in both caches. Past lengths stay on the device.
 
-torch holds the memory, and does the layers' norms and the sums of the residual
+torch holds the memory, does the layers' norms and the sums of the residual
 stream (charlotte_amd/batching.py has them of the library) and finds the drafts'
-largest logits. It brings a HIP
-runtime of its own, so a process imports torch (or this module) before the rest.
+largest logits. It brings a HIP runtime of its own, so a process imports torch
+(or this module) before the rest.
 """
 
 import argparse

@@ -481,6 +481,45 @@ def test_requests_that_share_pages(ctx, dev):
     pool.pool.free()
 
 
+def test_many_rows_over_long_pieces(ctx, dev):
+    """Pieces of more tiles than a workgroup keeps the places of, beside a short request; rows here and there against 64 bits."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+    from tests.support import serving_ref as ref
+
+    rng = np.random.default_rng(67)
+    heads, kv_heads, dim, page_tokens = 64, 2, 32, 64
+    past, counts = [67003, 40], [512, 2]
+    held = [-(-(p + c) // page_tokens) for p, c in zip(past, counts)]
+    pages, stride = sum(held), max(held)
+    order = rng.permutation(pages)
+    table = np.full((2, stride), NOWHERE, np.uint64)
+    table[0, :held[0]], table[1, :held[1]] = order[:held[0]], order[held[0]:]
+    slots = [np.arange(p + c) % page_tokens + table[r, np.arange(p + c) // page_tokens] * page_tokens
+             for r, (p, c) in enumerate(zip(past, counts))]
+    k, v = ([rng.standard_normal((len(x), kv_heads, dim)).astype(np.float32) for x in slots] for _ in range(2))
+    pool = _Pool(dev, "q8_0", pages, page_tokens, kv_heads, dim)
+    pool.write(*(np.concatenate(x).reshape(-1, kv_heads * dim) for x in (k, v)), np.concatenate(slots))
+    rows = sum(counts)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    need = sv.paged_attention_workspace_bytes(ctx, pool.pool, heads, 512)
+    work, _ = dev.room(need, np.uint8)
+    out, read = dev.room(rows * heads * dim)
+    sv.paged_attention(ctx, sv.PagedAttention(pool.pool, dev.put(q), out, heads, dim ** -0.5, 2, rows, dev.put(_words(past)),
+                                              dev.put(_words(counts)), dev.put(_words([0, 512, 514])), dev.put(_words(table)), stride,
+                                              most=512, workspace=work, workspace_bytes=need))
+    hx.sync()
+    got = read().reshape(rows, heads, dim)
+    assert np.isfinite(got).all()
+    held_kv = [[ref.stored(x, "q8_0") for x in kv] for kv in zip(k, v)]
+    for row in (0, 1, 255, 301, 511, 512, 513):
+        r, t = (0, row) if row < 512 else (1, row - 512)
+        n = past[r] + t + 1
+        want, weight, size = ref.attention(q[row:row + 1], *(x[:n] for x in held_kv[r]), past[r] + t, dim ** -0.5)
+        assert (np.abs(got[row:row + 1] - want) <= ref.attention_bound(weight, size, n + 32 * 256, dim)).all(), row
+    pool.pool.free()
+
+
 def test_rows_of_no_request_are_left_as_they_were(ctx, dev):
     _check_paged(dev, "q8_0", [(20, 3), (50, 1), (90, 2)], 4, 2, 64, rows=9, seed=2)
     _check_paged(dev, "q8_0", [(20, 3), (50, 1), (90, 2)], 4, 2, 64, granted=[3, 0, 2], seed=2)
