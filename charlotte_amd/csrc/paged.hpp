@@ -1,7 +1,7 @@
 // Attention of several requests' new tokens over their pages (attention.hpp's
 // arithmetic): attend_pages with few rows a workgroup, 16 or 32 of a key head, its
 // waves taking the tiles in turn through LDS rings and joined in LDS;
-// attend_page_rows, for the requests of a step that bring kManyRows and more,
+// attend_page_rows, for the requests of a step that bring many_from rows and more,
 // with 128 or 256, a tile laid out once for all of them.
 //
 // The requests' lengths are known to the device alone, and are anything: a
@@ -110,7 +110,7 @@ struct Request {
     bool over;              // its tokens pass the table's row
 };
 
-// `many`: requests of kManyRows rows and more are the other kernel's.
+// `many`: requests of many_from rows and more are the other kernel's.
 template <uint32_t ROWS>
 __device__ __forceinline__ void place_request(const PagedAttention& a, Request& r, bool many) {
     if (uint64_t{r.start} + r.count > a.rows) r.count = 0;
@@ -122,12 +122,12 @@ __device__ __forceinline__ void place_request(const PagedAttention& a, Request& 
         r.begin = 0, r.tiles = 1;
         return;
     }
-    if (many && rows >= kManyRows) r.groups = 0;
+    if (many && rows >= a.many_from) r.groups = 0;
     r.begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
     r.tiles = (static_cast<uint32_t>(end) + kTile - 1) / kTile - r.begin;
 }
 
-// Whether the requests of kManyRows rows and more are worth their own kernel: 32 rows by
+// Whether the requests of many_from rows and more are worth their own kernel: 32 rows by
 // a tile of theirs number a.many_load a workgroup and more. The same in every kernel
 // of the step.
 __device__ __forceinline__ bool many_rows(const PagedAttention& a) {
@@ -136,7 +136,7 @@ __device__ __forceinline__ bool many_rows(const PagedAttention& a) {
     uint32_t load = 0;
     for (uint32_t i = lane * share; i < min((lane + 1) * share, a.requests); ++i) {
         Request r{a.past[i], a.counts[i], a.starts[i], 0, 0, 0, false};
-        if (uint64_t{r.start} + r.count > a.rows || r.count * a.group < kManyRows) continue;
+        if (uint64_t{r.start} + r.count > a.rows || r.count * a.group < a.many_from) continue;
         const uint64_t end = uint64_t{r.past} + r.count;
         if (end > uint64_t{a.table_stride} * a.pool.capacity) continue;
         const uint32_t begin = a.window && r.past + 1 > a.window ? (r.past + 1 - a.window) / kTile : 0;
@@ -486,7 +486,7 @@ struct ManyLine {
 
     __device__ __forceinline__ Many many_of(uint32_t i) const {
         Many m{i, a.past[i], a.counts[i], a.starts[i], 0};
-        const bool mine = uint64_t{m.start} + m.count <= a.rows && m.count * a.group >= kManyRows &&
+        const bool mine = uint64_t{m.start} + m.count <= a.rows && m.count * a.group >= a.many_from &&
                           uint64_t{m.past} + m.count <= uint64_t{a.table_stride} * a.pool.capacity;
         if (mine) m.groups = (m.count * a.group + ROWS - 1) / ROWS;
         return m;

@@ -110,7 +110,7 @@ void check_table(uint32_t requests, uint32_t table_stride, uint32_t page_tokens)
 }
 
 // How a step of attention runs: requests of up to 16 rows of a key head by units of
-// 16, of more by units of 32, of kManyRows and more, where they are load enough, by
+// 16, of more by units of 32, of many_from and more, where they are load enough, by
 // units of `many`; each in launches of its own, of which one that finds no request of
 // its kind takes 4 - 5 us. One request, which is of one kind, and groups past 16 have no
 // launch of units of 16.
@@ -124,7 +124,7 @@ PagedPlan paged_plan(const chm::CacheShape& c, uint32_t group, uint32_t most, ui
     PagedPlan plan{requests > 1 && group <= 16, true, 0, 0};
     // the loads at which attention takes its form of many rows (attention_plan.cpp)
     const uint32_t load = c.head_dim <= 64 ? 112 : c.head_dim <= 128 ? 44 : 11;
-    if (rows >= chm::kManyRows && chm::many_rows_of(c.format, c.head_dim) && most_load >= load)
+    if (rows >= chm::many_from(c.head_dim) && chm::many_rows_of(c.format, c.head_dim) && most_load >= load)
         plan.many = c.head_dim <= 128 ? 256 : 128, plan.many_load = load;
     return plan;
 }
@@ -303,7 +303,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_paged_attention(charlotte_hip_m
                    : c.format == chm::kQ4_0 ? chm::launch_paged_q4_0(a, octets, s)
                                             : chm::launch_paged_q8_0(a, octets, s);
         };
-        a.many_load = plan.many_load;
+        a.many_from = chm::many_from(c.head_dim), a.many_load = plan.many_load;
         a.above = 0, a.upto = 0xFFFFFFFFu;
         if (plan.many)
             if (hipError_t e = run(plan.many, 0); e != hipSuccess) return e;

@@ -55,9 +55,9 @@ struct PagedAttention {
     uint32_t* counters;  // pieces of a unit that are done; 0 between launches
     uint32_t requests, rows, table_stride, group, window, parts;
     // attend_pages has the requests of more rows of a key head than `above`, up to
-    // `upto`; but those of kManyRows and more are attend_page_rows' where their load
+    // `upto`; but those of many_from and more are attend_page_rows' where their load
     // is many_load and more (0: never).
-    uint32_t above, upto, many_load;
+    uint32_t above, upto, many_from, many_load;
     uint32_t page_inverse;  // of a page's tiles, where they are two and more: 2^32 over them, rounded up
     float scale;
 };
@@ -65,8 +65,10 @@ struct PagedAttention {
 // Pieces of units that a step may leave, a workgroup.
 constexpr uint32_t kPieces = 2;
 // Rows of a key head from which a request has workgroups of many rows, in the
-// formats and widths that attention has them for (attention_plan.cpp).
-constexpr uint32_t kManyRows = 256;
+// formats and widths that attention has them for (attention_plan.cpp). 8 requests over
+// 4,000, 8 key heads in Q8_0, so and by units of 32: 128 rows of 128 values 101 us and 109,
+// of 64 61 and 44; 256 rows 129 and 200, 78 and 84.
+constexpr uint32_t many_from(uint32_t head_dim) { return head_dim <= 64 ? 256 : 128; }
 constexpr bool many_rows_of(uint32_t format, uint32_t head_dim) { return format == 1 /* F16 */ || head_dim <= 128; }
 // `octets`: 1 or 2 of attend_pages; 0: attend_page_rows, and what joins its pieces.
 hipError_t launch_paged_f16(const PagedAttention& a, uint32_t octets, hipStream_t stream);

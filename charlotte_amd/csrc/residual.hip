@@ -7,7 +7,7 @@
 // and, over its waves, one pass through LDS. The weights and the gate are read
 // with the row, ahead of the sums that they wait for.
 //
-// Bound by bytes, 16 a value with both results: 2,048 rows of 4,096 (134 MB) 28 us, 4.8
+// Bound by bytes, 16 a value with both results: 2,048 rows of 4,096 (134 MB) 28 us, 4.7
 // TB/s. One row of 1,024 2.4 us, latency; 333 gated ones of 1,155, at addresses that
 // are no fours', 5.2.
 #include "requests.hpp"

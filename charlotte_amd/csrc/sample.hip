@@ -27,9 +27,9 @@
 // written back or cleared for it.
 //
 // Bound by f64 arithmetic and by the chains of each row's last workgroups: 1 x 151,936 logits
-// 22 us (3.4 + 10.4 + 9.3: a chunk a workgroup, then the bins searched, then the list
-// sorted); 64 x 128,256, settings a row, 51 (7.3, read at 4.5 TB/s, + 25.2: 30 operations
-// of f64 a logit, 7 us at their full rate, two adds to LDS, the bins added up + 17.9);
+// 22 us (3.3 + 9.9 + 8.7: a chunk a workgroup, then the bins searched, then the list
+// sorted); 64 x 128,256, settings a row, 51 (8.2, read at 4.0 TB/s, + 25.5: 30 operations
+// of f64 a logit, 7 us at their full rate, two adds to LDS, the bins added up, + 17.6);
 // 24 x 262,144 by temperature alone 50. Weights of f32's exponential in the bins, with
 // bounds, and the exact ones summed in row_draw took as long where few tokens lay within
 // the bounds, and 200 - 600 us where a draw near the end of a flat row had thousands.
