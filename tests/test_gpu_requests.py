@@ -481,6 +481,13 @@ def test_requests_that_share_pages(ctx, dev):
     pool.pool.free()
 
 
+@pytest.mark.parametrize("format_,dim,rows", [("q8_0", 128, 128), ("q4_0", 64, 256), ("f16", 160, 128)])
+def test_requests_of_about_many_rows(ctx, dev, format_, dim, rows):
+    """A row less than takes the form of many rows, as many, one more, and few, in one step."""
+    _check_paged(dev, format_, [(3300, rows - 1), (3300, rows), (7, 1), (3301, rows + 1)], 16, 16, dim, page_tokens=64, seed=dim,
+                 twice=True)
+
+
 def test_many_rows_over_long_pieces(ctx, dev):
     """Pieces of more tiles than a workgroup keeps the places of, beside a short request; rows here and there against 64 bits."""
     from charlotte_amd import harness as hx
