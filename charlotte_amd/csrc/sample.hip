@@ -389,8 +389,9 @@ __device__ __forceinline__ Ends ends_of(const DrawChunks& c, uint32_t row) {
     return {most_of_wave(e.largest), least_of_wave(e.smallest)};
 }
 
-// An infinite logit, or two whose distance f32 does not hold: the row has no bins.
-__device__ __forceinline__ bool too_far(float most, float smallest) { return most - smallest == INFINITY; }
+// An infinite logit, or two whose distance f32 does not hold: the row has no bins. (Of +inf
+// and -inf alone the smallest is +inf too, and the distance a NaN.)
+__device__ __forceinline__ bool too_far(float most, float smallest) { return !(most - smallest < INFINITY); }
 
 // A logit's place among the bins: it does not fall as the logit does.
 __device__ __forceinline__ float place_of(float l, float most, float steps) {

@@ -796,6 +796,26 @@ def test_sample_rows_with_nothing_or_not_finite(ctx, dev, vocabulary):
         assert got[:3].tolist() == [-1, -1, 0]
 
 
+@pytest.mark.parametrize("vocabulary", [1, 2, 7, 5000, 151936])
+@pytest.mark.parametrize("settings", [(1.0, 0, 1.0, 0.0), (0.7, 3, 1.0, 0.0), (2.0, 0, 0.6, 0.0), (1.0, 0, 1.0, 0.3), (1e-3, 2, 0.9, 1.0)])
+def test_sample_rows_of_infinities_alone(ctx, dev, vocabulary, settings):
+    """A token forced by +inf among -inf, several of them, and nothing else: those of +inf weigh 2^40, the rest nothing."""
+    rng = np.random.default_rng(vocabulary)
+    logits = np.full((6, vocabulary), -np.inf, np.float32)
+    logits[0] = np.inf
+    logits[1, -1] = np.inf
+    logits[2, vocabulary // 2] = np.inf
+    logits[3, ::3] = np.inf
+    logits[4] = np.where(np.arange(vocabulary) % 2, np.float32(np.nan), np.float32(np.inf))
+    logits[5, vocabulary // 3:] = np.inf
+    for u in (0.0, 0.5, 0.99999994):
+        got = _check_sample(ctx, dev, logits, [(*settings, u)] * 6, {"stride": vocabulary + 3, "offset": 4})
+        assert got[1] == vocabulary - 1 and got[2] == vocabulary // 2
+    # each row's own setting, and rows with finite logits beside them
+    logits = np.concatenate([logits, rng.standard_normal((3, vocabulary)).astype(np.float32)])
+    _check_sample(ctx, dev, logits, _settings(rng, 9))
+
+
 @pytest.mark.parametrize("vocabulary", [40, 50001])
 def test_sample_settings_at_their_ends(ctx, dev, vocabulary):
     rng = np.random.default_rng(2)
