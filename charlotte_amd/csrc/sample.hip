@@ -48,10 +48,14 @@ constexpr uint32_t kList = 2048;  // tokens gathered of a row
 constexpr float kReach = 27.8f;
 constexpr double kWhole = 1099511627776.0;  // 2^40
 
+// log2(e) / temperature, in two parts.
+struct Octaves {
+    double high, low;
+};
 // A row's settings, as its kernels use them.
 struct Settings {
     double rate;       // 1 / temperature
-    double octaves;    // log2(e) / temperature
+    Octaves octaves;
     uint64_t top_k;    // tokens
     double top_p;      // 1: all
     uint64_t least;    // min_p's weight
@@ -66,8 +70,11 @@ __device__ __forceinline__ Settings settings_of(const Sample& a, uint32_t row) {
     const float u = a.uniforms[row];
     Settings s;
     s.greedy = !(t >= 1e-6f) || k == 1;
-    s.rate = s.greedy ? 1.0 : 1.0 / static_cast<double>(t);
-    s.octaves = s.rate * 1.44269504088896340736;
+    const double heat = s.greedy ? 1.0 : static_cast<double>(t);
+    s.rate = 1.0 / heat;
+    constexpr double kLog2E = 1.44269504088896340736, kLog2ELow = 2.0355273740931033e-17;
+    s.octaves.high = s.rate * kLog2E;
+    s.octaves.low = s.rate > 0.0 ? (__builtin_fma(-s.octaves.high, heat, kLog2E) + kLog2ELow) * s.rate : 0.0;
     s.top_k = k > 0 && static_cast<uint32_t>(k) < a.vocabulary ? static_cast<uint32_t>(k) : a.vocabulary;
     s.top_p = p < 1.0f ? fmax(static_cast<double>(p), 0.0) : 1.0;  // (a NaN: 1)
     s.least = static_cast<uint64_t>(ceil((m > 0.0f ? fmin(static_cast<double>(m), 1.0) : 0.0) * kWhole));
@@ -86,30 +93,33 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// floor(2^40 exp((l - m) rate)), `octaves` = rate log2(e), of a finite m: 2^z by its
-// series, z within half of a whole number (the 12th term is below 2^-47), all of it
-// within 2^-46. A whole number that f64 holds.
-__device__ __forceinline__ double whole_weight(float l, double most, double octaves) {
-    const double y = fmax((static_cast<double>(l) - most) * octaves, -64.0);
-    const double whole = rint(y), z = (y - whole) * 0.693147180559945309417;
-    double p = 1.0 / 39916800;
-    p = __builtin_fma(p, z, 1.0 / 3628800);
-    p = __builtin_fma(p, z, 1.0 / 362880);
-    p = __builtin_fma(p, z, 1.0 / 40320);
-    p = __builtin_fma(p, z, 1.0 / 5040);
-    p = __builtin_fma(p, z, 1.0 / 720);
-    p = __builtin_fma(p, z, 1.0 / 120);
-    p = __builtin_fma(p, z, 1.0 / 24);
-    p = __builtin_fma(p, z, 1.0 / 6);
-    p = __builtin_fma(p, z, 0.5);
-    p = __builtin_fma(p, z, 1.0);
+// floor(2^40 exp((l - m) / T)), l not so far below a finite m that the power has no
+// exponent: (l - m) log2(e) / T in two parts, whose nearest whole number is taken off
+// before it is rounded, and 2^z of what is left by the polynomial of degree 11 whose
+// largest relative error there is least (Remez's exchange; 2^-54.7 with its terms in f64).
+// In all within 1.25 units of f64's last place; a whole number that f64 holds.
+__device__ __forceinline__ double whole_weight(float l, double most, const Octaves& octaves) {
+    const double d = static_cast<double>(l) - most, whole = rint(d * octaves.high);
+    const double z = __builtin_fma(d, octaves.low, __builtin_fma(d, octaves.high, -whole));
+    double p = 4.4352819196017726e-10;
+    p = __builtin_fma(p, z, 7.074105632845698e-09);
+    p = __builtin_fma(p, z, 1.0178198028606432e-07);
+    p = __builtin_fma(p, z, 1.3215433089687149e-06);
+    p = __builtin_fma(p, z, 1.525273348996672e-05);
+    p = __builtin_fma(p, z, 0.0001540353046251404);
+    p = __builtin_fma(p, z, 0.001333355814678995);
+    p = __builtin_fma(p, z, 0.009618129107588335);
+    p = __builtin_fma(p, z, 0.055504108664819925);
+    p = __builtin_fma(p, z, 0.24022650695910155);
+    p = __builtin_fma(p, z, 0.6931471805599453);
     p = __builtin_fma(p, z, 1.0);
     return floor(ldexp(p, static_cast<int>(whole) + 40));
 }
 
-__device__ __forceinline__ uint64_t weight_of(float l, float most, double octaves) {
+__device__ __forceinline__ uint64_t weight_of(float l, float most, const Octaves& octaves) {
     if (l == most) return 1ull << 40;
     if (l == -INFINITY || most == INFINITY) return 0;
+    if ((static_cast<double>(l) - most) * octaves.high < -64.0) return 0;
     return static_cast<uint64_t>(whole_weight(l, most, octaves));
 }
 
@@ -140,7 +150,7 @@ struct DrawRow {
     const float* x;
     uint32_t lead, vocabulary;
     float most;
-    double octaves;
+    Octaves octaves;
 
     // f(logit, index) for each of the row's tokens.
     template <typename F>

@@ -849,7 +849,7 @@ charlotte_hip_matmul_status charlotte_hip_matmul_residual_norm(charlotte_hip_mat
  * the kept tokens' sum and r = floor(u 2^31) (u as verify takes it: one outside 0
  * .. 1 - 2^-24 as the nearer end, a NaN as 0), the token drawn is the first whose
  * running sum passes floor(W r / 2^31): in whole numbers, but for the exponential
- * (in f64, within a unit of its last place).
+ * (of l - m in f64, within 1.25 units of f64's last place) and top_p's product (f64).
  *
  * tokens gets the token, -1 for a row of nothing but -inf; chances, if given, its
  * weight over W (such a row: 0). The settings are a row's own where their array is

@@ -846,6 +846,70 @@ def test_sample_logits_as_far_apart_as_f32_has_them(ctx, dev):
     _check_sample(ctx, dev, logits, [(1e38, 0, 1.0, 0.0, 0.97), (2e38, 90, 1.0, 0.01, 0.999)])
 
 
+def _whole_weight(logit, temperature):
+    """2^40 exp(logit / temperature) of f32s, to 60 digits."""
+    import decimal
+
+    with decimal.localcontext() as c:
+        c.prec = 60
+        return (decimal.Decimal(float(logit)) / decimal.Decimal(float(temperature))).exp() * (1 << 40)
+
+
+def _about_a_whole_number(rng, temperature, above):
+    """A logit whose weight is 2 - 12 units of f64's last place above a whole number, or below one, and below 2^40 by less than half."""
+    while True:
+        logits = (-rng.random(4096) * 0.69 * temperature).astype(np.float32)
+        weights = np.exp(logits.astype(np.longdouble) / np.longdouble(temperature)) * (1 << 40)
+        parts = (weights % 1 if above else 1 - weights % 1) * 8192
+        for logit in logits[(parts > 2) & (parts < 12)]:
+            part = float(_whole_weight(logit, temperature) % 1) * 8192
+            if 2 < (part if above else 8192 - part) < 12:
+                return logit
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 3.3])
+@pytest.mark.parametrize("vocabulary", [37, 30001])
+def test_sample_weights_are_whole_numbers_of_the_exponential(ctx, dev, temperature, vocabulary):
+    """Rows whose weights are 2^40 and others that together are 2^40 + 1, or 2^40: with top_p of a half the first token is
+    not all that is kept, or is. Among them is one whose exponential lies 2 to 12 units of f64's last place from a whole
+    number, so that one that is off by as much makes it the other; those of the rest lie far from one."""
+    from charlotte_amd import harness as hx
+    from charlotte_amd import serving as sv
+
+    rng = np.random.default_rng(vocabulary)
+    t = np.float32(temperature)
+    rows, lines, want = 24, [], []
+    for row in range(rows):
+        above = row % 2 == 0  # what is too small by a unit falls below the whole number
+        logits = [np.float32(0), _about_a_whole_number(rng, t, above)]
+        left = (1 << 40) + (1 if above else 0) - int(_whole_weight(logits[1], t))
+        while left:
+            logit = np.float32(float(t) * np.log((left + 0.5) * 2.0 ** -40))
+            while not (int(_whole_weight(logit, t)) <= left and 0.1 < _whole_weight(logit, t) % 1 < 0.9):
+                logit = np.nextafter(logit, np.float32(-np.inf))
+            logits.append(logit)
+            left -= int(_whole_weight(logit, t))
+        weights = [int(_whole_weight(x, t)) for x in logits]
+        assert sum(weights) == (2 << 40) + (1 if above else 0)
+        line = np.full(vocabulary, -np.inf if row % 3 else -1e4, np.float32)
+        places = rng.permutation(vocabulary)[:len(logits)]
+        line[places] = logits
+        lines.append(line)
+        order = sorted(range(len(logits)), key=lambda i: (-logits[i], places[i]))
+        kept = order[:2] if above else order[:1]
+        total, u = sum(weights[i] for i in kept), 0.99999994
+        token = next(i for n, i in enumerate(kept) if sum(weights[j] for j in kept[:n + 1]) > total * int(u * 2.0 ** 31) >> 31)
+        want.append((places[token], weights[token] / total))
+    need = sv.sample_workspace_bytes(rows, vocabulary)
+    work, _ = dev.room(need, np.uint8)
+    (out, read), (chances, read_chances) = dev.room(rows, np.int32), dev.room(rows)
+    sv.sample(ctx, sv.Sample(dev.put(np.array(lines)), out, rows, vocabulary, dev.put(np.full(rows, 0.99999994, np.float32)),
+                             temperature, 0, 0.5, chances=chances, workspace=work, workspace_bytes=need))
+    hx.sync()
+    assert read().tolist() == [x for x, _ in want]
+    assert np.abs(read_chances() - [c for _, c in want]).max() <= 2.0 ** -24
+
+
 def test_samples_follow_the_weights(ctx, dev):
     """Every token's share of many draws over a grid of uniform numbers, to one draw."""
     from tests.support import requests_ref as ref
