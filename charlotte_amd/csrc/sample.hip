@@ -483,10 +483,13 @@ __device__ void plan_row(const Sample& a, const Settings& s, float steps, DrawRo
         low = max(d.sums[top_p.first], 1ull << 40), high = min(high, d.sums[top_p.last + 1]);
     }
     if (s.least > 0) {
-        // min_p's last token is in the bin of its distance or, by rounding, one beside it
-        const double at = -log(static_cast<double>(s.least) / kWhole) / s.rate * static_cast<double>(steps);
-        const uint32_t bin = static_cast<uint32_t>(fmin(at, static_cast<double>(kBins - 1)));
-        const uint32_t from = bin > 1 ? bin - 1 : 0, to = min(bin + 2, kBins);
+        // min_p's last token is in the bin of its distance or, by rounding, one beside it; of a
+        // temperature so far above the logits that f64's exponentials are alike over several
+        // bins, one of those (of an infinite one, where both are NaNs or infinite: of all)
+        const double bins = static_cast<double>(steps) / s.rate;
+        const double at = -log(static_cast<double>(s.least) / kWhole) * bins, off = 1.0 + 0x1p-50 * bins;
+        const uint32_t from = static_cast<uint32_t>(fmin(fmax(at - off, 0.0), static_cast<double>(kBins - 2)));
+        const uint32_t to = static_cast<uint32_t>(fmin(at + off, static_cast<double>(kBins - 1))) + 1;
         low = min(low, max(d.sums[from], 1ull << 40)), high = min(high, d.sums[to]);
         if (lane == 0) room.end_first = from, room.end_past = to, room.end_ahead = d.sums[from];
     }

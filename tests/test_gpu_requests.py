@@ -841,6 +841,31 @@ def test_sample_where_many_tokens_are_alike(ctx, dev, temperature):
     _check_sample(ctx, dev, logits, settings)
 
 
+@pytest.mark.parametrize("temperature", [1e12, 1e15, 3e16, 1e18, 3e38, float("inf")])
+@pytest.mark.parametrize("vocabulary", [40, 1000, 50001])
+def test_sample_among_weights_that_f64_does_not_tell_apart(ctx, dev, temperature, vocabulary, monkeypatch):
+    """Temperatures so far above the logits that the exponential of many, or of all, is one: min_p keeps them all. Here the
+    last bit decides what is kept, so the exponential is the correctly rounded one, 1 + expm1 where it is within 2^-26 of 1
+    (numpy's own is 1 - 2^-53 at -5e-17, and 1 - 2^-52 at -1.6e-16, where the nearest are 1 and 1 - 2^-53)."""
+    from tests.support import requests_ref as ref
+
+    class Rounded:
+        def __getattr__(self, name):
+            return getattr(np, name)
+
+        @staticmethod
+        def exp(x):
+            return 1 + np.expm1(x)
+
+    monkeypatch.setattr(ref, "np", Rounded())
+    rng = np.random.default_rng(vocabulary)
+    logits = (rng.standard_normal((10, vocabulary)) * 2).astype(np.float32)
+    logits[2] *= np.float32(1e-20)
+    settings = [(temperature, 0, 1.0, 1.0), (temperature, vocabulary // 2, 1.0, 1.0), (temperature, 0, 1.0, 1.0),
+                (temperature, 0, 0.7, 1.0), (temperature, 0, 1.0, 0.9999999)]
+    _check_sample(ctx, dev, logits, [(*s, u) for u in (0.3, 0.99999994) for s in settings])
+
+
 def test_sample_logits_as_far_apart_as_f32_has_them(ctx, dev):
     logits = np.array([[-3e38, 3e38, 0.0, 1e38, -1e38] * 40, [3.4e38, -3.4e38, 1.0, 2.0, -np.inf] * 40], np.float32)
     _check_sample(ctx, dev, logits, [(1e38, 0, 1.0, 0.0, 0.97), (2e38, 90, 1.0, 0.01, 0.999)])
