@@ -4,6 +4,7 @@
 // what they hold is checked by the kernels.
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "checks.hpp"
 #include "formats.hpp"
@@ -345,8 +346,9 @@ charlotte_hip_matmul_status charlotte_hip_matmul_residual_norm(charlotte_hip_mat
         if (d.residual_out && d.residual_out == d.normed) refuse("two results in one place");
         for (const float* shared : {d.branch_weight, d.weight})  // other rows read it
             if (shared && (shared == d.residual_out || shared == d.normed)) refuse("a result over a weight");
-        for (const float* input : {d.residual, d.branch, d.gate}) {
-            const uint64_t stride = input == d.residual ? a.residual_stride : input == d.branch ? a.branch_stride : a.gate_stride;
+        // each with a stride of its own, whichever of them are one memory
+        for (const auto& [input, stride] : {std::pair{d.residual, a.residual_stride}, std::pair{d.branch, a.branch_stride},
+                                            std::pair{d.gate, a.gate_stride}}) {
             in_place(d.residual_out, a.residual_out_stride, input, stride);
             in_place(d.normed, a.normed_stride, input, stride);
         }
