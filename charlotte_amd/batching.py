@@ -126,6 +126,10 @@ class Batch:
             raise ValueError("a request that the pool does not hold by itself")
         if not request.prompt:
             raise ValueError("a request without a prompt")
+        if len(request.taken) >= request.tokens:
+            raise ValueError(f"a request of {request.tokens} tokens, of which it has {len(request.taken)}")
+        if min(request.prompt) < 0 or max(request.prompt) >= self.model.config.vocabulary:
+            raise ValueError(f"a prompt with a token past the vocabulary of {self.model.config.vocabulary}")
         self.waiting.append(request)
 
     def _layers(self, rows, most, stream):
