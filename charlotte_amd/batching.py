@@ -42,6 +42,7 @@ class Request:
     seed: int = 0
     taken: list = field(default_factory=list)
     chances: list = field(default_factory=list)
+    failed: bool = False       # its logits had no number: it ended with the tokens before
 
     def __post_init__(self):
         self.random = np.random.default_rng(self.seed)
@@ -191,14 +192,16 @@ class Batch:
             sv.sample(self.ctx, self.draw, stream=stream)
         granted, tokens, chances = (t.cpu().numpy() for t in (self.granted, self.tokens, self.chances))
         for at, r in enumerate(drawing):
-            if granted[r]:
+            if granted[r] and tokens[at] < 0:  # a row of NaNs and -inf
+                self.active[r].failed = True
+            elif granted[r]:
                 self.active[r].taken.append(int(tokens[at]))
                 self.active[r].chances.append(float(chances[at]))
             else:
                 self.active[r].random = _before(self.active[r])
         self.read += granted
         self.steps += 1
-        done = [r for r in here if len(self.active[r].taken) >= self.active[r].tokens]
+        done = [r for r in here if self.active[r].failed or len(self.active[r].taken) >= self.active[r].tokens]
         for r in done:
             self.finished.append(self.active[r])
             self.active[r], self.read[r], self.crowded = None, 0, False

@@ -10,6 +10,7 @@ import torch
 from charlotte_amd import batching as ba
 from charlotte_amd import matmul as mm
 from charlotte_amd import speculative as sp
+from charlotte_amd import synthetic
 
 CONFIG = dict(vocabulary=1024, hidden=256, layers=3, draft_layers=1, heads=6, kv_heads=2, head_dim=64, feed_forward=512)
 
@@ -77,10 +78,40 @@ def refusals(ctx):
         raise AssertionError((together, rows, longest))
 
 
+def spoilt(ctx, cache):
+    """A request whose stream is not numbers ends as failed, without a token; those beside it are as they are without it."""
+    c = sp.Config(**CONFIG)
+    model = sp.Model(ctx, c, seed=4)
+    rows = np.frombuffer(synthetic.weight(np.random.default_rng(4), int(c.weights), c.vocabulary, c.hidden), np.uint8).copy()
+    blocks = rows.reshape(c.vocabulary, c.hidden // 32, -1)
+    bad = 77
+    blocks[bad, 3, :2] = np.array([0x7E00], "<u2").view(np.uint8)  # a block's scale, not a number
+    model.table.free()
+    model.table = mm.Weight(ctx, c.weights, c.vocabulary, c.hidden, rows.tobytes())
+    found = []
+    for with_it in (False, True):
+        requests = _requests(model, [5, 90, 33, 64, 17, 2], 12, temperature=0.9, top_k=40)
+        for r in requests:
+            r.prompt = [bad + 1 if t == bad else t for t in r.prompt]
+        requests.insert(3, ba.Request([5, 9, bad, 3] + [1] * 40, 12, temperature=0.9))
+        requests.insert(1, ba.Request([bad], 12))
+        fine = [r for r in requests if bad not in r.prompt]
+        assert len(fine) == 6
+        batch = ba.Batch(model, together=4, pages=14, rows=48, longest=256, cache_type=mm.TensorType[cache])
+        _taken(batch, requests if with_it else fine)
+        assert len(batch.finished) == (8 if with_it else 6)
+        if with_it:
+            assert all(r.failed and not r.taken and not r.chances for r in requests if bad in r.prompt)
+        assert not any(r.failed for r in fine) and all(len(r.taken) == 12 for r in fine)
+        found.append([r.taken for r in fine])
+        batch.free()
+    assert found[0] == found[1]
+
+
 def main():
     name, arguments = sys.argv[1], sys.argv[2:]
     with mm.Context(0) as ctx:
-        {"greedy": greedy, "drawn": drawn, "refusals": refusals}[name](ctx, *arguments)
+        {"greedy": greedy, "drawn": drawn, "refusals": refusals, "spoilt": spoilt}[name](ctx, *arguments)
     print("passed")
 
 

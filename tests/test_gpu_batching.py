@@ -19,3 +19,8 @@ def test_batching(check):
                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     print(run.stdout, flush=True)
     assert run.returncode == 0 and run.stdout.endswith("passed\n")
+
+
+@pytest.mark.parametrize("cache", ["Q8_0", "Q4_0", "F16"])
+def test_a_request_without_numbers(cache):
+    test_batching(["spoilt", cache])
