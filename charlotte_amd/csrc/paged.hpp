@@ -22,19 +22,27 @@
 // MBs, a launch of its own joins them.
 //
 // Few rows are bound by the cache's bytes: 64 requests of 50 - 32,768 tokens, 8 key
-// heads of 128 in Q8_0 (731 MB), 140 - 141 us, 5.2 TB/s, as a large copy. One token over
+// heads of 128 in Q8_0 (731 MB), 140 - 146 us, 5.0 - 5.2 TB/s, as a large copy. One token over
 // 65,536, 8 heads of 64 in Q4_0 (38 MB): 23.8 us, of which 4.5 go before the first tile,
 // 11 over the tiles (the VALU: 4-bit codes widened for four rows of 16) and 8 from a
 // workgroup's last tile to the units' join. 3 requests of up to 911 tokens: 15 us, of the
 // same parts. Many rows are bound by the VALU and the matrix cores in turn (two prompts of
-// 512 tokens over up to 8,000, 8 key heads of 64: 212 us; traced 217 in attend_page_rows,
+// 512 tokens over up to 8,000, 8 key heads of 64: 212 - 219 us; traced 217 in attend_page_rows,
 // matrix cores 35% busy, VALU 48%, beside 32 in the other launches); their requests in
-// units of 32 rows took 293.
+// units of 32 rows took 293. The launches are one after the other: requests of 17 rows up to
+// many_from beside single tokens are two chains of 15 - 20 us.
 //
 // Against one sequence's contiguous cache (attention.hpp), Q8_0, 8 key heads of 128, us:
 // 512 tokens over 15,873 368 beside 341, over 2,000 82 and 71, over none 37 and 36; 2,048 over
-// 2,048 312 and 314; one over 65,536 39 and 33; F16, one key head of 256, 512 over 8,000
-// 87 and 68 (more registers than 256: some of the tile's are spilled).
+// 2,048 312 and 314; one over 65,536 39 and 33. What finds the work stays in registers over
+// the tiles: every kernel here keeps 23 - 122 scalars in lanes of vector registers (attend_rows
+// at most 4), heads of 32 in many rows have 3 waves a SIMD (there 4), and some vector registers
+// spill, which none does there: 6 and 4 of attend_page_rows in Q8_0 and Q4_0 with heads of 128, 4, 2
+// and 11 in F16 with 160, 224 and 256 (512 over 8,000, one key head of 256 87 - 90 us and 67), 32
+// and 29 of attend_pages of 32 rows in Q8_0 and Q4_0 with heads of 256.
+// Q8_0 and Q4_0 with heads of 160 - 256 have no form of many rows, as attention has none: 512 over
+// 8,000, heads of 256, one key head 110 and 108 us (contiguous 97 and 91), eight 652 and 639 (644 and
+// 573; 122 by the formula's operations, 304 with operands in parts); of 160, eight 439 and 416 (410 both).
 #pragma once
 
 #include "attention.hpp"
@@ -43,8 +51,8 @@
 namespace chm {
 
 // What a unit costs beside its tiles, in tiles (its queries, its waves' join). One token
-// each of 64 requests of 50 - 32,768 tokens, 8 key heads of 128 in Q8_0: 181 us at none,
-// 163 - 169 at 8, 156 at 16, 160 at 24; of 200 requests of 50 - 2,000 115, 92, 92 and 92.
+// each of 64 requests of 50 - 32,768 tokens, 8 key heads of 128 in Q8_0: 164 - 170 us at none,
+// 149 at 8, 144 at 16, 146 at 24; of 200 requests of 50 - 2,000 115, 92, 92 and 92.
 constexpr uint32_t kUnitTiles = 16;
 // Tiles more than on the line that a workgroup may have for units cut in pieces:
 // about what a unit's ends cost that the line leaves in two workgroups. 8 requests of

@@ -69,6 +69,8 @@ constexpr uint32_t kPieces = 2;
 // 4,000, 8 key heads in Q8_0, so and by units of 32: 128 rows of 128 values 101 us and 109,
 // of 64 61 and 44; 256 rows 129 and 200, 78 and 84.
 constexpr uint32_t many_from(uint32_t head_dim) { return head_dim <= 64 ? 256 : 128; }
+// (Wider quantized heads: 4 waves' rows are too few to pay for laying codes out, 387 us beside 308 of a
+// contiguous cache, attention_plan.cpp; by units of 32 here: paged.hpp.)
 constexpr bool many_rows_of(uint32_t format, uint32_t head_dim) { return format == 1 /* F16 */ || head_dim <= 128; }
 // `octets`: 1 or 2 of attend_pages; 0: attend_page_rows, and what joins its pieces.
 hipError_t launch_paged_f16(const PagedAttention& a, uint32_t octets, hipStream_t stream);

@@ -7,9 +7,9 @@
 // and, over its waves, one pass through LDS. The weights and the gate are read
 // with the row, ahead of the sums that they wait for.
 //
-// Bound by bytes, 16 a value with both results: 2,048 rows of 4,096 (134 MB) 28 us, 4.7
-// TB/s. One row of 1,024 2.4 us, latency; 333 gated ones of 1,155, at addresses that
-// are no fours', 5.2.
+// Bound by bytes, 16 a value with both results: 2,048 rows of 4,096 (134 MB) out of memory
+// 26.7 - 28 us, 4.7 - 5.0 TB/s; 20.8 where the card's last cache has half of it. One row of
+// 1,024 2.4 us, latency; 333 gated ones of 1,155, at addresses that are no fours', 5.1 - 6.3.
 #include "requests.hpp"
 
 namespace chm {
@@ -136,9 +136,10 @@ static hipError_t launch_fours(const ResidualNorm& a, uint32_t threads, hipStrea
 
 hipError_t launch_residual_norm(const ResidualNorm& a, hipStream_t stream) {
     // A four a thread while the card holds all rows' threads about at once, else four of
-    // them: the same row in a quarter of the waves. Rows of 4,096, one and four: 1 row 3.9 us
-    // and 4.0, 333 7.5 and 6.9, 512 8.4 and 8.0, 1,024 15.4 and 12.3, 2,048 25.6 and
-    // 21.8; 333 of 1,155 5.1 and 6.8.
+    // them: the same row in a quarter of the waves. With a branch and both results, out of
+    // memory, one and four: rows of 4,096, 1 row 3.0 us and 3.2, 333 7.6 and 7.7, 512 8.2 and
+    // 8.2, 513 10.2 and 8.5, 1,024 15.9 and 11.8, 2,048 28.3 and 26.7; of 2,048, 513 5.7 and 5.8,
+    // 2,048 15.1 and 12.1; of 1,024 (always one), 2,048 8.1 and 8.2. 333 gated of 1,155 6.3 and 7.2.
     const uint32_t fours = (a.width + 3) / 4;
     auto threads = [&](uint32_t each) { return (fours + 64 * each - 1) / (64 * each) * 64; };
     if (threads(1) <= 256 || (threads(1) <= 64 * kMostWaves && a.rows <= 512)) return launch_fours<1>(a, threads(1), stream);

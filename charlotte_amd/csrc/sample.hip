@@ -26,13 +26,16 @@
 // each workgroup waits for its own to arrive, then counts itself; no cache is
 // written back or cleared for it.
 //
-// Bound by f64 arithmetic and by the chains of each row's last workgroups: 1 x 151,936 logits
-// 22 us (3.3 + 9.9 + 8.7: a chunk a workgroup, then the bins searched, then the list
-// sorted); 64 x 128,256, settings a row, 51 (8.2, read at 4.0 TB/s, + 25.5: 30 operations
-// of f64 a logit, 7 us at their full rate, two adds to LDS, the bins added up, + 17.6);
-// 24 x 262,144 by temperature alone 50. Weights of f32's exponential in the bins, with
-// bounds, and the exact ones summed in row_draw took as long where few tokens lay within
-// the bounds, and 200 - 600 us where a draw near the end of a flat row had thousands.
+// Bound by the weights' f64 and by what ends a row: 1 x 151,936 logits 22 - 24 us (3.4 + 9.8
+// + 9.3); 64 x 128,256, settings a row, 50 (8.2, read at 4.0 TB/s, + 26.0 + 17.7); 24 x
+// 262,144 by temperature alone 51. Of row_bins' 26.0 the logits and their bins are 8.0, the
+// weights 9.1 (21 of 50 instructions a logit are f64's: 4.4 at its full rate), adds to LDS 0.8,
+// to memory 3.0, the search by a row's last workgroup 5.0; of the one row's 9.8 they are 4.0,
+// 0.5, 0.1, 1.6 and 3.4. Weights of f32's exponential in the bins, with bounds, and whole
+// ones summed in row_draw took as long where few tokens lay within the bounds, and 200 -
+// 600 us where a draw near the end of a flat row had thousands. A flat row whose range a mask
+// of large finite values makes useless has hundreds of tokens a bin: past kList in those that
+// matter it is one workgroup's, as where many logits are equal.
 #include <algorithm>
 #include <cstddef>
 
