@@ -324,3 +324,16 @@ def test_two_streams_at_once(ctx, dev):
         stream.destroy()
     for step in steps:
         step.pool.pool.free()
+
+
+def test_units_that_are_not_in_pieces(ctx, dev):
+    """A unit a workgroup, each of one length, and as many of two lengths."""
+    from charlotte_amd import harness as hx
+
+    for requests in ([(416, 64)] * 64, [(416, 64), (380, 60)] * 40):
+        step = _Step(ctx, dev, "q8_0", requests, 16, 4, 128, seed=11)
+        step.run()
+        hx.sync()
+        assert step.form() is not None
+        step.check(step.got())
+        step.pool.pool.free()
